@@ -375,3 +375,71 @@ int attention_wide_launch(const float *qfull, int qfs, const float *kx, const fl
 // (attention_launch's last_hint; -1 = not known, narrow).  Only the launch
 // shape depends on it, never the result.
 bool attention_wide(int last_pos);
+
+// ------------------------------------------------------------ 16-bit element types
+// The element types of the serving operators: f16 and bf16 values in memory,
+// f32 in registers, rounded to nearest even.
+struct TypeF16 {
+  typedef _Float16 elem;
+  typedef half8_t vec8;
+};
+struct TypeBF16 {
+  typedef __bf16 elem;
+  typedef __bf16 vec8 __attribute__((ext_vector_type(8)));
+};
+
+// ------------------------------------------------------------ rope.hip
+struct cwen_rope {
+  int head_dim, n_rot, layout;
+  float mscale;
+  double turns[128];   // pair i turns by pos * turns[i] whole circles
+};
+struct RopeParams {
+  const void *q; long long q_ts, q_hs;   // source of the first n_head heads
+  void *qo; long long qo_ts, qo_hs;
+  const void *k, *v; long long k_ts, v_ts;   // null: no cache
+  cwen_kv kv;
+  int layer;
+  const int *seq, *slot, *pos;
+  int T, nh, inverse;
+};
+int rope_launch(const cwen_rope *r, int xtype, int ytype, const RopeParams &p, hipStream_t st);
+
+// ------------------------------------------------------------ kv.hip
+int kv_reset_launch(const cwen_kv &kv, hipStream_t st);
+int kv_reserve_launch(const cwen_kv &kv, const int *seqs, const int *n, int n_req, hipStream_t st);
+int kv_fork_launch(const cwen_kv &kv, const int *src, const int *dst, int n_req, hipStream_t st);
+int kv_keep_launch(const cwen_kv &kv, const int *seqs, const int *count, const int *path, int ps, int n_req,
+                   hipStream_t st);
+int kv_truncate_launch(const cwen_kv &kv, const int *seqs, const int *len, int n_req, hipStream_t st);
+int kv_take_status_launch(const cwen_kv &kv, int *out, hipStream_t st);
+
+// ------------------------------------------------------------ attn.hip
+struct PromptArgs {
+  const void *q, *k, *v;
+  void *o;
+  long long qs, ks, vs, os;
+  float *lse;
+  const int *cu_q, *cu_k;
+  int n_seq, total_q, total_k, nh, nkv;
+  float scale;
+};
+int attn_prompt_launch(const cwen_ctx *ctx, int type, int D, const PromptArgs &a, hipStream_t st);
+struct TreeArgs {
+  cwen_kv kv;
+  int layer;
+  const void *q;
+  void *o;
+  long long qs, os;
+  float *lse;
+  const int *seqs, *cu;
+  const unsigned long long *mask;
+  int mw, n_seq, total, max_nodes, max_len, nh;
+  float scale;
+};
+int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st);
+
+// ------------------------------------------------------------ cache pages (device)
+__device__ __forceinline__ void kv_raise(const cwen_kv &kv, int bits) {
+  __hip_atomic_fetch_or(kv.status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}

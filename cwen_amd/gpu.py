@@ -18,11 +18,12 @@ CWEN_OK = 0
 CWEN_ERANGE = -6
 ERRORS = {-1: "EINVAL", -2: "EHIP", -3: "ENOMEM", -4: "ETYPE", -5: "ESCRATCH", -6: "ERANGE", -7: "EIO"}
 
+T_F16, T_BF16 = 1, 30
 T_F32, T_Q4_0, T_Q4_1, T_Q8_0, T_Q5_K, T_Q6_K, T_Q4_0RS, T_Q4_0RSI = 0, 2, 3, 8, 13, 14, 101, 102
 BMAX = 16
 
 # (name, restype, argtypes) of every exported entry point.
-_VP, _I, _F = C.c_void_p, C.c_int, C.POINTER(C.c_float)
+_VP, _I, _F, _LL = C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_longlong
 SIGNATURES = [
     ("cwen_version", C.c_char_p, []),
     ("cwen_ctx_create", _I, [_I, C.POINTER(_VP)]),
@@ -47,6 +48,19 @@ SIGNATURES = [
     ("cwen_gdn_get_state", _I, [_VP, _I, _VP, _VP]),
     ("cwen_gdn_block", _I, [_VP, _VP, _VP, _I, _VP, _I, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, _VP]),
     ("cwen_gdn_commit", _I, [_VP, _I]),
+    ("cwen_rope_create", _I, [_VP, C.POINTER(_VP)]),
+    ("cwen_rope_free", _I, [_VP]),
+    ("cwen_rope_apply", _I, [_VP, _VP, _I, _VP, _LL, _LL, _I, _VP, _LL, _LL, _VP, _I, _I, _I, _VP]),
+    ("cwen_rope_kv", _I, [_VP, _VP, _I, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _VP]),
+    ("cwen_kv_reset", _I, [_VP, _VP, _VP]),
+    ("cwen_kv_reserve", _I, [_VP, _VP, _VP, _VP, _I, _VP]),
+    ("cwen_kv_fork", _I, [_VP, _VP, _VP, _VP, _I, _VP]),
+    ("cwen_kv_keep", _I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _VP]),
+    ("cwen_kv_truncate", _I, [_VP, _VP, _VP, _VP, _I, _VP]),
+    ("cwen_kv_status", _I, [_VP, _VP, C.POINTER(_I), _VP]),
+    ("cwen_attn_prompt", _I, [_VP, _I, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I,
+                              C.c_float, _VP]),
+    ("cwen_attn_tree", _I, [_VP, _VP, _I, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, C.c_float, _VP]),
     ("cwen_model_create", _I, [_VP, _VP, C.POINTER(_VP)]),
     ("cwen_model_free", _I, [_VP]),
     ("cwen_model_set", _I, [_VP, _I, _I, _I, _VP, _VP, _I, _I]),
@@ -164,7 +178,7 @@ class Context:
     def __init__(self, device: int = 0):
         h = C.c_void_p()
         check("cwen_ctx_create", lib().cwen_ctx_create(device, C.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
 
     def close(self) -> None:
         if self.h:
@@ -332,6 +346,228 @@ class GDN:
             self.free()
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------- serving operators
+ROPE_LAYOUTS = {"pairs": 0, "halves": 1}
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2}
+KV_FULL, KV_ARG, KV_PAGE = 1, 2, 4
+KV_REQ_MAX, TREE_MAX = 4096, 256
+
+
+def _type(t) -> int:
+    """CWEN_T_* of a float tensor."""
+    name = str(t.dtype)
+    if name not in ("torch.float32", "torch.float16", "torch.bfloat16"):
+        raise ValueError(f"float32, float16 or bfloat16 expected, got {name}")
+    return {"torch.float32": T_F32, "torch.float16": T_F16, "torch.bfloat16": T_BF16}[name]
+
+
+def _heads(name: str, t, shape=None, dtype=None) -> int:
+    """Check a [tokens, heads, head_dim] tensor with heads in a row; its token stride."""
+    if t.dim() != 3 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape or '[tokens, heads, head_dim]'}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: {t.dtype}, expected {dtype}")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+        raise ValueError(f"{name}: heads of a token must lie in a row")
+    if t.shape[0] <= 1:
+        return t.shape[1] * t.shape[2]
+    return t.stride(0)
+
+
+def _vec(name: str, t, n: int | None, dtype: str = "int32"):
+    """Check a contiguous device vector of n elements (None: any number)."""
+    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{name}: contiguous {dtype} of {n if n is not None else 'any number of'} elements expected")
+    return t
+
+
+def _on(ctx: "Context", **tensors) -> None:
+    """Every tensor (None skipped) is on the context's device."""
+    for name, t in tensors.items():
+        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
+            raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
+
+
+class RopeCfg(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("head_dim", "n_rot", "layout", "scaling", "freq_dim")] + \
+               [(n, C.c_double) for n in ("theta", "factor", "orig_ctx", "beta_fast", "beta_slow", "mscale")]
+
+
+class Rope:
+    """The tables of a rotary configuration (cwen_rope_create; no GPU needed)."""
+
+    def __init__(self, head_dim: int, n_rot: int | None = None, theta: float = 1e4, layout: str = "pairs",
+                 scaling: str = "plain", factor: float = 1.0, orig_ctx: float = 0.0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, mscale: float = 0.0, freq_dim: int = 0):
+        self.cfg = RopeCfg(head_dim, head_dim if n_rot is None else n_rot, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling],
+                           freq_dim, theta, factor, orig_ctx, beta_fast, beta_slow, mscale)
+        h = C.c_void_p()
+        check("cwen_rope_create", lib().cwen_rope_create(C.byref(self.cfg), C.byref(h)))
+        self.h, self.head_dim = h, head_dim
+
+    def free(self) -> None:
+        if self.h:
+            lib().cwen_rope_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def rope(ctx: Context, r: Rope, x, y, pos, inverse: bool = False, stream=None) -> None:
+    """y = x turned to its positions (cwen_rope_apply); x, y [tokens, heads, head_dim] of
+    any strides with the head's elements in a row, y may be x."""
+    T, H, D = x.shape
+    if tuple(y.shape) != (T, H, D) or D != r.head_dim:
+        raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, head_dim {r.head_dim}")
+    if x.numel() and (x.stride(2) != 1 or y.stride(2) != 1):
+        raise ValueError("a head's elements must lie in a row")
+    _on(ctx, x=x, y=y, pos=pos)
+    check("cwen_rope_apply", lib().cwen_rope_apply(
+        ctx.h, r.h, _type(x), _ptr(x), x.stride(0) if T > 1 else 0, x.stride(1) if H > 1 else 0, _type(y), _ptr(y),
+        y.stride(0) if T > 1 else 0, y.stride(1) if H > 1 else 0, _ptr(_vec("pos", pos, T)), T, H, int(inverse),
+        _stream(stream)))
+
+
+class KvCache(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "n_layers", "n_kv_head", "head_dim", "page", "n_pages", "max_seqs", "max_pages")] + \
+               [(n, C.c_void_p) for n in ("k", "v", "table", "len", "held", "ref", "work", "status")]
+
+
+class PagedKV:
+    """A paged KV cache over torch tensors (cwen_kv_*): k and v [layers, pages,
+    KV heads, page, head_dim], table [sequences, pages of one at most], len, held
+    [sequences], ref [pages], all int32 but the pools.  PagedKV.empty allocates one."""
+
+    def __init__(self, page: int, k, v, table, len, held, ref):
+        import torch
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) or \
+                k.shape[3] != page:
+            raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: contiguous [layers, pages, heads, {page}, head_dim] expected")
+        L, P, H, _, D = k.shape
+        if table.dim() != 2 or any(t.device != k.device for t in (v, table, len, held, ref)):
+            raise ValueError("table must be [sequences, pages], every tensor on one device")
+        S, M = table.shape
+        for name, t, n in (("table", table, S * M), ("len", len, S), ("held", held, S), ("ref", ref, P)):
+            _vec(name, t, n)
+        self.k, self.v, self.table, self.len, self.held, self.ref = k, v, table, len, held, ref
+        self.work = torch.empty(P + 4 * S + 4, dtype=torch.int32, device=k.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self.page, self.layers, self.heads, self.head_dim = page, L, H, D
+        self.c = KvCache(_type(k), L, H, D, page, P, S, M, *(_ptr(t) for t in (k, v, table, len, held, ref, self.work, self.status)))
+        self.ref_c = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, n_layers: int, n_kv_head: int, head_dim: int, page: int, n_pages: int, max_seqs: int, max_pages: int,
+              dtype, device="cuda") -> "PagedKV":
+        import torch
+        ints = lambda v, *n: torch.full(n, v, dtype=torch.int32, device=device)
+        pool = lambda: torch.zeros(n_layers, n_pages, n_kv_head, page, head_dim, dtype=dtype, device=device)
+        return cls(page, pool(), pool(), ints(-1, max_seqs, max_pages), ints(0, max_seqs), ints(0, max_seqs), ints(0, n_pages))
+
+    def reset(self, ctx: Context, stream=None) -> None:
+        _on(ctx, cache=self.k)
+        check("cwen_kv_reset", lib().cwen_kv_reset(ctx.h, self.ref_c, _stream(stream)))
+
+    def reserve(self, ctx: Context, seqs, n, stream=None) -> None:
+        """Room for n more positions of each sequence."""
+        _on(ctx, cache=self.k, seqs=seqs, n=n)
+        check("cwen_kv_reserve", lib().cwen_kv_reserve(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
+                                                       _ptr(_vec("n", n, seqs.numel())), seqs.numel(), _stream(stream)))
+
+    def fork(self, ctx: Context, src, dst, stream=None) -> None:
+        """dst sequences share the src sequences' pages."""
+        _on(ctx, cache=self.k, src=src, dst=dst)
+        check("cwen_kv_fork", lib().cwen_kv_fork(ctx.h, self.ref_c, _ptr(_vec("src", src, None)),
+                                                 _ptr(_vec("dst", dst, src.numel())), src.numel(), _stream(stream)))
+
+    def keep(self, ctx: Context, seqs, count, path=None, stream=None) -> None:
+        """Accept the rows path[i, :count[i]] (None: the first count[i]) behind each sequence."""
+        _on(ctx, cache=self.k, seqs=seqs, count=count, path=path)
+        n, ps = seqs.numel(), 0
+        if path is not None:
+            if path.dim() != 2 or path.shape[0] != n:
+                raise ValueError(f"path {tuple(path.shape)}: [{n}, rows] expected")
+            ps = path.shape[1]
+            _vec("path", path, n * ps)
+            if ps == 0:                           # nothing can be named: no row moves
+                path = None
+        check("cwen_kv_keep", lib().cwen_kv_keep(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
+                                                 _ptr(_vec("count", count, n)), _ptr(path), ps, n, _stream(stream)))
+
+    def truncate(self, ctx: Context, seqs, length=None, stream=None) -> None:
+        """Cut the sequences to `length` (None: 0) positions."""
+        _on(ctx, cache=self.k, seqs=seqs, length=length)
+        n = seqs.numel()
+        check("cwen_kv_truncate", lib().cwen_kv_truncate(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
+                                                         None if length is None else _ptr(_vec("length", length, n)), n,
+                                                         _stream(stream)))
+
+    def take_status(self, ctx: Context, stream=None) -> int:
+        """The KV_* bits raised since the last call, cleared.  Synchronous."""
+        _on(ctx, cache=self.k)
+        bits = C.c_int()
+        check("cwen_kv_status", lib().cwen_kv_status(ctx.h, self.ref_c, C.byref(bits), _stream(stream)))
+        return bits.value
+
+
+def rope_kv(ctx: Context, r: Rope, q, k, v, qo, kv: PagedKV, layer: int, seq, slot, pos, stream=None) -> None:
+    """A step's projections: q turned into qo, k turned and v into the cache's pages (cwen_rope_kv)."""
+    T, H, D = q.shape
+    if D != kv.head_dim or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype}, k {k.dtype}, v {v.dtype}: the cache's head_dim is {kv.head_dim}")
+    _on(ctx, q=q, k=k, v=v, qo=qo, cache=kv.k, seq=seq, slot=slot, pos=pos)
+    qs, qos = _heads("q", q), _heads("qo", qo, (T, H, D), kv.k.dtype)
+    ks, vs = _heads("k", k, (T, kv.heads, D)), _heads("v", v, (T, kv.heads, D))
+    check("cwen_rope_kv", lib().cwen_rope_kv(
+        ctx.h, r.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(qo), qos, kv.ref_c, layer, _ptr(_vec("seq", seq, T)),
+        _ptr(_vec("slot", slot, T)), _ptr(_vec("pos", pos, T)), T, H, _stream(stream)))
+
+
+def attn_prompt(ctx: Context, q, k, v, o, cu_q, cu_k=None, lse=None, scale: float | None = None, stream=None) -> None:
+    """Causal attention over packed sequences (cwen_attn_prompt); q, o [tokens, heads,
+    head_dim], k, v [tokens, KV heads, head_dim], cu_* the sequences' borders."""
+    (T, H, D), (Tk, Hk, _) = q.shape, k.shape
+    _on(ctx, q=q, k=k, v=v, o=o, cu_q=cu_q, cu_k=cu_k, lse=lse)
+    qs, os_ = _heads("q", q), _heads("o", o, (T, H, D), q.dtype)
+    ks, vs = _heads("k", k, (Tk, Hk, D), q.dtype), _heads("v", v, (Tk, Hk, D), q.dtype)
+    n = cu_q.numel() - 1
+    if n < 0:
+        raise ValueError("cu_q: at least one border expected")
+    if lse is not None:
+        _vec("lse", lse, T * H, "float32")
+    if cu_k is not None:
+        _vec("cu_k", cu_k, n + 1)
+    check("cwen_attn_prompt", lib().cwen_attn_prompt(
+        ctx.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(o), os_, _ptr(lse), _ptr(_vec("cu_q", cu_q, None)),
+        _ptr(cu_k), n, T, Tk, H, Hk, D, D ** -0.5 if scale is None else scale, _stream(stream)))
+
+
+def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: int, max_len: int, mask=None, lse=None,
+              scale: float | None = None, stream=None) -> None:
+    """Attention of drafted trees over the cache (cwen_attn_tree); q, o [nodes, heads, head_dim],
+    mask int64 [nodes, words] (None: chains), node i of a group in position len + i of its sequence."""
+    T, H, D = q.shape
+    if D != kv.head_dim:
+        raise ValueError(f"q {tuple(q.shape)}: the cache's head_dim is {kv.head_dim}")
+    _on(ctx, q=q, o=o, cache=kv.k, seqs=seqs, cu=cu, mask=mask, lse=lse)
+    qs, os_ = _heads("q", q, None, kv.k.dtype), _heads("o", o, (T, H, D), kv.k.dtype)
+    n, mw = seqs.numel(), 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != T:
+            raise ValueError(f"mask {tuple(mask.shape)}: [{T}, words] expected")
+        mw = mask.shape[1]
+        _vec("mask", mask, T * mw, "int64")
+    if lse is not None:
+        _vec("lse", lse, T * H, "float32")
+    check("cwen_attn_tree", lib().cwen_attn_tree(
+        ctx.h, kv.ref_c, layer, _ptr(q), qs, _ptr(o), os_, _ptr(lse), _ptr(_vec("seqs", seqs, None)), _ptr(_vec("cu", cu, n + 1)),
+        _ptr(mask), mw, n, T, max_nodes, max_len, H, D ** -0.5 if scale is None else scale, _stream(stream)))
 
 
 # ---------------------------------------------------------------- model

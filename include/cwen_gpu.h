@@ -44,6 +44,8 @@ extern "C" {
 
 /* ggml / CWENR weight type ids -- the same numeric ids as run.c:97-103 */
 #define CWEN_T_F32      0
+#define CWEN_T_F16      1    /* element types of the paged cache, of rotary     */
+#define CWEN_T_BF16    30    /* tensors and of the prompt and tree attention    */
 #define CWEN_T_Q4_0     2    /* GGUF 18-byte blocks {f16 d; u8 qs[16]}          */
 #define CWEN_T_Q4_1     3    /* GGUF 20-byte blocks {f16 d; f16 m; u8 qs[16]},
                                 w = n*d + m (run.c:111, 571-588, 1026-1099)     */
@@ -211,6 +213,163 @@ int cwen_gdn_block(cwen_ctx *ctx, cwen_gdn *g, const float *qkv, int qs, const f
  * + the replaying forward_block of a short walk (run.c:4975-4988) for this
  * layer. */
 int cwen_gdn_commit(cwen_gdn *g, int n);
+
+/* ---- rotary positions ----
+ * Turns the first n_rot dims of each head by angles a_i = pos * f_i, i <
+ * n_rot / 2: the pair (x, y) becomes m (x cos a - y sin a, x sin a + y cos a);
+ * the dims behind n_rot pass through.  The pairs are (2i, 2i + 1) (rope_apply,
+ * run.c:1936-1948) or (i, i + n_rot / 2).  With b_i = theta^(-2i / freq_dim):
+ *   PLAIN   f_i = b_i
+ *   LINEAR  f_i = b_i / factor
+ *   YARN    f_i = b_i (1 - r_i) + b_i / factor r_i, r_i = (i - low) / (high -
+ *           low) held to 0..1, low = floor(c(beta_fast)) >= 0, high =
+ *           ceil(c(beta_slow)) <= freq_dim - 1 (low + 0.001 when they meet),
+ *           c(b) = freq_dim ln(orig_ctx / (2 pi b)) / (2 ln theta)
+ * m = mscale; 0 there stands for 1, with YARN for 0.1 ln(factor) + 1.
+ * freq_dim 0 stands for n_rot (the model's tables, run.c:1903-1934, are
+ * freq_dim = 2 n_rot there).  Angles are reduced in 64 bits: exact to f32 at
+ * any int position. */
+typedef struct cwen_rope cwen_rope;
+enum { CWEN_ROPE_PAIRS = 0, CWEN_ROPE_HALVES = 1 };
+enum { CWEN_ROPE_PLAIN = 0, CWEN_ROPE_LINEAR = 1, CWEN_ROPE_YARN = 2 };
+typedef struct {
+  int head_dim;                     /* a multiple of 8, 8..512                          */
+  int n_rot;                        /* a multiple of 8 (HALVES: 16), 8..min(head_dim, 256) */
+  int layout, scaling;              /* CWEN_ROPE_*                                      */
+  int freq_dim;                     /* >= 0                                             */
+  double theta;                     /* > 1                                              */
+  double factor;                    /* >= 1 (LINEAR, YARN)                              */
+  double orig_ctx, beta_fast, beta_slow;   /* YARN: all > 0, beta_fast >= beta_slow     */
+  double mscale;                    /* >= 0                                             */
+} cwen_rope_cfg;
+/* The tables of a configuration, in host memory (no GPU needed; calls on any
+ * device and stream may share one, also at the same time). */
+int cwen_rope_create(const cwen_rope_cfg *cfg, cwen_rope **out);
+int cwen_rope_free(cwen_rope *r);
+/* y[t][h] = x[t][h] turned to pos[t] (device ints), t < T, h < n_head; element
+ * types xtype and ytype (F32, F16, BF16), computed in f32 and rounded once.
+ * Element (t, h, d) is at t * x_ts + h * x_hs + d.  With `inverse` the angles
+ * are negated: the gradient of the turn (for m = 1 its inverse).  y may be x
+ * itself (same type and strides), and must not overlap it otherwise.  x and y
+ * are 16-byte aligned and all strides multiples of 8; T may be 0. */
+int cwen_rope_apply(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *x, long long x_ts, long long x_hs,
+                    int ytype, void *y, long long y_ts, long long y_hs, const int *pos, int T, int n_head,
+                    int inverse, void *stream);
+
+/* ---- paged KV cache ----
+ * Sequences of positions in pages that several sequences may share.  The
+ * caller owns the memory; all of it is DEVICE memory and every call works on
+ * it in stream order, without a copy to the host, so calls can be captured.
+ * Calls on one cache must not overlap.  A page holds `page` positions of
+ * every layer and KV head: element (layer, page, head, slot, dim) of k and v
+ * is at (((layer * n_pages + page) * n_kv_head + head) * page_size + slot) *
+ * head_dim + dim.
+ * Sequence s owns the pages table[s * max_pages + i], i < held[s], in the
+ * order of its positions, of which the first len[s] are filled.  ref[p] counts
+ * the sequences that hold page p (0: free).  Unused table entries are -1.
+ * A request that cannot be met raises a bit of *status, which stays until
+ * cwen_kv_status clears it; the sequence it names is left as it was, and the
+ * call's other requests are carried out. */
+typedef struct {
+  int type;                /* CWEN_T_F16 or CWEN_T_BF16                            */
+  int n_layers, n_kv_head;
+  int head_dim;            /* a multiple of 8, 8..512 (attention: 64, 128, 256)    */
+  int page;                /* positions of a page: 16, 32, 64, 128 or 256          */
+  int n_pages;             /* 1..2^24                                              */
+  int max_seqs;            /* 1..65536                                             */
+  int max_pages;           /* pages of one sequence at most; max_pages * page < 2^30 */
+  void *k, *v;             /* 16-byte aligned                                      */
+  int *table;              /* [max_seqs][max_pages]                                */
+  int *len, *held;         /* [max_seqs]                                           */
+  int *ref;                /* [n_pages], 16-byte aligned                           */
+  int *work;               /* scratch of the calls: CWEN_KV_WORK(n_pages, max_seqs) ints */
+  int *status;             /* 1 int                                                */
+} cwen_kv;
+#define CWEN_KV_WORK(n_pages, max_seqs) ((size_t)(n_pages) + 4 * (size_t)(max_seqs) + 4)
+#define CWEN_KV_FULL 1     /* a reserve found too few free pages                   */
+#define CWEN_KV_ARG  2     /* a request's sequence, length, path or slot is invalid */
+#define CWEN_KV_PAGE 4     /* a table entry is no page; the result is unspecified  */
+/* Requests of one call at most (and never more than max_seqs). */
+#define CWEN_KV_REQ_MAX 4096
+/* Every sequence empty, every page free, status 0 (k and v as they are). */
+int cwen_kv_reset(cwen_ctx *ctx, const cwen_kv *kv, void *stream);
+/* Make room for n[i] (device, >= 0) positions behind len of sequence seqs[i]
+ * (device), i < n_req: held grows to cover them, and the page that holds
+ * position len, if other sequences hold it too, is replaced by a copy of its
+ * filled part in every layer.  The last holder of a shared page keeps it.
+ * Pages are taken lowest id first, in the order of the requests (a request's
+ * copy before its new pages).  All or nothing: with too few free pages
+ * (CWEN_KV_FULL) or any invalid request (CWEN_KV_ARG: an id out of range or
+ * named twice, a length past max_pages) nothing changes. */
+int cwen_kv_reserve(cwen_ctx *ctx, const cwen_kv *kv, const int *seqs, const int *n, int n_req, void *stream);
+/* dst[i] (empty: no pages) becomes a second holder of src[i]'s filled pages.
+ * A sequence may be the source of many, but a destination only once and never
+ * a source of the same call. */
+int cwen_kv_fork(cwen_ctx *ctx, const cwen_kv *kv, const int *src, const int *dst, int n_req, void *stream);
+/* Fill count[i] of the reserved positions: the rows at len + path[i * ps + j]
+ * (device, strictly increasing from >= 0, j < count[i] <= ps) become the rows
+ * len + j of every layer; then len grows by count[i] and the pages behind it
+ * are given back.  This keeps one branch of a drafted tree.  path NULL: the
+ * first count[i] rows stay where they are (ps unused).  Rows that move must
+ * be in pages of their own (reserved since the last fork). */
+int cwen_kv_keep(cwen_ctx *ctx, const cwen_kv *kv, const int *seqs, const int *count, const int *path, int ps,
+                 int n_req, void *stream);
+/* Cut sequences to len[i] <= their length (len NULL: to 0) and give back the
+ * pages behind it. */
+int cwen_kv_truncate(cwen_ctx *ctx, const cwen_kv *kv, const int *seqs, const int *len, int n_req, void *stream);
+/* Read the status bits to the HOST and clear them.  Synchronous. */
+int cwen_kv_status(cwen_ctx *ctx, const cwen_kv *kv, int *bits, void *stream);
+
+/* A step's projections into the cache: token t < T of sequence seq[t] (device)
+ * has q [n_head], k and v [n_kv_head] heads of head_dim at x + t * stride,
+ * element type xtype (F32, F16, BF16); q and k are turned to pos[t]; q goes to
+ * qo + t * qo_ts (the cache's type, heads in a row), k and v to position
+ * slot[t] of the sequence in `layer`, rounded to the cache's type once.  The
+ * position must be in a page that the sequence holds alone (cwen_kv_reserve);
+ * otherwise, and for an id out of range, nothing is written and CWEN_KV_ARG
+ * raised.  A token of slot < 0 is padding: its k and v are not written.
+ * Pointers 16-byte aligned, strides multiples of 8; qo must not overlap q,
+ * unless it is q itself in type and stride. */
+int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, long long q_ts, const void *k,
+                 long long k_ts, const void *v, long long v_ts, void *qo, long long qo_ts, const cwen_kv *kv, int layer,
+                 const int *seq, const int *slot, const int *pos, int T, int n_head, void *stream);
+
+/* ---- attention of prompts and drafted trees ----
+ * Both: f16 or bf16 operands, scores, softmax and sums in f32 on the matrix
+ * cores, the probabilities rounded to the operands' type before their product
+ * with v, the output rounded once.  n_head a multiple of n_kv_head (query head
+ * h reads KV head h / (n_head / n_kv_head)), head_dim 64, 128 or 256, scale >
+ * 0 and finite.  Heads of a token are in a row ([head][head_dim]), tokens
+ * `stride` elements apart; pointers 16-byte aligned, strides multiples of 8.
+ * lse (nullable, f32 [token][n_head]): the natural log of the row's sum of
+ * exp(scale * score).  A row that sees no key gives zeros and lse = -inf.
+ * Keys and values that a row does not see have no influence on it, whatever
+ * they hold (NaN and infinities included).  Outputs must not overlap inputs. */
+
+/* Causal attention over packed sequences.  Sequence s < n_seq holds queries
+ * cu_q[s] .. cu_q[s+1]-1 and keys cu_k[s] .. cu_k[s+1]-1 (device, n_seq + 1
+ * non-decreasing ints within 0..total_q and 0..total_k; cu_k NULL: cu_q);
+ * its query i sees keys j <= i + (keys - queries).  Rows of o that no
+ * sequence covers are left as they were; lengths may be 0. */
+int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, const void *k, long long k_ts,
+                     const void *v, long long v_ts, void *o, long long o_ts, float *lse, const int *cu_q,
+                     const int *cu_k, int n_seq, int total_q, int total_k, int n_head, int n_kv_head, int head_dim,
+                     float scale, void *stream);
+
+/* Attention of drafted trees over the paged cache.  Group s < n_seq is
+ * sequence seqs[s] (device) with the nodes cu[s] .. cu[s+1]-1 (device, as
+ * cu_q above, at most max_nodes <= CWEN_TREE_MAX each; nodes past max_nodes
+ * are left as they were).  Node i's key and value are in position len + i of
+ * the sequence (cwen_rope_kv put them there); node i sees the len cached
+ * positions and the nodes j of its group whose bit j is set in its row of
+ * mask (device, [total][mw] words of 64 bits; bits past the group are
+ * ignored).  mask NULL: a chain, j <= i; one node alone is a decode step.
+ * Works on the context's scratch.  max_len: the expected longest context; it
+ * guides the launch and may be wrong. */
+#define CWEN_TREE_MAX 256
+int cwen_attn_tree(cwen_ctx *ctx, const cwen_kv *kv, int layer, const void *q, long long q_ts, void *o, long long o_ts,
+                   float *lse, const int *seqs, const int *cu, const unsigned long long *mask, int mw, int n_seq,
+                   int total, int max_nodes, int max_len, int n_head, float scale, void *stream);
 
 /* ---- the block-verify model ----
  * The reference's hybrid decoder (run.c:80-92, 140-160) resident on one
