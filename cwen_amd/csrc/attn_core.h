@@ -1,0 +1,183 @@
+// The tile of prompt and tree attention: one wave's 32 query rows against BN
+// keys whose K and V rows lie in LDS.
+//
+// The scores are taken transposed, S^T = K Q^T (v_mfma_f32_32x32x16, K the
+// left operand): lane (n = lane & 31, hi = lane >> 5) then holds 16 scores of
+// query n per 32 keys, namely of the keys 8 i + 4 hi + j (i, j < 4).  So the
+// softmax's maximum and sum run over a lane's own registers with one exchange
+// between the wave's halves, and the probabilities are already where the next
+// product wants them: O^T = V^T P^T, P^T the right operand, whose lane (n, hi)
+// supplies 8 keys of query n.  A product's keys may be taken in any order as
+// long as both operands agree; V^T's lanes read the matching keys, 4 and 4,
+// with transposing LDS reads (ds_read_b64_tr_b16).
+//
+// Rows in LDS are D elements without padding (they arrive by loads that land
+// there directly); their 16-byte pieces are permuted instead, so that lanes that
+// read the same piece of different rows hit different banks.
+#pragma once
+#include <math.h>
+#include "cwen_internal.h"
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void attn_lds_t;
+typedef const __attribute__((address_space(1))) void attn_glb_t;
+
+template <typename T> struct AttnOps;
+template <> struct AttnOps<TypeF16> {
+  typedef TypeF16::vec8 vec8;
+  typedef _Float16 vec4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x16_t mma(vec8 a, vec8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ vec4 tr(const void *p) {
+    typedef __fp16 v4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        vec4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4 *)(attn_lds_t *)const_cast<void *>(p)));
+  }
+  // NaN when an element is not finite (times 0).
+  static __device__ __forceinline__ float probe(vec8 v, float acc) {
+    const half2_t z = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2((half2_t){v[i], v[i + 1]}, z, acc, false);
+    return acc;
+  }
+};
+template <> struct AttnOps<TypeBF16> {
+  typedef TypeBF16::vec8 vec8;
+  typedef __bf16 vec4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x16_t mma(vec8 a, vec8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ vec4 tr(const void *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) vec4 *)(attn_lds_t *)const_cast<void *>(p));
+  }
+  static __device__ __forceinline__ float probe(vec8 v, float acc) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc = fmaf((float)v[i], 0.f, acc);
+    return acc;
+  }
+};
+
+// Pieces (16 bytes) of a row, and where piece c of row r is kept.
+template <int D> __device__ __forceinline__ constexpr int k_piece(int r, int c) { return c ^ (r & (D >= 128 ? 15 : 7)); }
+template <int D> __device__ __forceinline__ constexpr int v_piece(int r, int c) {
+  return c ^ (D >= 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2);
+}
+
+__device__ __forceinline__ float max_halves(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  return __builtin_bit_cast(float, (int)p[0]) + __builtin_bit_cast(float, (int)p[1]);
+}
+
+// The maximum a row's exponents are taken against is renewed only when a row
+// outgrew it by more than 2^8: the probabilities stay below 2^8 (f16 holds
+// 65504), and most tiles then leave the output sums alone.
+constexpr float ATTN_SLACK = 8.f;
+
+template <typename T, int D, int BN> struct AttnWave {
+  typedef typename T::elem elem;
+  typedef typename AttnOps<T>::vec8 vec8;
+  typedef typename AttnOps<T>::vec4 vec4;
+  static constexpr int QS = D / 16, OB = D / 32, KB = BN / 32;
+
+  vec8 q[QS];        // dims 16 s + 8 hi .. + 7 of query n
+  f32x16_t o[OB];    // [i]: output dims 32 b + 8 (i / 4) + 4 hi + i % 4 of query n
+  float m, l;        // maximum (in powers of two) and this lane's part of the sum
+  float odd;         // NaN once a partly hidden tile held a value that is not finite
+
+  // row: the query's elements, null for a row that does not exist
+  __device__ __forceinline__ void start(const elem *row) {
+    const int hi = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) q[s] = row ? *(const vec8 *)(row + 16 * s + 8 * hi) : vec8{};
+#pragma unroll
+    for (int b = 0; b < OB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+    m = -INFINITY;
+    l = odd = 0.f;
+  }
+
+  // One tile.  K, V: LDS arrays of BN rows.  c: scale * log2(e).  HIDE: hide(j)
+  // tells whether this lane's query does not see key j of the tile.
+  template <bool HIDE, typename F> __device__ __forceinline__ void tile(const elem *K, const elem *V, float c, F hide) {
+    const int lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    f32x16_t s[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < QS; ++k)
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        const vec8 kf = *(const vec8 *)(K + (b * 32 + n) * D + 8 * k_piece<D>(n, 2 * k + hi));
+        s[b] = AttnOps<T>::mma(kf, q[k], s[b]);
+      }
+    if (HIDE) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (hide(b * 32 + 8 * (i >> 2) + 4 * hi + (i & 3))) s[b][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = max_halves(mx) * c;
+    if (__any(mx > m + ATTN_SLACK)) {
+      const float mn = fmaxf(m, mx), a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= a;
+#pragma unroll
+      for (int b = 0; b < OB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= a;
+      m = mn;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    vec8 p[2 * KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -ms));
+        l += e;
+        p[2 * b + (i >> 3)][i & 7] = (elem)e;     // half a step; the sum keeps all of it
+      }
+    // Lane i of a group of 16 addresses the 4 keys' rows 4 g + i / 4 and gets column i of all 4.
+    const int vi = lane & 15, vr = 4 * hi + (vi >> 2), vc = ((lane >> 4) & 1) * 2 + ((vi & 3) >> 1), ve = (vi & 1) * 4;
+#pragma unroll
+    for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+      for (int b = 0; b < OB; ++b) {
+        const elem *at = V + (16 * t + vr) * D + 8 * v_piece<D>(vr, 4 * b + vc) + ve;
+        const vec4 a = AttnOps<T>::tr(at), d = AttnOps<T>::tr(at + 8 * D);
+        const vec8 vf = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
+        if (HIDE) odd = AttnOps<T>::probe(vf, odd);
+        o[b] = AttnOps<T>::mma(vf, p[t], o[b]);
+      }
+  }
+
+  // The whole row's sum.
+  __device__ __forceinline__ float sum() const { return sum_halves(l); }
+};
+
+// Rows of a tile into LDS, by NW waves: row(r) gives row r's elements in memory
+// (r < BN).  A wave's pieces are consecutive in LDS, as the load requires.
+template <int D, int BN, bool ISV, int NW, typename elem, typename F>
+__device__ __forceinline__ void land_rows(elem *dst, int wave, F row) {
+  constexpr int C = D / 8;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < BN * C / (64 * NW); ++i) {
+    const int x0 = (i * NW + wave) * 64, x = x0 + lane, r = x / C, p = x % C;
+    const int c = ISV ? v_piece<D>(r, p) : k_piece<D>(r, p);
+    __builtin_amdgcn_global_load_lds((attn_glb_t *)(row(r) + 8 * c), (attn_lds_t *)(dst + 8 * x0), 16, 0, 0);
+  }
+}
