@@ -102,11 +102,9 @@ template <typename T, int D, int BN> struct AttnWave {
     l = odd = 0.f;
   }
 
-  // One tile.  K, V: LDS arrays of BN rows.  c: scale * log2(e).  HIDE: hide(j)
-  // tells whether this lane's query does not see key j of the tile.
-  template <bool HIDE, typename F> __device__ __forceinline__ void tile(const elem *K, const elem *V, float c, F hide) {
+  // The scores of one tile, K the LDS array of its BN rows.
+  __device__ __forceinline__ void scores(const elem *K, f32x16_t (&s)[KB]) {
     const int lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
-    f32x16_t s[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -118,6 +116,11 @@ template <typename T, int D, int BN> struct AttnWave {
         const vec8 kf = *(const vec8 *)(K + (b * 32 + n) * D + 8 * k_piece<D>(n, 2 * k + hi));
         s[b] = AttnOps<T>::mma(kf, q[k], s[b]);
       }
+  }
+  // Their softmax against the row's maximum so far.  c: scale * log2(e).  HIDE:
+  // hide(j) tells whether this lane's query does not see key j of the tile.
+  template <bool HIDE, typename F> __device__ __forceinline__ void soft(f32x16_t (&s)[KB], float c, F hide, vec8 (&p)[2 * KB]) {
+    const int hi = (threadIdx.x & 63) >> 5;
     if (HIDE) {
 #pragma unroll
       for (int b = 0; b < KB; ++b)
@@ -141,7 +144,6 @@ template <typename T, int D, int BN> struct AttnWave {
       m = mn;
     }
     const float ms = m == -INFINITY ? 0.f : m;
-    vec8 p[2 * KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -150,7 +152,11 @@ template <typename T, int D, int BN> struct AttnWave {
         l += e;
         p[2 * b + (i >> 3)][i & 7] = (elem)e;     // half a step; the sum keeps all of it
       }
-    // Lane i of a group of 16 addresses the 4 keys' rows 4 g + i / 4 and gets column i of all 4.
+  }
+  // The outputs' sums, V the LDS array of the tile's rows.  Lane i of a group of
+  // 16 addresses the 4 keys' rows 4 g + i / 4 and gets column i of all 4.
+  template <bool HIDE> __device__ __forceinline__ void outputs(const elem *V, const vec8 (&p)[2 * KB]) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5;
     const int vi = lane & 15, vr = 4 * hi + (vi >> 2), vc = ((lane >> 4) & 1) * 2 + ((vi & 3) >> 1), ve = (vi & 1) * 4;
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
@@ -162,6 +168,13 @@ template <typename T, int D, int BN> struct AttnWave {
         if (HIDE) odd = AttnOps<T>::probe(vf, odd);
         o[b] = AttnOps<T>::mma(vf, p[t], o[b]);
       }
+  }
+  template <bool HIDE, typename F> __device__ __forceinline__ void tile(const elem *K, const elem *V, float c, F hide) {
+    f32x16_t s[KB];
+    vec8 p[2 * KB];
+    scores(K, s);
+    soft<HIDE>(s, c, hide, p);
+    outputs<HIDE>(V, p);
   }
 
   // The whole row's sum.

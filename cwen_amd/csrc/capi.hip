@@ -21,6 +21,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 constexpr size_t kScratchHalves = (size_t)CWEN_BMAX * CWEN_KMAX;
 constexpr size_t kPartialFloats = (size_t)8 << 20;   // 32 MiB of split-K partials
 constexpr int kCounters = 1 << 16;
+constexpr size_t kAttnFloats = (size_t)16 << 20;     // 64 MiB: some 2 chunks per CU of 128 rows of 256
 
 // Scratch of the allocation-free entry point, one copy per GPU, held until
 // the process ends: the f16 operand of X and the f16 hidden activations
@@ -142,12 +143,14 @@ int cwen_ctx_create(int device, cwen_ctx **out) {
       hipMalloc((void **)&c->counters, kCounters * sizeof(int)) != hipSuccess ||
       hipMalloc((void **)&c->amax_keys, CWEN_BMAX * sizeof(unsigned long long)) != hipSuccess ||
       hipMalloc((void **)&c->amax_cnt, sizeof(int)) != hipSuccess ||
+      hipMalloc((void **)&c->attn_part, kAttnFloats * sizeof(float)) != hipSuccess ||
       hipMalloc((void **)&c->res, (2 + CWEN_BMAX) * sizeof(int)) != hipSuccess) {
     cwen_ctx_destroy(c);
     return CWEN_ENOMEM;
   }
   c->partials_floats = kPartialFloats;
   c->ncounters = kCounters;
+  c->attn_floats = kAttnFloats;
   if (hipMemset(c->counters, 0, kCounters * sizeof(int)) != hipSuccess ||
       hipMemset(c->amax_keys, 0, CWEN_BMAX * sizeof(unsigned long long)) != hipSuccess ||
       hipMemset(c->amax_cnt, 0, sizeof(int)) != hipSuccess ||
@@ -175,6 +178,7 @@ int cwen_ctx_destroy(cwen_ctx *ctx) {
   if (ctx->counters) (void)hipFree(ctx->counters);
   if (ctx->amax_keys) (void)hipFree(ctx->amax_keys);
   if (ctx->amax_cnt) (void)hipFree(ctx->amax_cnt);
+  if (ctx->attn_part) (void)hipFree(ctx->attn_part);
   if (ctx->res) (void)hipFree(ctx->res);
   free(ctx);
   return CWEN_OK;

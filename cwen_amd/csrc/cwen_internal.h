@@ -34,6 +34,8 @@ struct cwen_ctx {
   int ncounters;
   unsigned long long *amax_keys;  // per-column argmax keys [CWEN_BMAX], zero between launches
   int *amax_cnt;            // argmax arrival counter, zero between launches
+  float *attn_part;         // partial outputs of the tree attention
+  size_t attn_floats;
   int *res;                 // device result slots of the verify entry points [2 + CWEN_BMAX]
 };
 
