@@ -65,6 +65,13 @@ __device__ __forceinline__ int span(const int *cu, int s, int total, int *first)
   *first = a;
   return max(b - a, 0);
 }
+// The same for a wave's one sequence, in scalar registers.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int span1(const int *cu, int s, int total, int *first) {
+  const int n = scalar(span(cu, s, total, first));
+  *first = scalar(*first);
+  return n;
+}
 template <int BM> __device__ __forceinline__ Item find_item(const int *cu, int n_seq, int total, int it) {
   const int lane = threadIdx.x & 63;
   for (int s0 = 0; s0 < n_seq; s0 += 64) {
@@ -84,11 +91,12 @@ template <int BM> __device__ __forceinline__ Item find_item(const int *cu, int n
   return {-1, 0};
 }
 
-template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(PromptArgs a) {
+// NW waves of 32 QB queries of one head share double-buffered tiles of BN keys.
+template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void prompt_kernel(PromptArgs a) {
   typedef typename T::elem elem;
-  constexpr int BM = 32 * NW;
+  constexpr int WM = 32 * QB, BM = WM * NW;
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = a.nh / a.nkv;
   // Blocks of one kv head go to one or two XCDs (block b runs on XCD b % 8), long rows first.
   const int hh = blockIdx.x % a.nh, h = (hh % a.nkv) * g + hh / a.nkv, hkv = hh % a.nkv;
@@ -96,20 +104,23 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
   const Item item = find_item<BM>(a.cu_q, a.n_seq, a.total_q, items - 1 - (int)(blockIdx.x / a.nh));
   if (item.seq < 0) return;
   int q0, k0;
-  const int nq = span(a.cu_q, item.seq, a.total_q, &q0), nk = span(a.cu_k, item.seq, a.total_k, &k0), off = nk - nq;
-  const int w0 = item.tile * BM + wave * 32, n = lane & 31;
-  const int row = w0 + n;                                        // this lane's query of the sequence
-  const bool live = row < nq;
-  const int limit = live ? row + off : -1;                       // its last key
-  AttnWave<T, D, BN> w;
-  w.start(live ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
+  const int nq = span1(a.cu_q, item.seq, a.total_q, &q0), nk = span1(a.cu_k, item.seq, a.total_k, &k0), off = nk - nq;
+  const int first = item.tile * BM, w0 = first + wave * WM;      // the workgroup's and this wave's first query
+  AttnWave<T, D, BN, QB> w;
+  int limit[QB];                                                 // the last key of this lane's queries
+#pragma unroll
+  for (int y = 0; y < QB; ++y) {
+    const int row = w0 + 32 * y + n;
+    limit[y] = row < nq ? row + off : -1;
+    w.start(y, row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
+  }
   const elem *kp = (const elem *)a.k + (long long)k0 * a.ks + hkv * D, *vp = (const elem *)a.v + (long long)k0 * a.vs + hkv * D;
-  const int kend = min(min(item.tile * BM + BM, nq) + off, nk);  // keys that the workgroup's rows see
-  const int wend = min(min(w0 + 32, nq) + off, nk);              // and this wave's
+  const int kend = min(min(first + BM, nq) + off, nk);           // keys that the workgroup's rows see
+  const int wend = min(min(w0 + WM, nq) + off, nk);              // and this wave's
   const float c = a.scale * LOG2E;
   auto land = [&](elem *Kd, elem *Vd, int t0) __attribute__((always_inline)) {
-    land_rows<D, BN, false, NW>(Kd, wave, [&](int r) { return kp + min(t0 + r, nk - 1) * a.ks; });
-    land_rows<D, BN, true, NW>(Vd, wave, [&](int r) { return vp + min(t0 + r, nk - 1) * a.vs; });
+    land_rows<D, BN, false, NW>(Kd, wave, t0, nk - 1, (uint32_t)a.ks * 2, [&](int, int j) { return kp + j * a.ks; });
+    land_rows<D, BN, true, NW>(Vd, wave, t0, nk - 1, (uint32_t)a.vs * 2, [&](int, int j) { return vp + j * a.vs; });
   };
   auto ready = [&]() __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -118,30 +129,28 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
   };
   // Tiles that every row sees whole come first, two per turn; what is left has
   // its keys compared with each row's last.
-  const int full = max(min(item.tile * BM + off + 1, nk), 0) / (2 * BN) * (2 * BN);
+  const int full = max(min(first + off + 1, nk), 0) / (2 * BN) * (2 * BN);
   if (kend > 0) land(K0, V0, 0);
   int t0 = 0;
   for (; t0 < full; t0 += 2 * BN) {
     ready();
     land(K1, V1, t0 + BN);
-    w.template tile<false>(K0, V0, c, [](int) { return false; });
+    w.template tile<false>(K0, V0, c, [](int, int) { return false; });
     ready();
     if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    w.template tile<false>(K1, V1, c, [](int) { return false; });
+    w.template tile<false>(K1, V1, c, [](int, int) { return false; });
   }
   for (; t0 < kend; t0 += 2 * BN) {
     ready();
     if (t0 + BN < kend) land(K1, V1, t0 + BN);
-    if (t0 < wend) w.template tile<true>(K0, V0, c, [&](int j) { return t0 + j > limit; });
+    if (t0 < wend) w.template tile<true>(K0, V0, c, [&](int y, int j) { return t0 + j > limit[y]; });
     if (t0 + BN >= kend) break;
     ready();
     if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    if (t0 + BN < wend) w.template tile<true>(K1, V1, c, [&](int j) { return t0 + BN + j > limit; });
+    if (t0 + BN < wend) w.template tile<true>(K1, V1, c, [&](int y, int j) { return t0 + BN + j > limit[y]; });
   }
-  const float l = w.sum();
-  elem *orow = (elem *)a.o + (long long)(q0 + row) * a.os + h * D;
   if (__any(w.odd != w.odd)) {   // a hidden value may have leaked: these rows one by one
-    for (int i = 0; i < 32 && w0 + i < nq; ++i) {
+    for (int i = 0; i < WM && w0 + i < nq; ++i) {
       const long long t = q0 + w0 + i;
       AttnRow<T, D> x;
       x.run((const elem *)a.q + t * a.qs + h * D, 0, min(nk, w0 + i + off + 1), c, [](int) { return true; },
@@ -153,19 +162,23 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
     }
     return;
   }
-  if (!live) return;
-  const float inv = limit < 0 ? 0.f : 1.f / l;
 #pragma unroll
-  for (int b = 0; b < D / 32; ++b)
+  for (int y = 0; y < QB; ++y) {
+    const int row = w0 + 32 * y + n;
+    const float l = w.sum(y), inv = limit[y] < 0 ? 0.f : 1.f / l;
+    if (row >= nq) continue;
+    elem *orow = (elem *)a.o + (long long)(q0 + row) * a.os + h * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      typename AttnOps<T>::vec4 v;
+    for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (elem)(limit < 0 ? 0.f : w.o[b][4 * i + j] * inv);
-      *(typename AttnOps<T>::vec4 *)(orow + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
-    }
-  if (a.lse && lane < 32)
-    a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m + __builtin_amdgcn_logf(l));
+      for (int i = 0; i < 4; ++i) {
+        typename AttnOps<T>::vec4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (elem)(limit[y] < 0 ? 0.f : w.o[y][b][4 * i + j] * inv);
+        *(typename AttnOps<T>::vec4 *)(orow + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
+      }
+    if (a.lse && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
+  }
 }
 
 // ---- trees over the paged cache ----
@@ -194,6 +207,10 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int s) {
     q.keys = kv_readable(q.len, q.nodes, a.kv.held[q.id], a.kv.page, a.kv.max_pages, &q.bad);
   }
   return q;
+}
+__device__ __forceinline__ TreeSeq tree_seq1(const TreeArgs &a, int s) {     // in scalar registers
+  const TreeSeq q = tree_seq(a, s);
+  return {scalar(q.c0), scalar(q.nodes), scalar(q.len), scalar(q.keys), scalar(q.id), scalar(q.bad) != 0};
 }
 struct TreeItem {
   int s, tile, split, nsplit;   // group (< 0: none), row tile, key chunk and their number
@@ -248,6 +265,10 @@ __device__ __forceinline__ TreeItem tree_find(const TreeArgs &a, int it, bool no
   }
   return {-1, 0, 0, 1, 0, 0};
 }
+__device__ __forceinline__ TreeItem tree_item(const TreeArgs &a, int it, int rt, int unit, int target) {   // in scalar registers
+  const TreeItem x = tree_find(a, it, false, rt, unit, target);
+  return {scalar(x.s), scalar(x.tile), scalar(x.split), scalar(x.nsplit), scalar(x.slot), scalar(x.chunk)};
+}
 // Bit j: whether node i's row sees key u0 + j of the drafted ones (u0 < 0: a
 // cached position, seen), j < 32; n nodes.
 __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int mw, int i, int n, int u0) {
@@ -280,15 +301,18 @@ template <typename T, int D> struct TreeRows {
   const TreeArgs &a;
   const TreeSeq &q;
   int hkv, g, shift;                // shift: log2 of the page size
-  const int *tab;
+  // The sequence's pages, as constant memory: no kernel that reads them writes
+  // them, and with a uniform index the entry is a scalar load.
+  const __attribute__((address_space(4))) int *tab;
   __device__ __forceinline__ TreeRows(const TreeArgs &a, const TreeSeq &q, int hkv)
       : a(a), q(q), hkv(hkv), g(a.nh / a.kv.n_kv_head), shift(__builtin_ctz(a.kv.page)),
-        tab(a.kv.table + (size_t)q.id * a.kv.max_pages) {}
+        tab((const __attribute__((address_space(4))) int *)(a.kv.table + (size_t)q.id * a.kv.max_pages)) {}
   // The page that holds key j (past the last: the last).
   __device__ __forceinline__ int page(int j) const { return tab[min(j, q.keys - 1) >> shift]; }
+  // Key j of that page.
   __device__ __forceinline__ const elem *row(const void *pool, int page, int j, bool *bad) const {
     const int pg = kv_page_ok(page, a.kv.n_pages, bad);
-    return (const elem *)pool + kv_at(a.layer, pg, hkv, min(j, q.keys - 1) & (a.kv.page - 1), a.kv.n_pages, a.kv.n_kv_head, a.kv.page, D);
+    return (const elem *)pool + kv_at(a.layer, pg, hkv, j & (a.kv.page - 1), a.kv.n_pages, a.kv.n_kv_head, a.kv.page, D);
   }
   __device__ __forceinline__ const elem *query(int r) const {
     return (const elem *)a.q + (long long)(q.c0 + r / g) * a.qs + (hkv * g + r % g) * D;
@@ -339,9 +363,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
   __shared__ float2 s_ml[NW][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreeItem item = tree_find(a, blockIdx.x / nkv, false, 32, UNIT, p.target);
+  const TreeItem item = tree_item(a, blockIdx.x / nkv, 32, UNIT, p.target);
   if (item.s < 0) return;
-  const TreeSeq q = tree_seq(a, item.s);
+  const TreeSeq q = tree_seq1(a, item.s);
   if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
   const TreeRows<T, D> rows(a, q, hkv);
   const int base = item.tile * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;
@@ -350,11 +374,13 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
   elem *Kw = Ks + wave * BN * D, *Vw = Vs + wave * BN * D;
   bool bad = false;
   int t0 = begin + wave * BN;
-  AttnWave<T, D, BN> w;
+  AttnWave<T, D, BN, 1> w;
   // 16 rows never straddle a page: two lookups a tile, for the tile after the current one.
   int pg[2];
   auto land = [&](elem *dst, const void *pool, auto isv) __attribute__((always_inline)) {
-    land_rows<D, BN, decltype(isv)::value, 1>(dst, 0, [&](int x) { return rows.row(pool, x < 16 ? pg[0] : pg[1], t0 + x, &bad); });
+    constexpr int half = 16 / (64 / (D / 8));       // loads of 16 rows
+    land_rows<D, BN, decltype(isv)::value, 1>(dst, 0, t0, q.keys - 1, D * 2,
+                                              [&](int i, int j) { return rows.row(pool, pg[i / half], j, &bad); });
   };
   auto pages = [&]() __attribute__((always_inline)) {
     pg[0] = rows.page(t0);
@@ -365,7 +391,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
     land(Kw, a.kv.k, std::false_type{});
     land(Vw, a.kv.v, std::true_type{});
   }
-  w.start(live ? rows.query(r) : nullptr);
+  w.start(0, live ? rows.query(r) : nullptr);
   const float c = a.scale * LOG2E;
   const unsigned long long *mask = live ? rows.mask(r) : nullptr;
   const int node = r / rows.g;
@@ -374,27 +400,27 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
     const int u0 = t0 - q.len;
     t0 += UNIT;
     if (t0 < end) pages();
-    f32x16_t s[1];
-    typename AttnWave<T, D, BN>::vec8 pr[2];
+    f32x16_t s[1][1];
+    typename AttnWave<T, D, BN, 1>::vec8 pr[1][2];
     w.scores(Kw, s);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its rows are read
     if (t0 < end) land(Kw, a.kv.k, std::false_type{});
     if (u0 + BN > 0) {
       const uint32_t see = tree_sees(mask, a.mw, node, q.keys - q.len, u0);
       saw |= see != 0;
-      w.template soft<true>(s, c, [&](int j) { return !((see >> j) & 1); }, pr);
+      w.template soft<true>(s, c, [&](int, int j) { return !((see >> j) & 1); }, pr);
       w.template outputs<true>(Vw, pr);
     } else {
       saw = true;
-      w.template soft<false>(s, c, [](int) { return false; }, pr);
+      w.template soft<false>(s, c, [](int, int) { return false; }, pr);
       w.template outputs<false>(Vw, pr);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (t0 < end) land(Vw, a.kv.v, std::true_type{});
   }
   if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-  const float l = w.sum();
-  if (lane < 32) s_ml[wave][n] = make_float2(w.m, saw && l == 0.f ? NAN : l);
+  const float l = w.sum(0);
+  if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
   const bool whole = item.nsplit == 1;
   const size_t slot = ((size_t)hkv * p.slots + item.slot + item.split) * 32;
   if (__syncthreads_or(w.odd != w.odd)) {        // a hidden value may have leaked: the rows one by one
@@ -407,7 +433,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
   float M = -INFINITY;
 #pragma unroll
   for (int x = 0; x < NW; ++x) M = fmaxf(M, s_ml[x][n].x);
-  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M);
+  const float f = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
   auto area = [&](int x) { return (float *)(x < 2 ? Ks : Vs) + (x & 1) * 32 * D; };
   float *mine = area(wave);
 #pragma unroll
@@ -415,7 +441,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       *(float4 *)(mine + n * D + 4 * ((8 * b + 2 * i + hi) ^ (n & 15))) =
-          make_float4(w.o[b][4 * i] * f, w.o[b][4 * i + 1] * f, w.o[b][4 * i + 2] * f, w.o[b][4 * i + 3] * f);
+          make_float4(w.o[0][b][4 * i] * f, w.o[0][b][4 * i + 1] * f, w.o[0][b][4 * i + 2] * f, w.o[0][b][4 * i + 3] * f);
   __syncthreads();
   for (int x = tid; x < R * PC; x += 256) {
     const int y = x / PC, pc = x - y * PC;
@@ -442,28 +468,23 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
   }
 }
 
-// Many rows: NW waves of 32 rows share double-buffered tiles of BN keys.
-template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * NW, 2) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
+// Many rows: NW waves of 32 QB rows share double-buffered tiles of BN keys.
+template <typename T, int D, int NW, int BN, int QB, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
-  constexpr int RT = 32 * NW, PER = BN * D / 8 / (64 * NW);
+  constexpr int WM = 32 * QB, RT = WM * NW, PER = BN * D / 8 / (64 * NW);
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreeItem item = tree_find(a, blockIdx.x / nkv, false, RT, BN, p.target);
+  const TreeItem item = tree_item(a, blockIdx.x / nkv, RT, BN, p.target);
   if (item.s < 0) return;
-  const TreeSeq q = tree_seq(a, item.s);
+  const TreeSeq q = tree_seq1(a, item.s);
   if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
   const TreeRows<T, D> rows(a, q, hkv);
-  const int base = item.tile * RT + wave * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;   // R <= 0: no rows here
-  const bool live = n < R;
+  const int base = item.tile * RT + wave * WM, R = min(q.nodes * rows.g - base, WM);   // R <= 0: no rows here
   const int begin = item.split * item.chunk, end = min(begin + item.chunk, q.keys);
   bool bad = false;
-  AttnWave<T, D, BN> w;
-  w.start(live ? rows.query(r) : nullptr);
   const float c = a.scale * LOG2E;
-  const unsigned long long *mask = live ? rows.mask(r) : nullptr;
-  const int node = r / rows.g;
-  bool saw = false;
   // The page of each piece that this wave lands (its rows lie in one page), a tile ahead.
   int pg[PER];
   auto pages = [&](int t0) __attribute__((always_inline)) {
@@ -471,10 +492,8 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
     for (int i = 0; i < PER; ++i) pg[i] = rows.page(t0 + (i * NW + wave) * 64 / (D / 8));
   };
   auto land = [&](elem *Kd, elem *Vd, int t0) __attribute__((always_inline)) {
-    int i = 0;
-    land_rows<D, BN, false, NW>(Kd, wave, [&](int x) { return rows.row(a.kv.k, pg[i++], t0 + x, &bad); });
-    i = 0;
-    land_rows<D, BN, true, NW>(Vd, wave, [&](int x) { return rows.row(a.kv.v, pg[i++], t0 + x, &bad); });
+    land_rows<D, BN, false, NW>(Kd, wave, t0, q.keys - 1, D * 2, [&](int i, int j) { return rows.row(a.kv.k, pg[i], j, &bad); });
+    land_rows<D, BN, true, NW>(Vd, wave, t0, q.keys - 1, D * 2, [&](int i, int j) { return rows.row(a.kv.v, pg[i], j, &bad); });
     if (t0 + BN < end) pages(t0 + BN);
     __builtin_amdgcn_sched_barrier(0);              // the addresses' registers are free again before the tile
   };
@@ -482,13 +501,6 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
     asm volatile("" ::: "memory");
-  };
-  auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
-    uint32_t see[BN / 32], any = 0;
-#pragma unroll
-    for (int b = 0; b < BN / 32; ++b) any |= see[b] = tree_sees(mask, a.mw, node, q.keys - q.len, t0 + 32 * b - q.len);
-    saw |= any != 0;
-    w.template tile<true>(Kb, Vb, c, [&](int j) { return !((see[j >> 5] >> (j & 31)) & 1); });
   };
   if (begin < end) {
     pages(begin);
@@ -503,15 +515,32 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
     return;
   }
+  AttnWave<T, D, BN, QB> w;
+#pragma unroll
+  for (int y = 0; y < QB; ++y) w.start(y, 32 * y + n < R ? rows.query(base + 32 * y + n) : nullptr);
   const int full = begin + max(min(end, q.len) - begin, 0) / (2 * BN) * (2 * BN);   // whole tiles of cached positions
-  saw = full > begin;
+  uint32_t saw[QB];
+#pragma unroll
+  for (int y = 0; y < QB; ++y) saw[y] = full > begin;
+  auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
+    uint32_t see[QB][BN / 32];
+#pragma unroll
+    for (int y = 0; y < QB; ++y) {
+      const int r = base + 32 * y + n;
+      const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b)
+        saw[y] |= see[y][b] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, t0 + 32 * b - q.len);
+    }
+    w.template tile<true>(Kb, Vb, c, [&](int y, int j) { return !((see[y][j >> 5] >> (j & 31)) & 1); });
+  };
   for (; t0 < full; t0 += 2 * BN) {
     ready();
     land(K1, V1, t0 + BN);
-    w.template tile<false>(K0, V0, c, [](int) { return false; });
+    w.template tile<false>(K0, V0, c, [](int, int) { return false; });
     ready();
     if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
-    w.template tile<false>(K1, V1, c, [](int) { return false; });
+    w.template tile<false>(K1, V1, c, [](int, int) { return false; });
   }
   for (; t0 < end; t0 += 2 * BN) {
     ready();
@@ -523,30 +552,35 @@ template <typename T, int D, int NW, int BN> __global__ __launch_bounds__(64 * N
     part(K1, V1, t0 + BN);
   }
   if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-  const float l = w.sum();
   const bool whole = item.nsplit == 1;
-  const size_t slot = ((size_t)hkv * p.slots + item.slot + item.split) * RT + wave * 32;
+  const size_t slot = ((size_t)hkv * p.slots + item.slot + item.split) * RT + wave * WM;
   if (__any(w.odd != w.odd)) {
     for (int x = 0; x < R; ++x)
       rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
-  } else if (live) {
-    const float ls = saw && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+    return;
+  }
+#pragma unroll
+  for (int y = 0; y < QB; ++y) {
+    const int x = 32 * y + n;
+    const float l = w.sum(y), ls = saw[y] && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+    if (x >= R) continue;
 #pragma unroll
     for (int b = 0; b < D / 32; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 v = make_float4(w.o[b][4 * i] * inv, w.o[b][4 * i + 1] * inv, w.o[b][4 * i + 2] * inv, w.o[b][4 * i + 3] * inv);
+        const float4 v = make_float4(w.o[y][b][4 * i] * inv, w.o[y][b][4 * i + 1] * inv, w.o[y][b][4 * i + 2] * inv,
+                                     w.o[y][b][4 * i + 3] * inv);
         const int d = 32 * b + 8 * i + 4 * hi;
         if (whole) {
           const typename AttnOps<T>::vec4 e = {(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
-          *(typename AttnOps<T>::vec4 *)(rows.out(r) + d) = e;
+          *(typename AttnOps<T>::vec4 *)(rows.out(base + x) + d) = e;
         } else {
-          *(float4 *)(p.po + (slot + n) * D + d) = v;
+          *(float4 *)(p.po + (slot + x) * D + d) = v;
         }
       }
     if (lane < 32) {
-      if (!whole) p.ml[slot + n] = make_float2(w.m, ls);
-      else if (a.lse) *rows.lse(r) = LN2 * (w.m + __builtin_amdgcn_logf(l));
+      if (!whole) p.ml[slot + x] = make_float2(w.m[y], ls);
+      else if (a.lse) *rows.lse(base + x) = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
     }
   }
 }
@@ -612,13 +646,15 @@ template <typename F> int by_type(int type, int D, F f) {
 }  // namespace
 
 int attn_prompt_launch(const cwen_ctx *, int type, int D, const PromptArgs &a, hipStream_t st) {
-  constexpr int NW = 8;
-  const long long items = (a.total_q + 32 * NW - 1) / (32 * NW) + a.n_seq;
+  const int BM = D == 256 ? 128 : 256;
+  const long long items = (a.total_q + BM - 1) / BM + a.n_seq;
   if (items * a.nh > INT32_MAX) return CWEN_EINVAL;
   return by_type(type, D, [&](auto t, auto d) {
+    typedef decltype(t) T;
     constexpr int dim = decltype(d)::value;
-    hipLaunchKernelGGL((prompt_kernel<decltype(t), dim, NW, dim == 256 ? 32 : 64>), dim3((unsigned)(items * a.nh)),
-                       dim3(64 * NW), 0, st, a);
+    const dim3 grid((unsigned)(items * a.nh));
+    if constexpr (dim == 256) hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, 1, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prompt_kernel<T, dim, 8, 64, 1, 2>), grid, dim3(512), 0, st, a);
   });
 }
 int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
@@ -643,7 +679,8 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value, BN = dim == 256 ? 32 : 64;
     if (form == 1) hipLaunchKernelGGL((tree_few_kernel<T, dim>), grid, dim3(256), 0, st, a, p);
-    else hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN>), grid, dim3(256), 0, st, a, p);
+    else if constexpr (dim == 256) hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
   });
   if (rc || !p.target) return rc;
   return by_type(a.kv.type, D, [&](auto t, auto d) {

@@ -239,7 +239,7 @@ int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, con
   const long long qr = (long long)n_head * head_dim, kr = (long long)n_kv_head * head_dim;
   if (!ok_rows(q, q_ts, qr) || !ok_rows(o, o_ts, qr) || !cu_q || !aligned4(cu_q) || !aligned4(cu_k) || !aligned4(lse))
     return CWEN_EINVAL;
-  if (total_k && (!ok_rows(k, k_ts, kr) || !ok_rows(v, v_ts, kr))) return CWEN_EINVAL;
+  if (total_k && (!ok_rows(k, k_ts, kr) || !ok_rows(v, v_ts, kr) || k_ts >= 1 << 27 || v_ts >= 1 << 27)) return CWEN_EINVAL;
   const long long ob = ((total_q - 1) * o_ts + qr) * 2;
   if (overlap(q, ((total_q - 1) * q_ts + qr) * 2, o, ob)) return CWEN_EINVAL;
   if (total_k && (overlap(k, ((total_k - 1) * k_ts + kr) * 2, o, ob) || overlap(v, ((total_k - 1) * v_ts + kr) * 2, o, ob)))

@@ -355,39 +355,68 @@ KV_FULL, KV_ARG, KV_PAGE = 1, 2, 4
 KV_REQ_MAX, TREE_MAX = 4096, 256
 
 
+_FLOATS: dict = {}          # torch dtype -> CWEN_T_*, filled at the first use
+_DT: dict = {}              # "int32" -> torch.int32
+_raw_stream = None
+
+
+def _torch_tables() -> None:
+    global _raw_stream
+    import torch
+    _FLOATS.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16})
+    _DT.update(int32=torch.int32, int64=torch.int64, float32=torch.float32)
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _raw_stream = fast or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _stream_of(ctx: Context, stream) -> int:
+    """A stream argument; None: the current stream of the context's device."""
+    if stream is None:
+        if _raw_stream is None:
+            _torch_tables()
+        return _raw_stream(ctx.device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
 def _type(t) -> int:
     """CWEN_T_* of a float tensor."""
-    name = str(t.dtype)
-    if name not in ("torch.float32", "torch.float16", "torch.bfloat16"):
-        raise ValueError(f"float32, float16 or bfloat16 expected, got {name}")
-    return {"torch.float32": T_F32, "torch.float16": T_F16, "torch.bfloat16": T_BF16}[name]
+    if not _FLOATS:
+        _torch_tables()
+    typ = _FLOATS.get(t.dtype)
+    if typ is None:
+        raise ValueError(f"float32, float16 or bfloat16 expected, got {t.dtype}")
+    return typ
 
 
 def _heads(name: str, t, shape=None, dtype=None) -> int:
     """Check a [tokens, heads, head_dim] tensor with heads in a row; its token stride."""
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape or '[tokens, heads, head_dim]'}")
+    sh = t.shape
+    if len(sh) != 3 or (shape is not None and sh != shape):
+        raise ValueError(f"{name}: shape {tuple(sh)}, expected {shape or '[tokens, heads, head_dim]'}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name}: {t.dtype}, expected {dtype}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+    row = sh[1] * sh[2]
+    ts, hs, ds = t.stride()
+    if sh[0] * row and (ds != 1 or (sh[1] > 1 and hs != sh[2])):
         raise ValueError(f"{name}: heads of a token must lie in a row")
-    if t.shape[0] <= 1:
-        return t.shape[1] * t.shape[2]
-    return t.stride(0)
+    return ts if sh[0] > 1 else row
 
 
-def _vec(name: str, t, n: int | None, dtype: str = "int32"):
-    """Check a contiguous device vector of n elements (None: any number)."""
-    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or (n is not None and t.numel() != n):
+def _vec(name: str, t, n: int | None, dtype: str = "int32") -> int | None:
+    """Check a contiguous vector of n elements (None: any number); its address."""
+    if not _DT:
+        _torch_tables()
+    if t.dtype != _DT[dtype] or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{name}: contiguous {dtype} of {n if n is not None else 'any number of'} elements expected")
-    return t
+    return t.data_ptr()
 
 
-def _on(ctx: "Context", **tensors) -> None:
+def _on(ctx: Context, *tensors) -> None:
     """Every tensor (None skipped) is on the context's device."""
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
-            raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
+    dev = ctx.device
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the context on cuda:{dev}")
 
 
 class RopeCfg(C.Structure):
@@ -427,11 +456,11 @@ def rope(ctx: Context, r: Rope, x, y, pos, inverse: bool = False, stream=None) -
         raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, head_dim {r.head_dim}")
     if x.numel() and (x.stride(2) != 1 or y.stride(2) != 1):
         raise ValueError("a head's elements must lie in a row")
-    _on(ctx, x=x, y=y, pos=pos)
+    _on(ctx, x, y, pos)
     check("cwen_rope_apply", lib().cwen_rope_apply(
         ctx.h, r.h, _type(x), _ptr(x), x.stride(0) if T > 1 else 0, x.stride(1) if H > 1 else 0, _type(y), _ptr(y),
-        y.stride(0) if T > 1 else 0, y.stride(1) if H > 1 else 0, _ptr(_vec("pos", pos, T)), T, H, int(inverse),
-        _stream(stream)))
+        y.stride(0) if T > 1 else 0, y.stride(1) if H > 1 else 0, _vec("pos", pos, T), T, H, int(inverse),
+        _stream_of(ctx, stream)))
 
 
 class KvCache(C.Structure):
@@ -471,24 +500,24 @@ class PagedKV:
         return cls(page, pool(), pool(), ints(-1, max_seqs, max_pages), ints(0, max_seqs), ints(0, max_seqs), ints(0, n_pages))
 
     def reset(self, ctx: Context, stream=None) -> None:
-        _on(ctx, cache=self.k)
-        check("cwen_kv_reset", lib().cwen_kv_reset(ctx.h, self.ref_c, _stream(stream)))
+        _on(ctx, self.k)
+        check("cwen_kv_reset", lib().cwen_kv_reset(ctx.h, self.ref_c, _stream_of(ctx, stream)))
 
     def reserve(self, ctx: Context, seqs, n, stream=None) -> None:
         """Room for n more positions of each sequence."""
-        _on(ctx, cache=self.k, seqs=seqs, n=n)
-        check("cwen_kv_reserve", lib().cwen_kv_reserve(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
-                                                       _ptr(_vec("n", n, seqs.numel())), seqs.numel(), _stream(stream)))
+        _on(ctx, self.k, seqs, n)
+        check("cwen_kv_reserve", lib().cwen_kv_reserve(ctx.h, self.ref_c, _vec("seqs", seqs, None),
+                                                       _vec("n", n, seqs.numel()), seqs.numel(), _stream_of(ctx, stream)))
 
     def fork(self, ctx: Context, src, dst, stream=None) -> None:
         """dst sequences share the src sequences' pages."""
-        _on(ctx, cache=self.k, src=src, dst=dst)
-        check("cwen_kv_fork", lib().cwen_kv_fork(ctx.h, self.ref_c, _ptr(_vec("src", src, None)),
-                                                 _ptr(_vec("dst", dst, src.numel())), src.numel(), _stream(stream)))
+        _on(ctx, self.k, src, dst)
+        check("cwen_kv_fork", lib().cwen_kv_fork(ctx.h, self.ref_c, _vec("src", src, None),
+                                                 _vec("dst", dst, src.numel()), src.numel(), _stream_of(ctx, stream)))
 
     def keep(self, ctx: Context, seqs, count, path=None, stream=None) -> None:
         """Accept the rows path[i, :count[i]] (None: the first count[i]) behind each sequence."""
-        _on(ctx, cache=self.k, seqs=seqs, count=count, path=path)
+        _on(ctx, self.k, seqs, count, path)
         n, ps = seqs.numel(), 0
         if path is not None:
             if path.dim() != 2 or path.shape[0] != n:
@@ -497,22 +526,22 @@ class PagedKV:
             _vec("path", path, n * ps)
             if ps == 0:                           # nothing can be named: no row moves
                 path = None
-        check("cwen_kv_keep", lib().cwen_kv_keep(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
-                                                 _ptr(_vec("count", count, n)), _ptr(path), ps, n, _stream(stream)))
+        check("cwen_kv_keep", lib().cwen_kv_keep(ctx.h, self.ref_c, _vec("seqs", seqs, None),
+                                                 _vec("count", count, n), _ptr(path), ps, n, _stream_of(ctx, stream)))
 
     def truncate(self, ctx: Context, seqs, length=None, stream=None) -> None:
         """Cut the sequences to `length` (None: 0) positions."""
-        _on(ctx, cache=self.k, seqs=seqs, length=length)
+        _on(ctx, self.k, seqs, length)
         n = seqs.numel()
-        check("cwen_kv_truncate", lib().cwen_kv_truncate(ctx.h, self.ref_c, _ptr(_vec("seqs", seqs, None)),
-                                                         None if length is None else _ptr(_vec("length", length, n)), n,
-                                                         _stream(stream)))
+        check("cwen_kv_truncate", lib().cwen_kv_truncate(ctx.h, self.ref_c, _vec("seqs", seqs, None),
+                                                         None if length is None else _vec("length", length, n), n,
+                                                         _stream_of(ctx, stream)))
 
     def take_status(self, ctx: Context, stream=None) -> int:
         """The KV_* bits raised since the last call, cleared.  Synchronous."""
-        _on(ctx, cache=self.k)
+        _on(ctx, self.k)
         bits = C.c_int()
-        check("cwen_kv_status", lib().cwen_kv_status(ctx.h, self.ref_c, C.byref(bits), _stream(stream)))
+        check("cwen_kv_status", lib().cwen_kv_status(ctx.h, self.ref_c, C.byref(bits), _stream_of(ctx, stream)))
         return bits.value
 
 
@@ -521,19 +550,19 @@ def rope_kv(ctx: Context, r: Rope, q, k, v, qo, kv: PagedKV, layer: int, seq, sl
     T, H, D = q.shape
     if D != kv.head_dim or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype}, k {k.dtype}, v {v.dtype}: the cache's head_dim is {kv.head_dim}")
-    _on(ctx, q=q, k=k, v=v, qo=qo, cache=kv.k, seq=seq, slot=slot, pos=pos)
+    _on(ctx, q, k, v, qo, kv.k, seq, slot, pos)
     qs, qos = _heads("q", q), _heads("qo", qo, (T, H, D), kv.k.dtype)
     ks, vs = _heads("k", k, (T, kv.heads, D)), _heads("v", v, (T, kv.heads, D))
     check("cwen_rope_kv", lib().cwen_rope_kv(
-        ctx.h, r.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(qo), qos, kv.ref_c, layer, _ptr(_vec("seq", seq, T)),
-        _ptr(_vec("slot", slot, T)), _ptr(_vec("pos", pos, T)), T, H, _stream(stream)))
+        ctx.h, r.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(qo), qos, kv.ref_c, layer, _vec("seq", seq, T),
+        _vec("slot", slot, T), _vec("pos", pos, T), T, H, _stream_of(ctx, stream)))
 
 
 def attn_prompt(ctx: Context, q, k, v, o, cu_q, cu_k=None, lse=None, scale: float | None = None, stream=None) -> None:
     """Causal attention over packed sequences (cwen_attn_prompt); q, o [tokens, heads,
     head_dim], k, v [tokens, KV heads, head_dim], cu_* the sequences' borders."""
     (T, H, D), (Tk, Hk, _) = q.shape, k.shape
-    _on(ctx, q=q, k=k, v=v, o=o, cu_q=cu_q, cu_k=cu_k, lse=lse)
+    _on(ctx, q, k, v, o, cu_q, cu_k, lse)
     qs, os_ = _heads("q", q), _heads("o", o, (T, H, D), q.dtype)
     ks, vs = _heads("k", k, (Tk, Hk, D), q.dtype), _heads("v", v, (Tk, Hk, D), q.dtype)
     n = cu_q.numel() - 1
@@ -544,8 +573,8 @@ def attn_prompt(ctx: Context, q, k, v, o, cu_q, cu_k=None, lse=None, scale: floa
     if cu_k is not None:
         _vec("cu_k", cu_k, n + 1)
     check("cwen_attn_prompt", lib().cwen_attn_prompt(
-        ctx.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(o), os_, _ptr(lse), _ptr(_vec("cu_q", cu_q, None)),
-        _ptr(cu_k), n, T, Tk, H, Hk, D, D ** -0.5 if scale is None else scale, _stream(stream)))
+        ctx.h, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(o), os_, _ptr(lse), _vec("cu_q", cu_q, None),
+        _ptr(cu_k), n, T, Tk, H, Hk, D, D ** -0.5 if scale is None else scale, _stream_of(ctx, stream)))
 
 
 def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: int, max_len: int, mask=None, lse=None,
@@ -555,7 +584,7 @@ def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: 
     T, H, D = q.shape
     if D != kv.head_dim:
         raise ValueError(f"q {tuple(q.shape)}: the cache's head_dim is {kv.head_dim}")
-    _on(ctx, q=q, o=o, cache=kv.k, seqs=seqs, cu=cu, mask=mask, lse=lse)
+    _on(ctx, q, o, kv.k, seqs, cu, mask, lse)
     qs, os_ = _heads("q", q, None, kv.k.dtype), _heads("o", o, (T, H, D), kv.k.dtype)
     n, mw = seqs.numel(), 0
     if mask is not None:
@@ -566,8 +595,8 @@ def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: 
     if lse is not None:
         _vec("lse", lse, T * H, "float32")
     check("cwen_attn_tree", lib().cwen_attn_tree(
-        ctx.h, kv.ref_c, layer, _ptr(q), qs, _ptr(o), os_, _ptr(lse), _ptr(_vec("seqs", seqs, None)), _ptr(_vec("cu", cu, n + 1)),
-        _ptr(mask), mw, n, T, max_nodes, max_len, H, D ** -0.5 if scale is None else scale, _stream(stream)))
+        ctx.h, kv.ref_c, layer, _ptr(q), qs, _ptr(o), os_, _ptr(lse), _vec("seqs", seqs, None), _vec("cu", cu, n + 1),
+        _ptr(mask), mw, n, T, max_nodes, max_len, H, D ** -0.5 if scale is None else scale, _stream_of(ctx, stream)))
 
 
 # ---------------------------------------------------------------- model

@@ -112,7 +112,8 @@ def test_attention_refusals():
     for bad in (dict(ctx=None), dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(cu=None), dict(q=P + 2), dict(qs=504),
                 dict(ks=128), dict(vs=260), dict(os=256), dict(nh=3), dict(nkv=0), dict(D=96), dict(D=512), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(n=-1), dict(tq=-1), dict(tk=1 << 30),
-                dict(cuk=None, tk=3), dict(o=P), dict(o=P + 8192), dict(o=P + 16384), dict(cu=P + 2), dict(lse=P + 1), dict(n=65537)):
+                dict(cuk=None, tk=3), dict(o=P), dict(o=P + 8192), dict(o=P + 16384), dict(cu=P + 2), dict(lse=P + 1), dict(n=65537),
+                dict(ks=1 << 27), dict(vs=1 << 27)):
         assert prompt(**bad) == EINVAL, bad
 
     def tree(c=None, layer=0, q=P, qs=512, o=P + 8192, os=512, seqs=P, cu=P, mask=P, mw=1, n=1, total=2, mn=2, ml=5, nh=4, scale=1.0):
