@@ -1,6 +1,7 @@
 // Attention of packed prompts and of drafted trees over the paged cache.
 #include <math.h>
 #include <algorithm>
+#include <stdlib.h>
 #include "cwen_internal.h"
 #include "kv_table.h"
 #include "attn_core.h"
@@ -123,7 +124,7 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
     land_rows<D, BN, true, NW>(Vd, wave, t0, nk - 1, (uint32_t)a.vs * 2, [&](int, int j) { return vp + j * a.vs; });
   };
   auto ready = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_loads<0>();
     lds_barrier();
     asm volatile("" ::: "memory");
   };
@@ -186,11 +187,12 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
 // that share the kv head's keys lie side by side, so a group's n nodes are n g
 // rows against one stream of pages.  Few rows leave the work bound by that
 // stream, many by the matrix cores, and both want it cut along the keys, since
-// groups are few: row tiles of RT rows are cut into chunks of whole tiles of
-// keys, as many that about `target` items per kv head arise over all groups
-// (so that a long sequence among short ones does not set the time).  Nothing of
-// this is known on the host: every workgroup finds its item from the lengths on the
-// device, 64 groups at a time.
+// groups are few.  All row tiles (RT rows) of all groups are laid end to end, each
+// as long as its keys (in units of a tile of keys), and the line is cut into `lines`
+// equal pieces, one workgroup each: no long sequence sets the time, and a piece that
+// begins or ends inside a row tile leaves a partial result, at most two a
+// workgroup.  Nothing of this is known on the host: every workgroup finds
+// its pieces from the lengths on the device, 64 groups at a time.
 struct TreeSeq {
   int c0, nodes, len, keys, id;     // first node, nodes, cached positions, keys in all, sequence (0 when invalid)
   bool bad;
@@ -212,63 +214,67 @@ __device__ __forceinline__ TreeSeq tree_seq1(const TreeArgs &a, int s) {     // 
   const TreeSeq q = tree_seq(a, s);
   return {scalar(q.c0), scalar(q.nodes), scalar(q.len), scalar(q.keys), scalar(q.id), scalar(q.bad) != 0};
 }
-struct TreeItem {
-  int s, tile, split, nsplit;   // group (< 0: none), row tile, key chunk and their number
-  int slot;                     // the row tile's first partial
-  int chunk;                    // keys of a chunk
+struct TreeTile {
+  int s, tile;              // group (< 0: none) and row tile of it
+  int units;                // its length
+  long long at;             // where it begins on the line
 };
-// The item `it`, or with `node` the group whose nodes hold token `it` (tile and split 0).
-__device__ __forceinline__ TreeItem tree_find(const TreeArgs &a, int it, bool node, int rt, int unit, int target) {
-  const int lane = threadIdx.x & 63, g = a.nh / a.kv.n_kv_head;
-  auto at = [&](int s, int *tiles, int *units, TreeSeq *q) {
+__device__ __forceinline__ long long scan64(long long v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long long u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ long long lane64(long long v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), l);
+  return (long long)((unsigned long long)hi << 32 | lo);
+}
+struct TreePlan {
+  int rt, unit, lines;
+  long long total;          // the line's length
+  __device__ __forceinline__ void of(const TreeArgs &a, int s, TreeSeq *q, int *tiles, int *units) const {
+    *q = {};
     *tiles = *units = 0;
     if (s >= a.n_seq) return;
     *q = tree_seq(a, s);
-    *tiles = (q->nodes * g + rt - 1) / rt;
-    *units = (q->keys + unit - 1) / unit;
-  };
-  auto scan = [&](int v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int u = __shfl_up(v, d);
-      if (lane >= d) v += u;
-    }
-    return v;
-  };
-  TreeSeq q = {};
-  int tiles, units;
-  long long work = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-    at(s0 + lane, &tiles, &units, &q);
-    long long v = (long long)tiles * units;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    work += v;
+    *tiles = (q->nodes * (a.nh / a.kv.n_kv_head) + rt - 1) / rt;
+    *units = max((q->keys + unit - 1) / unit, 1);          // rows without keys are work too
   }
-  // units of a chunk; target 0: every row tile one chunk
-  const int per = (int)min(target ? max((work + target - 1) / target, 1ll) : 1ll << 30, (1ll << 30) / unit);
-  int slot = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-    if (a.n_seq > 64) at(s0 + lane, &tiles, &units, &q);     // with up to 64 groups the values are still there
-    const int ns = max((units + per - 1) / per, 1), items = tiles * ns, parts = ns > 1 ? items : 0;
-    const int inc = scan(items), pinc = scan(parts);
-    const bool mine = node ? s0 + lane < a.n_seq && it >= q.c0 && it < q.c0 + q.nodes : inc > it;
-    const unsigned long long hit = __ballot(mine);
-    if (hit) {
-      const int w = __builtin_ctzll(hit);
-      const int nsplit = __builtin_amdgcn_readlane(ns, w), r = node ? 0 : it - __builtin_amdgcn_readlane(inc - items, w);
-      const int tile = r / nsplit;
-      return {s0 + w, tile, r - tile * nsplit, nsplit, slot + __builtin_amdgcn_readlane(pinc - parts, w) + tile * nsplit, per * unit};
+  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rt, int unit, int most) : rt(rt), unit(unit), total(0) {
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+      TreeSeq q;
+      int tiles, units;
+      of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
+      total += lane64(scan64((long long)tiles * units), 63);
     }
-    if (!node) it -= __builtin_amdgcn_readlane(inc, 63);
-    slot += __builtin_amdgcn_readlane(pinc, 63);
+    lines = scalar((int)min((long long)most, total));
   }
-  return {-1, 0, 0, 1, 0, 0};
-}
-__device__ __forceinline__ TreeItem tree_item(const TreeArgs &a, int it, int rt, int unit, int target) {   // in scalar registers
-  const TreeItem x = tree_find(a, it, false, rt, unit, target);
-  return {scalar(x.s), scalar(x.tile), scalar(x.split), scalar(x.nsplit), scalar(x.slot), scalar(x.chunk)};
-}
+  // Where piece w begins, and the piece that holds position u.
+  __device__ __forceinline__ long long begin(int w) const { return total * w / lines; }
+  __device__ __forceinline__ int piece(long long u) const { return (int)(((u + 1) * lines - 1) / total); }
+  // The row tile at position u; or, with node >= 0, the group's first that holds it.
+  __device__ __forceinline__ TreeTile find(const TreeArgs &a, long long u, int node) const {
+    long long at = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+      TreeSeq q;
+      int tiles, units;
+      of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
+      const long long mine = (long long)tiles * units, inc = at + scan64(mine);
+      const unsigned long long hit = __ballot(node >= 0 ? node >= q.c0 && node < q.c0 + q.nodes : inc > u);
+      if (hit) {
+        const int w = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(units, w);
+        const long long first = lane64(inc - mine, w);
+        const int tile = node >= 0 ? 0 : (int)((u - first) / n);
+        return {scalar(s0 + w), scalar(tile), scalar(n), lane64(first + (long long)tile * n, 0)};
+      }
+      at = lane64(inc, 63);
+    }
+    return {-1, 0, 0, 0};
+  }
+};
 // Bit j: whether node i's row sees key u0 + j of the drafted ones (u0 < 0: a
 // cached position, seen), j < 32; n nodes.
 __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int mw, int i, int n, int u0) {
@@ -289,10 +295,9 @@ __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int
 }
 
 struct TreeLaunch {
-  int target;                   // items per kv head
-  float *po;                    // partial outputs [kv head][slot][row][D]
-  float2 *ml;                   // and their maxima and sums [kv head][slot][row]
-  int slots;
+  int lines;                    // pieces of a kv head's line
+  float *po;                    // partial outputs [kv head][2 lines][row][D]: piece w's first row tile, its last
+  float2 *ml;                   // and their maxima and sums [kv head][2 lines][row]
 };
 
 // One group's rows against the pages: what both forms share.
@@ -300,19 +305,26 @@ template <typename T, int D> struct TreeRows {
   typedef typename T::elem elem;
   const TreeArgs &a;
   const TreeSeq &q;
-  int hkv, g, shift;                // shift: log2 of the page size
+  int hkv, g;
+  const elem *kb, *vb;              // the layer's rows of the kv head in page 0
+  int64_t step;                     // elements from page to page
+  int shift, last, n_pages;         // log2 of the page size, the last key
   // The sequence's pages, as constant memory: no kernel that reads them writes
   // them, and with a uniform index the entry is a scalar load.
   const __attribute__((address_space(4))) int *tab;
   __device__ __forceinline__ TreeRows(const TreeArgs &a, const TreeSeq &q, int hkv)
-      : a(a), q(q), hkv(hkv), g(a.nh / a.kv.n_kv_head), shift(__builtin_ctz(a.kv.page)),
-        tab((const __attribute__((address_space(4))) int *)(a.kv.table + (size_t)q.id * a.kv.max_pages)) {}
+      : a(a), q(q), hkv(hkv), g(a.nh / a.kv.n_kv_head), step((int64_t)a.kv.n_kv_head * a.kv.page * D),
+        shift(__builtin_ctz(a.kv.page)), last(q.keys - 1), n_pages(a.kv.n_pages),
+        tab((const __attribute__((address_space(4))) int *)(a.kv.table + (size_t)q.id * a.kv.max_pages)) {
+    const int64_t first = kv_at(a.layer, 0, hkv, 0, a.kv.n_pages, a.kv.n_kv_head, a.kv.page, D);
+    kb = (const elem *)a.kv.k + first;
+    vb = (const elem *)a.kv.v + first;
+  }
   // The page that holds key j (past the last: the last).
-  __device__ __forceinline__ int page(int j) const { return tab[min(j, q.keys - 1) >> shift]; }
+  __device__ __forceinline__ int page(int j) const { return tab[min(j, last) >> shift]; }
   // Key j of that page.
-  __device__ __forceinline__ const elem *row(const void *pool, int page, int j, bool *bad) const {
-    const int pg = kv_page_ok(page, a.kv.n_pages, bad);
-    return (const elem *)pool + kv_at(a.layer, pg, hkv, j & (a.kv.page - 1), a.kv.n_pages, a.kv.n_kv_head, a.kv.page, D);
+  __device__ __forceinline__ const elem *row(const elem *pool, int page, int j, bool *bad) const {
+    return pool + kv_page_ok(page, n_pages, bad) * step + (j & ((1 << shift) - 1)) * D;
   }
   __device__ __forceinline__ const elem *query(int r) const {
     return (const elem *)a.q + (long long)(q.c0 + r / g) * a.qs + (hkv * g + r % g) * D;
@@ -338,8 +350,8 @@ template <typename T, int D> struct TreeRows {
           },
           [&](int j, const elem **k, const elem **v) {
             bool bad = false;
-            *k = row(a.kv.k, page(j), j, &bad);
-            *v = row(a.kv.v, page(j), j, &bad);
+            *k = row(kb, page(j), j, &bad);
+            *v = row(vb, page(j), j, &bad);
           });
     if (!po) {
       x.store(out(r), lse(r));
@@ -356,115 +368,128 @@ template <typename T, int D> struct TreeRows {
 // are requested when the scores are done, the next V rows after the outputs, so
 // that half of its LDS and more is always under way.  The waves' sums meet at the
 // end.
-template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_kernel(TreeArgs a, TreeLaunch p) {
+template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void tree_few_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
   constexpr int BN = 32, NW = 4, UNIT = BN * NW, PC = D / 4;      // PC: 16-byte pieces of an f32 row
+  constexpr int LOADS = BN * D / 8 / 64;                          // of one tile of K or V, by one wave
   __shared__ __align__(1024) elem Ks[NW * BN * D], Vs[NW * BN * D];
   __shared__ float2 s_ml[NW][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreeItem item = tree_item(a, blockIdx.x / nkv, 32, UNIT, p.target);
-  if (item.s < 0) return;
-  const TreeSeq q = tree_seq1(a, item.s);
-  if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
-  const TreeRows<T, D> rows(a, q, hkv);
-  const int base = item.tile * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;
-  const bool live = n < R;
-  const int begin = item.split * item.chunk, end = min(begin + item.chunk, q.keys);
-  elem *Kw = Ks + wave * BN * D, *Vw = Vs + wave * BN * D;
-  bool bad = false;
-  int t0 = begin + wave * BN;
-  AttnWave<T, D, BN, 1> w;
-  // 16 rows never straddle a page: two lookups a tile, for the tile after the current one.
-  int pg[2];
-  auto land = [&](elem *dst, const void *pool, auto isv) __attribute__((always_inline)) {
-    constexpr int half = 16 / (64 / (D / 8));       // loads of 16 rows
-    land_rows<D, BN, decltype(isv)::value, 1>(dst, 0, t0, q.keys - 1, D * 2,
-                                              [&](int i, int j) { return rows.row(pool, pg[i / half], j, &bad); });
-  };
-  auto pages = [&]() __attribute__((always_inline)) {
-    pg[0] = rows.page(t0);
-    pg[1] = rows.page(t0 + 16);
-  };
-  if (t0 < end) {
-    pages();
-    land(Kw, a.kv.k, std::false_type{});
-    land(Vw, a.kv.v, std::true_type{});
-  }
-  w.start(0, live ? rows.query(r) : nullptr);
-  const float c = a.scale * LOG2E;
-  const unsigned long long *mask = live ? rows.mask(r) : nullptr;
-  const int node = r / rows.g;
-  bool saw = false;
-  while (t0 < end) {
-    const int u0 = t0 - q.len;
-    t0 += UNIT;
-    if (t0 < end) pages();
-    f32x16_t s[1][1];
-    typename AttnWave<T, D, BN, 1>::vec8 pr[1][2];
-    w.scores(Kw, s);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its rows are read
-    if (t0 < end) land(Kw, a.kv.k, std::false_type{});
-    if (u0 + BN > 0) {
-      const uint32_t see = tree_sees(mask, a.mw, node, q.keys - q.len, u0);
-      saw |= see != 0;
-      w.template soft<true>(s, c, [&](int, int j) { return !((see >> j) & 1); }, pr);
-      w.template outputs<true>(Vw, pr);
-    } else {
-      saw = true;
-      w.template soft<false>(s, c, [](int, int) { return false; }, pr);
-      w.template outputs<false>(Vw, pr);
+  const TreePlan plan(a, 32, UNIT, p.lines);
+  const int piece = blockIdx.x / nkv;
+  if (piece >= plan.lines) return;
+  const long long stop = lane64(plan.begin(piece + 1), 0);
+  bool first = true;
+  for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
+    const TreeTile item = plan.find(a, u, -1);
+    const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
+    u += count;
+    const TreeSeq q = tree_seq1(a, item.s);
+    if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
+    const TreeRows<T, D> rows(a, q, hkv);
+    const int base = item.tile * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;
+    const bool live = n < R;
+    const int begin = skip * UNIT, end = min(begin + count * UNIT, q.keys);
+    elem *Kw = Ks + wave * BN * D, *Vw = Vs + wave * BN * D;
+    bool bad = false;
+    int t0 = begin + wave * BN;
+    AttnWave<T, D, BN, 1> w;
+    // 16 rows never straddle a page: two lookups a tile, for the tile after the current one.
+    int pg[2];
+    auto land = [&](elem *dst, const elem *pool, auto isv) __attribute__((always_inline)) {
+      constexpr int half = 16 / (64 / (D / 8));       // loads of 16 rows
+      land_rows<D, BN, decltype(isv)::value, 1>(dst, 0, t0, rows.last, D * 2,
+                                                [&](int i, int j) { return rows.row(pool, pg[i / half], j, &bad); });
+    };
+    auto pages = [&]() __attribute__((always_inline)) {
+      pg[0] = rows.page(t0);
+      pg[1] = rows.page(t0 + 16);
+    };
+    if (t0 < end) {
+      pages();
+      land(Kw, rows.kb, std::false_type{});
+      land(Vw, rows.vb, std::true_type{});
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t0 < end) land(Vw, a.kv.v, std::true_type{});
-  }
-  if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-  const float l = w.sum(0);
-  if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
-  const bool whole = item.nsplit == 1;
-  const size_t slot = ((size_t)hkv * p.slots + item.slot + item.split) * 32;
-  if (__syncthreads_or(w.odd != w.odd)) {        // a hidden value may have leaked: the rows one by one
-    for (int x = wave; x < R; x += NW)
-      rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
-    return;
-  }
-  // Each wave's outputs against the row's common maximum, through LDS (rows of D
-  // floats, their pieces permuted by the row), then summed in the waves' order.
-  float M = -INFINITY;
-#pragma unroll
-  for (int x = 0; x < NW; ++x) M = fmaxf(M, s_ml[x][n].x);
-  const float f = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
-  auto area = [&](int x) { return (float *)(x < 2 ? Ks : Vs) + (x & 1) * 32 * D; };
-  float *mine = area(wave);
-#pragma unroll
-  for (int b = 0; b < D / 32; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *(float4 *)(mine + n * D + 4 * ((8 * b + 2 * i + hi) ^ (n & 15))) =
-          make_float4(w.o[0][b][4 * i] * f, w.o[0][b][4 * i + 1] * f, w.o[0][b][4 * i + 2] * f, w.o[0][b][4 * i + 3] * f);
-  __syncthreads();
-  for (int x = tid; x < R * PC; x += 256) {
-    const int y = x / PC, pc = x - y * PC;
-    float Mr = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int u = 0; u < NW; ++u) Mr = fmaxf(Mr, s_ml[u][y].x);
-#pragma unroll
-    for (int u = 0; u < NW; ++u) L += s_ml[u][y].x == -INFINITY ? s_ml[u][y].y : s_ml[u][y].y * __builtin_amdgcn_exp2f(s_ml[u][y].x - Mr);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < NW; ++u) {
-      const float4 v = *(const float4 *)(area(u) + y * D + 4 * (pc ^ (y & 15)));
-      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+    w.start(0, live ? rows.query(r) : nullptr);
+    const float c = a.scale * LOG2E;
+    const unsigned long long *mask = live ? rows.mask(r) : nullptr;
+    const int node = r / rows.g;
+    uint32_t saw = 0;
+    auto step = [&](auto hide) __attribute__((always_inline)) {
+      constexpr bool H = decltype(hide)::value;
+      const int u0 = t0 - q.len;
+      t0 += UNIT;
+      if (t0 < end) pages();
+      f32x16_t s[1][1];
+      typename AttnWave<T, D, BN, 1>::vec8 pr[1][2];
+      // Loads land in the order of their requests: K's are there when no more
+      // than V's are still under way, V's when no more than the next K's.
+      wait_loads<LOADS>();
+      w.scores(Kw, s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its rows are read
+      if (t0 < end) land(Kw, rows.kb, std::false_type{});
+      const uint32_t see = H ? tree_sees(mask, a.mw, node, q.keys - q.len, u0) : ~0u;
+      saw |= see;
+      w.template soft<H>(s, c, [&](int, int j) { return !((see >> j) & 1); }, pr);
+      if (t0 < end) wait_loads<LOADS>();
+      else wait_loads<0>();
+      w.template outputs<H>(Vw, pr);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (t0 < end) land(Vw, rows.vb, std::true_type{});
+    };
+    while (t0 < min(end, q.len - BN + 1)) step(std::false_type{});  // tiles of cached positions
+    while (t0 < end) step(std::true_type{});
+    if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
+    const float l = w.sum(0);
+    if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
+    const bool whole = count == item.units;
+    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * piece + !first) * 32;
+    if (__syncthreads_or(w.odd != w.odd)) {        // a hidden value may have leaked: the rows one by one
+      for (int x = wave; x < R; x += NW)
+        rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
+      __syncthreads();
+      continue;
     }
-    if (whole) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
-      *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
-      if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (Mr + __builtin_amdgcn_logf(L));
-    } else {
-      *(float4 *)(p.po + (slot + y) * D + 4 * pc) = o;
-      if (pc == 0) p.ml[slot + y] = make_float2(Mr, L);
+    // Each wave's outputs against the row's common maximum, through LDS (rows of D
+    // floats, their pieces permuted by the row), then summed in the waves' order.
+    float M = -INFINITY;
+  #pragma unroll
+    for (int x = 0; x < NW; ++x) M = fmaxf(M, s_ml[x][n].x);
+    const float f = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
+    auto area = [&](int x) { return (float *)(x < 2 ? Ks : Vs) + (x & 1) * 32 * D; };
+    float *mine = area(wave);
+  #pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+  #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(float4 *)(mine + n * D + 4 * ((8 * b + 2 * i + hi) ^ (n & 15))) =
+            make_float4(w.o[0][b][4 * i] * f, w.o[0][b][4 * i + 1] * f, w.o[0][b][4 * i + 2] * f, w.o[0][b][4 * i + 3] * f);
+    __syncthreads();
+    for (int x = tid; x < R * PC; x += 256) {
+      const int y = x / PC, pc = x - y * PC;
+      float Mr = -INFINITY, L = 0.f;
+  #pragma unroll
+      for (int u = 0; u < NW; ++u) Mr = fmaxf(Mr, s_ml[u][y].x);
+  #pragma unroll
+      for (int u = 0; u < NW; ++u) L += s_ml[u][y].x == -INFINITY ? s_ml[u][y].y : s_ml[u][y].y * __builtin_amdgcn_exp2f(s_ml[u][y].x - Mr);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  #pragma unroll
+      for (int u = 0; u < NW; ++u) {
+        const float4 v = *(const float4 *)(area(u) + y * D + 4 * (pc ^ (y & 15)));
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+      }
+      if (whole) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
+        *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
+        if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (Mr + __builtin_amdgcn_logf(L));
+      } else {
+        *(float4 *)(p.po + (slot + y) * D + 4 * pc) = o;
+        if (pc == 0) p.ml[slot + y] = make_float2(Mr, L);
+      }
     }
+    __syncthreads();                               // LDS is free for the next row tile
   }
 }
 
@@ -472,161 +497,188 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void tree_few_
 template <typename T, int D, int NW, int BN, int QB, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
-  constexpr int WM = 32 * QB, RT = WM * NW, PER = BN * D / 8 / (64 * NW);
+  constexpr int WM = 32 * QB, RT = WM * NW, PER = BN * D / 8 / (64 * NW), UNIT = 2 * BN;
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreeItem item = tree_item(a, blockIdx.x / nkv, RT, BN, p.target);
-  if (item.s < 0) return;
-  const TreeSeq q = tree_seq1(a, item.s);
-  if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
-  const TreeRows<T, D> rows(a, q, hkv);
-  const int base = item.tile * RT + wave * WM, R = min(q.nodes * rows.g - base, WM);   // R <= 0: no rows here
-  const int begin = item.split * item.chunk, end = min(begin + item.chunk, q.keys);
-  bool bad = false;
-  const float c = a.scale * LOG2E;
-  // The page of each piece that this wave lands (its rows lie in one page), a tile ahead.
-  int pg[PER];
-  auto pages = [&](int t0) __attribute__((always_inline)) {
+  const TreePlan plan(a, RT, UNIT, p.lines);
+  const int piece = blockIdx.x / nkv;
+  if (piece >= plan.lines) return;
+  const long long stop = lane64(plan.begin(piece + 1), 0);
+  bool first = true;
+  for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
+    const TreeTile item = plan.find(a, u, -1);
+    const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
+    u += count;
+    const TreeSeq q = tree_seq1(a, item.s);
+    if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
+    const TreeRows<T, D> rows(a, q, hkv);
+    const int base = item.tile * RT + wave * WM, R = min(q.nodes * rows.g - base, WM);   // R <= 0: no rows here
+    const int begin = skip * UNIT, end = min(begin + count * UNIT, q.keys);
+    bool bad = false;
+    const float c = a.scale * LOG2E;
+    // The page of each piece that this wave lands (its rows lie in one page), a tile ahead.
+    int pg[PER];
+    auto pages = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) pg[i] = rows.page(t0 + (i * NW + wave) * 64 / (D / 8));
-  };
-  auto land = [&](elem *Kd, elem *Vd, int t0) __attribute__((always_inline)) {
-    land_rows<D, BN, false, NW>(Kd, wave, t0, q.keys - 1, D * 2, [&](int i, int j) { return rows.row(a.kv.k, pg[i], j, &bad); });
-    land_rows<D, BN, true, NW>(Vd, wave, t0, q.keys - 1, D * 2, [&](int i, int j) { return rows.row(a.kv.v, pg[i], j, &bad); });
-    if (t0 + BN < end) pages(t0 + BN);
-    __builtin_amdgcn_sched_barrier(0);              // the addresses' registers are free again before the tile
-  };
-  auto ready = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
-    asm volatile("" ::: "memory");
-  };
-  if (begin < end) {
-    pages(begin);
-    land(K0, V0, begin);
-  }
-  int t0 = begin;
-  if (R <= 0) {                                     // a wave without rows lands its share and does no more
-    for (bool one = true; t0 < end; t0 += BN, one = !one) {
+      for (int i = 0; i < PER; ++i) pg[i] = rows.page(t0 + (i * NW + wave) * 64 / (D / 8));
+    };
+    auto land = [&](elem *Kd, elem *Vd, int t0) __attribute__((always_inline)) {
+      land_rows<D, BN, false, NW>(Kd, wave, t0, rows.last, D * 2, [&](int i, int j) { return rows.row(rows.kb, pg[i], j, &bad); });
+      land_rows<D, BN, true, NW>(Vd, wave, t0, rows.last, D * 2, [&](int i, int j) { return rows.row(rows.vb, pg[i], j, &bad); });
+      if (t0 + BN < end) pages(t0 + BN);
+      __builtin_amdgcn_sched_barrier(0);              // the addresses' registers are free again before the tile
+    };
+    auto ready = [&]() __attribute__((always_inline)) {
+      wait_loads<0>();
+      lds_barrier();
+      asm volatile("" ::: "memory");
+    };
+    if (begin < end) {
+      pages(begin);
+      land(K0, V0, begin);
+    }
+    int t0 = begin;
+    if (R <= 0) {                                     // a wave without rows lands its share and does no more
+      for (bool one = true; t0 < end; t0 += BN, one = !one) {
+        ready();
+        if (t0 + BN < end) land(one ? K1 : K0, one ? V1 : V0, t0 + BN);
+      }
+      if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
+      lds_barrier();
+      continue;
+    }
+    AttnWave<T, D, BN, QB> w;
+#pragma unroll
+    for (int y = 0; y < QB; ++y) w.start(y, 32 * y + n < R ? rows.query(base + 32 * y + n) : nullptr);
+    const int full = begin + max(min(end, q.len) - begin, 0) / (2 * BN) * (2 * BN);   // whole tiles of cached positions
+    uint32_t saw[QB];
+#pragma unroll
+    for (int y = 0; y < QB; ++y) saw[y] = full > begin;
+    auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
+      uint32_t see[QB][BN / 32];
+#pragma unroll
+      for (int y = 0; y < QB; ++y) {
+        const int r = base + 32 * y + n;
+        const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b)
+          saw[y] |= see[y][b] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, t0 + 32 * b - q.len);
+      }
+      w.template tile<true>(Kb, Vb, c, [&](int y, int j) { return !((see[y][j >> 5] >> (j & 31)) & 1); });
+    };
+    for (; t0 < full; t0 += 2 * BN) {
       ready();
-      if (t0 + BN < end) land(one ? K1 : K0, one ? V1 : V0, t0 + BN);
+      land(K1, V1, t0 + BN);
+      w.template tile<false>(K0, V0, c, [](int, int) { return false; });
+      ready();
+      if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
+      w.template tile<false>(K1, V1, c, [](int, int) { return false; });
+    }
+    for (; t0 < end; t0 += 2 * BN) {
+      ready();
+      if (t0 + BN < end) land(K1, V1, t0 + BN);
+      part(K0, V0, t0);
+      if (t0 + BN >= end) break;
+      ready();
+      if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
+      part(K1, V1, t0 + BN);
     }
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-    return;
-  }
-  AttnWave<T, D, BN, QB> w;
-#pragma unroll
-  for (int y = 0; y < QB; ++y) w.start(y, 32 * y + n < R ? rows.query(base + 32 * y + n) : nullptr);
-  const int full = begin + max(min(end, q.len) - begin, 0) / (2 * BN) * (2 * BN);   // whole tiles of cached positions
-  uint32_t saw[QB];
-#pragma unroll
-  for (int y = 0; y < QB; ++y) saw[y] = full > begin;
-  auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
-    uint32_t see[QB][BN / 32];
+    const bool whole = count == item.units;
+    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * piece + !first) * RT + wave * WM;
+    if (__any(w.odd != w.odd)) {
+      for (int x = 0; x < R; ++x)
+        rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
+      lds_barrier();
+      continue;
+    }
 #pragma unroll
     for (int y = 0; y < QB; ++y) {
-      const int r = base + 32 * y + n;
-      const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
+      const int x = 32 * y + n;
+      const float l = w.sum(y), ls = saw[y] && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+      if (x >= R) continue;
 #pragma unroll
-      for (int b = 0; b < BN / 32; ++b)
-        saw[y] |= see[y][b] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, t0 + 32 * b - q.len);
-    }
-    w.template tile<true>(Kb, Vb, c, [&](int y, int j) { return !((see[y][j >> 5] >> (j & 31)) & 1); });
-  };
-  for (; t0 < full; t0 += 2 * BN) {
-    ready();
-    land(K1, V1, t0 + BN);
-    w.template tile<false>(K0, V0, c, [](int, int) { return false; });
-    ready();
-    if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
-    w.template tile<false>(K1, V1, c, [](int, int) { return false; });
-  }
-  for (; t0 < end; t0 += 2 * BN) {
-    ready();
-    if (t0 + BN < end) land(K1, V1, t0 + BN);
-    part(K0, V0, t0);
-    if (t0 + BN >= end) break;
-    ready();
-    if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
-    part(K1, V1, t0 + BN);
-  }
-  if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-  const bool whole = item.nsplit == 1;
-  const size_t slot = ((size_t)hkv * p.slots + item.slot + item.split) * RT + wave * WM;
-  if (__any(w.odd != w.odd)) {
-    for (int x = 0; x < R; ++x)
-      rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
-    return;
-  }
+      for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-  for (int y = 0; y < QB; ++y) {
-    const int x = 32 * y + n;
-    const float l = w.sum(y), ls = saw[y] && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
-    if (x >= R) continue;
-#pragma unroll
-    for (int b = 0; b < D / 32; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 v = make_float4(w.o[y][b][4 * i] * inv, w.o[y][b][4 * i + 1] * inv, w.o[y][b][4 * i + 2] * inv,
-                                     w.o[y][b][4 * i + 3] * inv);
-        const int d = 32 * b + 8 * i + 4 * hi;
-        if (whole) {
-          const typename AttnOps<T>::vec4 e = {(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
-          *(typename AttnOps<T>::vec4 *)(rows.out(base + x) + d) = e;
-        } else {
-          *(float4 *)(p.po + (slot + x) * D + d) = v;
+        for (int i = 0; i < 4; ++i) {
+          const float4 v = make_float4(w.o[y][b][4 * i] * inv, w.o[y][b][4 * i + 1] * inv, w.o[y][b][4 * i + 2] * inv,
+                                       w.o[y][b][4 * i + 3] * inv);
+          const int d = 32 * b + 8 * i + 4 * hi;
+          if (whole) {
+            const typename AttnOps<T>::vec4 e = {(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
+            *(typename AttnOps<T>::vec4 *)(rows.out(base + x) + d) = e;
+          } else {
+            *(float4 *)(p.po + (slot + x) * D + d) = v;
+          }
         }
+      if (lane < 32) {
+        if (!whole) p.ml[slot + x] = make_float2(w.m[y], ls);
+        else if (a.lse) *rows.lse(base + x) = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
       }
-    if (lane < 32) {
-      if (!whole) p.ml[slot + x] = make_float2(w.m[y], ls);
-      else if (a.lse) *rows.lse(base + x) = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
     }
+    lds_barrier();                                 // LDS is free for the next row tile
   }
 }
 
-// The chunks of a row joined: one workgroup per (node, head), each of its waves a
-// contiguous quarter of the chunks in order, the quarters then added in order.
-template <typename T, int D> __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int unit) {
+// The chunks of a row joined.  Few rows (hpw 1): a workgroup per row, each of its
+// waves a contiguous quarter of the chunks in order, the quarters then added in
+// order.  Many: a workgroup per hpw heads of a node, a wave per row, so that finding
+// the node's group and its chunks, a microsecond or two, is done once for them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int unit, int hpw) {
   typedef typename T::elem elem;
   constexpr int E = D / 64;
-  __shared__ float s_o[4][D], s_m[4], s_l[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = blockIdx.x % a.nh, g = a.nh / a.kv.n_kv_head, hkv = h / g;
-  const int t = blockIdx.x / a.nh;
-  const TreeItem item = tree_find(a, t, true, rt, unit, p.target);
-  if (item.s < 0 || item.nsplit == 1) return;
+  __shared__ float s_o[4][D], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+  const int blocks = (a.nh + hpw - 1) / hpw, t = blockIdx.x / blocks, h0 = (blockIdx.x - t * blocks) * hpw;
+  const TreePlan plan(a, rt, unit, p.lines);
+  const TreeTile group = plan.find(a, 0, t);
+  if (group.s < 0) return;
   int c0;
-  span(a.cu, item.s, a.total, &c0);
-  const int r = (t - c0) * g + h % g, tile = r / rt;
-  const size_t first = ((size_t)hkv * p.slots + item.slot + tile * item.nsplit) * rt + r % rt;    // chunk x: first + x * rt
-  float M = -INFINITY;
-  for (int x = lane; x < item.nsplit; x += 64) M = fmaxf(M, p.ml[first + (size_t)x * rt].x);
+  span(a.cu, group.s, a.total, &c0);
+  const int g = a.nh / a.kv.n_kv_head;
+  for (int h = h0 + (hpw == 1 ? 0 : wave); h < min(h0 + hpw, a.nh); h += hpw == 1 ? 1 : 4) {
+    const int hkv = h / g, r = (t - c0) * g + h - hkv * g, tile = r / rt;
+    const long long at0 = group.at + (long long)tile * group.units;
+    const int w0 = scalar(plan.piece(at0)), nsplit = scalar(plan.piece(at0 + group.units - 1)) - w0 + 1;
+    if (nsplit == 1) continue;
+    // Chunk x is piece w0 + x's: its first row tile's, but for chunk 0 if the piece began before this tile.
+    const size_t first = ((size_t)hkv * 2 * p.lines + 2 * w0) * rt + r % rt, odd0 = plan.begin(w0) < at0 ? rt : 0;
+    auto slot = [&](int x) { return first + (size_t)x * 2 * rt + (x ? 0 : odd0); };
+    float M = -INFINITY;
+    for (int x = lane; x < nsplit; x += 64) M = fmaxf(M, p.ml[slot(x)].x);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-  const int per = (item.nsplit + 3) / 4, x0 = wave * per, x1 = min(x0 + per, item.nsplit);
-  float L = 0.f, o[E];
+    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
+    const int per = (nsplit + 3) / 4, x0 = hpw == 1 ? wave * per : 0, x1 = hpw == 1 ? min(x0 + per, nsplit) : nsplit;
+    float L = 0.f, o[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-  for (int x = x0; x < x1; ++x) {
-    const size_t at = first + (size_t)x * rt;
-    const float2 ml = p.ml[at];
-    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : __builtin_amdgcn_exp2f(ml.x - M);   // NaN stays
-    L += ml.x == -INFINITY ? f : ml.y * f;
+    for (int x = x0; x < x1; ++x) {
+      const size_t at = slot(x);
+      const float2 ml = p.ml[at];
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : __builtin_amdgcn_exp2f(ml.x - M);   // NaN stays
+      L += ml.x == -INFINITY ? f : ml.y * f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(p.po[at * D + lane * E + e], f, o[e]);
+      for (int e = 0; e < E; ++e) o[e] = fmaf(p.po[at * D + lane * E + e], f, o[e]);
+    }
+    if (hpw == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_o[wave][lane * E + e] = o[e];
+      if (lane == 0) s_l[wave] = L;
+      __syncthreads();
+      if (wave) return;
+      L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = s_o[0][lane * E + e] + s_o[1][lane * E + e] + s_o[2][lane * E + e] + s_o[3][lane * E + e];
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    elem *out = (elem *)a.o + (long long)t * a.os + h * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = (elem)(o[e] * inv);
+    if (a.lse && lane == 0) a.lse[(long long)t * a.nh + h] = LN2 * (M + __builtin_amdgcn_logf(L));
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_o[wave][lane * E + e] = o[e];
-  if (lane == 0) s_l[wave] = L;
-  __syncthreads();
-  (void)s_m;
-  L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  for (int d = tid; d < D; d += 256)
-    ((elem *)a.o)[(long long)t * a.os + h * D + d] = (elem)((s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) * inv);
-  if (a.lse && tid == 0) a.lse[(long long)t * a.nh + h] = LN2 * (M + __builtin_amdgcn_logf(L));
 }
 
 template <typename F> int by_type(int type, int D, F f) {
@@ -661,18 +713,16 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const int nkv = a.kv.n_kv_head, g = a.nh / nkv, D = a.kv.head_dim;
   const long long rows = (long long)a.max_nodes * g;
   const int form = rows <= 32 ? 1 : 4;                           // row tiles of 32 of a workgroup
-  const int rt = 32 * form, unit = form == 1 ? 128 : D == 256 ? 32 : 64;
-  const long long tiles = (rows + rt - 1) / rt;                  // of one group at most
-  const long long room = (long long)ctx->attn_floats / ((D + 2ll) * rt * nkv);   // slots that the scratch holds
+  const int rt = 32 * form, unit = form == 1 || D < 256 ? 128 : 64;
+  const long long room = (long long)ctx->attn_floats / ((D + 2ll) * rt * nkv * 2);   // pieces whose partials the scratch holds
+  static const int mul = getenv("MUL") ? atoi(getenv("MUL")) : 1;
+  const int per_cu = form == 1 ? 256 / D : D == 64 ? 3 : 2;      // workgroups that a CU holds at once
   TreeLaunch p;
-  long long want = std::max(1ll, 2ll * ctx->ncu / nkv);
-  p.target = (int)std::max(1ll, std::min(want, room / 2));
-  if (2ll * p.target > room) return CWEN_ESCRATCH;
-  if (a.max_len + a.max_nodes <= unit) p.target = 0;             // no chunks worth joining
-  p.slots = 2 * p.target;
+  p.lines = (int)std::max(1ll, std::min((long long)mul * per_cu * ctx->ncu / nkv, room));
+  if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
-  p.po = ctx->attn_part + (((size_t)nkv * p.slots * rt * 2 + 3) & ~(size_t)3);
-  const long long items = p.target + a.n_seq * tiles;            // at most
+  p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
+  const long long items = p.lines;
   if (items * nkv > INT32_MAX || (long long)a.total * a.nh > INT32_MAX) return CWEN_EINVAL;
   const dim3 grid((unsigned)(items * nkv));
   int rc = by_type(a.kv.type, D, [&](auto t, auto d) {
@@ -682,9 +732,13 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
     else if constexpr (dim == 256) hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
     else hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
   });
-  if (rc || !p.target) return rc;
+  if (rc || p.lines == 1) return rc;
+  // Up to 4 rows per CU: a workgroup each; past them as many heads to a workgroup as leave 2 per CU.
+  const long long all = (long long)a.total * a.nh;
+  int hpw = 1;
+  if (all > 4ll * ctx->ncu) hpw = (int)std::min<long long>(a.nh, std::max(4ll, all / (2ll * ctx->ncu)) + 3 & ~3ll);
   return by_type(a.kv.type, D, [&](auto t, auto d) {
-    hipLaunchKernelGGL((tree_join_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)a.total * a.nh), dim3(256), 0, st, a, p,
-                       rt, unit);
+    hipLaunchKernelGGL((tree_join_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)(a.total * ((a.nh + hpw - 1) / hpw))),
+                       dim3(256), 0, st, a, p, rt, unit, hpw);
   });
 }

@@ -58,6 +58,16 @@ template <> struct AttnOps<TypeBF16> {
   }
 };
 
+// Wait until at most N of the wave's loads are under way.  The builtin and not
+// asm: the compiler then knows that the older ones have landed and adds no
+// wait of its own before it reads them from LDS (vmcnt(0) there, which would
+// also wait for the next tile, took a third of the tree attention's time).
+template <int N> __device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 0x70 | 0xF00 | (N >> 4) << 14);   // gfx9 encoding: vmcnt(N), the others unchanged
+  asm volatile("" ::: "memory");
+}
+
 // Pieces (16 bytes) of a row, and where piece c of row r is kept.
 template <int D> __device__ __forceinline__ constexpr int k_piece(int r, int c) { return c ^ (r & (D >= 128 ? 15 : 7)); }
 template <int D> __device__ __forceinline__ constexpr int v_piece(int r, int c) {

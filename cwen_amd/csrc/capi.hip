@@ -21,7 +21,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 constexpr size_t kScratchHalves = (size_t)CWEN_BMAX * CWEN_KMAX;
 constexpr size_t kPartialFloats = (size_t)8 << 20;   // 32 MiB of split-K partials
 constexpr int kCounters = 1 << 16;
-constexpr size_t kAttnFloats = (size_t)16 << 20;     // 64 MiB: some 2 chunks per CU of 128 rows of 256
+constexpr size_t kAttnFloats = (size_t)36 << 20;     // 144 MiB: two partials of 128 rows of 256 for 2 workgroups per CU
 
 // Scratch of the allocation-free entry point, one copy per GPU, held until
 // the process ends: the f16 operand of X and the f16 hidden activations
