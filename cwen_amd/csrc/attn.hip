@@ -232,9 +232,15 @@ __device__ __forceinline__ long long lane64(long long v, int l) {
   const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), l);
   return (long long)((unsigned long long)hi << 32 | lo);
 }
+// Where every group has the same number of row tiles (`levels`, more than one of
+// them for many rows), each level has a line of its own, as long as the groups'
+// keys, cut alike: the workgroups that read the same keys for different rows then
+// run at the same time on the same XCD and find them in its L2.  On one line, 288
+// rows behind 32000 positions read every key from memory three times (106 us
+// against 89 with lines that happened to be cut alike).
 struct TreePlan {
-  int rt, unit, lines;
-  long long total;          // the line's length
+  int rt, unit, levels, lines;   // levels 1: one line for all (or one row tile a group)
+  long long total;               // a line's length
   __device__ __forceinline__ void of(const TreeArgs &a, int s, TreeSeq *q, int *tiles, int *units) const {
     *q = {};
     *tiles = *units = 0;
@@ -243,38 +249,52 @@ struct TreePlan {
     *tiles = (q->nodes * (a.nh / a.kv.n_kv_head) + rt - 1) / rt;
     *units = max((q->keys + unit - 1) / unit, 1);          // rows without keys are work too
   }
-  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rt, int unit, int most) : rt(rt), unit(unit), total(0) {
+  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rt, int unit, int want, int most) : rt(rt), unit(unit) {
+    long long sum = 0, one = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
       TreeSeq q;
       int tiles, units;
       of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
-      total += lane64(scan64((long long)tiles * units), 63);
+      sum += lane64(scan64((long long)tiles * units), 63);
+      if (want > 1) one += lane64(scan64((long long)(tiles ? units : 0)), 63);
     }
-    lines = scalar((int)min((long long)most, total));
+    levels = want > 1 && sum == one * want ? want : 1;
+    total = levels > 1 ? one : sum;
+    lines = scalar((int)min((long long)(most / levels), total));
   }
   // Where piece w begins, and the piece that holds position u.
   __device__ __forceinline__ long long begin(int w) const { return total * w / lines; }
   __device__ __forceinline__ int piece(long long u) const { return (int)(((u + 1) * lines - 1) / total); }
-  // The row tile at position u; or, with node >= 0, the group's first that holds it.
-  __device__ __forceinline__ TreeTile find(const TreeArgs &a, long long u, int node) const {
+  // The row tile at position u of a level's line; or, with node >= 0, the first one of
+  // the group that holds it.
+  __device__ __forceinline__ TreeTile find(const TreeArgs &a, int level, long long u, int node) const {
     long long at = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
       TreeSeq q;
       int tiles, units;
       of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
-      const long long mine = (long long)tiles * units, inc = at + scan64(mine);
+      const long long mine = (long long)(levels > 1 ? tiles > 0 : tiles) * units, inc = at + scan64(mine);
       const unsigned long long hit = __ballot(node >= 0 ? node >= q.c0 && node < q.c0 + q.nodes : inc > u);
       if (hit) {
         const int w = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(units, w);
         const long long first = lane64(inc - mine, w);
         const int tile = node >= 0 ? 0 : (int)((u - first) / n);
-        return {scalar(s0 + w), scalar(tile), scalar(n), lane64(first + (long long)tile * n, 0)};
+        return {scalar(s0 + w), scalar(levels > 1 ? level : tile), scalar(n), lane64(first + (long long)tile * n, 0)};
       }
       at = lane64(inc, 63);
     }
     return {-1, 0, 0, 0};
   }
 };
+// The level, piece and kv head of a workgroup: blocks run on XCD b % 8, and a
+// piece's levels follow each other there.
+struct TreeBlock {
+  int level, piece, hkv;
+};
+__device__ __forceinline__ TreeBlock tree_block(const TreePlan &p, int nkv) {
+  const int b = blockIdx.x, q = b >> 3, pair = q / p.levels * 8 + (b & 7);
+  return {q % p.levels, pair / nkv, pair % nkv};
+}
 // Bit j: whether node i's row sees key u0 + j of the drafted ones (u0 < 0: a
 // cached position, seen), j < 32; n nodes.
 __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int mw, int i, int n, int u0) {
@@ -295,7 +315,7 @@ __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int
 }
 
 struct TreeLaunch {
-  int lines;                    // pieces of a kv head's line
+  int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most
   float *po;                    // partial outputs [kv head][2 lines][row][D]: piece w's first row tile, its last
   float2 *ml;                   // and their maxima and sums [kv head][2 lines][row]
 };
@@ -375,14 +395,15 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
   __shared__ __align__(1024) elem Ks[NW * BN * D], Vs[NW * BN * D];
   __shared__ float2 s_ml[NW][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreePlan plan(a, 32, UNIT, p.lines);
-  const int piece = blockIdx.x / nkv;
+  const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
+  const TreePlan plan(a, 32, UNIT, p.levels, p.lines);
+  const TreeBlock me = tree_block(plan, nkv);
+  const int piece = scalar(me.piece), hkv = scalar(me.hkv);
   if (piece >= plan.lines) return;
   const long long stop = lane64(plan.begin(piece + 1), 0);
   bool first = true;
   for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
-    const TreeTile item = plan.find(a, u, -1);
+    const TreeTile item = plan.find(a, me.level, u, -1);
     const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
     u += count;
     const TreeSeq q = tree_seq1(a, item.s);
@@ -444,7 +465,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     const float l = w.sum(0);
     if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
     const bool whole = count == item.units;
-    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * piece + !first) * 32;
+    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * 32;
     if (__syncthreads_or(w.odd != w.odd)) {        // a hidden value may have leaked: the rows one by one
       for (int x = wave; x < R; x += NW)
         rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
@@ -499,15 +520,18 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
   typedef typename T::elem elem;
   constexpr int WM = 32 * QB, RT = WM * NW, PER = BN * D / 8 / (64 * NW), UNIT = 2 * BN;
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+  constexpr int WORDS = CWEN_TREE_MAX / 32;
+  __shared__ uint32_t s_see[NW][QB][WORDS][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nkv = a.kv.n_kv_head, hkv = blockIdx.x % nkv, n = lane & 31, hi = lane >> 5;
-  const TreePlan plan(a, RT, UNIT, p.lines);
-  const int piece = blockIdx.x / nkv;
+  const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
+  const TreePlan plan(a, RT, UNIT, p.levels, p.lines);
+  const TreeBlock me = tree_block(plan, nkv);
+  const int piece = scalar(me.piece), hkv = scalar(me.hkv);
   if (piece >= plan.lines) return;
   const long long stop = lane64(plan.begin(piece + 1), 0);
   bool first = true;
   for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
-    const TreeTile item = plan.find(a, u, -1);
+    const TreeTile item = plan.find(a, me.level, u, -1);
     const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
     u += count;
     const TreeSeq q = tree_seq1(a, item.s);
@@ -517,7 +541,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
     const int begin = skip * UNIT, end = min(begin + count * UNIT, q.keys);
     bool bad = false;
     const float c = a.scale * LOG2E;
-    // The page of each piece that this wave lands (its rows lie in one page), a tile ahead.
+    // The page of each load's rows (they lie in one page), a tile ahead.
     int pg[PER];
     auto pages = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
@@ -548,6 +572,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
       lds_barrier();
       continue;
     }
+    // What the rows see of the drafted nodes, before the tiles need the registers.
+    if (end > q.len) {
+#pragma unroll
+      for (int y = 0; y < QB; ++y) {
+        const int r = base + 32 * y + n;
+        const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
+        for (int k = hi; k < WORDS; k += 2) s_see[wave][y][k][n] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, 32 * k);
+      }
+    }
     AttnWave<T, D, BN, QB> w;
 #pragma unroll
     for (int y = 0; y < QB; ++y) w.start(y, 32 * y + n < R ? rows.query(base + 32 * y + n) : nullptr);
@@ -558,13 +591,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
     auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
       uint32_t see[QB][BN / 32];
 #pragma unroll
-      for (int y = 0; y < QB; ++y) {
-        const int r = base + 32 * y + n;
-        const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
+      for (int y = 0; y < QB; ++y)
 #pragma unroll
-        for (int b = 0; b < BN / 32; ++b)
-          saw[y] |= see[y][b] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, t0 + 32 * b - q.len);
-      }
+        for (int b = 0; b < BN / 32; ++b) {
+          const int u0 = t0 + 32 * b - q.len, k = u0 >> 5;            // 32 bits across two words
+          const uint32_t lo = k < 0 ? ~0u : k < WORDS ? s_see[wave][y][k][n] : 0;
+          const uint32_t up = k < -1 ? ~0u : k + 1 < WORDS ? s_see[wave][y][k + 1][n] : 0;
+          saw[y] |= see[y][b] = __builtin_amdgcn_alignbit(up, lo, u0 & 31);
+        }
       w.template tile<true>(Kb, Vb, c, [&](int y, int j) { return !((see[y][j >> 5] >> (j & 31)) & 1); });
     };
     for (; t0 < full; t0 += 2 * BN) {
@@ -575,18 +609,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
       if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
       w.template tile<false>(K1, V1, c, [](int, int) { return false; });
     }
-    for (; t0 < end; t0 += 2 * BN) {
+    for (bool one = false; t0 < end; t0 += BN, one = !one) {
       ready();
-      if (t0 + BN < end) land(K1, V1, t0 + BN);
-      part(K0, V0, t0);
-      if (t0 + BN >= end) break;
-      ready();
-      if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
-      part(K1, V1, t0 + BN);
+      if (t0 + BN < end) land(one ? K0 : K1, one ? V0 : V1, t0 + BN);
+      part(one ? K1 : K0, one ? V1 : V0, t0);
     }
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
     const bool whole = count == item.units;
-    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * piece + !first) * RT + wave * WM;
+    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * RT + wave * WM;
     if (__any(w.odd != w.odd)) {
       for (int x = 0; x < R; ++x)
         rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
@@ -632,20 +662,22 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
   __shared__ float s_o[4][D], s_l[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
   const int blocks = (a.nh + hpw - 1) / hpw, t = blockIdx.x / blocks, h0 = (blockIdx.x - t * blocks) * hpw;
-  const TreePlan plan(a, rt, unit, p.lines);
-  const TreeTile group = plan.find(a, 0, t);
+  const TreePlan plan(a, rt, unit, p.levels, p.lines);
+  const TreeTile group = plan.find(a, 0, 0, t);
   if (group.s < 0) return;
   int c0;
   span(a.cu, group.s, a.total, &c0);
   const int g = a.nh / a.kv.n_kv_head;
   for (int h = h0 + (hpw == 1 ? 0 : wave); h < min(h0 + hpw, a.nh); h += hpw == 1 ? 1 : 4) {
     const int hkv = h / g, r = (t - c0) * g + h - hkv * g, tile = r / rt;
-    const long long at0 = group.at + (long long)tile * group.units;
+    const int level = plan.levels > 1 ? tile : 0;
+    const long long at0 = group.at + (long long)(tile - level) * group.units;
     const int w0 = scalar(plan.piece(at0)), nsplit = scalar(plan.piece(at0 + group.units - 1)) - w0 + 1;
     if (nsplit == 1) continue;
     // Chunk x is piece w0 + x's: its first row tile's, but for chunk 0 if the piece began before this tile.
-    const size_t first = ((size_t)hkv * 2 * p.lines + 2 * w0) * rt + r % rt, odd0 = plan.begin(w0) < at0 ? rt : 0;
-    auto slot = [&](int x) { return first + (size_t)x * 2 * rt + (x ? 0 : odd0); };
+    const size_t first = ((size_t)hkv * 2 * p.lines + 2 * (w0 * plan.levels + level)) * rt + r % rt;
+    const size_t odd0 = plan.begin(w0) < at0 ? rt : 0;
+    auto slot = [&](int x) { return first + (size_t)x * 2 * plan.levels * rt + (x ? 0 : odd0); };
     float M = -INFINITY;
     for (int x = lane; x < nsplit; x += 64) M = fmaxf(M, p.ml[slot(x)].x);
 #pragma unroll
@@ -719,12 +751,15 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const int per_cu = form == 1 ? 256 / D : D == 64 ? 3 : 2;      // workgroups that a CU holds at once
   TreeLaunch p;
   p.lines = (int)std::max(1ll, std::min((long long)mul * per_cu * ctx->ncu / nkv, room));
+  if (getenv("LINES")) p.lines = atoi(getenv("LINES"));
   if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
   p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
-  const long long items = p.lines;
-  if (items * nkv > INT32_MAX || (long long)a.total * a.nh > INT32_MAX) return CWEN_EINVAL;
-  const dim3 grid((unsigned)(items * nkv));
+  p.levels = (int)std::min((rows + rt - 1) / rt, (long long)p.lines);
+  const long long blocks = 8ll * std::max((long long)p.levels * (((long long)nkv * (p.lines / p.levels) + 7) / 8),
+                                          ((long long)nkv * p.lines + 7) / 8);
+  if (blocks > INT32_MAX || (long long)a.total * a.nh > INT32_MAX) return CWEN_EINVAL;
+  const dim3 grid((unsigned)blocks);
   int rc = by_type(a.kv.type, D, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value, BN = dim == 256 ? 32 : 64;
