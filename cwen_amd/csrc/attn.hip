@@ -1,7 +1,6 @@
 // Attention of packed prompts and of drafted trees over the paged cache.
 #include <math.h>
 #include <algorithm>
-#include <stdlib.h>
 #include "cwen_internal.h"
 #include "kv_table.h"
 #include "attn_core.h"
@@ -210,28 +209,24 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int s) {
   }
   return q;
 }
-__device__ __forceinline__ TreeSeq tree_seq1(const TreeArgs &a, int s) {     // in scalar registers
-  const TreeSeq q = tree_seq(a, s);
-  return {scalar(q.c0), scalar(q.nodes), scalar(q.len), scalar(q.keys), scalar(q.id), scalar(q.bad) != 0};
-}
 struct TreeTile {
   int s, tile;              // group (< 0: none) and row tile of it
   int units;                // its length
-  long long at;             // where it begins on the line
+  int at;                   // where it begins on the line
 };
-__device__ __forceinline__ long long scan64(long long v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long long u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
+// Inclusive sum over the wave's lanes (row shifts, then row broadcasts).
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
 }
-__device__ __forceinline__ long long lane64(long long v, int l) {
-  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), l);
-  return (long long)((unsigned long long)hi << 32 | lo);
+__device__ __forceinline__ int scan64(int v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
 }
+__device__ __forceinline__ int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 // Where every group has the same number of row tiles (`levels`, more than one of
 // them for many rows), each level has a line of its own, as long as the groups'
 // keys, cut alike: the workgroups that read the same keys for different rows then
@@ -240,48 +235,54 @@ __device__ __forceinline__ long long lane64(long long v, int l) {
 // against 89 with lines that happened to be cut alike).
 struct TreePlan {
   int rt, unit, levels, lines;   // levels 1: one line for all (or one row tile a group)
-  long long total;               // a line's length
-  __device__ __forceinline__ void of(const TreeArgs &a, int s, TreeSeq *q, int *tiles, int *units) const {
-    *q = {};
-    *tiles = *units = 0;
-    if (s >= a.n_seq) return;
-    *q = tree_seq(a, s);
-    *tiles = (q->nodes * (a.nh / a.kv.n_kv_head) + rt - 1) / rt;
-    *units = max((q->keys + unit - 1) / unit, 1);          // rows without keys are work too
+  int total;                     // a line's length; the launch has made sure that the sums fit 32 bits
+  // A lane's group: its sequence, row tiles and units.
+  struct Mine {
+    TreeSeq q;
+    int tiles, units;
+  };
+  __device__ __forceinline__ Mine load(const TreeArgs &a, int s0) const {
+    const int s = s0 + (int)(threadIdx.x & 63);
+    Mine m = {};
+    if (s >= a.n_seq) return m;
+    m.q = tree_seq(a, s);
+    m.tiles = (m.q.nodes * (a.nh / a.kv.n_kv_head) + rt - 1) / rt;
+    m.units = max((m.q.keys + unit - 1) / unit, 1);          // rows without keys are work too
+    return m;
   }
-  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rt, int unit, int want, int most) : rt(rt), unit(unit) {
-    long long sum = 0, one = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-      TreeSeq q;
-      int tiles, units;
-      of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
-      sum += lane64(scan64((long long)tiles * units), 63);
-      if (want > 1) one += lane64(scan64((long long)(tiles ? units : 0)), 63);
+  // m: load(a, 0)
+  __device__ __forceinline__ TreePlan(int rt, int unit) : rt(rt), unit(unit) {}
+  __device__ __forceinline__ void lay(const TreeArgs &a, Mine m, int want, int most) {
+    int sum = 0, one = 0;
+    for (int s0 = 0;;) {
+      sum += lane_of(scan64(m.tiles * m.units), 63);
+      if (want > 1) one += lane_of(scan64(m.tiles ? m.units : 0), 63);
+      if ((s0 += 64) >= a.n_seq) break;
+      m = load(a, s0);
     }
     levels = want > 1 && sum == one * want ? want : 1;
     total = levels > 1 ? one : sum;
-    lines = scalar((int)min((long long)(most / levels), total));
+    lines = min(most / levels, total);
   }
   // Where piece w begins, and the piece that holds position u.
-  __device__ __forceinline__ long long begin(int w) const { return total * w / lines; }
-  __device__ __forceinline__ int piece(long long u) const { return (int)(((u + 1) * lines - 1) / total); }
+  __device__ __forceinline__ int begin(int w) const { return total / lines * w + total % lines * w / lines; }
+  __device__ __forceinline__ int piece(int u) const { return (int)(((long long)(u + 1) * lines - 1) / total); }
   // The row tile at position u of a level's line; or, with node >= 0, the first one of
-  // the group that holds it.
-  __device__ __forceinline__ TreeTile find(const TreeArgs &a, int level, long long u, int node) const {
-    long long at = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-      TreeSeq q;
-      int tiles, units;
-      of(a, s0 + (int)(threadIdx.x & 63), &q, &tiles, &units);
-      const long long mine = (long long)(levels > 1 ? tiles > 0 : tiles) * units, inc = at + scan64(mine);
-      const unsigned long long hit = __ballot(node >= 0 ? node >= q.c0 && node < q.c0 + q.nodes : inc > u);
+  // the group that holds it.  q: the group's sequence.
+  __device__ __forceinline__ TreeTile find(const TreeArgs &a, Mine m, int level, int u, int node, TreeSeq *q) const {
+    int at = 0;
+    for (int s0 = 0; s0 < a.n_seq;) {
+      const int mine = (levels > 1 ? m.tiles > 0 : m.tiles) * m.units, inc = at + scan64(mine);
+      const unsigned long long hit = __ballot(node >= 0 ? node >= m.q.c0 && node < m.q.c0 + m.q.nodes : inc > u);
       if (hit) {
-        const int w = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(units, w);
-        const long long first = lane64(inc - mine, w);
-        const int tile = node >= 0 ? 0 : (int)((u - first) / n);
-        return {scalar(s0 + w), scalar(levels > 1 ? level : tile), scalar(n), lane64(first + (long long)tile * n, 0)};
+        const int w = __builtin_ctzll(hit), n = lane_of(m.units, w), first = lane_of(inc - mine, w);
+        const int tile = node >= 0 ? 0 : (u - first) / n;
+        *q = {lane_of(m.q.c0, w), lane_of(m.q.nodes, w), lane_of(m.q.len, w), lane_of(m.q.keys, w), lane_of(m.q.id, w),
+              lane_of(m.q.bad, w) != 0};
+        return {scalar(s0 + w), scalar(levels > 1 ? level : tile), n, scalar(first + tile * n)};
       }
-      at = lane64(inc, 63);
+      at = lane_of(inc, 63);
+      if ((s0 += 64) < a.n_seq) m = load(a, s0);
     }
     return {-1, 0, 0, 0};
   }
@@ -318,6 +319,7 @@ struct TreeLaunch {
   int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most
   float *po;                    // partial outputs [kv head][2 lines][row][D]: piece w's first row tile, its last
   float2 *ml;                   // and their maxima and sums [kv head][2 lines][row]
+  int *count;                   // few rows: arrivals per (kv head, group), zero between launches; null: joined by a launch
 };
 
 // One group's rows against the pages: what both forms share.
@@ -383,30 +385,56 @@ template <typename T, int D> struct TreeRows {
   }
 };
 
+// A chunk's share of a row: how its sums count against the row's maximum M (NaN
+// stays), and what it adds to the row's sum.
+__device__ __forceinline__ float chunk_weight(float2 ml, float M, float *sum) {
+  const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : __builtin_amdgcn_exp2f(ml.x - M);
+  *sum += ml.x == -INFINITY ? f : ml.y * f;
+  return f;
+}
+// Values that other workgroups of this launch wrote: at the device's coherence point.
+__device__ __forceinline__ void put2(void *p, float x, float y) {
+  __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const void *p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ float max64(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+
 // Few rows: one tile of 32, the chunk's keys dealt to 4 waves 32 at a time.  A wave
 // has its own K and V rows in LDS and no barrier in its loop: the next K rows
 // are requested when the scores are done, the next V rows after the outputs, so
 // that half of its LDS and more is always under way.  The waves' sums meet at the
-// end.
+// end.  Where the chunks of a group are few, the last workgroup to leave one joins
+// them in the same launch.
 template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void tree_few_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
   constexpr int BN = 32, NW = 4, UNIT = BN * NW, PC = D / 4;      // PC: 16-byte pieces of an f32 row
   constexpr int LOADS = BN * D / 8 / 64;                          // of one tile of K or V, by one wave
+  constexpr int JOIN = 16;
   __shared__ __align__(1024) elem Ks[NW * BN * D], Vs[NW * BN * D];
   __shared__ float2 s_ml[NW][32];
+  __shared__ int s_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
-  const TreePlan plan(a, 32, UNIT, p.levels, p.lines);
+  TreePlan plan(32, UNIT);
+  TreePlan::Mine groups = plan.load(a, 0);
+  plan.lay(a, groups, p.levels, p.lines);
   const TreeBlock me = tree_block(plan, nkv);
   const int piece = scalar(me.piece), hkv = scalar(me.hkv);
   if (piece >= plan.lines) return;
-  const long long stop = lane64(plan.begin(piece + 1), 0);
+  const int stop = scalar(plan.begin(piece + 1));
   bool first = true;
-  for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
-    const TreeTile item = plan.find(a, me.level, u, -1);
-    const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
+  for (int u = scalar(plan.begin(piece)); u < stop; first = false) {
+    if (!first) groups = plan.load(a, 0);          // not kept through the tiles
+    TreeSeq q;
+    const TreeTile item = plan.find(a, groups, me.level, u, -1, &q);
+    const int skip = u - item.at, count = min(item.at + item.units, stop) - u;
     u += count;
-    const TreeSeq q = tree_seq1(a, item.s);
     if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
     const TreeRows<T, D> rows(a, q, hkv);
     const int base = item.tile * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;
@@ -466,9 +494,68 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
     const bool whole = count == item.units;
     const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * 32;
+    auto join = [&]() __attribute__((always_inline)) {
+      const int at0 = item.at, p0 = plan.piece(at0), nsplit = plan.piece(at0 + item.units - 1) - p0 + 1;
+      int *count = p.count + hkv * a.n_seq + item.s;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the partial has arrived
+      __syncthreads();
+      if (tid == 0) s_end = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nsplit - 1;
+      __syncthreads();
+      if (!s_end) return;
+      const size_t first0 = ((size_t)hkv * p.lines + p0) * 2 * 32, odd0 = plan.begin(p0) < at0 ? 32 : 0;
+      auto place = [&](int x, int y) { return first0 + (size_t)x * 64 + (x ? 0 : odd0) + y; };
+      // The chunks' weights of as many rows as LDS holds, then 16 bytes a thread of
+      // their outputs, JOIN chunks under way at a time: each round is a trip to memory.
+      float *weight = (float *)Ks;
+      const int batch = min(R, NW * BN * D / 2 / nsplit);
+      for (int y0 = 0; y0 < R; y0 += batch) {
+        const int y1 = min(y0 + batch, R);
+        for (int y = y0 + wave; y < y1; y += NW) {
+          float M = -INFINITY, L = 0.f;
+          for (int x = lane; x < nsplit; x += 64) M = fmaxf(M, get2(p.ml + place(x, y)).x);
+          M = max64(M);
+          for (int x = lane; x < nsplit; x += 64) weight[(y - y0) * nsplit + x] = chunk_weight(get2(p.ml + place(x, y)), M, &L);
+          L = sum64(L);
+          if (lane == 0) s_ml[0][y] = make_float2(M, L);
+        }
+        __syncthreads();
+        for (int z = tid; z < (y1 - y0) * PC; z += 256) {
+          const int y = y0 + z / PC, pc = z % PC;
+          const float *wy = weight + (y - y0) * nsplit;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int x = 0; x < nsplit; x += JOIN) {
+            float2 v[JOIN][2];
+#pragma unroll
+            for (int u = 0; u < JOIN; ++u) {
+              const float *po = p.po + place(min(x + u, nsplit - 1), y) * D + 4 * pc;
+              v[u][0] = get2(po);
+              v[u][1] = get2(po + 2);
+            }
+#pragma unroll
+            for (int u = 0; u < JOIN; ++u) {
+              if (x + u >= nsplit) break;
+              const float f = wy[x + u];
+              o.x = fmaf(v[u][0].x, f, o.x); o.y = fmaf(v[u][0].y, f, o.y);
+              o.z = fmaf(v[u][1].x, f, o.z); o.w = fmaf(v[u][1].y, f, o.w);
+            }
+          }
+          const float2 ml = s_ml[0][y];
+          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+          const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
+          *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
+          if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));
+        }
+        __syncthreads();
+      }
+      if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
     if (__syncthreads_or(w.odd != w.odd)) {        // a hidden value may have leaked: the rows one by one
       for (int x = wave; x < R; x += NW)
         rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
+      if (!whole && p.count) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+        join();
+      }
       __syncthreads();
       continue;
     }
@@ -505,11 +592,17 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
         const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
         *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
         if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (Mr + __builtin_amdgcn_logf(L));
+      } else if (p.count) {
+        float *po = p.po + (slot + y) * D + 4 * pc;
+        put2(po, o.x, o.y);
+        put2(po + 2, o.z, o.w);
+        if (pc == 0) put2(p.ml + slot + y, Mr, L);
       } else {
         *(float4 *)(p.po + (slot + y) * D + 4 * pc) = o;
         if (pc == 0) p.ml[slot + y] = make_float2(Mr, L);
       }
     }
+    if (!whole && p.count) join();
     __syncthreads();                               // LDS is free for the next row tile
   }
 }
@@ -524,17 +617,20 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
   __shared__ uint32_t s_see[NW][QB][WORDS][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
-  const TreePlan plan(a, RT, UNIT, p.levels, p.lines);
+  TreePlan plan(RT, UNIT);
+  TreePlan::Mine groups = plan.load(a, 0);
+  plan.lay(a, groups, p.levels, p.lines);
   const TreeBlock me = tree_block(plan, nkv);
   const int piece = scalar(me.piece), hkv = scalar(me.hkv);
   if (piece >= plan.lines) return;
-  const long long stop = lane64(plan.begin(piece + 1), 0);
+  const int stop = scalar(plan.begin(piece + 1));
   bool first = true;
-  for (long long u = lane64(plan.begin(piece), 0); u < stop; first = false) {
-    const TreeTile item = plan.find(a, me.level, u, -1);
-    const int skip = scalar((int)(u - item.at)), count = scalar((int)(min(item.at + item.units, stop) - u));
+  for (int u = scalar(plan.begin(piece)); u < stop; first = false) {
+    if (!first) groups = plan.load(a, 0);          // not kept through the tiles
+    TreeSeq q;
+    const TreeTile item = plan.find(a, groups, me.level, u, -1, &q);
+    const int skip = u - item.at, count = min(item.at + item.units, stop) - u;
     u += count;
-    const TreeSeq q = tree_seq1(a, item.s);
     if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
     const TreeRows<T, D> rows(a, q, hkv);
     const int base = item.tile * RT + wave * WM, R = min(q.nodes * rows.g - base, WM);   // R <= 0: no rows here
@@ -651,65 +747,100 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
   }
 }
 
-// The chunks of a row joined.  Few rows (hpw 1): a workgroup per row, each of its
-// waves a contiguous quarter of the chunks in order, the quarters then added in
-// order.  Many: a workgroup per hpw heads of a node, a wave per row, so that finding
-// the node's group and its chunks, a microsecond or two, is done once for them.
-template <typename T, int D>
+// The chunks of rows joined: a workgroup takes `hpw` heads of a node.  LR lanes find
+// a row's chunks and their weights, into LDS; then each thread adds 16 bytes of a
+// row's outputs, or, with fewer of those than threads, a share of its chunks. So
+// the trips to memory are few however many rows a workgroup has: one after the
+// other they took 28 us of a batch of 580 nodes.
+constexpr int JOIN_HEADS = 32;
+template <typename T, int D, int LR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int unit, int hpw) {
   typedef typename T::elem elem;
-  constexpr int E = D / 64;
-  __shared__ float s_o[4][D], s_l[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
-  const int blocks = (a.nh + hpw - 1) / hpw, t = blockIdx.x / blocks, h0 = (blockIdx.x - t * blocks) * hpw;
-  const TreePlan plan(a, rt, unit, p.levels, p.lines);
-  const TreeTile group = plan.find(a, 0, 0, t);
-  if (group.s < 0) return;
-  int c0;
-  span(a.cu, group.s, a.total, &c0);
-  const int g = a.nh / a.kv.n_kv_head;
-  for (int h = h0 + (hpw == 1 ? 0 : wave); h < min(h0 + hpw, a.nh); h += hpw == 1 ? 1 : 4) {
-    const int hkv = h / g, r = (t - c0) * g + h - hkv * g, tile = r / rt;
-    const int level = plan.levels > 1 ? tile : 0;
-    const long long at0 = group.at + (long long)(tile - level) * group.units;
-    const int w0 = scalar(plan.piece(at0)), nsplit = scalar(plan.piece(at0 + group.units - 1)) - w0 + 1;
-    if (nsplit == 1) continue;
-    // Chunk x is piece w0 + x's: its first row tile's, but for chunk 0 if the piece began before this tile.
-    const size_t first = ((size_t)hkv * 2 * p.lines + 2 * (w0 * plan.levels + level)) * rt + r % rt;
-    const size_t odd0 = plan.begin(w0) < at0 ? rt : 0;
-    auto slot = [&](int x) { return first + (size_t)x * 2 * plan.levels * rt + (x ? 0 : odd0); };
-    float M = -INFINITY;
-    for (int x = lane; x < nsplit; x += 64) M = fmaxf(M, p.ml[slot(x)].x);
+  constexpr int PC = D / 4, CAP = 4096, U = 8;
+  __shared__ float s_w[CAP];
+  __shared__ float2 s_ml[JOIN_HEADS];
+  __shared__ long long s_first[JOIN_HEADS];
+  __shared__ int s_n[JOIN_HEADS], s_odd[JOIN_HEADS];
+  __shared__ float4 s_o[256];
+  const int tid = threadIdx.x, blocks = (a.nh + hpw - 1) / hpw, t = blockIdx.x / blocks, h0 = (blockIdx.x - t * blocks) * hpw;
+  TreePlan plan(rt, unit);
+  const TreePlan::Mine groups = plan.load(a, 0);
+  plan.lay(a, groups, p.levels, p.lines);
+  TreeSeq q;
+  const TreeTile group = plan.find(a, groups, 0, 0, t, &q);
+  if (group.s < 0 || plan.lines == 1) return;
+  const int g = a.nh / a.kv.n_kv_head, rows = min(hpw, a.nh - h0), step = 2 * plan.levels * rt;
+  const int batch = min(rows, CAP / plan.lines);                  // at most 4 workgroups a CU: lines <= 1024 <= CAP
+  for (int y0 = 0; y0 < rows; y0 += batch) {
+    const int nb = min(batch, rows - y0);
+    for (int i = tid / LR; i < nb; i += 256 / LR) {
+      const int h = h0 + y0 + i, hkv = h / g, r = (t - q.c0) * g + h - hkv * g, tile = r / rt, level = plan.levels > 1 ? tile : 0;
+      const int at0 = group.at + (tile - level) * group.units, w0 = plan.piece(at0);
+      const int n = plan.piece(at0 + group.units - 1) - w0 + 1, l = tid % LR;
+      // Chunk x is piece w0 + x's: its first row tile's, but for chunk 0 if the piece began before this tile.
+      const long long first = ((long long)hkv * 2 * p.lines + 2 * (w0 * plan.levels + level)) * rt + r % rt;
+      const int odd = plan.begin(w0) < at0 ? rt : 0;
+      float M = -INFINITY, L = 0.f;
+      if (n > 1) {
+        for (int x = l; x < n; x += LR) M = fmaxf(M, p.ml[first + (long long)x * step + (x ? 0 : odd)].x);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-    const int per = (nsplit + 3) / 4, x0 = hpw == 1 ? wave * per : 0, x1 = hpw == 1 ? min(x0 + per, nsplit) : nsplit;
-    float L = 0.f, o[E];
+        for (int d = 1; d < LR; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
+        for (int x = l; x < n; x += LR)
+          s_w[i * plan.lines + x] = chunk_weight(p.ml[first + (long long)x * step + (x ? 0 : odd)], M, &L);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int x = x0; x < x1; ++x) {
-      const size_t at = slot(x);
-      const float2 ml = p.ml[at];
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : __builtin_amdgcn_exp2f(ml.x - M);   // NaN stays
-      L += ml.x == -INFINITY ? f : ml.y * f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(p.po[at * D + lane * E + e], f, o[e]);
+        for (int d = 1; d < LR; d *= 2) L += __shfl_xor(L, d);
+      }
+      if (l == 0) {
+        s_n[i] = n;
+        s_first[i] = first;
+        s_odd[i] = odd;
+        s_ml[i] = make_float2(M, L);
+      }
     }
-    if (hpw == 1) {
+    __syncthreads();
+    const int items = nb * PC, shares = max(256 / items, 1);
+    for (int z0 = 0; z0 < items; z0 += 256) {
+      const int z = z0 + tid % (items < 256 ? items : 256), share = items < 256 ? tid / items : 0;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (z < items && share < shares) {
+        const int i = z / PC, pc = z % PC, n = s_n[i] > 1 ? s_n[i] : 0, per = (n + shares - 1) / shares, x1 = min((share + 1) * per, n);
+        for (int x = share * per; x < x1; x += U) {
+          float4 v[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) s_o[wave][lane * E + e] = o[e];
-      if (lane == 0) s_l[wave] = L;
-      __syncthreads();
-      if (wave) return;
-      L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+          for (int u = 0; u < U; ++u) {
+            const int at = min(x + u, x1 - 1);
+            v[u] = *(const float4 *)(p.po + (s_first[i] + (long long)at * step + (at ? 0 : s_odd[i])) * D + 4 * pc);
+          }
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = s_o[0][lane * E + e] + s_o[1][lane * E + e] + s_o[2][lane * E + e] + s_o[3][lane * E + e];
+          for (int u = 0; u < U; ++u) {
+            if (x + u >= x1) break;
+            const float f = s_w[i * plan.lines + x + u];
+            o.x = fmaf(v[u].x, f, o.x); o.y = fmaf(v[u].y, f, o.y);
+            o.z = fmaf(v[u].z, f, o.z); o.w = fmaf(v[u].w, f, o.w);
+          }
+        }
+      }
+      if (shares > 1) {
+        s_o[tid] = o;
+        __syncthreads();
+        if (share == 0)
+          for (int u = 1; u < shares; ++u) {
+            const float4 v = s_o[tid + u * items];
+            o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+          }
+      }
+      if (z < items && share == 0) {
+        const int i = z / PC, pc = z % PC, h = h0 + y0 + i;
+        if (s_n[i] > 1) {
+          const float2 ml = s_ml[i];
+          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+          const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
+          *(typename AttnOps<T>::vec4 *)((elem *)a.o + (long long)t * a.os + h * D + 4 * pc) = e;
+          if (a.lse && pc == 0) a.lse[(long long)t * a.nh + h] = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));
+        }
+      }
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    elem *out = (elem *)a.o + (long long)t * a.os + h * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = (elem)(o[e] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)t * a.nh + h] = LN2 * (M + __builtin_amdgcn_logf(L));
+    __syncthreads();
   }
 }
 
@@ -747,17 +878,23 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const int form = rows <= 32 ? 1 : 4;                           // row tiles of 32 of a workgroup
   const int rt = 32 * form, unit = form == 1 || D < 256 ? 128 : 64;
   const long long room = (long long)ctx->attn_floats / ((D + 2ll) * rt * nkv * 2);   // pieces whose partials the scratch holds
-  static const int mul = getenv("MUL") ? atoi(getenv("MUL")) : 1;
   const int per_cu = form == 1 ? 256 / D : D == 64 ? 3 : 2;      // workgroups that a CU holds at once
   TreeLaunch p;
-  p.lines = (int)std::max(1ll, std::min((long long)mul * per_cu * ctx->ncu / nkv, room));
-  if (getenv("LINES")) p.lines = atoi(getenv("LINES"));
+  p.lines = (int)std::max(1ll, std::min((long long)per_cu * ctx->ncu / nkv, room));
   if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
+  // Up to 128 (row, chunk) partials of a group are joined in the launch: one token of 6 heads behind 1000
+  // positions 14.4 us so, 15.7 in two launches; behind 4096 20.0 and 16.8.
+  const long long chunks = std::min((long long)p.lines, ((long long)a.max_len + a.max_nodes + unit - 1) / unit);
+  p.count = form == 1 && chunks * rows <= 128 && (long long)nkv * a.n_seq <= ctx->ncounters ? ctx->counters : nullptr;
   p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
-  p.levels = (int)std::min((rows + rt - 1) / rt, (long long)p.lines);
+  const long long tiles = (rows + rt - 1) / rt;                  // of one group at most
+  p.levels = (int)std::min(tiles, (long long)p.lines);
   const long long blocks = 8ll * std::max((long long)p.levels * (((long long)nkv * (p.lines / p.levels) + 7) / 8),
                                           ((long long)nkv * p.lines + 7) / 8);
+  // Every line's positions fit 32 bits.
+  const long long units = ((long long)a.kv.max_pages * a.kv.page + unit - 1) / unit + 1;
+  if ((a.n_seq + 64ll) * tiles * units > INT32_MAX) return CWEN_EINVAL;
   if (blocks > INT32_MAX || (long long)a.total * a.nh > INT32_MAX) return CWEN_EINVAL;
   const dim3 grid((unsigned)blocks);
   int rc = by_type(a.kv.type, D, [&](auto t, auto d) {
@@ -767,13 +904,16 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
     else if constexpr (dim == 256) hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
     else hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
   });
-  if (rc || p.lines == 1) return rc;
+  if (rc || p.lines == 1 || p.count) return rc;
   // Up to 4 rows per CU: a workgroup each; past them as many heads to a workgroup as leave 2 per CU.
   const long long all = (long long)a.total * a.nh;
   int hpw = 1;
-  if (all > 4ll * ctx->ncu) hpw = (int)std::min<long long>(a.nh, std::max(4ll, all / (2ll * ctx->ncu)) + 3 & ~3ll);
+  if (all > 4ll * ctx->ncu) hpw = (int)std::min<long long>(std::min(a.nh, JOIN_HEADS), std::max(2ll, all / (2ll * ctx->ncu)));
   return by_type(a.kv.type, D, [&](auto t, auto d) {
-    hipLaunchKernelGGL((tree_join_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)(a.total * ((a.nh + hpw - 1) / hpw))),
-                       dim3(256), 0, st, a, p, rt, unit, hpw);
+    typedef decltype(t) T;
+    constexpr int dim = decltype(d)::value;
+    const dim3 grid((unsigned)(a.total * ((a.nh + hpw - 1) / hpw)));
+    if (hpw <= 4) hipLaunchKernelGGL((tree_join_kernel<T, dim, 64>), grid, dim3(256), 0, st, a, p, rt, unit, hpw);
+    else hipLaunchKernelGGL((tree_join_kernel<T, dim, 16>), grid, dim3(256), 0, st, a, p, rt, unit, hpw);
   });
 }
