@@ -54,41 +54,90 @@ template <typename T, int D> struct AttnRow {
   }
 };
 
+// Inclusive sum over the wave's lanes (row shifts, then row broadcasts).
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ int scan64(int v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
+}
+__device__ __forceinline__ int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ int max64(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v = max(v, __shfl_xor(v, d));
+  return v;
+}
+
 // ---- packed prompts ----
-// Sequence and tile of item `it`: the sequences' tiles of BM queries, counted
-// one after the other.  Every wave finds it by itself (64 sequences at a time).
+// Sequence and tile of item `it` of the sequences' tiles of BM queries.  Every wave
+// finds it by itself.
 struct Item {
   int seq, tile;      // seq < 0: past the last one
+  int q0, nq, k0, nk; // the sequence's first query, queries, first key, keys
 };
 __device__ __forceinline__ int span(const int *cu, int s, int total, int *first) {
   const int a = min(max(cu[s], 0), total), b = min(max(cu[s + 1], 0), total);
   *first = a;
   return max(b - a, 0);
 }
-// The same for a wave's one sequence, in scalar registers.
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int span1(const int *cu, int s, int total, int *first) {
-  const int n = scalar(span(cu, s, total, first));
-  *first = scalar(*first);
-  return n;
-}
-template <int BM> __device__ __forceinline__ Item find_item(const int *cu, int n_seq, int total, int it) {
+// Long tiles first: the sequences' last tiles, then those before, all that have as
+// many keys behind each other (up to 64 sequences; past them sequence by sequence
+// from the last).  In the sequences' own order a long one's last tiles may start when the
+// others are done.
+template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a, int it) {
   const int lane = threadIdx.x & 63;
-  for (int s0 = 0; s0 < n_seq; s0 += 64) {
-    int first, v = s0 + lane < n_seq ? (span(cu, s0 + lane, total, &first) + BM - 1) / BM : 0, inc = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int u = __shfl_up(inc, d);
-      if (lane >= d) inc += u;
+  int q0 = 0, nq = 0, k0 = 0, nk = 0;
+  auto load = [&](int s) {
+    nq = nk = 0;
+    if (s >= a.n_seq) return;
+    nq = span(a.cu_q, s, a.total_q, &q0);
+    nk = span(a.cu_k, s, a.total_k, &k0);
+  };
+  auto item = [&](int s0, int w, int tile) {
+    return Item{scalar(s0 + w), scalar(tile), lane_of(q0, w), lane_of(nq, w), lane_of(k0, w), lane_of(nk, w)};
+  };
+  load(lane);
+  int tiles = (nq + BM - 1) / BM;
+  if (a.n_seq <= 64) {
+    // The level: the largest tile index i such that more than `it` tiles have an index >= i.
+    if (lane_of(scan64(tiles), 63) <= it) return {-1};
+    int lo = 0, hi = lane_of(max64(tiles), 0);            // tiles of an index >= hi: none
+    while (lo + 1 < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (lane_of(scan64(max(tiles - mid, 0)), 63) > it) lo = mid;
+      else hi = mid;
     }
+    it -= lane_of(scan64(max(tiles - lo - 1, 0)), 63);     // which of the level's sequences
+    const unsigned long long have = __ballot(tiles > lo);
+    const int rank = __builtin_popcountll(have & ((1ull << lane) - 1));
+    return item(0, __builtin_ctzll(__ballot(tiles > lo && rank == it)), lo);
+  }
+  // From the last sequence's last tile on: the total first.
+  int all = lane_of(scan64(tiles), 63);
+  for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
+    load(s0 + lane);
+    all += lane_of(scan64((nq + BM - 1) / BM), 63);
+  }
+  it = all - 1 - it;
+  if (it < 0) return {-1};
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    load(s0 + lane);
+    tiles = (nq + BM - 1) / BM;
+    const int inc = scan64(tiles);
     const unsigned long long past = __ballot(inc > it);
     if (past) {
       const int w = __builtin_ctzll(past);
-      return {s0 + w, it - __builtin_amdgcn_readlane(inc - v, w)};
+      return item(s0, w, it - lane_of(inc - tiles, w));
     }
-    it -= __builtin_amdgcn_readlane(inc, 63);
+    it -= lane_of(inc, 63);
   }
-  return {-1, 0};
+  return {-1};
 }
 
 // NW waves of 32 QB queries of one head share double-buffered tiles of BN keys.
@@ -100,20 +149,10 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
   const int g = a.nh / a.nkv;
   // Blocks of one kv head go to one or two XCDs (block b runs on XCD b % 8), long rows first.
   const int hh = blockIdx.x % a.nh, h = (hh % a.nkv) * g + hh / a.nkv, hkv = hh % a.nkv;
-  const int items = gridDim.x / a.nh;
-  const Item item = find_item<BM>(a.cu_q, a.n_seq, a.total_q, items - 1 - (int)(blockIdx.x / a.nh));
+  const Item item = find_item<BM>(a, blockIdx.x / a.nh);
   if (item.seq < 0) return;
-  int q0, k0;
-  const int nq = span1(a.cu_q, item.seq, a.total_q, &q0), nk = span1(a.cu_k, item.seq, a.total_k, &k0), off = nk - nq;
-  const int first = item.tile * BM, w0 = first + wave * WM;      // the workgroup's and this wave's first query
-  AttnWave<T, D, BN, QB> w;
-  int limit[QB];                                                 // the last key of this lane's queries
-#pragma unroll
-  for (int y = 0; y < QB; ++y) {
-    const int row = w0 + 32 * y + n;
-    limit[y] = row < nq ? row + off : -1;
-    w.start(y, row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
-  }
+  const int tile = item.tile, q0 = item.q0, nq = item.nq, k0 = item.k0, nk = item.nk, off = nk - nq;
+  const int first = tile * BM, w0 = first + wave * WM;      // the workgroup's and this wave's first query
   const elem *kp = (const elem *)a.k + (long long)k0 * a.ks + hkv * D, *vp = (const elem *)a.v + (long long)k0 * a.vs + hkv * D;
   const int kend = min(min(first + BM, nq) + off, nk);           // keys that the workgroup's rows see
   const int wend = min(min(w0 + WM, nq) + off, nk);              // and this wave's
@@ -131,6 +170,14 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
   // its keys compared with each row's last.
   const int full = max(min(first + off + 1, nk), 0) / (2 * BN) * (2 * BN);
   if (kend > 0) land(K0, V0, 0);
+  AttnWave<T, D, BN, QB> w;
+  int limit[QB];                                                 // the last key of this lane's queries
+#pragma unroll
+  for (int y = 0; y < QB; ++y) {
+    const int row = w0 + 32 * y + n;
+    limit[y] = row < nq ? row + off : -1;
+    w.start(y, row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
+  }
   int t0 = 0;
   for (; t0 < full; t0 += 2 * BN) {
     ready();
@@ -214,19 +261,6 @@ struct TreeTile {
   int units;                // its length
   int at;                   // where it begins on the line
 };
-// Inclusive sum over the wave's lanes (row shifts, then row broadcasts).
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
-}
-__device__ __forceinline__ int scan64(int v) {
-  v = dpp_add<0x111, 0xF>(v);
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);
-  return dpp_add<0x143, 0xC>(v);
-}
-__device__ __forceinline__ int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 // Where every group has the same number of row tiles (`levels`, more than one of
 // them for many rows), each level has a line of its own, as long as the groups'
 // keys, cut alike: the workgroups that read the same keys for different rows then
@@ -861,15 +895,24 @@ template <typename F> int by_type(int type, int D, F f) {
 }  // namespace
 
 int attn_prompt_launch(const cwen_ctx *, int type, int D, const PromptArgs &a, hipStream_t st) {
-  const int BM = D == 256 ? 128 : 256;
+  // Sequences of 4096 tokens and more on average: workgroups of 8 waves read K and V half as often as
+  // those of 4, which leave fewer waves idle in short sequences and more workgroups to a CU (heads of 128,
+  // 32/8: one prompt of 32768 7.57 ms against 7.90, of 8192 0.52 and 0.56; of 2048 62 us against 54; 9 of
+  // 700..3800 446 us against 441).  Heads of 64 gain nothing from 8 (32768: 4.9 ms against 4.7).
+  const bool wide = D != 64 && a.total_q >= 4096ll * a.n_seq;
+  const int BM = wide ? 256 : 128;
   const long long items = (a.total_q + BM - 1) / BM + a.n_seq;
   if (items * a.nh > INT32_MAX) return CWEN_EINVAL;
   return by_type(type, D, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value;
     const dim3 grid((unsigned)(items * a.nh));
-    if constexpr (dim == 256) hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, 1, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((prompt_kernel<T, dim, 8, 64, 1, 2>), grid, dim3(512), 0, st, a);
+    if constexpr (dim == 64) {
+      hipLaunchKernelGGL((prompt_kernel<T, 64, 4, 32, 1, 3>), grid, dim3(256), 0, st, a);
+    } else {
+      if (wide) hipLaunchKernelGGL((prompt_kernel<T, dim, 8, dim == 256 ? 32 : 64, 1, 2>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, 1, dim == 256 ? 2 : 3>), grid, dim3(256), 0, st, a);
+    }
   });
 }
 int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {

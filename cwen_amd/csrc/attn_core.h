@@ -52,8 +52,10 @@ template <> struct AttnOps<TypeBF16> {
     return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) vec4 *)(attn_lds_t *)const_cast<void *>(p));
   }
   static __device__ __forceinline__ float probe(vec8 v, float acc) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    const v2 z = {(__bf16)0.f, (__bf16)0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = fmaf((float)v[i], 0.f, acc);
+    for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2_f32_bf16((v2){v[i], v[i + 1]}, z, acc, false);
     return acc;
   }
 };
