@@ -135,10 +135,28 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(cwen_kv kv, const int *src
   }
 }
 
+// The filled rows of a shared page that a reserve replaced, in the slices l0 .. l1 - 1 (slice
+// 2 l: layer l's keys, 2 l + 1: its values), by the workgroup's N threads; a head's
+// rows are contiguous in both pages.  job: {old, new, rows, -} (old < 0: none).
+template <int N> __device__ __forceinline__ void copy_page(const cwen_kv &kv, const int *job, int l0, int l1) {
+  const int old = job[0];
+  if (old < 0) return;
+  const int pg = job[1], n16 = job[2] * kv.head_dim / 8;    // 16-byte pieces of one head
+  const int slice = n16 * kv.n_kv_head;
+  for (int x = threadIdx.x; x < slice * (l1 - l0); x += N) {
+    const int l = l0 + x / slice, y = x % slice, h = y / n16;
+    uint16_t *pool = (uint16_t *)(l & 1 ? kv.v : kv.k);
+    const size_t o = (size_t)h * kv.page * kv.head_dim + 8 * (size_t)(y - h * n16);
+    *(u32x4_t *)(pool + kv_at(l >> 1, pg, 0, 0, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim) + o) =
+        *(const u32x4_t *)(pool + kv_at(l >> 1, old, 0, 0, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim) + o);
+  }
+}
+
 // The plan of a reserve: one workgroup.  work: the free pages found, then per
 // request the copy to make, {old, new, rows, -} (old < 0: none).
+// With `copy` it makes the copies too (few and small ones: a launch saved).
 constexpr int RES = 1024;
-__global__ __launch_bounds__(RES) void kv_reserve_kernel(cwen_kv kv, const int *seqs, const int *grow, int n) {
+__global__ __launch_bounds__(RES) void kv_reserve_kernel(cwen_kv kv, const int *seqs, const int *grow, int n, int copy) {
   __shared__ int s_first[CWEN_KV_REQ_MAX + 1];     // pages taken by the requests before
   __shared__ int s_last[CWEN_KV_REQ_MAX];          // the shared page that a request would write to, or -1
   __shared__ uint32_t s_seen[65536 / 32];
@@ -251,23 +269,12 @@ __global__ __launch_bounds__(RES) void kv_reserve_kernel(cwen_kv kv, const int *
   }
   __syncthreads();
   for (int i = tid; i < n; i += RES) kv.held[seqs[i]] += s_first[i + 1] - s_first[i] - (jobs[4 * i] >= 0);
+  if (copy)
+    for (int i = 0; i < n; ++i) copy_page<RES>(kv, jobs + 4 * i, 0, 2 * kv.n_layers);
 }
-
-// The filled rows of the shared pages that a reserve replaced.  Grid (requests,
-// layers, k and v); a head's rows are contiguous in both pages.
+// Grid (requests, slices).
 __global__ __launch_bounds__(256) void kv_copy_kernel(cwen_kv kv) {
-  const int *job = kv.work + ((kv.n_pages + 3) & ~3) + 4 * blockIdx.x;
-  const int old = job[0];
-  if (old < 0) return;
-  const int pg = job[1], n16 = job[2] * kv.head_dim / 8;    // 16-byte pieces of one head
-  uint16_t *pool = (uint16_t *)(blockIdx.z ? kv.v : kv.k);
-  const uint16_t *a = pool + kv_at(blockIdx.y, old, 0, 0, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim);
-  uint16_t *b = pool + kv_at(blockIdx.y, pg, 0, 0, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim);
-  for (int h = 0; h < kv.n_kv_head; ++h)
-    for (int i = threadIdx.x; i < n16; i += 256) {
-      const size_t o = (size_t)h * kv.page * kv.head_dim + 8 * (size_t)i;
-      *(u32x4_t *)(b + o) = *(const u32x4_t *)(a + o);
-    }
+  copy_page<256>(kv, kv.work + ((kv.n_pages + 3) & ~3) + 4 * blockIdx.x, blockIdx.y, blockIdx.y + 1);
 }
 
 // Whether request i of a keep can be met (workgroup-uniform).  len and held
@@ -296,51 +303,71 @@ __device__ __forceinline__ bool keep_ok(const cwen_kv &kv, const int *seqs, cons
   return !__syncthreads_or(bad);
 }
 
-// The rows of an accepted branch.  Grid (requests, layers, k and v).  A thread
-// owns 16 bytes of the row (all heads side by side) and takes the branch's rows in
-// order, KEEP at a time: a destination never lies behind a later source, so
-// nothing is overwritten before it is read, and no thread depends on another.
+// The rows of an accepted branch, layers l0 .. l1 - 1.  Those that stay where they
+// are come first (the path increases), and only the others are touched: 256 of them
+// at a time have their places worked out in LDS, then a thread owns 16 bytes of the row (k
+// and v, all heads side by side) and takes the rows in order, KEEP at a time.  A
+// destination never lies behind a later source, so nothing is overwritten before
+// it is read, and no thread depends on another.  With every place looked up by
+// every thread, and every row moved, 64 branches of 32 rows in 16 layers took 44 us.
 constexpr int KEEP = 8;
+__device__ __forceinline__ void keep_rows(const cwen_kv &kv, int s, int len, int c, const int *row, int l0, int l1) {
+  __shared__ long long s_src[256], s_dst[256];
+  const int *tab = kv.table + (size_t)s * kv.max_pages;
+  const int tid = threadIdx.x, per = kv.head_dim / 8, pieces = per * kv.n_kv_head;
+  int first = 0;
+  for (int j0 = 0; j0 < c; j0 += 256) first += __syncthreads_count(j0 + tid < c && row[j0 + tid] == j0 + tid);
+  auto at = [&](int pos) {
+    bool bad = false;
+    const int pg = kv_page_ok(tab[pos / kv.page], kv.n_pages, &bad);
+    return kv_at(0, pg, 0, pos % kv.page, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim);
+  };
+  const long long layer = (long long)kv.n_pages * kv.n_kv_head * kv.page * kv.head_dim;
+  for (int j0 = first; j0 < c; j0 += 256) {
+    const int n = min(256, c - j0);
+    if (tid < n) {
+      s_src[tid] = at(len + row[j0 + tid]);
+      s_dst[tid] = at(len + j0 + tid);
+    }
+    __syncthreads();
+    for (int x = tid; x < 2 * pieces * (l1 - l0); x += 256) {
+      const int l = l0 + x / (2 * pieces), y = x % (2 * pieces), v = y >= pieces, z = y - v * pieces, h = z / per;
+      uint16_t *pool = (uint16_t *)(v ? kv.v : kv.k) + l * layer + (long long)h * kv.page * kv.head_dim + 8 * (z - h * per);
+      for (int u0 = 0; u0 < n; u0 += KEEP) {
+        u32x4_t val[KEEP];
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) val[u] = *(const u32x4_t *)(pool + s_src[min(u0 + u, n - 1)]);
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u)
+          if (u0 + u < n) *(u32x4_t *)(pool + s_dst[u0 + u]) = val[u];
+      }
+    }
+    __syncthreads();
+  }
+}
+// Grid (requests, layers).
 __global__ __launch_bounds__(256) void kv_keep_kernel(cwen_kv kv, const int *seqs, const int *count, const int *path, int ps,
                                                       int n) {
   const int i = blockIdx.x;
   int len, held;
   if (!keep_ok<256>(kv, seqs, count, path, ps, i, n, &len, &held)) return;   // kv_keep_end_kernel raises the flag
-  const int c = count[i], *row = path + (size_t)i * ps;
-  const int *tab = kv.table + (size_t)seqs[i] * kv.max_pages;
-  uint16_t *pool = (uint16_t *)(blockIdx.z ? kv.v : kv.k);
-  const int per = kv.head_dim / 8;                 // 16-byte pieces of one head's row
-  auto at = [&](int pos, int h, int d) {
-    bool bad = false;
-    const int pg = kv_page_ok(tab[pos / kv.page], kv.n_pages, &bad);
-    return kv_at(blockIdx.y, pg, h, pos % kv.page, kv.n_pages, kv.n_kv_head, kv.page, kv.head_dim) + 8 * d;
-  };
-  for (int x = threadIdx.x; x < per * kv.n_kv_head; x += 256) {
-    const int h = x / per, d = x - h * per;
-    for (int j0 = 0; j0 < c; j0 += KEEP) {
-      u32x4_t v[KEEP];
-#pragma unroll
-      for (int u = 0; u < KEEP; ++u)
-        if (j0 + u < c) v[u] = *(const u32x4_t *)(pool + at(len + row[j0 + u], h, d));
-#pragma unroll
-      for (int u = 0; u < KEEP; ++u)
-        if (j0 + u < c) *(u32x4_t *)(pool + at(len + j0 + u, h, d)) = v[u];
-    }
-  }
+  keep_rows(kv, seqs[i], len, count[i], path + (size_t)i * ps, blockIdx.y, blockIdx.y + 1);
 }
-// The new lengths, and the pages behind them given back.
+// The new lengths, and the pages behind them given back; with `rows` (few layers
+// and requests: a launch saved) the rows first.  Grid: requests.
 __global__ __launch_bounds__(256) void kv_keep_end_kernel(cwen_kv kv, const int *seqs, const int *count, const int *path,
-                                                          int ps, int n) {
+                                                          int ps, int n, int rows) {
   const int i = blockIdx.x;
   int len, held;
   if (!keep_ok<256>(kv, seqs, count, path, ps, i, n, &len, &held)) {
     if (threadIdx.x == 0) kv_raise(kv, CWEN_KV_ARG);
     return;
   }
-  const int s = seqs[i], pages = kv_cover(len + count[i], kv.page);
+  const int s = seqs[i], c = count[i], pages = kv_cover(len + c, kv.page);
+  if (rows) keep_rows(kv, s, len, c, path + (size_t)i * ps, 0, kv.n_layers);
   release_from<256>(kv, s, pages, held);
   if (threadIdx.x == 0) {
-    kv.len[s] = len + count[i];
+    kv.len[s] = len + c;
     kv.held[s] = pages;
   }
 }
@@ -357,10 +384,16 @@ int kv_take_status_launch(const cwen_kv &kv, int *out, hipStream_t st) {
   CWEN_HIP_TRY(hipGetLastError());
   return CWEN_OK;
 }
+// Whether one workgroup per request moves a request's rows of every layer in about the time of a launch.
+static bool few_rows(const cwen_kv &kv, int n_req, int rows) {
+  return (long long)n_req * kv.n_layers * rows * kv.n_kv_head * kv.head_dim <= 1 << 17;
+}
 int kv_reserve_launch(const cwen_kv &kv, const int *seqs, const int *n, int n_req, hipStream_t st) {
-  hipLaunchKernelGGL(kv_reserve_kernel, dim3(1), dim3(RES), 0, st, kv, seqs, n, n_req);
+  const bool few = few_rows(kv, n_req, kv.page);
+  hipLaunchKernelGGL(kv_reserve_kernel, dim3(1), dim3(RES), 0, st, kv, seqs, n, n_req, (int)few);
   CWEN_HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(kv_copy_kernel, dim3(n_req, kv.n_layers, 2), dim3(256), 0, st, kv);
+  if (few) return CWEN_OK;
+  hipLaunchKernelGGL(kv_copy_kernel, dim3(n_req, 2 * kv.n_layers), dim3(256), 0, st, kv);
   CWEN_HIP_TRY(hipGetLastError());
   return CWEN_OK;
 }
@@ -371,11 +404,12 @@ int kv_fork_launch(const cwen_kv &kv, const int *src, const int *dst, int n_req,
 }
 int kv_keep_launch(const cwen_kv &kv, const int *seqs, const int *count, const int *path, int ps, int n_req,
                    hipStream_t st) {
-  if (path) {
-    hipLaunchKernelGGL(kv_keep_kernel, dim3(n_req, kv.n_layers, 2), dim3(256), 0, st, kv, seqs, count, path, ps, n_req);
+  const bool few = path && few_rows(kv, 1, ps);
+  if (path && !few) {
+    hipLaunchKernelGGL(kv_keep_kernel, dim3(n_req, kv.n_layers), dim3(256), 0, st, kv, seqs, count, path, ps, n_req);
     CWEN_HIP_TRY(hipGetLastError());
   }
-  hipLaunchKernelGGL(kv_keep_end_kernel, dim3(n_req), dim3(256), 0, st, kv, seqs, count, path, ps, n_req);
+  hipLaunchKernelGGL(kv_keep_end_kernel, dim3(n_req), dim3(256), 0, st, kv, seqs, count, path, ps, n_req, (int)few);
   CWEN_HIP_TRY(hipGetLastError());
   return CWEN_OK;
 }

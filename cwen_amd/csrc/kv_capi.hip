@@ -33,7 +33,7 @@ struct OnDevice {
 int check_kv(const cwen_kv *kv) {
   if (!kv) return CWEN_EINVAL;
   if (kv->type != CWEN_T_F16 && kv->type != CWEN_T_BF16) return CWEN_ETYPE;
-  if (kv->n_layers < 1 || kv->n_layers > 65535 || kv->n_kv_head < 1 || kv->n_kv_head > 65535) return CWEN_EINVAL;
+  if (kv->n_layers < 1 || kv->n_layers > 32767 || kv->n_kv_head < 1 || kv->n_kv_head > 65535) return CWEN_EINVAL;
   if (kv->head_dim < 8 || kv->head_dim > 512 || kv->head_dim % 8) return CWEN_EINVAL;
   if (kv->page < 16 || kv->page > 256 || (kv->page & (kv->page - 1))) return CWEN_EINVAL;
   if (kv->n_pages < 1 || kv->n_pages > (1 << 24) || kv->max_seqs < 1 || kv->max_seqs > 65536) return CWEN_EINVAL;
