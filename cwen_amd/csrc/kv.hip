@@ -295,7 +295,9 @@ __device__ __forceinline__ bool keep_ok(const cwen_kv &kv, const int *seqs, cons
       bad |= r <= before || !kv_fits(*len, r, kv.page, *held) || *len + r >= *held * kv.page;
       if (!bad && r != j) {                         // a row that moves: into pages held alone
         bool bp = false;
-        const int pg = kv_page_ok(kv.table[(size_t)s * kv.max_pages + (*len + j) / kv.page], kv.n_pages, &bp);
+        const int *tab = kv.table + (size_t)s * kv.max_pages;
+        const int pg = kv_page_ok(tab[(*len + j) / kv.page], kv.n_pages, &bp);
+        kv_page_ok(tab[(*len + r) / kv.page], kv.n_pages, &bp);
         bad |= bp || kv.ref[pg] != 1;
       }
     }

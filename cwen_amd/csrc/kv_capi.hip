@@ -38,6 +38,7 @@ int check_kv(const cwen_kv *kv) {
   if (kv->page < 16 || kv->page > 256 || (kv->page & (kv->page - 1))) return CWEN_EINVAL;
   if (kv->n_pages < 1 || kv->n_pages > (1 << 24) || kv->max_seqs < 1 || kv->max_seqs > 65536) return CWEN_EINVAL;
   if (kv->max_pages < 1 || (long long)kv->max_pages * kv->page >= 1ll << 30) return CWEN_EINVAL;
+  if ((long long)kv->max_pages * kv->max_seqs > INT32_MAX) return CWEN_EINVAL;
   if (!kv->k || !kv->v || !aligned16(kv->k) || !aligned16(kv->v)) return CWEN_EINVAL;
   if (!kv->table || !kv->len || !kv->held || !kv->ref || !kv->work || !kv->status) return CWEN_EINVAL;
   if (!aligned16(kv->ref) || !aligned4(kv->table) || !aligned4(kv->len) || !aligned4(kv->held) || !aligned4(kv->work) ||
@@ -61,6 +62,16 @@ bool ok_rows(const void *p, long long ts, long long row) {
 bool overlap(const void *a, long long abytes, const void *b, long long bbytes) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return x < y + (uintptr_t)bbytes && y < x + (uintptr_t)abytes;
+}
+
+// Whether rows of xr bytes at x keep clear of T rows of yr bytes at y: no common memory at all,
+// or (`inside`) rows of the same stride that lie side by side, as the parts of one product do.
+bool clear_of(const void *x, long long x_ts, long long xr, const void *y, long long y_ts, long long yr, int T, bool inside) {
+  if (!overlap(x, (T - 1) * x_ts + xr, y, (T - 1) * y_ts + yr)) return true;
+  if (!inside || T == 1 || x_ts != y_ts) return false;
+  long long off = (long long)((intptr_t)x - (intptr_t)y) % y_ts;
+  if (off < 0) off += y_ts;
+  return off >= yr && off + xr <= y_ts;
 }
 
 }  // namespace
@@ -115,7 +126,7 @@ int cwen_rope_free(cwen_rope *r) {
 
 int cwen_rope_apply(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *x, long long x_ts, long long x_hs, int ytype,
                     void *y, long long y_ts, long long y_hs, const int *pos, int T, int n_head, int inverse, void *stream) {
-  if (!ctx || !r || T < 0 || n_head < 1 || n_head > 65535) return CWEN_EINVAL;
+  if (!ctx || !r || T < 0 || T >= 1 << 24 || n_head < 1 || n_head > 65535) return CWEN_EINVAL;
   const int xe = elem_size(xtype), ye = elem_size(ytype);
   if (!xe || !ye) return CWEN_ETYPE;
   if (T == 0) return CWEN_OK;
@@ -141,7 +152,7 @@ int cwen_rope_apply(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *x,
 int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, long long q_ts, const void *k, long long k_ts,
                  const void *v, long long v_ts, void *qo, long long qo_ts, const cwen_kv *kv, int layer, const int *seq,
                  const int *slot, const int *pos, int T, int n_head, void *stream) {
-  if (!ctx || !r || T < 0 || n_head < 1 || n_head > 65535) return CWEN_EINVAL;
+  if (!ctx || !r || T < 0 || T >= 1 << 24 || n_head < 1 || n_head > 65535) return CWEN_EINVAL;
   const int rc = check_kv(kv);
   if (rc) return rc;
   const int xe = elem_size(xtype);
@@ -156,8 +167,8 @@ int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, lo
   const bool same = q == qo && xtype == kv->type && (T == 1 || q_ts == qo_ts);
   const long long qo_bytes = ((T - 1) * qo_ts + qr) * 2;
   if (!same && overlap(q, ((T - 1) * q_ts + qr) * xe, qo, qo_bytes)) return CWEN_EINVAL;
-  if (overlap(k, ((T - 1) * k_ts + kr) * xe, qo, qo_bytes) && !(k_ts == qo_ts && same)) return CWEN_EINVAL;
-  if (overlap(v, ((T - 1) * v_ts + kr) * xe, qo, qo_bytes) && !(v_ts == qo_ts && same)) return CWEN_EINVAL;
+  if (!clear_of(k, k_ts * xe, kr * xe, qo, qo_ts * 2, qr * 2, T, same)) return CWEN_EINVAL;
+  if (!clear_of(v, v_ts * xe, kr * xe, qo, qo_ts * 2, qr * 2, T, same)) return CWEN_EINVAL;
   OnDevice dev(ctx->device);
   if (dev.rc) return dev.rc;
   RopeParams p = {};

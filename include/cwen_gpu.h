@@ -251,7 +251,7 @@ int cwen_rope_free(cwen_rope *r);
  * Element (t, h, d) is at t * x_ts + h * x_hs + d.  With `inverse` the angles
  * are negated: the gradient of the turn (for m = 1 its inverse).  y may be x
  * itself (same type and strides), and must not overlap it otherwise.  x and y
- * are 16-byte aligned and all strides multiples of 8; T may be 0. */
+ * are 16-byte aligned and all strides multiples of 8; 0 <= T < 2^24. */
 int cwen_rope_apply(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *x, long long x_ts, long long x_hs,
                     int ytype, void *y, long long y_ts, long long y_hs, const int *pos, int T, int n_head,
                     int inverse, void *stream);
@@ -277,7 +277,8 @@ typedef struct {
   int page;                /* positions of a page: 16, 32, 64, 128 or 256          */
   int n_pages;             /* 1..2^24                                              */
   int max_seqs;            /* 1..65536                                             */
-  int max_pages;           /* pages of one sequence at most; max_pages * page < 2^30 */
+  int max_pages;           /* pages of one sequence at most; max_pages * page < 2^30,
+                              max_pages * max_seqs < 2^31                      */
   void *k, *v;             /* 16-byte aligned                                      */
   int *table;              /* [max_seqs][max_pages]                                */
   int *len, *held;         /* [max_seqs]                                           */
@@ -327,9 +328,11 @@ int cwen_kv_status(cwen_ctx *ctx, const cwen_kv *kv, int *bits, void *stream);
  * slot[t] of the sequence in `layer`, rounded to the cache's type once.  The
  * position must be in a page that the sequence holds alone (cwen_kv_reserve);
  * otherwise, and for an id out of range, nothing is written and CWEN_KV_ARG
- * raised.  A token of slot < 0 is padding: its k and v are not written.
- * Pointers 16-byte aligned, strides multiples of 8; qo must not overlap q,
- * unless it is q itself in type and stride. */
+ * raised.  A token of slot < 0 is padding: its k and v are not written.  No
+ * two tokens of a call may name one position (which of them stays would be
+ * open).  Pointers 16-byte aligned, strides multiples of 8, T < 2^24; qo must
+ * not overlap the inputs, unless it is q itself in type and stride (then k and
+ * v may lie beside q in the rows of one product). */
 int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, long long q_ts, const void *k,
                  long long k_ts, const void *v, long long v_ts, void *qo, long long qo_ts, const cwen_kv *kv, int layer,
                  const int *seq, const int *slot, const int *pos, int T, int n_head, void *stream);
@@ -365,8 +368,11 @@ int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, con
  * positions and the nodes j of its group whose bit j is set in its row of
  * mask (device, [total][mw] words of 64 bits; bits past the group are
  * ignored).  mask NULL: a chain, j <= i; one node alone is a decode step.
- * Works on the context's scratch.  max_len: the expected longest context; it
- * guides the launch and may be wrong. */
+ * Works on the context's scratch and counters: calls on one context must not
+ * overlap, nor replays of graphs that captured them.  max_len: the expected
+ * longest context; it guides the launch and may be wrong.  CWEN_EINVAL also
+ * when (n_seq + 64) * (row tiles of max_nodes * heads per KV head) * (tiles of
+ * max_pages * page positions) passes 2^31. */
 #define CWEN_TREE_MAX 256
 int cwen_attn_tree(cwen_ctx *ctx, const cwen_kv *kv, int layer, const void *q, long long q_ts, void *o, long long o_ts,
                    float *lse, const int *seqs, const int *cu, const unsigned long long *mask, int mw, int n_seq,

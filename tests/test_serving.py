@@ -102,6 +102,22 @@ def test_rope_call_refusals():
         assert fused(**bad) == EINVAL, bad
 
 
+def test_rope_kv_in_place_refusals():
+    """q in place: k and v beside it in the rows of one product, never under its heads."""
+    L, r = gpu.lib(), gpu.Rope(128, 64)
+
+    def call(k, v, qs=512 + 1024, T=2, xt=gpu.T_F16, ks=None):
+        return L.cwen_rope_kv(CTX, r.h, xt, P, qs, k, ks or qs, v, qs, P, qs, kv(), 0, P, P, P, T, 4, None)
+    for k, v in ((P + 1024 - 16, P + 2048), (P + 1024, P + 2048 + 16), (P + 512, P + 2048), (P + 1024, P), (P + 1024, P + 3072 - 16),
+                 (P + 3072 + 512, P + 2048), (P - 16, P + 2048)):
+        assert call(k, v) == EINVAL, (k - P, v - P)
+    assert call(P + 1024, P + 2048, ks=1024) == EINVAL
+    assert call(P + 1024 - 16, P + 2048, T=1) == EINVAL
+    assert call(P + 1024, P + 2048, T=1 << 24) == EINVAL
+    assert L.cwen_rope_apply(CTX, r.h, gpu.T_F16, P, 512, 128, gpu.T_F16, P, 512, 128, P, 1 << 24, 4, 0, None) == EINVAL
+    assert L.cwen_kv_reset(CTX, kv(max_seqs=65536, max_pages=32768), None) == EINVAL      # 2^31 table entries
+
+
 def test_attention_refusals():
     L = gpu.lib()
 

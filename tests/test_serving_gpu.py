@@ -338,6 +338,37 @@ def test_shared_last_page_is_copied_for_all_but_its_last_holder(env):
         assert all(torch.equal(a, b) for a, b in zip(gather(kv, s, 37), want))
 
 
+def test_keep_long_paths(env):
+    """Paths of more rows than one sweep of the kernel holds, over many pages and layers, beside a
+    short one and one that stays; an entry that is no page refuses its request."""
+    gpu, ctx = env
+    g = gen(33)
+    kv = gpu.PagedKV.empty(3, 2, 72, 32, 150, 6, 60, BF16)
+    kv.k.copy_(randn(g, *kv.k.shape)), kv.v.copy_(randn(g, *kv.v.shape))
+    kv.reserve(ctx, ints([0, 1, 2]), ints([100, 40, 7]))
+    kv.keep(ctx, ints([0, 1, 2]), ints([100, 40, 7]))
+    kv.reserve(ctx, ints([0, 1, 2]), ints([1700, 1000, 90]))
+    rng = random.Random(1)
+    paths = [sorted(rng.sample(range(1700), 900)), list(range(300)) + sorted(rng.sample(range(300, 1000), 333)), list(range(64))]
+    want = []
+    for s, (n, row) in enumerate(zip((100, 40, 7), paths)):
+        a = gather(kv, s, int(kv.held[s]) * 32)
+        at = torch.tensor(list(range(n)) + [n + r for r in row], device="cuda")
+        want.append([x[:, at] for x in a])
+    table = [p + [-1] * (900 - len(p)) for p in paths]
+    kv.keep(ctx, ints([0, 1, 2]), ints([len(p) for p in paths]), ints(table))
+    assert kv.len.tolist()[:3] == [1000, 673, 71] and kv.take_status(ctx) == 0
+    for s in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(gather(kv, s, int(kv.len[s])), want[s])), s
+    assert int((kv.ref > 0).sum()) == sum(-(-n // 32) for n in (1000, 673, 71))
+    kv.reserve(ctx, ints([2, 1]), ints([90, 5]))
+    kv.table[2, 4] = 150
+    before = [t.clone() for t in (kv.k, kv.v)]
+    kv.keep(ctx, ints([2, 1]), ints([1, 2]), ints([[80, 0], [0, 1]]))
+    assert kv.take_status(ctx) & gpu.KV_ARG and kv.len.tolist()[:3] == [1000, 675, 71]
+    assert torch.equal(before[0], kv.k) and torch.equal(before[1], kv.v)
+
+
 # ---------------------------------------------------------------- projections into the cache
 @pytest.mark.parametrize("src,typ,page,layout", [(F32, F16, 16, "pairs"), (BF16, BF16, 64, "halves"), (F16, F16, 256, "halves"),
                                                  (F32, BF16, 32, "pairs")])
@@ -374,6 +405,28 @@ def test_rope_kv(env, src, typ, page, layout):
             assert torch.equal(kv.v[1, pg, :, row], v[t].to(typ)), ("v", t)
             kv.k[1, pg, :, row], kv.v[1, pg, :, row] = k0[1, pg, :, row], v0[1, pg, :, row]
     assert torch.equal(kv.k, k0) and torch.equal(kv.v, v0)      # and nothing else
+
+
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+def test_rope_kv_in_place(env, layout):
+    """q turned where it lies, k and v beside it in the same rows: what two tensors give."""
+    gpu, ctx = env
+    g, D, H, K, T = gen(23), 64, 5, 2, 301
+    r = gpu.Rope(head_dim=D, n_rot=48, theta=1e4, layout=layout)
+    kv = gpu.PagedKV.empty(1, K, D, 16, 20, 1, 20, BF16)
+    kv.reserve(ctx, ints([0]), ints([T]))
+    wide = randn(g, T, (H + 2 * K) * D + 8, dtype=BF16)
+    q, k, v = (wide[:, a * D:b * D].unflatten(1, (-1, D)) for a, b in ((0, H), (H, H + K), (H + K, H + 2 * K)))
+    at, before, qo = ints(list(range(T))), wide.clone(), torch.empty(T, H, D, device="cuda", dtype=BF16)
+    gpu.rope_kv(ctx, r, q, k, v, qo, kv, 0, at * 0, at, at)
+    want = [kv.k.clone(), kv.v.clone()]
+    kv.k.fill_(1), kv.v.fill_(1)
+    gpu.rope_kv(ctx, r, q, k, v, q, kv, 0, at * 0, at, at)
+    used = kv.table[0, :-(-T // 16)].long()
+    for pool, w in zip((kv.k, kv.v), want):
+        a, b = (x[0, used].transpose(1, 2).reshape(-1, K, D)[:T] for x in (pool, w))
+        assert torch.equal(a, b)
+    assert torch.equal(q, qo) and torch.equal(wide[:, H * D:], before[:, H * D:]) and kv.take_status(ctx) == 0
 
 
 # ---------------------------------------------------------------- prompt attention
@@ -454,6 +507,38 @@ def test_prompt_hidden_values_have_no_influence(env, typ, D):
         k[-3:], v[-3:] = float("nan"), float("inf")             # the gap behind the last sequence
         v[200, 1] = float("nan")
     check_prompt(prompt_case(gpu, ctx, gen(8), typ, 4, 2, D, [60, 140, 40, 1], gap=3, nan=spoil), typ)
+
+
+def test_prompt_many_sequences(env):
+    """The search for a workgroup's tile: 64 sequences, 65, 200; long ones between short and empty ones."""
+    gpu, ctx = env
+    rng = random.Random(9)
+    for S, D in ((64, 64), (65, 128), (200, 64)):
+        lens = [rng.choice([0, 1, rng.randint(1, 60), rng.randint(1, 200)]) for _ in range(S)]
+        lens[3], lens[S - 2] = 700, 333
+        check_prompt(prompt_case(gpu, ctx, gen(S), F16, 2, 1, D, lens, gap=2), F16, heads=[0])
+    lk = [n + rng.randint(0, 90) for n in lens]
+    check_prompt(prompt_case(gpu, ctx, gen(2), BF16, 2, 1, 64, lens, lk), BF16, heads=[1])
+
+
+def test_prompt_wide_workgroups(env):
+    """Sequences of 4096 tokens and more take workgroups of 8 waves."""
+    gpu, ctx = env
+    check_prompt(prompt_case(gpu, ctx, gen(1), BF16, 2, 1, 128, [4500]), BF16, heads=[1])
+    check_prompt(prompt_case(gpu, ctx, gen(2), F16, 1, 1, 256, [4101], [4133]), F16)
+
+
+def test_prompt_offsets_past_32_bits(env):
+    """Tokens 2^26 elements apart: the last keys lie past 4 GiB."""
+    gpu, ctx = env
+    g, n, D = gen(5), 70, 64
+    big = torch.zeros(n, 1 << 25, dtype=F16, device="cuda")             # 4.4 GiB
+    q = randn(g, n, 2, D, dtype=F16)
+    big[:, :2 * D] = randn(g, n, 2 * D)
+    k, v = big[:, :D].unflatten(1, (1, D)), big[:, D:2 * D].unflatten(1, (1, D))
+    o, z = torch.empty_like(q), torch.empty(n, 2, device="cuda")
+    gpu.attn_prompt(ctx, q, k, v, o, ints([0, 3, n]), lse=z)
+    check_prompt((q, k, v, o, z, [3, n - 3], [3, n - 3]), F16)
 
 
 def test_prompt_many_heads_sampled(env):
@@ -573,6 +658,62 @@ def test_tree_long_context(env):
         check_tree(kv, 0, q, o, z, lens, nodes, bits, typ)
 
 
+@pytest.mark.parametrize("D,typ,per,nodes", [(64, F16, 2, 1), (128, BF16, 4, 3), (256, F16, 1, 2), (64, BF16, 8, 9), (128, F16, 5, 20)])
+def test_tree_many_groups(env, D, typ, per, nodes):
+    """More groups than a wave has lanes, contexts from 0 to 900, groups without nodes; joined in the
+    launch and by one of its own."""
+    gpu, ctx = env
+    for S in (17, 40, 130):
+        rng = random.Random(S + D)
+        lens = [rng.choice([0, 1, rng.randint(1, 100), rng.randint(1, 900)]) for _ in range(S)]
+        n = [rng.choice([0, 1, rng.randint(1, nodes), nodes]) for _ in range(S)]
+        g = gen(S)
+        kv = tree_cache(gpu, ctx, g, typ, 2, D, 16, lens, n, L=1)
+        q = randn(g, sum(n), 2 * per, D, dtype=typ)
+        bits = [b for m in n for b in random_tree(rng, m, 1)]
+        for hint in (max(lens), 100000):
+            o, z = run_tree(gpu, ctx, kv, 0, q, lens, n, bits, max_len=hint)
+            check_tree(kv, 0, q, o, z, lens, n, bits, typ, heads=[0, 2 * per - 1])
+        assert kv.take_status(ctx) == 0
+
+
+def test_tree_row_tiles_side_by_side(env):
+    """Every group with the same number of row tiles (2 and more), and groups that differ by one row."""
+    gpu, ctx = env
+    for D, H, K, lens, nodes in ((128, 16, 2, [700, 33, 1500], [40, 40, 33]), (256, 6, 1, [2100], [48]), (64, 8, 1, [900, 64], [64, 33]),
+                                 (256, 12, 2, [300, 0, 77], [43, 22, 43]), (128, 8, 1, [640, 640], [17, 16])):
+        g, rng = gen(D), random.Random(D)
+        kv = tree_cache(gpu, ctx, g, F16, K, D, 64, lens, nodes, L=1)
+        q = randn(g, sum(nodes), H, D, dtype=F16)
+        bits = [b for m in nodes for b in random_tree(rng, m, 1)]
+        o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, bits)
+        check_tree(kv, 0, q, o, z, lens, nodes, bits, F16, heads=[0, H - 1])
+
+
+def test_tree_offsets_past_32_bits(env):
+    """A cache of more than 2^31 elements: the pages used lie at its two ends."""
+    gpu, ctx = env
+    g, P = gen(7), 34000
+    kv = gpu.PagedKV(256, *(torch.zeros(1, P, 1, 256, 256, dtype=F16, device="cuda") for _ in range(2)),
+                     torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), ints([0, 0]), ints([0, 0]), torch.zeros(P, dtype=torch.int32, device="cuda"))
+    kv.ref[3:P - 3] = 1
+    kv.reserve(ctx, ints([1]), ints([1300]))
+    assert kv.table[1].tolist() == [0, 1, 2, P - 3, P - 2, P - 1, -1, -1]
+    used = kv.table[1, :6].long()
+    kv.k[:, used], kv.v[:, used] = randn(g, 1, 6, 1, 256, 256, dtype=F16), randn(g, 1, 6, 1, 256, 256, dtype=F16)
+    kv.keep(ctx, ints([1]), ints([1290]))
+    for H in (6, 40):
+        q = randn(g, 3, H, 256, dtype=F16)
+        o = torch.empty_like(q)
+        gpu.attn_tree(ctx, kv, 0, q, o, ints([1]), ints([0, 3]), 3, 1290)
+        view = gpu.PagedKV(256, kv.k, kv.v, kv.table[1:], kv.len[1:], kv.held[1:], kv.ref)
+        check_tree(view, 0, q, o, None, [1290], [3], None, F16, heads=[0, H - 1])
+    kv.fork(ctx, ints([1]), ints([0]))
+    kv.ref[5] = 0
+    kv.reserve(ctx, ints([0]), ints([4]))                      # copies the filled rows of the last page into page 5
+    assert torch.equal(kv.k[:, 5, :, :10], kv.k[:, P - 1, :, :10]) and kv.take_status(ctx) == 0
+
+
 @pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("H,K,D", [(4, 2, 64), (2, 2, 128), (20, 2, 128), (6, 1, 256)])
 def test_tree_hidden_values_have_no_influence(env, typ, H, K, D):
@@ -597,6 +738,22 @@ def test_tree_hidden_values_have_no_influence(env, typ, H, K, D):
     q = randn(g, sum(nodes), H, D, dtype=typ)
     o, z = run_tree(gpu, ctx, kv, 1, q, lens, nodes, bits)
     check_tree(kv, 1, q, o, z, lens, nodes, bits, typ)
+
+
+@pytest.mark.parametrize("H,K,D,hint", [(6, 1, 256, 2500), (4, 1, 64, 200), (40, 2, 128, 2500)])
+def test_tree_hidden_values_across_chunks(env, H, K, D, hint):
+    """A hidden node's NaN and infinities where the keys are cut into chunks (joined in the launch and
+    behind it): the other rows are those of the formula, the rows that see them are NaN or infinite."""
+    gpu, ctx = env
+    lens, nodes, g = [2500, 700], [4, 3], gen(17)
+    kv = tree_cache(gpu, ctx, g, F16, K, D, 64, lens, nodes, L=1)
+    bits = [0b1, 0b11, 0b101, 0b1101, 0b1, 0b10, 0b110]
+    for s, node, val in ((0, 1, float("nan")), (0, 3, float("inf")), (1, 0, -float("inf"))):
+        r = lens[s] + node
+        kv.v[:, int(kv.table[s, r // 64]), :, r % 64, ::5] = val
+    q = randn(g, 7, H, D, dtype=F16)
+    o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, bits, max_len=hint)
+    check_tree(kv, 0, q, o, z, lens, nodes, bits, F16, heads=[0, H - 1])
 
 
 def test_tree_nodes_past_the_bound_and_bad_state(env):
@@ -687,6 +844,64 @@ def test_repeats_are_bit_equal_and_graphs_replay(env):
         step()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out(), want))
+
+
+@pytest.mark.parametrize("nodes,H", [(1, 4), (1, 12), (9, 8)])
+def test_decode_step_in_a_graph(env, nodes, H):
+    """A captured decode step (joined in its launch or not) replayed with eager steps of other shapes
+    between: bit for bit the eager result, also as the context grows."""
+    gpu, ctx = env
+    g, lens = gen(5), [700, 90, 1100]
+    kv = tree_cache(gpu, ctx, g, F16, 2, 128, 32, [x + 40 for x in lens], [nodes] * 3, L=1)
+    q, big = randn(g, 3 * nodes, H, 128, dtype=F16), randn(g, 3 * 40, 16, 128, dtype=F16)
+    o, ob = torch.empty_like(q), torch.empty_like(big)
+    cu, cub, seqs = ints([i * nodes for i in range(4)]), ints([0, 40, 80, 120]), ints([0, 1, 2])
+    run = lambda: gpu.attn_tree(ctx, kv, 0, q, o, seqs, cu, nodes, 1100)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    run()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    for i in range(5):
+        kv.len[:3] = ints([x + 7 * i for x in lens])
+        run()
+        want = o.clone()
+        gpu.attn_tree(ctx, kv, 0, big, ob, seqs, cub, 40, 1100)
+        o.fill_(3)
+        graph.replay()
+        assert torch.equal(o, want), i
+        check_tree(kv, 0, q, o, None, [x + 7 * i for x in lens], [nodes] * 3, None, F16, heads=[0, H - 1])
+
+
+def test_two_contexts_on_two_streams(env):
+    """Calls on two contexts and caches at the same time give what they give alone."""
+    gpu, _ = env
+    jobs = []
+    for i, (typ, D, H, lens, nodes) in enumerate(((F16, 256, 6, [3000], [1]), (BF16, 128, 16, [900, 2000], [20, 12]))):
+        g, c = gen(i), gpu.Context(0)
+        kv = tree_cache(gpu, c, g, typ, 2, D, 16, lens, nodes, L=1)
+        q, pq, pk = randn(g, sum(nodes), H, D, dtype=typ), randn(g, 1500, 4, D, dtype=typ), randn(g, 1500, 2, D, dtype=typ)
+        jobs.append(dict(c=c, kv=kv, q=q, o=torch.empty_like(q), pq=pq, pk=pk, po=torch.empty_like(pq), seqs=ints(list(range(len(lens)))),
+                         cu=ints([sum(nodes[:k]) for k in range(len(nodes) + 1)]), n=max(nodes), m=max(lens), st=torch.cuda.Stream()))
+    border = ints([0, 700, 1500])
+
+    def run(j, stream=None):
+        gpu.attn_tree(j["c"], j["kv"], 0, j["q"], j["o"], j["seqs"], j["cu"], j["n"], j["m"], stream=stream)
+        gpu.attn_prompt(j["c"], j["pq"], j["pk"], j["pk"], j["po"], border, stream=stream)
+    alone = []
+    for j in jobs:
+        run(j)
+        torch.cuda.synchronize()
+        alone.append((j["o"].clone(), j["po"].clone()))
+        j["o"].fill_(0), j["po"].fill_(0)
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for j in jobs:
+            run(j, j["st"])
+    torch.cuda.synchronize()
+    for j, (o, po) in zip(jobs, alone):
+        assert torch.equal(j["o"], o) and torch.equal(j["po"], po)
 
 
 # ---------------------------------------------------------------- a request, as it is served
