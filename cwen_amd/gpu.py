@@ -520,12 +520,10 @@ class PagedKV:
         _on(ctx, self.k, seqs, count, path)
         n, ps = seqs.numel(), 0
         if path is not None:
-            if path.dim() != 2 or path.shape[0] != n:
-                raise ValueError(f"path {tuple(path.shape)}: [{n}, rows] expected")
+            if path.dim() != 2 or path.shape[0] != n or path.shape[1] == 0:
+                raise ValueError(f"path {tuple(path.shape)}: [{n}, rows] expected, rows >= 1")
             ps = path.shape[1]
             _vec("path", path, n * ps)
-            if ps == 0:                           # nothing can be named: no row moves
-                path = None
         check("cwen_kv_keep", lib().cwen_kv_keep(ctx.h, self.ref_c, _vec("seqs", seqs, None),
                                                  _vec("count", count, n), _ptr(path), ps, n, _stream_of(ctx, stream)))
 

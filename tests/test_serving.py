@@ -162,6 +162,19 @@ def test_wrapper_checks():
             f(*a)
 
 
+def test_wrapper_refuses_paths_without_rows():
+    """A path of no rows names nothing; it is not "the first rows stay"."""
+    torch = pytest.importorskip("torch")
+    pool, ints = torch.zeros(1, 4, 2, 16, 64, dtype=torch.float16), lambda *n: torch.zeros(n, dtype=torch.int32)
+    c = gpu.PagedKV(16, pool, pool.clone(), ints(2, 3), ints(2), ints(2), ints(4))
+
+    class Ctx:
+        device, h = -1, None                              # where host tensors are
+    for path in (ints(1, 0), ints(2, 3), ints(3)):
+        with pytest.raises(ValueError):
+            c.keep(Ctx, ints(1), ints(1), path, stream=0)
+
+
 # ---------------------------------------------------------------- page arithmetic on bad state
 HARNESS = r"""
 #include "kv_table.h"
