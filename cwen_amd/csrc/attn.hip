@@ -140,10 +140,10 @@ template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a,
   return {-1};
 }
 
-// NW waves of 32 QB queries of one head share double-buffered tiles of BN keys.
-template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void prompt_kernel(PromptArgs a) {
+// NW waves of 32 queries of one head share double-buffered tiles of BN keys.
+template <typename T, int D, int NW, int BN, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void prompt_kernel(PromptArgs a) {
   typedef typename T::elem elem;
-  constexpr int WM = 32 * QB, BM = WM * NW;
+  constexpr int WM = 32, BM = WM * NW;
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = a.nh / a.nkv;
@@ -170,31 +170,26 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
   // its keys compared with each row's last.
   const int full = max(min(first + off + 1, nk), 0) / (2 * BN) * (2 * BN);
   if (kend > 0) land(K0, V0, 0);
-  AttnWave<T, D, BN, QB> w;
-  int limit[QB];                                                 // the last key of this lane's queries
-#pragma unroll
-  for (int y = 0; y < QB; ++y) {
-    const int row = w0 + 32 * y + n;
-    limit[y] = row < nq ? row + off : -1;
-    w.start(y, row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
-  }
+  AttnWave<T, D, BN> w;
+  const int row = w0 + n, limit = row < nq ? row + off : -1;     // this lane's query and its last key
+  w.start(row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
   int t0 = 0;
   for (; t0 < full; t0 += 2 * BN) {
     ready();
     land(K1, V1, t0 + BN);
-    w.template tile<false>(K0, V0, c, [](int, int) { return false; });
+    w.template tile<false>(K0, V0, c, [](int) { return false; });
     ready();
     if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    w.template tile<false>(K1, V1, c, [](int, int) { return false; });
+    w.template tile<false>(K1, V1, c, [](int) { return false; });
   }
   for (; t0 < kend; t0 += 2 * BN) {
     ready();
     if (t0 + BN < kend) land(K1, V1, t0 + BN);
-    if (t0 < wend) w.template tile<true>(K0, V0, c, [&](int y, int j) { return t0 + j > limit[y]; });
+    if (t0 < wend) w.template tile<true>(K0, V0, c, [&](int j) { return t0 + j > limit; });
     if (t0 + BN >= kend) break;
     ready();
     if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    if (t0 + BN < wend) w.template tile<true>(K1, V1, c, [&](int y, int j) { return t0 + BN + j > limit[y]; });
+    if (t0 + BN < wend) w.template tile<true>(K1, V1, c, [&](int j) { return t0 + BN + j > limit; });
   }
   if (__any(w.odd != w.odd)) {   // a hidden value may have leaked: these rows one by one
     for (int i = 0; i < WM && w0 + i < nq; ++i) {
@@ -209,23 +204,19 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
     }
     return;
   }
+  const float l = w.sum(), inv = limit < 0 ? 0.f : 1.f / l;
+  if (row >= nq) return;
+  elem *orow = (elem *)a.o + (long long)(q0 + row) * a.os + h * D;
 #pragma unroll
-  for (int y = 0; y < QB; ++y) {
-    const int row = w0 + 32 * y + n;
-    const float l = w.sum(y), inv = limit[y] < 0 ? 0.f : 1.f / l;
-    if (row >= nq) continue;
-    elem *orow = (elem *)a.o + (long long)(q0 + row) * a.os + h * D;
+  for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-    for (int b = 0; b < D / 32; ++b)
+    for (int i = 0; i < 4; ++i) {
+      typename AttnOps<T>::vec4 v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        typename AttnOps<T>::vec4 v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (elem)(limit[y] < 0 ? 0.f : w.o[y][b][4 * i + j] * inv);
-        *(typename AttnOps<T>::vec4 *)(orow + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
-      }
-    if (a.lse && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
-  }
+      for (int j = 0; j < 4; ++j) v[j] = (elem)(limit < 0 ? 0.f : w.o[b][4 * i + j] * inv);
+      *(typename AttnOps<T>::vec4 *)(orow + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
+    }
+  if (a.lse && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m + __builtin_amdgcn_logf(l));
 }
 
 // ---- trees over the paged cache ----
@@ -234,7 +225,7 @@ template <typename T, int D, int NW, int BN, int QB, int OCC> __global__ __launc
 // rows against one stream of pages.  Few rows leave the work bound by that
 // stream, many by the matrix cores, and both want it cut along the keys, since
 // groups are few.  All row tiles (RT rows) of all groups are laid end to end, each
-// as long as its keys (in units of a tile of keys), and the line is cut into `lines`
+// as long as its keys (in units of 128), and the line is cut into `lines`
 // equal pieces, one workgroup each: no long sequence sets the time, and a piece that
 // begins or ends inside a row tile leaves a partial result, at most two a
 // workgroup.  Nothing of this is known on the host: every workgroup finds
@@ -258,7 +249,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int s) {
 }
 struct TreeTile {
   int s, tile;              // group (< 0: none) and row tile of it
-  int units;                // its length
+  int units;                // its length without the `extra` behind it
   int at;                   // where it begins on the line
 };
 // Where every group has the same number of row tiles (`levels`, more than one of
@@ -267,8 +258,15 @@ struct TreeTile {
 // run at the same time on the same XCD and find them in its L2.  On one line, 288
 // rows behind 32000 positions read every key from memory three times (106 us
 // against 89 with lines that happened to be cut alike).
+// A row tile takes longer than its keys: its pages are looked up, its outputs leave, its drafted
+// keys are slower.  `extra` units behind its keys, with no work in them, stand for that, so a piece
+// that holds the end of one gets fewer keys: 48 trees behind up to 12000 positions (32/8 heads of
+// 128) 131 us against 147 without, behind 2000 32 against 42.
+// Pieces shorter than 128 keys leave more partials than they save time: 288 rows of 256 behind
+// 2000 positions 31 us, cut by 64 keys 38 (behind 300 26 and 25).
+constexpr int UNIT = 128;
 struct TreePlan {
-  int rt, unit, levels, lines;   // levels 1: one line for all (or one row tile a group)
+  int rt, extra, levels, lines;   // levels 1: one line for all (or one row tile a group)
   int total;                     // a line's length; the launch has made sure that the sums fit 32 bits
   // A lane's group: its sequence, row tiles and units.
   struct Mine {
@@ -281,11 +279,11 @@ struct TreePlan {
     if (s >= a.n_seq) return m;
     m.q = tree_seq(a, s);
     m.tiles = (m.q.nodes * (a.nh / a.kv.n_kv_head) + rt - 1) / rt;
-    m.units = max((m.q.keys + unit - 1) / unit, 1);          // rows without keys are work too
+    m.units = max((m.q.keys + UNIT - 1) / UNIT, 1) + extra;  // rows without keys are work too
     return m;
   }
   // m: load(a, 0)
-  __device__ __forceinline__ TreePlan(int rt, int unit) : rt(rt), unit(unit) {}
+  __device__ __forceinline__ TreePlan(int rt, int extra) : rt(rt), extra(extra) {}
   __device__ __forceinline__ void lay(const TreeArgs &a, Mine m, int want, int most) {
     int sum = 0, one = 0;
     for (int s0 = 0;;) {
@@ -313,7 +311,7 @@ struct TreePlan {
         const int tile = node >= 0 ? 0 : (u - first) / n;
         *q = {lane_of(m.q.c0, w), lane_of(m.q.nodes, w), lane_of(m.q.len, w), lane_of(m.q.keys, w), lane_of(m.q.id, w),
               lane_of(m.q.bad, w) != 0};
-        return {scalar(s0 + w), scalar(levels > 1 ? level : tile), n, scalar(first + tile * n)};
+        return {scalar(s0 + w), scalar(levels > 1 ? level : tile), n - extra, scalar(first + tile * n)};
       }
       at = lane_of(inc, 63);
       if ((s0 += 64) < a.n_seq) m = load(a, s0);
@@ -351,6 +349,7 @@ __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int
 
 struct TreeLaunch {
   int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most
+  int extra;                    // units that a row tile counts beyond its keys
   float *po;                    // partial outputs [kv head][2 lines][row][D]: piece w's first row tile, its last
   float2 *ml;                   // and their maxima and sums [kv head][2 lines][row]
   int *count;                   // few rows: arrivals per (kv head, group), zero between launches; null: joined by a launch
@@ -447,7 +446,7 @@ __device__ __forceinline__ float max64(float v) {
 // them in the same launch.
 template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(256))) void tree_few_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
-  constexpr int BN = 32, NW = 4, UNIT = BN * NW, PC = D / 4;      // PC: 16-byte pieces of an f32 row
+  constexpr int BN = 32, NW = 4, PC = D / 4;      // PC: 16-byte pieces of an f32 row
   constexpr int LOADS = BN * D / 8 / 64;                          // of one tile of K or V, by one wave
   constexpr int JOIN = 16;
   __shared__ __align__(1024) elem Ks[NW * BN * D], Vs[NW * BN * D];
@@ -455,7 +454,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
   __shared__ int s_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
-  TreePlan plan(32, UNIT);
+  TreePlan plan(32, p.extra);
   TreePlan::Mine groups = plan.load(a, 0);
   plan.lay(a, groups, p.levels, p.lines);
   const TreeBlock me = tree_block(plan, nkv);
@@ -468,7 +467,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     TreeSeq q;
     const TreeTile item = plan.find(a, groups, me.level, u, -1, &q);
     const int skip = u - item.at, count = min(item.at + item.units, stop) - u;
-    u += count;
+    u = min(item.at + item.units + plan.extra, stop);
+    if (count <= 0) continue;
     if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
     const TreeRows<T, D> rows(a, q, hkv);
     const int base = item.tile * 32, R = min(q.nodes * rows.g - base, 32), r = base + n;
@@ -477,7 +477,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     elem *Kw = Ks + wave * BN * D, *Vw = Vs + wave * BN * D;
     bool bad = false;
     int t0 = begin + wave * BN;
-    AttnWave<T, D, BN, 1> w;
+    AttnWave<T, D, BN> w;
     // 16 rows never straddle a page: two lookups a tile, for the tile after the current one.
     int pg[2];
     auto land = [&](elem *dst, const elem *pool, auto isv) __attribute__((always_inline)) {
@@ -494,7 +494,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
       land(Kw, rows.kb, std::false_type{});
       land(Vw, rows.vb, std::true_type{});
     }
-    w.start(0, live ? rows.query(r) : nullptr);
+    w.start(live ? rows.query(r) : nullptr);
     const float c = a.scale * LOG2E;
     const unsigned long long *mask = live ? rows.mask(r) : nullptr;
     const int node = r / rows.g;
@@ -504,8 +504,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
       const int u0 = t0 - q.len;
       t0 += UNIT;
       if (t0 < end) pages();
-      f32x16_t s[1][1];
-      typename AttnWave<T, D, BN, 1>::vec8 pr[1][2];
+      f32x16_t s[1];
+      typename AttnWave<T, D, BN>::vec8 pr[2];
       // Loads land in the order of their requests: K's are there when no more
       // than V's are still under way, V's when no more than the next K's.
       wait_loads<LOADS>();
@@ -514,7 +514,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
       if (t0 < end) land(Kw, rows.kb, std::false_type{});
       const uint32_t see = H ? tree_sees(mask, a.mw, node, q.keys - q.len, u0) : ~0u;
       saw |= see;
-      w.template soft<H>(s, c, [&](int, int j) { return !((see >> j) & 1); }, pr);
+      w.template soft<H>(s, c, [&](int j) { return !((see >> j) & 1); }, pr);
       if (t0 < end) wait_loads<LOADS>();
       else wait_loads<0>();
       w.template outputs<H>(Vw, pr);
@@ -524,8 +524,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     while (t0 < min(end, q.len - BN + 1)) step(std::false_type{});  // tiles of cached positions
     while (t0 < end) step(std::true_type{});
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
-    const float l = w.sum(0);
-    if (lane < 32) s_ml[wave][n] = make_float2(w.m[0], saw && l == 0.f ? NAN : l);
+    const float l = w.sum();
+    if (lane < 32) s_ml[wave][n] = make_float2(w.m, saw && l == 0.f ? NAN : l);
     const bool whole = count == item.units;
     const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * 32;
     auto join = [&]() __attribute__((always_inline)) {
@@ -596,27 +596,27 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     // Each wave's outputs against the row's common maximum, through LDS (rows of D
     // floats, their pieces permuted by the row), then summed in the waves' order.
     float M = -INFINITY;
-  #pragma unroll
+#pragma unroll
     for (int x = 0; x < NW; ++x) M = fmaxf(M, s_ml[x][n].x);
-    const float f = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
+    const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M);
     auto area = [&](int x) { return (float *)(x < 2 ? Ks : Vs) + (x & 1) * 32 * D; };
     float *mine = area(wave);
-  #pragma unroll
+#pragma unroll
     for (int b = 0; b < D / 32; ++b)
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 4; ++i)
         *(float4 *)(mine + n * D + 4 * ((8 * b + 2 * i + hi) ^ (n & 15))) =
-            make_float4(w.o[0][b][4 * i] * f, w.o[0][b][4 * i + 1] * f, w.o[0][b][4 * i + 2] * f, w.o[0][b][4 * i + 3] * f);
+            make_float4(w.o[b][4 * i] * f, w.o[b][4 * i + 1] * f, w.o[b][4 * i + 2] * f, w.o[b][4 * i + 3] * f);
     __syncthreads();
     for (int x = tid; x < R * PC; x += 256) {
       const int y = x / PC, pc = x - y * PC;
       float Mr = -INFINITY, L = 0.f;
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < NW; ++u) Mr = fmaxf(Mr, s_ml[u][y].x);
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < NW; ++u) L += s_ml[u][y].x == -INFINITY ? s_ml[u][y].y : s_ml[u][y].y * __builtin_amdgcn_exp2f(s_ml[u][y].x - Mr);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < NW; ++u) {
         const float4 v = *(const float4 *)(area(u) + y * D + 4 * (pc ^ (y & 15)));
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
@@ -641,17 +641,17 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
   }
 }
 
-// Many rows: NW waves of 32 QB rows share double-buffered tiles of BN keys.
-template <typename T, int D, int NW, int BN, int QB, int OCC>
-__global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
+// Many rows: 4 waves of 32 rows share double-buffered tiles of BN keys.
+template <typename T, int D, int BN>
+__global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
   typedef typename T::elem elem;
-  constexpr int WM = 32 * QB, RT = WM * NW, PER = BN * D / 8 / (64 * NW), UNIT = 2 * BN;
+  constexpr int NW = 4, RT = 32 * NW, PER = BN * D / 8 / (64 * NW);
   __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
   constexpr int WORDS = CWEN_TREE_MAX / 32;
-  __shared__ uint32_t s_see[NW][QB][WORDS][32];
+  __shared__ uint32_t s_see[NW][WORDS][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nkv = a.kv.n_kv_head, n = lane & 31, hi = lane >> 5;
-  TreePlan plan(RT, UNIT);
+  TreePlan plan(RT, p.extra);
   TreePlan::Mine groups = plan.load(a, 0);
   plan.lay(a, groups, p.levels, p.lines);
   const TreeBlock me = tree_block(plan, nkv);
@@ -664,10 +664,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
     TreeSeq q;
     const TreeTile item = plan.find(a, groups, me.level, u, -1, &q);
     const int skip = u - item.at, count = min(item.at + item.units, stop) - u;
-    u += count;
+    u = min(item.at + item.units + plan.extra, stop);
+    if (count <= 0) continue;
     if (q.bad && tid == 0) kv_raise(a.kv, CWEN_KV_PAGE);
     const TreeRows<T, D> rows(a, q, hkv);
-    const int base = item.tile * RT + wave * WM, R = min(q.nodes * rows.g - base, WM);   // R <= 0: no rows here
+    const int base = item.tile * RT + wave * 32, R = min(q.nodes * rows.g - base, 32);   // R <= 0: no rows here
     const int begin = skip * UNIT, end = min(begin + count * UNIT, q.keys);
     bool bad = false;
     const float c = a.scale * LOG2E;
@@ -700,44 +701,37 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
       }
       if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
       lds_barrier();
+      lds_barrier();
       continue;
     }
     // What the rows see of the drafted nodes, before the tiles need the registers.
+    const int words = (q.keys - q.len + 31) / 32;
     if (end > q.len) {
-#pragma unroll
-      for (int y = 0; y < QB; ++y) {
-        const int r = base + 32 * y + n;
-        const unsigned long long *mask = 32 * y + n < R ? rows.mask(r) : nullptr;
-        for (int k = hi; k < WORDS; k += 2) s_see[wave][y][k][n] = tree_sees(mask, a.mw, r / rows.g, q.keys - q.len, 32 * k);
-      }
+      const unsigned long long *mask = n < R ? rows.mask(base + n) : nullptr;
+      for (int k = hi; k < words; k += 2) s_see[wave][k][n] = tree_sees(mask, a.mw, (base + n) / rows.g, q.keys - q.len, 32 * k);
     }
-    AttnWave<T, D, BN, QB> w;
-#pragma unroll
-    for (int y = 0; y < QB; ++y) w.start(y, 32 * y + n < R ? rows.query(base + 32 * y + n) : nullptr);
+    AttnWave<T, D, BN> w;
+    w.start(n < R ? rows.query(base + n) : nullptr);
     const int full = begin + max(min(end, q.len) - begin, 0) / (2 * BN) * (2 * BN);   // whole tiles of cached positions
-    uint32_t saw[QB];
-#pragma unroll
-    for (int y = 0; y < QB; ++y) saw[y] = full > begin;
+    uint32_t saw = full > begin;
     auto part = [&](const elem *Kb, const elem *Vb, int t0) __attribute__((always_inline)) {
-      uint32_t see[QB][BN / 32];
+      uint32_t see[BN / 32];
 #pragma unroll
-      for (int y = 0; y < QB; ++y)
-#pragma unroll
-        for (int b = 0; b < BN / 32; ++b) {
-          const int u0 = t0 + 32 * b - q.len, k = u0 >> 5;            // 32 bits across two words
-          const uint32_t lo = k < 0 ? ~0u : k < WORDS ? s_see[wave][y][k][n] : 0;
-          const uint32_t up = k < -1 ? ~0u : k + 1 < WORDS ? s_see[wave][y][k + 1][n] : 0;
-          saw[y] |= see[y][b] = __builtin_amdgcn_alignbit(up, lo, u0 & 31);
-        }
-      w.template tile<true>(Kb, Vb, c, [&](int y, int j) { return !((see[y][j >> 5] >> (j & 31)) & 1); });
+      for (int b = 0; b < BN / 32; ++b) {
+        const int u0 = t0 + 32 * b - q.len, k = u0 >> 5;              // 32 bits across two words
+        const uint32_t lo = k < 0 ? ~0u : k < words ? s_see[wave][k][n] : 0;
+        const uint32_t up = k < -1 ? ~0u : k + 1 < words ? s_see[wave][k + 1][n] : 0;
+        saw |= see[b] = __builtin_amdgcn_alignbit(up, lo, u0 & 31);
+      }
+      w.template tile<true>(Kb, Vb, c, [&](int j) { return !((see[j >> 5] >> (j & 31)) & 1); });
     };
     for (; t0 < full; t0 += 2 * BN) {
       ready();
       land(K1, V1, t0 + BN);
-      w.template tile<false>(K0, V0, c, [](int, int) { return false; });
+      w.template tile<false>(K0, V0, c, [](int) { return false; });
       ready();
       if (t0 + 2 * BN < end) land(K0, V0, t0 + 2 * BN);
-      w.template tile<false>(K1, V1, c, [](int, int) { return false; });
+      w.template tile<false>(K1, V1, c, [](int) { return false; });
     }
     for (bool one = false; t0 < end; t0 += BN, one = !one) {
       ready();
@@ -746,36 +740,46 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
     }
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
     const bool whole = count == item.units;
-    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * RT + wave * WM;
+    const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * RT + wave * 32;
+    lds_barrier();                                    // every wave is through with the tiles
     if (__any(w.odd != w.odd)) {
       for (int x = 0; x < R; ++x)
         rows.plain(base + x, begin, end, whole ? nullptr : p.po + (slot + x) * D, whole ? nullptr : p.ml + slot + x);
       lds_barrier();
       continue;
     }
+    constexpr int DC = BN * D / 64, PC = DC / 4, RPI = 64 / PC;   // columns, 16-byte pieces and rows of a load
+    int me_lane = lane;                               // opaque: its addresses are not kept through the tiles
+    asm volatile("" : "+v"(me_lane));
+    const int row = me_lane & 31, half = me_lane >> 5, pc = me_lane % PC;
+    const float l = w.sum(), ls = saw && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+    if (me_lane < min(R, 32)) {
+      if (!whole) p.ml[slot + row] = make_float2(w.m, ls);
+      else if (a.lse) *rows.lse(base + row) = LN2 * (w.m + __builtin_amdgcn_logf(l));
+    }
+    // The outputs through LDS, DC columns of a wave's rows at a time, so that lanes side by side
+    // store what lies side by side: from the registers a store touches 32 rows, 32 bytes of each,
+    // and 128 rows of 256 took 4.3 us.
+    float *mine = (float *)(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
 #pragma unroll
-    for (int y = 0; y < QB; ++y) {
-      const int x = 32 * y + n;
-      const float l = w.sum(y), ls = saw[y] && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
-      if (x >= R) continue;
+    for (int d0 = 0; d0 < D; d0 += DC) {
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
+      for (int b = d0 / 32; b < (d0 + DC) / 32; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 v = make_float4(w.o[y][b][4 * i] * inv, w.o[y][b][4 * i + 1] * inv, w.o[y][b][4 * i + 2] * inv,
-                                       w.o[y][b][4 * i + 3] * inv);
-          const int d = 32 * b + 8 * i + 4 * hi;
-          if (whole) {
-            const typename AttnOps<T>::vec4 e = {(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
-            *(typename AttnOps<T>::vec4 *)(rows.out(base + x) + d) = e;
-          } else {
-            *(float4 *)(p.po + (slot + x) * D + d) = v;
-          }
+        for (int i = 0; i < 4; ++i)
+          *(float4 *)(mine + row * DC + 4 * ((8 * (b - d0 / 32) + 2 * i + half) ^ (row & 15))) =
+              make_float4(w.o[b][4 * i] * inv, w.o[b][4 * i + 1] * inv, w.o[b][4 * i + 2] * inv, w.o[b][4 * i + 3] * inv);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int x = me_lane / PC; x < R; x += RPI) {
+        const float4 v = *(const float4 *)(mine + x * DC + 4 * (pc ^ (x & 15)));
+        if (whole) {
+          const typename AttnOps<T>::vec4 e = {(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
+          *(typename AttnOps<T>::vec4 *)(rows.out(base + x) + d0 + 4 * pc) = e;
+        } else {
+          *(float4 *)(p.po + (slot + x) * D + d0 + 4 * pc) = v;
         }
-      if (lane < 32) {
-        if (!whole) p.ml[slot + x] = make_float2(w.m[y], ls);
-        else if (a.lse) *rows.lse(base + x) = LN2 * (w.m[y] + __builtin_amdgcn_logf(l));
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     lds_barrier();                                 // LDS is free for the next row tile
   }
@@ -788,7 +792,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void tree_many_kernel(TreeArgs a, Tre
 // other they took 28 us of a batch of 580 nodes.
 constexpr int JOIN_HEADS = 32;
 template <typename T, int D, int LR>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int unit, int hpw) {
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int hpw) {
   typedef typename T::elem elem;
   constexpr int PC = D / 4, CAP = 4096, U = 8;
   __shared__ float s_w[CAP];
@@ -797,7 +801,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
   __shared__ int s_n[JOIN_HEADS], s_odd[JOIN_HEADS];
   __shared__ float4 s_o[256];
   const int tid = threadIdx.x, blocks = (a.nh + hpw - 1) / hpw, t = blockIdx.x / blocks, h0 = (blockIdx.x - t * blocks) * hpw;
-  TreePlan plan(rt, unit);
+  TreePlan plan(rt, p.extra);
   const TreePlan::Mine groups = plan.load(a, 0);
   plan.lay(a, groups, p.levels, p.lines);
   TreeSeq q;
@@ -809,7 +813,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
     const int nb = min(batch, rows - y0);
     for (int i = tid / LR; i < nb; i += 256 / LR) {
       const int h = h0 + y0 + i, hkv = h / g, r = (t - q.c0) * g + h - hkv * g, tile = r / rt, level = plan.levels > 1 ? tile : 0;
-      const int at0 = group.at + (tile - level) * group.units, w0 = plan.piece(at0);
+      const int at0 = group.at + (tile - level) * (group.units + p.extra), w0 = plan.piece(at0);
       const int n = plan.piece(at0 + group.units - 1) - w0 + 1, l = tid % LR;
       // Chunk x is piece w0 + x's: its first row tile's, but for chunk 0 if the piece began before this tile.
       const long long first = ((long long)hkv * 2 * p.lines + 2 * (w0 * plan.levels + level)) * rt + r % rt;
@@ -908,10 +912,10 @@ int attn_prompt_launch(const cwen_ctx *, int type, int D, const PromptArgs &a, h
     constexpr int dim = decltype(d)::value;
     const dim3 grid((unsigned)(items * a.nh));
     if constexpr (dim == 64) {
-      hipLaunchKernelGGL((prompt_kernel<T, 64, 4, 32, 1, 3>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((prompt_kernel<T, 64, 4, 32, 3>), grid, dim3(256), 0, st, a);
     } else {
-      if (wide) hipLaunchKernelGGL((prompt_kernel<T, dim, 8, dim == 256 ? 32 : 64, 1, 2>), grid, dim3(512), 0, st, a);
-      else hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, 1, dim == 256 ? 2 : 3>), grid, dim3(256), 0, st, a);
+      if (wide) hipLaunchKernelGGL((prompt_kernel<T, dim, 8, dim == 256 ? 32 : 64, 2>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, dim == 256 ? 2 : 3>), grid, dim3(256), 0, st, a);
     }
   });
 }
@@ -919,16 +923,17 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const int nkv = a.kv.n_kv_head, g = a.nh / nkv, D = a.kv.head_dim;
   const long long rows = (long long)a.max_nodes * g;
   const int form = rows <= 32 ? 1 : 4;                           // row tiles of 32 of a workgroup
-  const int rt = 32 * form, unit = form == 1 || D < 256 ? 128 : 64;
+  const int rt = 32 * form;
   const long long room = (long long)ctx->attn_floats / ((D + 2ll) * rt * nkv * 2);   // pieces whose partials the scratch holds
   const int per_cu = form == 1 ? 256 / D : D == 64 ? 3 : 2;      // workgroups that a CU holds at once
   TreeLaunch p;
+  p.extra = D == 256 ? 1 : 2;                                    // the units of 256 take twice as long
   p.lines = (int)std::max(1ll, std::min((long long)per_cu * ctx->ncu / nkv, room));
   if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
   // Up to 128 (row, chunk) partials of a group are joined in the launch: one token of 6 heads behind 1000
   // positions 14.4 us so, 15.7 in two launches; behind 4096 20.0 and 16.8.
-  const long long chunks = std::min((long long)p.lines, ((long long)a.max_len + a.max_nodes + unit - 1) / unit);
+  const long long chunks = std::min((long long)p.lines, ((long long)a.max_len + a.max_nodes + UNIT - 1) / UNIT);
   p.count = form == 1 && chunks * rows <= 128 && (long long)nkv * a.n_seq <= ctx->ncounters ? ctx->counters : nullptr;
   p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
   const long long tiles = (rows + rt - 1) / rt;                  // of one group at most
@@ -936,7 +941,7 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const long long blocks = 8ll * std::max((long long)p.levels * (((long long)nkv * (p.lines / p.levels) + 7) / 8),
                                           ((long long)nkv * p.lines + 7) / 8);
   // Every line's positions fit 32 bits.
-  const long long units = ((long long)a.kv.max_pages * a.kv.page + unit - 1) / unit + 1;
+  const long long units = ((long long)a.kv.max_pages * a.kv.page + UNIT - 1) / UNIT + 1 + p.extra;
   if ((a.n_seq + 64ll) * tiles * units > INT32_MAX) return CWEN_EINVAL;
   if (blocks > INT32_MAX || (long long)a.total * a.nh > INT32_MAX) return CWEN_EINVAL;
   const dim3 grid((unsigned)blocks);
@@ -944,8 +949,7 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value, BN = dim == 256 ? 32 : 64;
     if (form == 1) hipLaunchKernelGGL((tree_few_kernel<T, dim>), grid, dim3(256), 0, st, a, p);
-    else if constexpr (dim == 256) hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
-    else hipLaunchKernelGGL((tree_many_kernel<T, dim, 4, BN, 1, 2>), grid, dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((tree_many_kernel<T, dim, BN>), grid, dim3(256), 0, st, a, p);
   });
   if (rc || p.lines == 1 || p.count) return rc;
   // Up to 4 rows per CU: a workgroup each; past them as many heads to a workgroup as leave 2 per CU.
@@ -956,7 +960,7 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value;
     const dim3 grid((unsigned)(a.total * ((a.nh + hpw - 1) / hpw)));
-    if (hpw <= 4) hipLaunchKernelGGL((tree_join_kernel<T, dim, 64>), grid, dim3(256), 0, st, a, p, rt, unit, hpw);
-    else hipLaunchKernelGGL((tree_join_kernel<T, dim, 16>), grid, dim3(256), 0, st, a, p, rt, unit, hpw);
+    if (hpw <= 4) hipLaunchKernelGGL((tree_join_kernel<T, dim, 64>), grid, dim3(256), 0, st, a, p, rt, hpw);
+    else hipLaunchKernelGGL((tree_join_kernel<T, dim, 16>), grid, dim3(256), 0, st, a, p, rt, hpw);
   });
 }

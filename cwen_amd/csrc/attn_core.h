@@ -90,34 +90,35 @@ __device__ __forceinline__ float sum_halves(float x) {
 // 65504), and most tiles then leave the output sums alone.
 constexpr float ATTN_SLACK = 8.f;
 
-// A wave holds QB times 32 query rows: each K and V fragment read from LDS then
-// feeds QB products.
-template <typename T, int D, int BN, int QB> struct AttnWave {
+// A wave holds 32 query rows.  64 of them, which would read each fragment from LDS half as
+// often, do not fit the registers with heads of 256 and gain nothing with shorter ones: the
+// reads are hidden behind the products.
+template <typename T, int D, int BN> struct AttnWave {
   typedef typename T::elem elem;
   typedef typename AttnOps<T>::vec8 vec8;
   typedef typename AttnOps<T>::vec4 vec4;
   static constexpr int QS = D / 16, OB = D / 32, KB = BN / 32;
 
-  vec8 q[QB][QS];        // dims 16 s + 8 hi .. + 7 of query n
-  f32x16_t o[QB][OB];    // [i]: output dims 32 b + 8 (i / 4) + 4 hi + i % 4 of query n
-  float m[QB], l[QB];    // maximum (in powers of two) and this lane's part of the sum
+  vec8 q[QS];            // dims 16 s + 8 hi .. + 7 of query n
+  f32x16_t o[OB];        // [i]: output dims 32 b + 8 (i / 4) + 4 hi + i % 4 of query n
+  float m, l;            // maximum (in powers of two) and this lane's part of the sum
   float odd;             // NaN once a partly hidden tile held a value that is not finite
 
-  // row: the elements of query n of block y, null for a row that does not exist
-  __device__ __forceinline__ void start(int y, const elem *row) {
+  // row: the elements of query n, null for a row that does not exist
+  __device__ __forceinline__ void start(const elem *row) {
     const int hi = (threadIdx.x & 63) >> 5;
 #pragma unroll
-    for (int s = 0; s < QS; ++s) q[y][s] = row ? *(const vec8 *)(row + 16 * s + 8 * hi) : vec8{};
+    for (int s = 0; s < QS; ++s) q[s] = row ? *(const vec8 *)(row + 16 * s + 8 * hi) : vec8{};
 #pragma unroll
     for (int b = 0; b < OB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[y][b][i] = 0.f;
-    m[y] = -INFINITY;
-    l[y] = odd = 0.f;
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+    m = -INFINITY;
+    l = odd = 0.f;
   }
 
   // The scores of one tile, K the LDS array of its BN rows.
-  __device__ __forceinline__ void scores(const elem *K, f32x16_t (&s)[QB][KB]) {
+  __device__ __forceinline__ void scores(const elem *K, f32x16_t (&s)[KB]) {
     const int lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
     // Byte of piece hi of row n; piece 2 k + hi is an exclusive or away (k_piece).
     // Opaque, so that the addresses are formed when they are used: kept, they
@@ -125,63 +126,57 @@ template <typename T, int D, int BN, int QB> struct AttnWave {
     uint32_t at = (uint32_t)(n * D * 2 + 16 * k_piece<D>(n, hi));
     asm("" : "+v"(at));
 #pragma unroll
-    for (int y = 0; y < QB; ++y)
+    for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[y][b][i] = 0.f;
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < QS; ++k)
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
         const vec8 kf = *(const vec8 *)((const char *)K + (at ^ (32u * (k & 7))) + 256 * (k >> 3) + b * 64 * D);
-#pragma unroll
-        for (int y = 0; y < QB; ++y) s[y][b] = AttnOps<T>::mma(kf, q[y][k], s[y][b]);
+        s[b] = AttnOps<T>::mma(kf, q[k], s[b]);
       }
   }
   // Their softmax against the row's maximum so far.  c: scale * log2(e).  HIDE:
-  // hide(y, j) tells whether this lane's query of block y does not see key j of the tile.
+  // hide(j) tells whether this lane's query does not see key j of the tile.
   template <bool HIDE, typename F>
-  __device__ __forceinline__ void soft(f32x16_t (&s)[QB][KB], float c, F hide, vec8 (&p)[QB][2 * KB]) {
+  __device__ __forceinline__ void soft(f32x16_t (&s)[KB], float c, F hide, vec8 (&p)[2 * KB]) {
     const int hi = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int y = 0; y < QB; ++y) {
-      if (HIDE) {
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (hide(y, b * 32 + 8 * (i >> 2) + 4 * hi + (i & 3))) s[y][b][i] = -INFINITY;
-      }
-      float mx = s[y][0][0];
+    if (HIDE) {
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[y][b][i]);
-      mx = max_halves(mx) * c;
-      if (__any(mx > m[y] + ATTN_SLACK)) {
-        const float mn = fmaxf(m[y], mx), a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[y] - mn);
-        l[y] *= a;
-#pragma unroll
-        for (int b = 0; b < OB; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[y][b][i] *= a;
-        m[y] = mn;
-      }
-      const float ms = m[y] == -INFINITY ? 0.f : m[y];
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[y][b][i], c, -ms));
-          l[y] += e;
-          p[y][2 * b + (i >> 3)][i & 7] = (elem)e;     // half a step; the sum keeps all of it
-        }
+        for (int i = 0; i < 16; ++i)
+          if (hide(b * 32 + 8 * (i >> 2) + 4 * hi + (i & 3))) s[b][i] = -INFINITY;
     }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = max_halves(mx) * c;
+    if (__any(mx > m + ATTN_SLACK)) {
+      const float mn = fmaxf(m, mx), a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= a;
+#pragma unroll
+      for (int b = 0; b < OB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= a;
+      m = mn;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -ms));
+        l += e;
+        p[2 * b + (i >> 3)][i & 7] = (elem)e;     // half a step; the sum keeps all of it
+      }
   }
   // The outputs' sums, V the LDS array of the tile's rows.  Lane i of a group of
   // 16 addresses the 4 keys' rows 4 g + i / 4 and gets column i of all 4.
-  template <bool HIDE> __device__ __forceinline__ void outputs(const elem *V, const vec8 (&p)[QB][2 * KB]) {
+  template <bool HIDE> __device__ __forceinline__ void outputs(const elem *V, const vec8 (&p)[2 * KB]) {
     const int lane = threadIdx.x & 63, hi = lane >> 5;
     const int vi = lane & 15, vr = 4 * hi + (vi >> 2), vc = ((lane >> 4) & 1) * 2 + ((vi & 3) >> 1), ve = (vi & 1) * 4;
     uint32_t at = (uint32_t)(vr * D * 2 + 16 * v_piece<D>(vr, vc) + 2 * ve);
@@ -194,20 +189,19 @@ template <typename T, int D, int BN, int QB> struct AttnWave {
         const vec4 a = AttnOps<T>::tr(r), d = AttnOps<T>::tr(r + 16 * D);
         const vec8 vf = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
         if (HIDE) odd = AttnOps<T>::probe(vf, odd);
-#pragma unroll
-        for (int y = 0; y < QB; ++y) o[y][b] = AttnOps<T>::mma(vf, p[y][t], o[y][b]);
+        o[b] = AttnOps<T>::mma(vf, p[t], o[b]);
       }
   }
   template <bool HIDE, typename F> __device__ __forceinline__ void tile(const elem *K, const elem *V, float c, F hide) {
-    f32x16_t s[QB][KB];
-    vec8 p[QB][2 * KB];
+    f32x16_t s[KB];
+    vec8 p[2 * KB];
     scores(K, s);
     soft<HIDE>(s, c, hide, p);
     outputs<HIDE>(V, p);
   }
 
   // The whole row's sum.
-  __device__ __forceinline__ float sum(int y) const { return sum_halves(l[y]); }
+  __device__ __forceinline__ float sum() const { return sum_halves(l); }
 };
 
 // Rows t0 .. t0 + BN - 1 into LDS, by NW waves; rows past `last` are copies of
