@@ -140,11 +140,14 @@ template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a,
   return {-1};
 }
 
-// NW waves of 32 queries of one head share double-buffered tiles of BN keys.
-template <typename T, int D, int NW, int BN, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void prompt_kernel(PromptArgs a) {
+// RW KW waves share double-buffered tiles of KW BN keys: RW of them have 32 queries
+// of one head each, and with KW = 2 the first RW take one half of every tile's keys, the
+// others, for the same queries, the other; their sums meet at the end.
+template <typename T, int D, int RW, int KW, int BN, int OCC>
+__global__ __launch_bounds__(64 * RW * KW, OCC) void prompt_kernel(PromptArgs a) {
   typedef typename T::elem elem;
-  constexpr int WM = 32, BM = WM * NW;
-  __shared__ __align__(1024) elem K0[BN * D], K1[BN * D], V0[BN * D], V1[BN * D];
+  constexpr int NW = RW * KW, WM = 32, BM = WM * RW, BT = KW * BN;
+  __shared__ __align__(1024) elem K0[BT * D], K1[BT * D], V0[BT * D], V1[BT * D];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = a.nh / a.nkv;
   // Blocks of one kv head go to one or two XCDs (block b runs on XCD b % 8), long rows first.
@@ -152,14 +155,15 @@ template <typename T, int D, int NW, int BN, int OCC> __global__ __launch_bounds
   const Item item = find_item<BM>(a, blockIdx.x / a.nh);
   if (item.seq < 0) return;
   const int tile = item.tile, q0 = item.q0, nq = item.nq, k0 = item.k0, nk = item.nk, off = nk - nq;
-  const int first = tile * BM, w0 = first + wave * WM;      // the workgroup's and this wave's first query
+  const int rw = wave % RW, kw = wave / RW;
+  const int first = tile * BM, w0 = first + rw * WM;        // the workgroup's and this wave's first query
   const elem *kp = (const elem *)a.k + (long long)k0 * a.ks + hkv * D, *vp = (const elem *)a.v + (long long)k0 * a.vs + hkv * D;
   const int kend = min(min(first + BM, nq) + off, nk);           // keys that the workgroup's rows see
   const int wend = min(min(w0 + WM, nq) + off, nk);              // and this wave's
   const float c = a.scale * LOG2E;
   auto land = [&](elem *Kd, elem *Vd, int t0) __attribute__((always_inline)) {
-    land_rows<D, BN, false, NW>(Kd, wave, t0, nk - 1, (uint32_t)a.ks * 2, [&](int, int j) { return kp + j * a.ks; });
-    land_rows<D, BN, true, NW>(Vd, wave, t0, nk - 1, (uint32_t)a.vs * 2, [&](int, int j) { return vp + j * a.vs; });
+    land_rows<D, BT, false, NW>(Kd, wave, t0, nk - 1, (uint32_t)a.ks * 2, [&](int, int j) { return kp + j * a.ks; });
+    land_rows<D, BT, true, NW>(Vd, wave, t0, nk - 1, (uint32_t)a.vs * 2, [&](int, int j) { return vp + j * a.vs; });
   };
   auto ready = [&]() __attribute__((always_inline)) {
     wait_loads<0>();
@@ -168,28 +172,63 @@ template <typename T, int D, int NW, int BN, int OCC> __global__ __launch_bounds
   };
   // Tiles that every row sees whole come first, two per turn; what is left has
   // its keys compared with each row's last.
-  const int full = max(min(first + off + 1, nk), 0) / (2 * BN) * (2 * BN);
+  const int full = max(min(first + off + 1, nk), 0) / (2 * BT) * (2 * BT);
   if (kend > 0) land(K0, V0, 0);
   AttnWave<T, D, BN> w;
   const int row = w0 + n, limit = row < nq ? row + off : -1;     // this lane's query and its last key
   w.start(row < nq ? (const elem *)a.q + (long long)(q0 + row) * a.qs + h * D : nullptr);
+  const int k0w = kw * BN, at = k0w * D;                         // this wave's keys of a tile
   int t0 = 0;
-  for (; t0 < full; t0 += 2 * BN) {
+  for (; t0 < full; t0 += 2 * BT) {
     ready();
-    land(K1, V1, t0 + BN);
-    w.template tile<false>(K0, V0, c, [](int) { return false; });
+    land(K1, V1, t0 + BT);
+    w.template tile<false>(K0 + at, V0 + at, c, [](int) { return false; });
     ready();
-    if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    w.template tile<false>(K1, V1, c, [](int) { return false; });
+    if (t0 + 2 * BT < kend) land(K0, V0, t0 + 2 * BT);
+    w.template tile<false>(K1 + at, V1 + at, c, [](int) { return false; });
   }
-  for (; t0 < kend; t0 += 2 * BN) {
+  for (; t0 < kend; t0 += 2 * BT) {
     ready();
-    if (t0 + BN < kend) land(K1, V1, t0 + BN);
-    if (t0 < wend) w.template tile<true>(K0, V0, c, [&](int j) { return t0 + j > limit; });
-    if (t0 + BN >= kend) break;
+    if (t0 + BT < kend) land(K1, V1, t0 + BT);
+    if (t0 + k0w < wend) w.template tile<true>(K0 + at, V0 + at, c, [&](int j) { return t0 + k0w + j > limit; });
+    if (t0 + BT >= kend) break;
     ready();
-    if (t0 + 2 * BN < kend) land(K0, V0, t0 + 2 * BN);
-    if (t0 + BN < wend) w.template tile<true>(K1, V1, c, [&](int j) { return t0 + BN + j > limit; });
+    if (t0 + 2 * BT < kend) land(K0, V0, t0 + 2 * BT);
+    if (t0 + BT + k0w < wend) w.template tile<true>(K1 + at, V1 + at, c, [&](int j) { return t0 + BT + k0w + j > limit; });
+  }
+  lds_barrier();                 // every wave is through with the tiles
+  elem *mine = (rw * 4 / RW == 0 ? K0 : rw * 4 / RW == 1 ? K1 : rw * 4 / RW == 2 ? V0 : V1) + rw % (RW / 4) * (4 * BT * D / RW);
+  if constexpr (KW == 2) {       // the second half's sums, lane by lane as they lie in registers
+    static_assert(RW == 4 && BT * sizeof(elem) >= 32 * sizeof(float), "a wave's outputs fill an array");
+    __shared__ float s_ml[RW][3][64];
+    float4 *x = (float4 *)mine + lane;
+    if (kw) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[64 * (4 * b + i)] = make_float4(w.o[b][4 * i], w.o[b][4 * i + 1], w.o[b][4 * i + 2], w.o[b][4 * i + 3]);
+      s_ml[rw][0][lane] = w.m;
+      s_ml[rw][1][lane] = w.l;
+      s_ml[rw][2][lane] = w.odd;
+    }
+    lds_barrier();
+    if (kw) return;
+    const float m = s_ml[rw][0][lane], M = fmaxf(w.m, m);
+    const float f0 = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M), f1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    w.m = M;
+    w.l = w.l * f0 + s_ml[rw][1][lane] * f1;
+    w.odd += s_ml[rw][2][lane];
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = x[64 * (4 * b + i)];
+        w.o[b][4 * i] = w.o[b][4 * i] * f0 + v.x * f1;
+        w.o[b][4 * i + 1] = w.o[b][4 * i + 1] * f0 + v.y * f1;
+        w.o[b][4 * i + 2] = w.o[b][4 * i + 2] * f0 + v.z * f1;
+        w.o[b][4 * i + 3] = w.o[b][4 * i + 3] * f0 + v.w * f1;
+      }
   }
   if (__any(w.odd != w.odd)) {   // a hidden value may have leaked: these rows one by one
     for (int i = 0; i < WM && w0 + i < nq; ++i) {
@@ -205,18 +244,38 @@ template <typename T, int D, int NW, int BN, int OCC> __global__ __launch_bounds
     return;
   }
   const float l = w.sum(), inv = limit < 0 ? 0.f : 1.f / l;
-  if (row >= nq) return;
-  elem *orow = (elem *)a.o + (long long)(q0 + row) * a.os + h * D;
+  if (a.lse && row < nq && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m + __builtin_amdgcn_logf(l));
+  // The outputs through LDS, DC columns of a wave's rows at a time, so that a store takes whole
+  // rows.  From the registers it takes 32 rows, 16 bytes of each, whose distance often puts them
+  // all in one channel of the L2: 10 us for 256 rows of 24 heads of 256.
+  constexpr int DC = BT * D / (8 * RW) < D ? BT * D / (8 * RW) : D, PC = DC / 8, RPI = 64 / PC, IN = 32 / RPI, XOR = PC < 16 ? PC - 1 : 15;
+  int me = lane;                 // opaque: its addresses are not kept through the tiles
+  asm volatile("" : "+v"(me));
+  const int x = me & 31, half = me >> 5, pc = me % PC, y0 = me / PC;
+  elem *to = (elem *)a.o + (long long)(q0 + w0 + y0) * a.os + h * D + 8 * pc;
 #pragma unroll
-  for (int b = 0; b < D / 32; ++b)
+  for (int d0 = 0; d0 < D; d0 += DC) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      typename AttnOps<T>::vec4 v;
+    for (int b = d0 / 32; b < (d0 + DC) / 32; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (elem)(limit < 0 ? 0.f : w.o[b][4 * i + j] * inv);
-      *(typename AttnOps<T>::vec4 *)(orow + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
+      for (int i = 0; i < 4; ++i) {
+        typename AttnOps<T>::vec4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (elem)(limit < 0 ? 0.f : w.o[b][4 * i + j] * inv);
+        *(typename AttnOps<T>::vec4 *)(mine + x * DC + 8 * ((4 * (b - d0 / 32) + i) ^ (x & XOR)) + 4 * half) = v;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    typename AttnOps<T>::vec8 v[IN];
+#pragma unroll
+    for (int u = 0; u < IN; ++u) {
+      const int y = y0 + u * RPI;
+      v[u] = *(const typename AttnOps<T>::vec8 *)(mine + y * DC + 8 * (pc ^ (y & XOR)));
     }
-  if (a.lse && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m + __builtin_amdgcn_logf(l));
+#pragma unroll
+    for (int u = 0; u < IN; ++u)
+      if (w0 + y0 + u * RPI < nq) *(typename AttnOps<T>::vec8 *)(to + (long long)u * RPI * a.os + d0) = v[u];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
 }
 
 // ---- trees over the paged cache ----
@@ -898,12 +957,18 @@ template <typename F> int by_type(int type, int D, F f) {
 
 }  // namespace
 
-int attn_prompt_launch(const cwen_ctx *, int type, int D, const PromptArgs &a, hipStream_t st) {
+int attn_prompt_launch(const cwen_ctx *ctx, int type, int D, const PromptArgs &a, hipStream_t st) {
+  const long long tiles = (a.total_q + 127) / 128 + a.n_seq;      // of 128 rows, at most
+  // Up to 2.5 workgroups per CU (heads of 64: 4.5) the longest row sets the time, so its keys
+  // go to two halves of a workgroup: heads of 128, 32/8: 2048 tokens 47 us against 62 (4096, 4 per
+  // CU: 158 against 143); of 256, 24/4: 2048 79 against 112 (4096 260 against 252); of 64, 16/4: 2048
+  // 26 against 38, 8192 174 against 184 (40 prompts of 125 20 against 16).
+  const bool split = 2 * tiles * a.nh <= (D == 64 ? 9ll : 5ll) * ctx->ncu;
   // Sequences of 4096 tokens and more on average: workgroups of 8 waves read K and V half as often as
   // those of 4, which leave fewer waves idle in short sequences and more workgroups to a CU (heads of 128,
-  // 32/8: one prompt of 32768 7.57 ms against 7.90, of 8192 0.52 and 0.56; of 2048 62 us against 54; 9 of
-  // 700..3800 446 us against 441).  Heads of 64 gain nothing from 8 (32768: 4.9 ms against 4.7).
-  const bool wide = D != 64 && a.total_q >= 4096ll * a.n_seq;
+  // 32/8: one prompt of 32768 7.57 ms against 7.90, 4 of 4096 757 us against 720; of 256, 24/4: 4096
+  // 247 us against 252, 16384 2.91 ms and 3.10).  Heads of 64 gain nothing (32768: 4.9 ms and 4.7).
+  const bool wide = !split && D != 64 && a.total_q >= 4096ll * a.n_seq;
   const int BM = wide ? 256 : 128;
   const long long items = (a.total_q + BM - 1) / BM + a.n_seq;
   if (items * a.nh > INT32_MAX) return CWEN_EINVAL;
@@ -911,12 +976,9 @@ int attn_prompt_launch(const cwen_ctx *, int type, int D, const PromptArgs &a, h
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value;
     const dim3 grid((unsigned)(items * a.nh));
-    if constexpr (dim == 64) {
-      hipLaunchKernelGGL((prompt_kernel<T, 64, 4, 32, 3>), grid, dim3(256), 0, st, a);
-    } else {
-      if (wide) hipLaunchKernelGGL((prompt_kernel<T, dim, 8, dim == 256 ? 32 : 64, 2>), grid, dim3(512), 0, st, a);
-      else hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 32, dim == 256 ? 2 : 3>), grid, dim3(256), 0, st, a);
-    }
+    if (split) hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 2, 32, 2>), grid, dim3(512), 0, st, a);
+    else if (!wide) hipLaunchKernelGGL((prompt_kernel<T, dim, 4, 1, 32, dim == 256 ? 2 : 3>), grid, dim3(256), 0, st, a);
+    else if constexpr (dim != 64) hipLaunchKernelGGL((prompt_kernel<T, dim, 8, 1, dim == 256 ? 32 : 64, 2>), grid, dim3(512), 0, st, a);
   });
 }
 int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {

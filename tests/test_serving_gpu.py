@@ -528,6 +528,35 @@ def test_prompt_wide_workgroups(env):
     check_prompt(prompt_case(gpu, ctx, gen(2), F16, 1, 1, 256, [4101], [4133]), F16)
 
 
+@pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_many_workgroups(env, D, typ):
+    """Heads enough that no tile's keys are halved between waves (they are where workgroups are few,
+    as in most tests here): lengths around the tiles, keys and queries that differ, hidden NaN."""
+    gpu, ctx = env
+    H = 1500 if D == 64 else 800
+    for i, (lq, lk) in enumerate([([1], None), ([31, 0, 33], [64, 5, 33]), ([64, 65], [65, 64]), ([70, 5], [131, 5]), ([129, 128], None),
+                                  ([200], [199]), ([257], [321])]):
+        check_prompt(prompt_case(gpu, ctx, gen(60 + i), typ, H, 2, D, lq, lk, gap=i % 2), typ, heads=[0, H // 2 - 1, H - 1])
+
+    def spoil(k, v):
+        v[37, 0, 5], v[90, 1, 6] = float("nan"), float("inf")
+        k[120, 0, :] = float("nan")
+        k[-3:], v[-3:] = float("nan"), float("inf")
+    check_prompt(prompt_case(gpu, ctx, gen(8), typ, H, 2, D, [60, 100, 1], gap=3, nan=spoil), typ, heads=[0, 7, H - 1])
+
+
+def test_prompt_few_workgroups_long(env):
+    """Halved keys over many tiles, a late maximum in either half, and more queries than keys."""
+    gpu, ctx = env
+    for D, typ, n in ((64, BF16, 1111), (128, F16, 1030), (256, F16, 900)):
+        for half in (0, 1):
+            def late(k, v):                                     # the highest scores lie in one half of the tiles
+                j = torch.arange(k.shape[0], device="cuda")
+                k.mul_((1 + 3.0 * ((j // 32) % 2 == half) * j / n)[:, None, None].to(k.dtype))
+            check_prompt(prompt_case(gpu, ctx, gen(n + half), typ, 2, 1, D, [n, 40], [n + 33, 9], nan=late), typ)
+
+
 def test_prompt_offsets_past_32_bits(env):
     """Tokens 2^26 elements apart: the last keys lie past 4 GiB."""
     gpu, ctx = env
