@@ -19,7 +19,8 @@ template <typename T, int D> struct AttnRow {
   bool sees;
   template <typename SEES, typename ROWS>
   __device__ __forceinline__ void run(const typename T::elem *q, int begin, int end, float c, SEES see, ROWS rows) {
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;    // opaque: what follows from it is not kept through the tiles
+    asm volatile("" : "+v"(lane));
     float x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -47,7 +48,8 @@ template <typename T, int D> struct AttnRow {
     }
   }
   __device__ __forceinline__ void store(typename T::elem *o, float *lse) const {
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int e = 0; e < E; ++e) o[lane * E + e] = (typename T::elem)(sees ? acc[e] / l : 0.f);
     if (lse && lane == 0) *lse = LN2 * (m + __builtin_amdgcn_logf(l));
@@ -190,11 +192,11 @@ __global__ __launch_bounds__(64 * RW * KW, OCC) void prompt_kernel(PromptArgs a)
   for (; t0 < kend; t0 += 2 * BT) {
     ready();
     if (t0 + BT < kend) land(K1, V1, t0 + BT);
-    if (t0 + k0w < wend) w.template tile<true>(K0 + at, V0 + at, c, [&](int j) { return t0 + k0w + j > limit; });
+    if (t0 + k0w < wend) w.template tile<true>(K0 + at, V0 + at, c, [&](int j) { return t0 + k0w + j + 4 * (lane >> 5) > limit; });
     if (t0 + BT >= kend) break;
     ready();
     if (t0 + 2 * BT < kend) land(K0, V0, t0 + 2 * BT);
-    if (t0 + BT + k0w < wend) w.template tile<true>(K1 + at, V1 + at, c, [&](int j) { return t0 + BT + k0w + j > limit; });
+    if (t0 + BT + k0w < wend) w.template tile<true>(K1 + at, V1 + at, c, [&](int j) { return t0 + BT + k0w + j + 4 * (lane >> 5) > limit; });
   }
   lds_barrier();                 // every wave is through with the tiles
   elem *mine = (rw * 4 / RW == 0 ? K0 : rw * 4 / RW == 1 ? K1 : rw * 4 / RW == 2 ? V0 : V1) + rw % (RW / 4) * (4 * BT * D / RW);
@@ -455,7 +457,9 @@ template <typename T, int D> struct TreeRows {
   // Row r alone over the keys begin .. end - 1; po, ml: its partial, or null.
   __device__ __forceinline__ void plain(int r, int begin, int end, float *po, float2 *ml) const {
     const unsigned long long *mk = mask(r);
-    const int i = r / g, lane = threadIdx.x & 63;
+    const int i = r / g;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
     AttnRow<T, D> x;
     x.run(query(r), begin, end, a.scale * LOG2E,
           [&](int j) {
@@ -573,7 +577,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
       if (t0 < end) land(Kw, rows.kb, std::false_type{});
       const uint32_t see = H ? tree_sees(mask, a.mw, node, q.keys - q.len, u0) : ~0u;
       saw |= see;
-      w.template soft<H>(s, c, [&](int j) { return !((see >> j) & 1); }, pr);
+      const uint32_t mine = see >> 4 * hi;
+      w.template soft<H>(s, c, [&](int j) { return !((mine >> j) & 1); }, pr);
       if (t0 < end) wait_loads<LOADS>();
       else wait_loads<0>();
       w.template outputs<H>(Vw, pr);
@@ -780,7 +785,9 @@ __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunc
         const int u0 = t0 + 32 * b - q.len, k = u0 >> 5;              // 32 bits across two words
         const uint32_t lo = k < 0 ? ~0u : k < words ? s_see[wave][k][n] : 0;
         const uint32_t up = k < -1 ? ~0u : k + 1 < words ? s_see[wave][k + 1][n] : 0;
-        saw |= see[b] = __builtin_amdgcn_alignbit(up, lo, u0 & 31);
+        see[b] = __builtin_amdgcn_alignbit(up, lo, u0 & 31);
+        saw |= see[b];
+        see[b] >>= 4 * hi;
       }
       w.template tile<true>(Kb, Vb, c, [&](int j) { return !((see[j >> 5] >> (j & 31)) & 1); });
     };

@@ -138,16 +138,16 @@ template <typename T, int D, int BN> struct AttnWave {
       }
   }
   // Their softmax against the row's maximum so far.  c: scale * log2(e).  HIDE:
-  // hide(j) tells whether this lane's query does not see key j of the tile.
+  // hide(j) tells whether this lane's query does not see key j + 4 hi of
+  // the tile (j is a constant then: with 4 hi in it the compiler kept 16 masks in registers).
   template <bool HIDE, typename F>
   __device__ __forceinline__ void soft(f32x16_t (&s)[KB], float c, F hide, vec8 (&p)[2 * KB]) {
-    const int hi = (threadIdx.x & 63) >> 5;
     if (HIDE) {
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (hide(b * 32 + 8 * (i >> 2) + 4 * hi + (i & 3))) s[b][i] = -INFINITY;
+          if (hide(b * 32 + 8 * (i >> 2) + (i & 3))) s[b][i] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
