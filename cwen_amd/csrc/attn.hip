@@ -1000,10 +1000,13 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   p.lines = (int)std::max(1ll, std::min((long long)per_cu * ctx->ncu / nkv, room));
   if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
-  // Up to 128 (row, chunk) partials of a group are joined in the launch: one token of 6 heads behind 1000
-  // positions 14.4 us so, 15.7 in two launches; behind 4096 20.0 and 16.8.
-  const long long chunks = std::min((long long)p.lines, ((long long)a.max_len + a.max_nodes + UNIT - 1) / UNIT);
-  p.count = form == 1 && chunks * rows <= 128 && (long long)nkv * a.n_seq <= ctx->ncounters ? ctx->counters : nullptr;
+  // Up to 96 (row, chunk) partials of a group are joined in the launch: one token of 6 heads behind 1000
+  // positions 14.6 us so, 16.1 in two launches; behind 2600 17.1 and 16.0.  Of many groups one is taken
+  // to hold at most twice its share of the pieces: 48 tokens of 32/8 heads behind up to 12000
+  // positions 113 us and 117; with 6 nodes each (24 rows) 164 and 162.
+  const long long share = 2ll * ((p.lines + a.n_seq - 1) / a.n_seq) + 1;
+  const long long chunks = std::min({(long long)p.lines, share, ((long long)a.max_len + a.max_nodes + UNIT - 1) / UNIT});
+  p.count = form == 1 && chunks * rows <= 96 && (long long)nkv * a.n_seq <= ctx->ncounters ? ctx->counters : nullptr;
   p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
   const long long tiles = (rows + rt - 1) / rt;                  // of one group at most
   p.levels = (int)std::min(tiles, (long long)p.lines);
