@@ -903,6 +903,43 @@ def test_decode_step_in_a_graph(env, nodes, H):
         check_tree(kv, 0, q, o, None, [x + 7 * i for x in lens], [nodes] * 3, None, F16, heads=[0, H - 1])
 
 
+def test_counters_are_shared_with_the_gemvs(env):
+    """Joins in the launch and GEMVs split over K count arrivals in the same words of a context: in
+    turn, without a wait between, each gives the bits that it gives alone."""
+    gpu, ctx = env
+    from cwen_amd import synth
+    qs, sc = synth.q4_rs(5, 48, 5120)
+    W = gpu.Weight(ctx, 101, qs, sc, 5120, 48)                 # few rows: K is split
+    g, lens = gen(31), [1900, 60, 1200]
+    kv = tree_cache(gpu, ctx, g, F16, 4, 256, 16, lens, [1, 1, 1], L=1)
+    q = randn(g, 3, 24, 256, dtype=F16)
+    x, seqs, cu = randn(g, 8, 5120), ints([0, 1, 2]), ints([0, 1, 2, 3])
+    o, y = torch.empty_like(q), torch.empty(8, 48, device="cuda")
+    gpu.attn_tree(ctx, kv, 0, q, o, seqs, cu, 1, 1900)
+    gpu.gemvb(ctx, W, x, y, 8)
+    torch.cuda.synchronize()
+    check_tree(kv, 0, q, o, None, lens, [1, 1, 1], None, F16, heads=[0, 23])
+    o0, y0 = o.clone(), y.clone()
+    for _ in range(20):
+        o.fill_(0), y.fill_(0)
+        gpu.attn_tree(ctx, kv, 0, q, o, seqs, cu, 1, 1900)
+        gpu.gemvb(ctx, W, x, y, 8)
+        gpu.attn_tree(ctx, kv, 0, q, o, seqs, cu, 1, 1900)
+        assert torch.equal(o, o0) and torch.equal(y, y0)
+
+
+def test_one_long_context_among_short_ones(env):
+    """A batch whose one long context holds nearly all the pieces: more than the launch expects."""
+    gpu, ctx = env
+    for D, H, K in ((256, 6, 1), (64, 2, 1), (128, 24, 8)):
+        lens, nodes = [3] * 20 + [9000] + [0] * 11, [1] * 32
+        g = gen(D)
+        kv = tree_cache(gpu, ctx, g, BF16, K, D, 64, lens, nodes, L=1)
+        q = randn(g, 32, H, D, dtype=BF16)
+        o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, [1] * 32)
+        check_tree(kv, 0, q, o, z, lens, nodes, [1] * 32, BF16, heads=[0, H - 1])
+
+
 def test_two_contexts_on_two_streams(env):
     """Calls on two contexts and caches at the same time give what they give alone."""
     gpu, _ = env
