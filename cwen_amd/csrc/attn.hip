@@ -142,6 +142,10 @@ template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a,
   return {-1};
 }
 
+// Bound by the matrix cores, and there by power: 32768 tokens of 32/8 heads of 128 in bf16 take
+// 7.6 ms, 1.16 PFLOP/s with the matrix pipes 57 % busy at 1.94 GHz (a product of 8192^3 reaches
+// 1.21); 9 prompts of 16301 tokens in all 339 us (0.91), 4096 tokens of 24/4 heads of 256 in f16
+// 228 us (0.90: the longest row sets the time).
 // RW KW waves share double-buffered tiles of KW BN keys: RW of them have 32 queries
 // of one head each, and with KW = 2 the first RW take one half of every tile's keys, the
 // others, for the same queries, the other; their sums meet at the end.
@@ -249,7 +253,8 @@ __global__ __launch_bounds__(64 * RW * KW, OCC) void prompt_kernel(PromptArgs a)
   if (a.lse && row < nq && lane < 32) a.lse[(long long)(q0 + row) * a.nh + h] = LN2 * (w.m + __builtin_amdgcn_logf(l));
   // The outputs through LDS, DC columns of a wave's rows at a time, so that a store takes whole
   // rows.  From the registers it takes 32 rows, 16 bytes of each, whose distance often puts them
-  // all in one channel of the L2: 10 us for 256 rows of 24 heads of 256.
+  // all in one channel of the L2: 1.5 % of a prompt of 4096 tokens with heads of 256, 2.5 % of 40
+  // prompts of 125 with heads of 64.
   constexpr int DC = BT * D / (8 * RW) < D ? BT * D / (8 * RW) : D, PC = DC / 8, RPI = 64 / PC, IN = 32 / RPI, XOR = PC < 16 ? PC - 1 : 15;
   int me = lane;                 // opaque: its addresses are not kept through the tiles
   asm volatile("" : "+v"(me));
@@ -501,6 +506,8 @@ __device__ __forceinline__ float max64(float v) {
   return v;
 }
 
+// Bound by a chain of six trips to memory, then by the pages' bytes: one node of 24/4 heads of 256
+// behind 4096 positions 10.8 us (16.8 MB), 64 of them behind up to 8000 102 us.
 // Few rows: one tile of 32, the chunk's keys dealt to 4 waves 32 at a time.  A wave
 // has its own K and V rows in LDS and no barrier in its loop: the next K rows
 // are requested when the scores are done, the next V rows after the outputs, so
@@ -705,6 +712,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
   }
 }
 
+// Bound by the pages' bytes while rows are few (48 trees of up to 24 nodes behind up to 12000
+// positions, 32/8 heads of 128: 130 us, 617 MB, 4.75 TB/s), by matrix work and the partials with
+// more (48 nodes of 24/4 heads of 256 behind 32000: 65 us).
 // Many rows: 4 waves of 32 rows share double-buffered tiles of BN keys.
 template <typename T, int D, int BN>
 __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
@@ -824,8 +834,8 @@ __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunc
       else if (a.lse) *rows.lse(base + row) = LN2 * (w.m + __builtin_amdgcn_logf(l));
     }
     // The outputs through LDS, DC columns of a wave's rows at a time, so that lanes side by side
-    // store what lies side by side: from the registers a store touches 32 rows, 32 bytes of each,
-    // and 128 rows of 256 took 4.3 us.
+    // store what lies side by side: from the registers a store touches 32 rows, 32 bytes of each
+    // (48 nodes behind 32000 positions, heads of 256: 70 us so, 66 through LDS).
     float *mine = (float *)(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += DC) {
@@ -855,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunc
 // a row's chunks and their weights, into LDS; then each thread adds 16 bytes of a
 // row's outputs, or, with fewer of those than threads, a share of its chunks. So
 // the trips to memory are few however many rows a workgroup has: one after the
-// other they took 28 us of a batch of 580 nodes.
+// other they took 28 us of a batch of 580 nodes, now 14; 33 chunks of one node take 6.4.
 constexpr int JOIN_HEADS = 32;
 template <typename T, int D, int LR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int hpw) {

@@ -58,8 +58,9 @@ __device__ __forceinline__ void turn(float &x, float &y, float2 cs) {
 // Grid (tokens, row groups).  A row is one head of the token: its work items are
 // 8 elements of the passed-through tail or of the turned part, with HALVES two
 // times 8 (both ends of 8 pairs).  One token to a workgroup and its heads over as
-// many as give every thread one item: a decode step of 28 heads takes 3.5 us, 2048
-// tokens of 32/8 heads of 128 42 us (201 MB, 4.8 TB/s, the rate of a copy).
+// many as give every thread one item.  A decode step of 32 heads takes 3.0 us, a launch's
+// own length; 8192 tokens of 32/8 heads of 128 in bf16 38 us (201 MB, 5.2 TB/s: a large
+// copy reaches 4.8).  With several tokens to a workgroup the divisions cost 10 us there.
 template <typename TX, typename TY, bool HALVES>
 __global__ __launch_bounds__(THREADS) void rope_kernel(RopeParams p, RopeTab tab) {
   __shared__ float2 s_cs[128];

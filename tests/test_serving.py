@@ -106,10 +106,10 @@ def test_rope_kv_in_place_refusals():
     """q in place: k and v beside it in the rows of one product, never under its heads."""
     L, r = gpu.lib(), gpu.Rope(128, 64)
 
-    def call(k, v, qs=512 + 1024, T=2, xt=gpu.T_F16, ks=None):
+    def call(k, v, qs=512 + 1152, T=2, xt=gpu.T_F16, ks=None):
         return L.cwen_rope_kv(CTX, r.h, xt, P, qs, k, ks or qs, v, qs, P, qs, kv(), 0, P, P, P, T, 4, None)
-    for k, v in ((P + 1024 - 16, P + 2048), (P + 1024, P + 2048 + 16), (P + 512, P + 2048), (P + 1024, P), (P + 1024, P + 3072 - 16),
-                 (P + 3072 + 512, P + 2048), (P - 16, P + 2048)):
+    for k, v in ((P + 1024 - 16, P + 2048), (P + 1024, P + 2304 + 16), (P + 512, P + 2048), (P + 1024, P), (P + 1024, P + 3328 - 16),
+                 (P + 3328 + 512, P + 2048), (P - 16, P + 2048)):
         assert call(k, v) == EINVAL, (k - P, v - P)
     assert call(P + 1024, P + 2048, ks=1024) == EINVAL
     assert call(P + 1024 - 16, P + 2048, T=1) == EINVAL
