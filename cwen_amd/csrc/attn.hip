@@ -865,12 +865,12 @@ __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunc
 // a row's chunks and their weights, into LDS; then each thread adds 16 bytes of a
 // row's outputs, or, with fewer of those than threads, a share of its chunks. So
 // the trips to memory are few however many rows a workgroup has: one after the
-// other they took 28 us of a batch of 580 nodes, now 14; 33 chunks of one node take 6.4.
+// other they took 28 us of a batch of 580 nodes, now 12; 33 chunks of one node take 6.4.
 constexpr int JOIN_HEADS = 32;
 template <typename T, int D, int LR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p, int rt, int hpw) {
   typedef typename T::elem elem;
-  constexpr int PC = D / 4, CAP = 4096, U = 8;
+  constexpr int PC = D / 4, CAP = 4096, U = 8, Z = 2, C = 4;
   __shared__ float s_w[CAP];
   __shared__ float2 s_ml[JOIN_HEADS];
   __shared__ long long s_first[JOIN_HEADS];
@@ -896,11 +896,13 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
       const int odd = plan.begin(w0) < at0 ? rt : 0;
       float M = -INFINITY, L = 0.f;
       if (n > 1) {
-        for (int x = l; x < n; x += LR) M = fmaxf(M, p.ml[first + (long long)x * step + (x ? 0 : odd)].x);
+        auto ml = [&](int x) { return p.ml[first + (long long)x * step + (x ? 0 : odd)]; };
+        const float2 mine = ml(min(l, n - 1));
+        if (l < n) M = mine.x;
+        for (int x = l + LR; x < n; x += LR) M = fmaxf(M, ml(x).x);
 #pragma unroll
         for (int d = 1; d < LR; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-        for (int x = l; x < n; x += LR)
-          s_w[i * plan.lines + x] = chunk_weight(p.ml[first + (long long)x * step + (x ? 0 : odd)], M, &L);
+        for (int x = l; x < n; x += LR) s_w[i * plan.lines + x] = chunk_weight(x == l ? mine : ml(x), M, &L);
 #pragma unroll
         for (int d = 1; d < LR; d *= 2) L += __shfl_xor(L, d);
       }
@@ -912,46 +914,76 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
       }
     }
     __syncthreads();
-    const int items = nb * PC, shares = max(256 / items, 1);
-    for (int z0 = 0; z0 < items; z0 += 256) {
-      const int z = z0 + tid % (items < 256 ? items : 256), share = items < 256 ? tid / items : 0;
+    auto chunk = [&](int i, int pc, int x) {
+      return *(const float4 *)(p.po + (s_first[i] + (long long)x * step + (x ? 0 : s_odd[i])) * D + 4 * pc);
+    };
+    auto add = [&](float4 &o, float4 v, float f) {
+      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    };
+    auto leave = [&](int i, int pc, float4 o) {
+      const int h = h0 + y0 + i;
+      const float2 ml = s_ml[i];
+      const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+      const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
+      *(typename AttnOps<T>::vec4 *)((elem *)a.o + (long long)t * a.os + h * D + 4 * pc) = e;
+      if (a.lse && pc == 0) a.lse[(long long)t * a.nh + h] = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));
+    };
+    const int items = nb * PC;
+    // Z pieces a thread, C chunks of each under way at a time (16 trees of 16 nodes, heads of 256: 12.0 us;
+    // 4 pieces cost the registers that hold a fifth workgroup on the CU: 17.0; 1 piece of 8 chunks 13.8).
+    if (items >= 256) {
+      for (int z0 = tid; z0 < items; z0 += 256 * Z) {
+        float4 o[Z];
+        int n[Z], most = 0;
+#pragma unroll
+        for (int k = 0; k < Z; ++k) {
+          o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          n[k] = z0 + 256 * k < items ? s_n[(z0 + 256 * k) / PC] : 0;
+          if (n[k] == 1) n[k] = 0;
+          most = max(most, n[k]);
+        }
+        for (int x = 0; x < most; x += C) {
+          float4 v[Z][C];
+#pragma unroll
+          for (int k = 0; k < Z; ++k)
+#pragma unroll
+            for (int u = 0; u < C; ++u) {
+              const int z = min(z0 + 256 * k, items - 1);
+              v[k][u] = chunk(z / PC, z % PC, min(x + u, max(n[k] - 1, 0)));
+            }
+#pragma unroll
+          for (int k = 0; k < Z; ++k)
+#pragma unroll
+            for (int u = 0; u < C; ++u)
+              if (x + u < n[k]) add(o[k], v[k][u], s_w[(z0 + 256 * k) / PC * plan.lines + x + u]);
+        }
+#pragma unroll
+        for (int k = 0; k < Z; ++k)
+          if (n[k]) leave((z0 + 256 * k) / PC, (z0 + 256 * k) % PC, o[k]);
+      }
+    } else {                     // a share of a row's chunks each
+      const int shares = 256 / items, z = tid % items, share = tid / items, i = z / PC, pc = z % PC;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (z < items && share < shares) {
-        const int i = z / PC, pc = z % PC, n = s_n[i] > 1 ? s_n[i] : 0, per = (n + shares - 1) / shares, x1 = min((share + 1) * per, n);
+      if (share < shares) {
+        const int n = s_n[i] > 1 ? s_n[i] : 0, per = (n + shares - 1) / shares, x1 = min((share + 1) * per, n);
         for (int x = share * per; x < x1; x += U) {
           float4 v[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int at = min(x + u, x1 - 1);
-            v[u] = *(const float4 *)(p.po + (s_first[i] + (long long)at * step + (at ? 0 : s_odd[i])) * D + 4 * pc);
-          }
+          for (int u = 0; u < U; ++u) v[u] = chunk(i, pc, min(x + u, x1 - 1));
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if (x + u >= x1) break;
-            const float f = s_w[i * plan.lines + x + u];
-            o.x = fmaf(v[u].x, f, o.x); o.y = fmaf(v[u].y, f, o.y);
-            o.z = fmaf(v[u].z, f, o.z); o.w = fmaf(v[u].w, f, o.w);
-          }
+          for (int u = 0; u < U; ++u)
+            if (x + u < x1) add(o, v[u], s_w[i * plan.lines + x + u]);
         }
       }
-      if (shares > 1) {
-        s_o[tid] = o;
-        __syncthreads();
-        if (share == 0)
-          for (int u = 1; u < shares; ++u) {
-            const float4 v = s_o[tid + u * items];
-            o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-          }
-      }
-      if (z < items && share == 0) {
-        const int i = z / PC, pc = z % PC, h = h0 + y0 + i;
-        if (s_n[i] > 1) {
-          const float2 ml = s_ml[i];
-          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
-          const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
-          *(typename AttnOps<T>::vec4 *)((elem *)a.o + (long long)t * a.os + h * D + 4 * pc) = e;
-          if (a.lse && pc == 0) a.lse[(long long)t * a.nh + h] = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));
+      s_o[tid] = o;
+      __syncthreads();
+      if (share == 0 && s_n[i] > 1) {
+        for (int u = 1; u < shares; ++u) {
+          const float4 v = s_o[tid + u * items];
+          o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
         }
+        leave(i, pc, o);
       }
     }
     __syncthreads();
