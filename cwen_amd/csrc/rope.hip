@@ -19,6 +19,7 @@ struct RopeTab {
   double turns[128];
   float mscale;
   int D, n_rot;
+  int tok;                       // tokens of a workgroup
 };
 
 template <typename T> struct Io;
@@ -55,24 +56,44 @@ __device__ __forceinline__ void turn(float &x, float &y, float2 cs) {
   x = a;
 }
 
-// Grid (tokens, row groups).  A row is one head of the token: its work items are
-// 8 elements of the passed-through tail or of the turned part, with HALVES two
-// times 8 (both ends of 8 pairs).  One token to a workgroup and its heads over as
-// many as give every thread one item.  A decode step of 32 heads takes 3.0 us, a launch's
-// own length; 8192 tokens of 32/8 heads of 128 in bf16 38 us (201 MB, 5.2 TB/s: a large
-// copy reaches 4.8).  With several tokens to a workgroup the divisions cost 10 us there.
-template <typename TX, typename TY, bool HALVES>
+// Work items of a row, one head of a token: 8 elements of the passed-through tail or
+// of the turned part, with HALVES two times 8 (both ends of 8 pairs).
+__host__ __device__ constexpr int rope_items(int D, int n_rot, bool halves) { return (D - n_rot) / 8 + n_rot / (halves ? 16 : 8); }
+
+// A thread has one item.  Grid (tokens, row groups), or, where the rows of three tokens and
+// more fit a workgroup, (groups of tok tokens, 1): about one workgroup starts a ns, so 8192
+// tokens of 5/1 heads of 128 take 9.3 us instead of 13.6, 100000 of one head of 64 12 instead
+// of 56 (two tokens to a workgroup lose to one in f32: 16 heads of 64 15 against 12.5).  A
+// decode step of 32 heads takes 3.2 us, a launch's own length; 8192 tokens of 32/8
+// heads of 128 in bf16 32 us (201 MB, 6.3 TB/s: a large copy reaches 4.8).
+template <typename TX, typename TY, bool HALVES, bool GROUP>
 __global__ __launch_bounds__(THREADS) void rope_kernel(RopeParams p, RopeTab tab) {
-  __shared__ float2 s_cs[128];
-  const int np = tab.n_rot / 2, D = tab.D, t = blockIdx.x;
-  if (threadIdx.x < np) {
-    const double a = (double)p.pos[t] * tab.turns[threadIdx.x];
+  __shared__ float2 s_cs[GROUP ? 2048 : 128];   // tok n_rot / 2 <= 256 / items * 8 items
+  const int np = tab.n_rot / 2, D = tab.D, tok = GROUP ? tab.tok : 1, t0 = blockIdx.x * tok, nt = min(tok, p.T - t0);
+  const int items = rope_items(D, tab.n_rot, HALVES), per = THREADS / items, turned = tab.n_rot / (HALVES ? 16 : 8);
+  const int n_kv = p.k ? p.kv.n_kv_head : 0, H = p.nh + 2 * n_kv;
+  const int r = threadIdx.x / items, c = threadIdx.x - r * items, lt = GROUP ? r / H : 0, t = t0 + lt;
+  const int h = GROUP ? r - lt * H : blockIdx.y * per + r;
+  const bool live = (int)threadIdx.x < per * items && h < H && lt < nt, both = HALVES && c < turned;
+  const int d = HALVES && !both ? tab.n_rot + 8 * (c - turned) : 8 * c;      // the first element
+  float x[8], y[8];
+  auto load = [&]() {
+    const int hk = h - p.nh;
+    const TX *src = hk < 0 ? (const TX *)p.q + t * p.q_ts + h * p.q_hs
+                    : hk < n_kv ? (const TX *)p.k + t * p.k_ts + (long long)hk * D : (const TX *)p.v + t * p.v_ts + (long long)(hk - n_kv) * D;
+    Io<TX>::load(src + d, x);
+    if (both) Io<TX>::load(src + np + d, y);
+  };
+  if (GROUP && live) load();
+  for (int i = threadIdx.x; i < nt * np; i += THREADS) {
+    const int u = GROUP ? i / np : 0;
+    const double a = (double)p.pos[t0 + u] * tab.turns[i - u * np];
     float sn, cs;
     sincospif(2.f * (float)(a - rint(a)), &sn, &cs);
-    s_cs[threadIdx.x] = make_float2(cs * tab.mscale, (p.inverse ? -sn : sn) * tab.mscale);
+    s_cs[i] = make_float2(cs * tab.mscale, (p.inverse ? -sn : sn) * tab.mscale);
   }
   long long row = -1;            // element offset of the token's cache row of head 0; < 0: none
-  if (p.k) {
+  if (p.k && live) {
     const int s = p.seq[t], slot = p.slot[t];
     if (slot >= 0) {
       bool bad = (unsigned)s >= (unsigned)p.kv.max_seqs;
@@ -87,63 +108,38 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeParams p, RopeTab tab
       }
       if (bad) {
         row = -1;
-        if (blockIdx.y == 0 && threadIdx.x == 0) kv_raise(p.kv, CWEN_KV_ARG);
+        if (h == 0 && c == 0) kv_raise(p.kv, CWEN_KV_ARG);
       }
     }
   }
   __syncthreads();
-
-  const int n_kv = p.k ? p.kv.n_kv_head : 0, H = p.nh + 2 * n_kv;
-  const int turned = HALVES ? tab.n_rot / 16 : tab.n_rot / 8;
-  const int items = turned + (D - tab.n_rot) / 8;          // of one row
-  const int per = THREADS / items;                          // rows side by side
-  const int c = threadIdx.x % items;
-  for (int h = blockIdx.y * per + threadIdx.x / items; h < H; h += gridDim.y * per) {
-    if ((int)threadIdx.x >= per * items) break;
-    const TX *src;
-    TY *dst;
-    bool rot = c < turned;
-    if (h < p.nh) {
-      src = (const TX *)p.q + t * p.q_ts + h * p.q_hs;
-      dst = (TY *)p.qo + t * p.qo_ts + h * p.qo_hs;
-    } else {
-      if (row < 0) continue;
-      const bool isv = h >= p.nh + n_kv;
-      const int hk = h - p.nh - (isv ? n_kv : 0);
-      src = isv ? (const TX *)p.v + t * p.v_ts + (long long)hk * D : (const TX *)p.k + t * p.k_ts + (long long)hk * D;
-      dst = (TY *)(isv ? p.kv.v : p.kv.k) + row + (long long)hk * p.kv.page * D;
-      rot = rot && !isv;
-    }
-    float x[8];
-    if (HALVES) {
-      if (c < turned) {
-        float y[8];
-        Io<TX>::load(src + 8 * c, x);
-        Io<TX>::load(src + np + 8 * c, y);
-        if (rot)
+  if (!live || (h >= p.nh && row < 0)) return;
+  if (!GROUP) load();
+  const int hk = h - p.nh;
+  const bool isv = hk >= n_kv;
+  TY *dst = hk < 0 ? (TY *)p.qo + t * p.qo_ts + h * p.qo_hs
+                   : (TY *)(isv ? p.kv.v : p.kv.k) + row + (long long)(hk - (isv ? n_kv : 0)) * p.kv.page * D;
+  if (c < turned && !(hk >= 0 && isv)) {
+    if (HALVES)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) turn(x[j], y[j], s_cs[8 * c + j]);
-        Io<TY>::store(dst + 8 * c, x);
-        Io<TY>::store(dst + np + 8 * c, y);
-      } else {
-        const int d = tab.n_rot + 8 * (c - turned);
-        Io<TX>::load(src + d, x);
-        Io<TY>::store(dst + d, x);
-      }
-    } else {
-      Io<TX>::load(src + 8 * c, x);
-      if (rot)
+      for (int j = 0; j < 8; ++j) turn(x[j], y[j], s_cs[lt * np + 8 * c + j]);
+    else
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turn(x[2 * j], x[2 * j + 1], s_cs[4 * c + j]);
-      Io<TY>::store(dst + 8 * c, x);
-    }
+      for (int j = 0; j < 4; ++j) turn(x[2 * j], x[2 * j + 1], s_cs[lt * np + 4 * c + j]);
   }
+  Io<TY>::store(dst + d, x);
+  if (both) Io<TY>::store(dst + np + d, y);
 }
 
 template <typename TX, typename TY>
 void launch(bool halves, dim3 g, const RopeParams &p, const RopeTab &t, hipStream_t st) {
-  if (halves) hipLaunchKernelGGL((rope_kernel<TX, TY, true>), g, dim3(THREADS), 0, st, p, t);
-  else hipLaunchKernelGGL((rope_kernel<TX, TY, false>), g, dim3(THREADS), 0, st, p, t);
+  if (halves) {
+    if (t.tok > 1) hipLaunchKernelGGL((rope_kernel<TX, TY, true, true>), g, dim3(THREADS), 0, st, p, t);
+    else hipLaunchKernelGGL((rope_kernel<TX, TY, true, false>), g, dim3(THREADS), 0, st, p, t);
+  } else {
+    if (t.tok > 1) hipLaunchKernelGGL((rope_kernel<TX, TY, false, true>), g, dim3(THREADS), 0, st, p, t);
+    else hipLaunchKernelGGL((rope_kernel<TX, TY, false, false>), g, dim3(THREADS), 0, st, p, t);
+  }
 }
 template <typename TX>
 void launch_y(int ytype, bool halves, dim3 g, const RopeParams &p, const RopeTab &t, hipStream_t st) {
@@ -161,8 +157,9 @@ int rope_launch(const cwen_rope *r, int xtype, int ytype, const RopeParams &p, h
   t.D = r->head_dim;
   t.n_rot = r->n_rot;
   const int rows = p.nh + (p.k ? 2 * p.kv.n_kv_head : 0);
-  const int per = THREADS * 8 / r->head_dim;
-  const dim3 g((unsigned)p.T, (unsigned)((rows + per - 1) / per));
+  const int per = THREADS / rope_items(r->head_dim, r->n_rot, r->layout == CWEN_ROPE_HALVES);
+  t.tok = per / rows >= 3 ? per / rows : 1;
+  const dim3 g((unsigned)((p.T + t.tok - 1) / t.tok), (unsigned)((rows + per - 1) / per));
   const bool halves = r->layout == CWEN_ROPE_HALVES;
   if (xtype == CWEN_T_F32) launch_y<float>(ytype, halves, g, p, t, st);
   else if (xtype == CWEN_T_F16) launch_y<TypeF16::elem>(ytype, halves, g, p, t, st);

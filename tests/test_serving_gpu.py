@@ -408,6 +408,34 @@ def test_rope_kv(env, src, typ, page, layout):
 
 
 @pytest.mark.parametrize("layout", ["pairs", "halves"])
+@pytest.mark.parametrize("T", [1, 2, 7, 301])
+def test_rope_small_rows_share_workgroups(env, layout, T):
+    """Few heads: several tokens to a workgroup; many: one.  The same bits, the same refusals, padding
+    and bad tokens among the others."""
+    gpu, ctx = env
+    g, D, K = gen(T), 64, 1
+    r = gpu.Rope(head_dim=D, n_rot=48, theta=1e4, layout=layout)
+    q, k, v = randn(g, T, 40, D, dtype=F16), randn(g, T, K, D, dtype=F16), randn(g, T, K, D, dtype=F16)
+    pos = torch.randint(0, 1 << 30, (T,), device="cuda", dtype=torch.int32, generator=g)
+    rng = random.Random(T)
+    slot = [rng.choice([i, i, i, i, -1, 10 ** 6]) for i in range(T)]
+    seq = [rng.choice([1, 1, 1, 1, 1, 7, -3]) for _ in range(T)]
+    got = []
+    for H in (40, 1, 2, 5):
+        kv = gpu.PagedKV.empty(1, K, D, 16, 20, 2, 20, BF16)
+        kv.reserve(ctx, ints([1]), ints([T]))
+        qo = torch.empty(T, H, D, device="cuda", dtype=BF16)
+        gpu.rope_kv(ctx, r, q[:, :H].contiguous(), k, v, qo, kv, 0, ints(seq), ints(slot), pos)
+        y = torch.empty(T, H, D, device="cuda", dtype=F32)
+        gpu.rope(ctx, r, q[:, :H], y, pos, inverse=True)
+        got.append((qo, y, kv.k, kv.v, kv.take_status(ctx)))
+    for H, one in zip((1, 2, 5), got[1:]):
+        assert torch.equal(one[0], got[0][0][:, :H]) and torch.equal(one[1], got[0][1][:, :H])
+        assert torch.equal(one[2], got[0][2]) and torch.equal(one[3], got[0][3]) and one[4] == got[0][4]
+    assert (got[0][4] != 0) == any(s >= 0 and (s > 10 ** 5 or i != 1) for s, i in zip(slot, seq))
+
+
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
 def test_rope_kv_in_place(env, layout):
     """q turned where it lies, k and v beside it in the same rows: what two tensors give."""
     gpu, ctx = env
