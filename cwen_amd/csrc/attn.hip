@@ -308,8 +308,9 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int s) {
   if (q.bad) {
     q.id = q.len = q.keys = 0;
   } else {
-    q.len = a.kv.len[q.id];
-    q.keys = kv_readable(q.len, q.nodes, a.kv.held[q.id], a.kv.page, a.kv.max_pages, &q.bad);
+    const int len = a.kv.len[q.id];
+    q.keys = kv_readable(len, q.nodes, a.kv.held[q.id], a.kv.page, a.kv.max_pages, &q.bad);
+    q.len = kv_cached(len, q.keys);       // what the masks' words are counted by
   }
   return q;
 }

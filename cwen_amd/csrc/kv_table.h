@@ -40,6 +40,9 @@ KV_FN int kv_readable(int len, int extra, int held, int page, int max_pages, boo
   *bad = true;
   return (int)most;
 }
+// The part of a claimed length that lies below the `keys` positions of kv_readable, so that
+// 0 <= keys - kv_cached <= extra whatever the state claims.
+KV_FN int kv_cached(int len, int keys) { return len < 0 ? 0 : len < keys ? len : keys; }
 // The element offset of (layer, page, head, row) of the pools.
 KV_FN int64_t kv_at(int layer, int pg, int head, int row, int n_pages, int n_kv_head, int page, int head_dim) {
   return ((((int64_t)layer * n_pages + pg) * n_kv_head + head) * page + row) * head_dim;

@@ -214,3 +214,30 @@ def test_page_arithmetic(pages):
         assert n == want and bool(bad.value) == (n != len_ + extra), (len_, extra, held)
     # offsets past 32 bits
     assert L.at(15, (1 << 24) - 1, 7, 255, 1 << 24, 8, 256, 256) == (((15 * 2 ** 24 + 2 ** 24 - 1) * 8 + 7) * 256 + 255) * 256
+
+
+BAD_STATE = r"""
+#include "kv_table.h"
+extern "C" int drafted(int len, int extra, int held, int page, int max_pages) {
+  bool b = false;
+  const int keys = kv_readable(len, extra, held, page, max_pages, &b);
+  return keys - kv_cached(len, keys); }
+"""
+
+
+def harness(tmp_path, source):
+    (tmp_path / "h.cpp").write_text(source)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", f"-I{ROOT / 'cwen_amd' / 'csrc'}", str(tmp_path / "h.cpp"), "-o", str(tmp_path / "h.so")],
+                   check=True)
+    return C.CDLL(str(tmp_path / "h.so"))
+
+
+def test_drafted_keys_of_bad_lengths(tmp_path):
+    """The keys that a tree's masks are read for: as many as the group has nodes at most, and none of a
+    sequence whose length is no length."""
+    L, big = harness(tmp_path, BAD_STATE), 2 ** 31 - 1
+    for extra in (0, 1, 64, 256):
+        for held in (-1, 0, 1, 8, 9):
+            for len_ in (-2 ** 31, -100000, -1, 0, 1, 15, 16, 127, 128, 129, 100000, big - 256, big):
+                n, fits = L.drafted(len_, extra, held, 16, 8), 0 <= held <= 8 and 0 <= len_ and len_ + extra <= 16 * held
+                assert 0 <= n <= extra and (n == extra or not fits) and (n == 0 or len_ >= 0), (len_, extra, held, n)

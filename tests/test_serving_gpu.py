@@ -1062,3 +1062,28 @@ def test_a_request_from_prompt_to_branch(env, typ, H, K, D, page):
     a, b = gather(kv, 2, 134)
     assert torch.equal(a[0, 130:], tkr[[0, 2, 5, 7]]) and torch.equal(b[0, 130:], tv[[0, 2, 5, 7]].to(typ))
     assert torch.equal(a[0, :130], rows[0][1]) and torch.equal(b[0, :130], rows[1][1])
+
+
+# ---------------------------------------------------------------- state that is no state
+@pytest.mark.parametrize("H,K,D,n", [(4, 2, 64, 3), (12, 2, 128, 40), (6, 1, 256, 33)])
+def test_tree_lengths_that_are_none(env, H, K, D, n):
+    """A length below 0 or past the pages raises the flag in every form, with masks and without; the
+    other groups are those of the formula and nothing outside the group is written."""
+    gpu, ctx = env
+    lens, nodes, g = [50, 80, 300], [n, n, n], gen(n)
+    kv = tree_cache(gpu, ctx, g, F16, K, D, 16, lens, nodes, L=1)
+    q = randn(g, 3 * n, H, D, dtype=F16)
+    bits = [b for m in nodes for b in random_tree(random.Random(n), m, 1)]
+    for bad in (-1, -100000, -2 ** 31, 2 ** 31 - 1):
+        for mask in (bits, None):
+            c = gpu.PagedKV(16, kv.k, kv.v, kv.table, kv.len.clone(), kv.held, kv.ref)
+            c.len[1] = bad
+            o = torch.full((3 * n + 1, H, D), 7.0, device="cuda", dtype=F16)
+            gpu.attn_tree(ctx, c, 0, q, o[:-1], ints([0, 1, 2]), ints([0, n, 2 * n, 3 * n]), n, 300,
+                          mask=None if mask is None else as_words(mask, 1))
+            assert c.take_status(ctx) == gpu.KV_PAGE, bad
+            assert bool((o[-1] == 7).all())
+            for s in (0, 2):
+                view = gpu.PagedKV(16, kv.k, kv.v, kv.table[s:], kv.len[s:], kv.held[s:], kv.ref)
+                a, b = s * n, (s + 1) * n
+                check_tree(view, 0, q[a:b], o[a:b], None, lens[s:s + 1], [n], None if mask is None else bits[a:b], F16, heads=[0, H - 1])
