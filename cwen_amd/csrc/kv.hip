@@ -84,19 +84,18 @@ __global__ __launch_bounds__(256) void kv_truncate_kernel(cwen_kv kv, const int 
     if (threadIdx.x == 0) kv_raise(kv, CWEN_KV_ARG);
     return;
   }
-  const int s = seqs[i], to = len ? len[i] : 0, cur = kv.len[s];
-  bool bad = to < 0 || to > cur;
-  const int held = kv_held_ok(kv.held[s], kv.max_pages, &bad);
+  const int s = seqs[i], to = len ? len[i] : 0;
+  bool bad = false;
+  const int held = kv_held_ok(kv.held[s], kv.max_pages, &bad), pages = kv_cut(to, kv.len[s], held, kv.page);
   __syncthreads();                               // every thread has read len and held
-  if (bad) {
+  if (bad || pages < 0) {
     if (threadIdx.x == 0) kv_raise(kv, CWEN_KV_ARG);
     return;
   }
-  const int pages = kv_cover(to, kv.page);
   release_from<256>(kv, s, pages, held);
   if (threadIdx.x == 0) {
     kv.len[s] = to;
-    kv.held[s] = min(pages, held);
+    kv.held[s] = pages;
   }
 }
 

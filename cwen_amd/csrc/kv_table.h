@@ -15,6 +15,11 @@ KV_FN int kv_cover(int n, int page) { return (n + page - 1) / page; }
 KV_FN bool kv_fits(int len, int n, int page, int max_pages) {
   return len >= 0 && n >= 0 && (int64_t)len + n <= (int64_t)max_pages * page;
 }
+// Pages that a cut of a sequence of `cur` positions to `to` leaves of its `held` ones, or -1
+// when it cannot be made: `cur` may claim more than the pages hold.
+KV_FN int kv_cut(int to, int cur, int held, int page) {
+  return to > cur || !kv_fits(to, 0, page, held) ? -1 : kv_cover(to, page);
+}
 // A table entry as an index that is safe to use; *bad when it is none.
 KV_FN int kv_page_ok(int entry, int n_pages, bool *bad) {
   if ((unsigned)entry < (unsigned)n_pages) return entry;

@@ -241,3 +241,15 @@ def test_drafted_keys_of_bad_lengths(tmp_path):
             for len_ in (-2 ** 31, -100000, -1, 0, 1, 15, 16, 127, 128, 129, 100000, big - 256, big):
                 n, fits = L.drafted(len_, extra, held, 16, 8), 0 <= held <= 8 and 0 <= len_ and len_ + extra <= 16 * held
                 assert 0 <= n <= extra and (n == extra or not fits) and (n == 0 or len_ >= 0), (len_, extra, held, n)
+
+
+def test_cuts_of_bad_lengths(tmp_path):
+    """What a cut leaves is never more than the pages held, nor an index before the first."""
+    L = harness(tmp_path, '#include "kv_table.h"\nextern "C" int cut(int to, int cur, int held, int page) { return kv_cut(to, cur, held, page); }')
+    some = (-2 ** 31, -1, 0, 1, 16, 17, 64, 65, 2 ** 30, 2 ** 31 - 16, 2 ** 31 - 1)
+    for page in (16, 256):
+        for held in (0, 1, 4, 2 ** 20):
+            for cur in some:
+                for to in some:
+                    want = -(-to // page) if 0 <= to <= min(cur, held * page) else -1
+                    assert L.cut(to, cur, held, page) == want, (to, cur, held, page)

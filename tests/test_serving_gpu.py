@@ -1087,3 +1087,21 @@ def test_tree_lengths_that_are_none(env, H, K, D, n):
                 view = gpu.PagedKV(16, kv.k, kv.v, kv.table[s:], kv.len[s:], kv.held[s:], kv.ref)
                 a, b = s * n, (s + 1) * n
                 check_tree(view, 0, q[a:b], o[a:b], None, lens[s:s + 1], [n], None if mask is None else bits[a:b], F16, heads=[0, H - 1])
+
+
+def test_truncate_of_a_length_past_its_pages(env):
+    """A corrupt length: a cut that its pages do not hold is refused and changes nothing, in its own row
+    of the table or a neighbour's; one that they hold makes the sequence whole again."""
+    gpu, ctx = env
+    kv = gpu.PagedKV.empty(1, 1, 64, 16, 40, 3, 10, F16)
+    kv.reserve(ctx, ints([0, 1, 2]), ints([160, 40, 90]))
+    kv.keep(ctx, ints([0, 1, 2]), ints([160, 40, 90]))
+    kv.len[1] = 2 ** 31 - 1
+    before = [t.clone() for t in (kv.table, kv.len, kv.held, kv.ref)]
+    for to in (2 ** 31 - 1, 2 ** 31 - 16, 49, -2 ** 31):
+        kv.truncate(ctx, ints([1]), ints([to]))
+        assert kv.take_status(ctx) == gpu.KV_ARG
+        assert all(torch.equal(a, b) for a, b in zip(before, (kv.table, kv.len, kv.held, kv.ref))), to
+    kv.truncate(ctx, ints([1, 2]), ints([20, 90]))
+    assert kv.take_status(ctx) == 0 and kv.len.tolist() == [160, 20, 90] and kv.held.tolist() == [10, 2, 6]
+    assert int((kv.ref > 0).sum()) == 18 and int(kv.table[1, 2]) == -1 and torch.equal(kv.table[0], before[0][0])
