@@ -359,7 +359,7 @@ struct TreePlan {
       if ((s0 += 64) >= a.n_seq) break;
       m = load(a, s0);
     }
-    levels = want > 1 && sum == one * want ? want : 1;
+    levels = want > 1 && sum == one * want ? want : 1;   // no group has more than `want`: all have as many
     total = levels > 1 ? one : sum;
     lines = min(most / levels, total);
   }
@@ -415,7 +415,7 @@ __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int
 }
 
 struct TreeLaunch {
-  int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most
+  int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most, or 1
   int extra;                    // units that a row tile counts beyond its keys
   float *po;                    // partial outputs [kv head][2 lines][row][D]: piece w's first row tile, its last
   float2 *ml;                   // and their maxima and sums [kv head][2 lines][row]
@@ -1052,7 +1052,7 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   p.count = form == 1 && chunks * rows <= 96 && (long long)nkv * a.n_seq <= ctx->ncounters ? ctx->counters : nullptr;
   p.po = ctx->attn_part + (((size_t)nkv * p.lines * 2 * rt * 2 + 3) & ~(size_t)3);
   const long long tiles = (rows + rt - 1) / rt;                  // of one group at most
-  p.levels = (int)std::min(tiles, (long long)p.lines);
+  p.levels = tree_levels(tiles, p.lines);
   const long long blocks = 8ll * std::max((long long)p.levels * (((long long)nkv * (p.lines / p.levels) + 7) / 8),
                                           ((long long)nkv * p.lines + 7) / 8);
   // Every line's positions fit 32 bits.

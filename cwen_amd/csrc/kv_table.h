@@ -52,3 +52,7 @@ KV_FN int kv_cached(int len, int keys) { return len < 0 ? 0 : len < keys ? len :
 KV_FN int64_t kv_at(int layer, int pg, int head, int row, int n_pages, int n_kv_head, int page, int head_dim) {
   return ((((int64_t)layer * n_pages + pg) * n_kv_head + head) * page + row) * head_dim;
 }
+// Lines of the tree attention's keys (one for each row tile of a group) when a group has `tiles` of
+// them at most and there are `pieces` workgroups: as many as tiles, or one.  With fewer lines than
+// tiles, groups of unequal tiles could add up to what equal ones do.
+KV_FN int tree_levels(int64_t tiles, int pieces) { return tiles <= pieces ? (int)tiles : 1; }

@@ -253,3 +253,19 @@ def test_cuts_of_bad_lengths(tmp_path):
                 for to in some:
                     want = -(-to // page) if 0 <= to <= min(cur, held * page) else -1
                     assert L.cut(to, cur, held, page) == want, (to, cur, held, page)
+
+
+def test_levels_are_taken_for_equal_groups_only(tmp_path):
+    """The tree attention gives each row tile a line of its own when the groups' tiles, weighed by their keys,
+    add up to as many as equal groups have: no mixture of up to `tiles` may reach that."""
+    L = harness(tmp_path, '#include "kv_table.h"\nextern "C" int levels(long long tiles, int pieces) { return tree_levels(tiles, pieces); }')
+    L.levels.argtypes = [C.c_longlong, C.c_int]
+    for tiles in range(1, 40):
+        for pieces in range(1, 40):
+            n = L.levels(tiles, pieces)
+            assert n == tiles <= pieces or n == 1, (tiles, pieces)
+            for a in range(1, tiles + 1):
+                for b in range(1, tiles + 1):
+                    equal = n > 1 and 3 * a + 5 * b == (3 + 5) * n     # groups of 3 and of 5 units
+                    assert not equal or a == b == n
+    assert L.levels(2 ** 33, 1024) == 1

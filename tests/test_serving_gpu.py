@@ -1105,3 +1105,15 @@ def test_truncate_of_a_length_past_its_pages(env):
     kv.truncate(ctx, ints([1, 2]), ints([20, 90]))
     assert kv.take_status(ctx) == 0 and kv.len.tolist() == [160, 20, 90] and kv.held.tolist() == [10, 2, 6]
     assert int((kv.ref > 0).sum()) == 18 and int(kv.table[1, 2]) == -1 and torch.equal(kv.table[0], before[0][0])
+
+
+@pytest.mark.parametrize("H,K,D,lens,nodes", [(384, 192, 128, [936, 808], [64, 192]), (384, 192, 128, [900, 900, 900], [64, 192, 128]),
+                                              (512, 128, 128, [500, 500], [64, 192]), (800, 400, 64, [700, 600], [20, 200])])
+def test_tree_row_tiles_that_average_the_pieces(env, H, K, D, lens, nodes):
+    """Fewer pieces than a group has row tiles, and groups whose tiles add up to those of equal ones."""
+    gpu, ctx = env
+    g = gen(H)
+    kv = tree_cache(gpu, ctx, g, F16, K, D, 64, lens, nodes, L=1)
+    q = randn(g, sum(nodes), H, D, dtype=F16)
+    o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, None)
+    check_tree(kv, 0, q, o, z, lens, nodes, None, F16, heads=[0, H // 2 - 1, H - 1])
