@@ -414,6 +414,22 @@ __device__ __forceinline__ uint32_t tree_sees(const unsigned long long *row, int
   return (uint32_t)(w << before) | (uint32_t)((1ull << before) - 1);
 }
 
+// A share of a row's keys leaves its maximum and sum {m, l}; the score that set a finite maximum adds
+// about 1 to the sum (the maximum's own rounding away).  With a maximum of -inf, l is 0 where the row saw
+// none of the keys, LOWEST where all that it saw have scores of -inf, and NaN.  Such keys weigh
+// nothing beside others, and 2^-100 is lost in their sum; a row that sees no others, whose
+// sum is then that of up to 1024 shares, is NaN (0 / 0), its lse -inf.
+constexpr float LOWEST = 0x1p-100f;
+__device__ __forceinline__ float share_sum(bool saw, float l) { return saw && l == 0.f ? LOWEST : l; }
+// How a share's sums count against the row's maximum M (NaN stays), and what it adds to the row's sum.
+__device__ __forceinline__ float chunk_weight(float2 ml, float M, float *sum) {
+  const float f = ml.x == -INFINITY ? 0.f * ml.y : __builtin_amdgcn_exp2f(ml.x - M);
+  *sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+  return f;
+}
+// What a row's sums are multiplied by.
+__device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : l < 0x1p-80f ? NAN : 1.f / l; }
+
 struct TreeLaunch {
   int lines, levels;            // pieces of a kv head, of all levels; row tiles of a group at most, or 1
   int extra;                    // units that a row tile counts beyond its keys
@@ -483,17 +499,10 @@ template <typename T, int D> struct TreeRows {
     }
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) po[lane * (D / 64) + e] = x.acc[e];
-    if (lane == 0) *ml = make_float2(x.m, x.sees && x.l == 0.f ? NAN : x.l);
+    if (lane == 0) *ml = make_float2(x.m, share_sum(x.sees, x.l));
   }
 };
 
-// A chunk's share of a row: how its sums count against the row's maximum M (NaN
-// stays), and what it adds to the row's sum.
-__device__ __forceinline__ float chunk_weight(float2 ml, float M, float *sum) {
-  const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : __builtin_amdgcn_exp2f(ml.x - M);
-  *sum += ml.x == -INFINITY ? f : ml.y * f;
-  return f;
-}
 // Values that other workgroups of this launch wrote: at the device's coherence point.
 __device__ __forceinline__ void put2(void *p, float x, float y) {
   __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -597,7 +606,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
     while (t0 < end) step(std::true_type{});
     if (bad) kv_raise(a.kv, CWEN_KV_PAGE);
     const float l = w.sum();
-    if (lane < 32) s_ml[wave][n] = make_float2(w.m, saw && l == 0.f ? NAN : l);
+    if (lane < 32) s_ml[wave][n] = make_float2(w.m, share_sum(saw != 0, l));
     const bool whole = count == item.units;
     const size_t slot = ((size_t)hkv * 2 * p.lines + 2 * (piece * plan.levels + me.level) + !first) * 32;
     auto join = [&]() __attribute__((always_inline)) {
@@ -646,7 +655,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
             }
           }
           const float2 ml = s_ml[0][y];
-          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+          const float inv = row_scale(ml.y);
           const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
           *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
           if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));
@@ -686,7 +695,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
 #pragma unroll
       for (int u = 0; u < NW; ++u) Mr = fmaxf(Mr, s_ml[u][y].x);
 #pragma unroll
-      for (int u = 0; u < NW; ++u) L += s_ml[u][y].x == -INFINITY ? s_ml[u][y].y : s_ml[u][y].y * __builtin_amdgcn_exp2f(s_ml[u][y].x - Mr);
+      for (int u = 0; u < NW; ++u) chunk_weight(s_ml[u][y], Mr, &L);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int u = 0; u < NW; ++u) {
@@ -694,7 +703,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
       }
       if (whole) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = row_scale(L);
         const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
         *(typename AttnOps<T>::vec4 *)(rows.out(base + y) + 4 * pc) = e;
         if (pc == 0 && a.lse) *rows.lse(base + y) = LN2 * (Mr + __builtin_amdgcn_logf(L));
@@ -829,9 +838,9 @@ __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunc
     int me_lane = lane;                               // opaque: its addresses are not kept through the tiles
     asm volatile("" : "+v"(me_lane));
     const int row = me_lane & 31, half = me_lane >> 5, pc = me_lane % PC;
-    const float l = w.sum(), ls = saw && l == 0.f ? NAN : l, inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+    const float l = share_sum(saw != 0, w.sum()), inv = whole ? row_scale(l) : 1.f;
     if (me_lane < min(R, 32)) {
-      if (!whole) p.ml[slot + row] = make_float2(w.m, ls);
+      if (!whole) p.ml[slot + row] = make_float2(w.m, l);
       else if (a.lse) *rows.lse(base + row) = LN2 * (w.m + __builtin_amdgcn_logf(l));
     }
     // The outputs through LDS, DC columns of a wave's rows at a time, so that lanes side by side
@@ -925,7 +934,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, TreeLaunch p
     auto leave = [&](int i, int pc, float4 o) {
       const int h = h0 + y0 + i;
       const float2 ml = s_ml[i];
-      const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+      const float inv = row_scale(ml.y);
       const typename AttnOps<T>::vec4 e = {(elem)(o.x * inv), (elem)(o.y * inv), (elem)(o.z * inv), (elem)(o.w * inv)};
       *(typename AttnOps<T>::vec4 *)((elem *)a.o + (long long)t * a.os + h * D + 4 * pc) = e;
       if (a.lse && pc == 0) a.lse[(long long)t * a.nh + h] = LN2 * (ml.x + __builtin_amdgcn_logf(ml.y));

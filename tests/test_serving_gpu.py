@@ -1117,3 +1117,46 @@ def test_tree_row_tiles_that_average_the_pieces(env, H, K, D, lens, nodes):
     q = randn(g, sum(nodes), H, D, dtype=F16)
     o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, None)
     check_tree(kv, 0, q, o, z, lens, nodes, None, F16, heads=[0, H // 2 - 1, H - 1])
+
+
+# ---------------------------------------------------------------- shares of a row that hold only scores of -inf
+@pytest.mark.parametrize("lens,nodes,at", [([32], [1], {0: [32]}), ([700], [2], {0: range(128, 256)}), ([700, 33], [3, 1], {0: range(700), 1: range(33)}),
+                                           ([700, 0], [2, 2], {0: range(702), 1: [0]}), ([2500], [3], {0: [2500, 2502]})],
+                         ids=["a wave", "a unit", "all cached", "all", "nodes"])
+@pytest.mark.parametrize("H,K,D,hint", [(6, 1, 256, 2500), (4, 1, 64, 200), (40, 2, 128, 2500), (24, 2, 128, 0)])
+def test_tree_scores_of_minus_infinity(env, H, K, D, hint, lens, nodes, at):
+    """Visible keys whose scores are -inf weigh nothing, wherever the keys are cut; a row that
+    sees no others is NaN with lse -inf, and so is a dim where a value of weight 0 is NaN.  Also with
+    a hidden NaN, which takes the rows one by one."""
+    gpu, ctx = env
+    for odd in (False, True):
+        g = gen(91)
+        kv = tree_cache(gpu, ctx, g, F16, K, D, 64, lens, nodes, L=1)
+        row = lambda pool, s, r: pool[:, int(kv.table[s, r // 64]), :, r % 64]
+        for s, rows in at.items():
+            for r in rows:
+                row(kv.k, s, r)[..., 0] = -math.inf
+        if odd:                                                # the last node of each group is hidden from the others
+            for s, (m, n) in enumerate(zip(lens, nodes)):
+                if n > 1:
+                    row(kv.v, s, m + n - 1)[..., 3] = float("nan")
+        q = randn(g, sum(nodes), H, D, dtype=F16)
+        q[..., 0] = 1
+        o, z = run_tree(gpu, ctx, kv, 0, q, lens, nodes, None, max_len=hint)
+        a = 0
+        for s, (m, n) in enumerate(zip(lens, nodes)):
+            j = torch.arange(m + n, device="cuda")
+            pg = kv.table[s, j // 64].long()
+            k, v = kv.k[0][pg, :, j % 64], kv.v[0][pg, :, j % 64]
+            sees = j[None] <= m + torch.arange(n, device="cuda")[:, None]
+            counts = torch.isfinite(k[:, 0, 0])[None] & sees
+            for h in (0, H - 1):
+                w = R.attention(q[a:a + n, h], k[:, h // (H // K)].nan_to_num(neginf=0), v[:, h // (H // K)], counts, D ** -0.5)
+                eo, el = R.attention_bounds(*w, m + n, D, F16)
+                some = counts.any(1)
+                nan = ((sees & ~counts).float() @ torch.isnan(v[:, h // (H // K)]).float()) > 0       # 0 * NaN
+                want = torch.where(some[:, None] & ~nan, w[0], torch.full_like(w[0], float("nan")))
+                close(o[a:a + n, h], want, eo, ("o", odd, s, h))
+                close(z[a:a + n, h], w[1], el, ("lse", odd, s, h))
+            a += n
+        assert kv.take_status(ctx) == 0
