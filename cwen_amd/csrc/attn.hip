@@ -1049,8 +1049,8 @@ int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st) {
   const int per_cu = form == 1 ? 256 / D : D == 64 ? 3 : 2;      // workgroups that a CU holds at once
   TreeLaunch p;
   p.extra = D == 256 ? 1 : 2;                                    // the units of 256 take twice as long
+  // One piece a KV head at least: it holds whole rows and leaves no partials, so it needs no room.
   p.lines = (int)std::max(1ll, std::min((long long)per_cu * ctx->ncu / nkv, room));
-  if (room < 1) return CWEN_ESCRATCH;
   p.ml = (float2 *)ctx->attn_part;
   // Up to 96 (row, chunk) partials of a group are joined in the launch: one token of 6 heads behind 1000
   // positions 14.6 us so, 16.1 in two launches; behind 2600 17.1 and 16.0.  Of many groups one is taken

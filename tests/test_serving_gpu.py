@@ -1160,3 +1160,15 @@ def test_tree_scores_of_minus_infinity(env, H, K, D, hint, lens, nodes, at):
                 close(z[a:a + n, h], w[1], el, ("lse", odd, s, h))
             a += n
         assert kv.take_status(ctx) == 0
+
+
+# ---------------------------------------------------------------- more KV heads than the partials' scratch has room for
+@pytest.mark.parametrize("K,D,nodes", [(600, 256, 40), (2400, 256, 3), (2300, 64, 70)])
+def test_tree_more_heads_than_the_scratch_holds(env, K, D, nodes):
+    """One workgroup then takes all of a head's rows and leaves no partials."""
+    gpu, ctx = env
+    g, lens, n = gen(K), [150, 3], [nodes, 1]
+    kv = tree_cache(gpu, ctx, g, BF16, K, D, 16, lens, n, L=1)
+    q = randn(g, sum(n), K, D, dtype=BF16)
+    o, z = run_tree(gpu, ctx, kv, 0, q, lens, n, None)
+    check_tree(kv, 0, q, o, z, lens, n, None, BF16, heads=[0, 7, K - 1])
