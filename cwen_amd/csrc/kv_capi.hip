@@ -234,7 +234,7 @@ int cwen_kv_status(cwen_ctx *ctx, const cwen_kv *kv, int *bits, void *stream) {
 // ------------------------------------------------------------ attention
 static int check_heads(int nh, int nkv, int D, float scale) {
   if (nh < 1 || nkv < 1 || nh > 65535 || nh % nkv || (D != 64 && D != 128 && D != 256)) return CWEN_EINVAL;
-  return scale > 0 && isfinite(scale) ? CWEN_OK : CWEN_EINVAL;
+  return scale > 0 && isfinite(scale * 1.44269504f) ? CWEN_OK : CWEN_EINVAL;     // exponents are powers of two
 }
 
 int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, const void *k, long long k_ts, const void *v,

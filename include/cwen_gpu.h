@@ -342,7 +342,7 @@ int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, lo
  * cores, the probabilities rounded to the operands' type before their product
  * with v, the output rounded once.  n_head a multiple of n_kv_head (query head
  * h reads KV head h / (n_head / n_kv_head)), head_dim 64, 128 or 256, scale >
- * 0 and finite.  Heads of a token are in a row ([head][head_dim]), tokens
+ * 0 and below 2^127.  Heads of a token are in a row ([head][head_dim]), tokens
  * `stride` elements apart; pointers 16-byte aligned, strides multiples of 8
  * (those of k and v below 2^27).
  * lse (nullable, f32 [token][n_head]): the natural log of the row's sum of

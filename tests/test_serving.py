@@ -269,3 +269,15 @@ def test_levels_are_taken_for_equal_groups_only(tmp_path):
                     equal = n > 1 and 3 * a + 5 * b == (3 + 5) * n     # groups of 3 and of 5 units
                     assert not equal or a == b == n
     assert L.levels(2 ** 33, 1024) == 1
+
+
+@pytest.mark.parametrize("scale,rc", [(3e38, EINVAL), (2.4e38, EINVAL), (1e38, None)])
+def test_scales_past_the_powers_of_two(scale, rc):
+    """scale * log2(e) has to be a float: with infinity there a score of 0 would be NaN.  (Taken scales
+    go on to the device, which is not here; no launch is made without one.)"""
+    L = gpu.lib()
+    if rc is None and __import__("torch").cuda.is_available():
+        pytest.skip("made-up addresses")
+    got = (L.cwen_attn_prompt(CTX, gpu.T_F16, P, 512, P + 8192, 256, P + 16384, 256, P + 24576, 512, None, P, P, 1, 2, 2, 4, 2, 128, scale, None),
+           L.cwen_attn_tree(CTX, kv(), 0, P, 512, P + 8192, 512, None, P, P, None, 0, 1, 2, 2, 5, 4, scale, None))
+    assert got == (rc, rc) if rc else EINVAL not in got
