@@ -1172,3 +1172,24 @@ def test_tree_more_heads_than_the_scratch_holds(env, K, D, nodes):
     q = randn(g, sum(n), K, D, dtype=BF16)
     o, z = run_tree(gpu, ctx, kv, 0, q, lens, n, None)
     check_tree(kv, 0, q, o, z, lens, n, None, BF16, heads=[0, 7, K - 1])
+
+
+def test_rope_turns_as_the_model_does(env, oracle):
+    """The configuration of the 27B shape's attention layers against the decoder's own rotation (run.c:1903-1948),
+    whose frequencies and angles are f32: at most 6 roundings of the angle.  With freq_dim 0 it is another one."""
+    gpu, ctx = env
+    cfg = dict(head_dim=256, n_rot=64, theta=1e7, layout="pairs", freq_dim=128)
+    g, pos = gen(77), [0, 1, 5, 97, 1000, 4095]
+    x = randn(g, len(pos), 3, 256)
+    y, other = torch.empty_like(x), torch.empty_like(x)
+    gpu.rope(ctx, gpu.Rope(**cfg), x, y, ints(pos))
+    gpu.rope(ctx, gpu.Rope(**{**cfg, "freq_dim": 0}), x, other, ints(pos))
+    f, m = R.rope_freqs(64, 1e7, freq_dim=128)
+    for t, p in enumerate(pos):
+        want = torch.from_numpy(oracle.rope(x[t].cpu().numpy(), p)).double()
+        mag = x[t].double().cpu().abs()
+        pair = (mag[:, 0:64:2] + mag[:, 1:64:2]).repeat_interleave(2, 1)
+        bound = torch.zeros_like(want)
+        bound[:, :64] = pair * (6 * 2.0 ** -24 * p * torch.tensor(f, dtype=torch.float64).repeat_interleave(2) + (math.pi + 7 + 4) * 2.0 ** -24)
+        close(y[t], want, bound, ("model", p))
+        assert p == 0 or float((other[t].double().cpu() - want)[:, :64].abs().max()) > 0.01
