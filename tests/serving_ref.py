@@ -103,3 +103,21 @@ def attention_bounds(o, lse, A, S, V, n_keys, D, typ):
     eo = eo + u * (o.abs() + eo) + (2.0 ** -25 if typ == torch.float16 else 0)
     el = d + (n_keys + 4) * 2.0 ** -24 + 2.0 ** -22 * (1 + lse.abs().nan_to_num(posinf=0))
     return eo, el
+
+
+def signature(n, D):
+    """Keys whose place shows in the output: key j has the score -level[j] in powers of two (0 to 3, by units of
+    128 keys) and the value 1 in dim dims[j] only, another one for every 16 keys.  All weights are powers of two and
+    exact in 16 bits, so a row's output is 2^-level summed by dim over its whole sum."""
+    j = torch.arange(n)
+    return (j // 128 * 5 + j // 1024) % 4, (j // 16 * 7 + j // 4096) % D
+
+
+def signature_output(level, dims, D):
+    w = 2.0 ** -level.double()
+    return torch.zeros(D, dtype=torch.float64).index_add_(0, dims, w) / w.sum()
+
+
+def signature_bound(want, n, typ):
+    """The output's rounding; the sum in f32, its n terms in lanes and waves of which one adds n / 2 at most; the exponents and factors."""
+    return want * (UNIT[typ] + n / 2 * 2.0 ** -24 + 2.0 ** -20)

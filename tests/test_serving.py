@@ -281,3 +281,26 @@ def test_scales_past_the_powers_of_two(scale, rc):
     got = (L.cwen_attn_prompt(CTX, gpu.T_F16, P, 512, P + 8192, 256, P + 16384, 256, P + 24576, 512, None, P, P, 1, 2, 2, 4, 2, 128, scale, None),
            L.cwen_attn_tree(CTX, kv(), 0, P, 512, P + 8192, 512, None, P, P, None, 0, 1, 2, 2, 5, 4, scale, None))
     assert got == (rc, rc) if rc else EINVAL not in got
+
+
+@pytest.mark.parametrize("n", [1100, 3001, 9000, 20000])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_signatures_show_a_lost_or_wrong_block(n, D):
+    """The long-context tests' values: 16 keys left out, taken twice, or read where other 16 lie exceed the bound
+    twice (once for the roundings that a right row may have, once to be seen beside them), in bf16 too."""
+    torch = pytest.importorskip("torch")
+    import serving_ref as R
+    level, dims = R.signature(n, D)
+    want = R.signature_output(level, dims, D)
+    bound = R.signature_bound(want, n, torch.bfloat16)
+    seen = lambda other: bool(((other - want).abs() > 2 * bound).any())
+    j = torch.arange(n)
+    for b in range(0, n - 32, 16 * 7):
+        one = (j // 16) == b // 16
+        assert seen(R.signature_output(level[~one], dims[~one], D)), ("lost", b)
+        assert seen(R.signature_output(torch.cat([level, level[one]]), torch.cat([dims, dims[one]]), D)), ("twice", b)
+        for away in (16, 32, 128, 512):                    # values of a block that lies elsewhere
+            if b + away + 16 <= n:
+                moved = dims.clone()
+                moved[one] = dims[b + away:b + away + 16]
+                assert seen(R.signature_output(level, moved, D)), ("wrong", b, away)

@@ -1193,3 +1193,58 @@ def test_rope_turns_as_the_model_does(env, oracle):
         bound[:, :64] = pair * (6 * 2.0 ** -24 * p * torch.tensor(f, dtype=torch.float64).repeat_interleave(2) + (math.pi + 7 + 4) * 2.0 ** -24)
         close(y[t], want, bound, ("model", p))
         assert p == 0 or float((other[t].double().cpu() - want)[:, :64].abs().max()) > 0.01
+
+
+# ---------------------------------------------------------------- every key in its place
+@pytest.mark.parametrize("ctx_len,nodes,H,K,D,typ,page", [(20000, 1, 6, 1, 256, F16, 16), (19991, 1, 8, 2, 128, BF16, 64), (9000, 3, 4, 1, 64, F16, 16),
+                                                          (9000, 20, 8, 2, 128, BF16, 16), (20000, 48, 6, 1, 256, F16, 64), (3001, 40, 4, 1, 64, BF16, 32),
+                                                          (1100, 1, 24, 4, 256, F16, 16)])
+def test_tree_long_context_key_by_key(env, ctx_len, nodes, H, K, D, typ, page):
+    """Values that show which keys were taken with which weight: a block of 16 left out, taken twice or read from
+    another page exceeds the bound."""
+    gpu, ctx = env
+    n, g = ctx_len + nodes, gen(ctx_len)
+    kv = tree_cache(gpu, ctx, g, typ, K, D, page, [ctx_len], [nodes], L=1)
+    level, dims = R.signature(n, D)
+    j = torch.arange(n, device="cuda")
+    pg = kv.table[0, j // page].long()
+    kv.k.fill_(float("nan")), kv.v.fill_(float("nan"))                                 # whatever else is read shows too
+    key, val = torch.zeros(n, D, dtype=typ, device="cuda"), torch.zeros(n, D, dtype=typ, device="cuda")
+    key[:, 0] = -level.cuda().to(typ)
+    val[j, dims.cuda()] = 1
+    for h in range(K):                                                                 # a head's values lie a dim further
+        kv.k[0, pg, h, j % page], kv.v[0, pg, h, j % page] = key, val.roll(h, 1)
+    q = randn(g, nodes, H, D, dtype=typ)
+    q[..., 0] = 1
+    o, z = torch.empty_like(q), torch.empty(nodes, H, device="cuda")
+    gpu.attn_tree(ctx, kv, 0, q, o, ints([0]), ints([0, nodes]), nodes, ctx_len, lse=z, scale=math.log(2))
+    for i in {0, nodes // 2, nodes - 1}:
+        m = ctx_len + i + 1
+        want = R.signature_output(level[:m], dims[:m], D)
+        total = float((2.0 ** -level[:m].double()).sum())
+        for h in range(H):
+            w = want.roll(h // (H // K))
+            close(o[i, h], w, R.signature_bound(w, m, typ), ("o", i, h))
+            assert abs(float(z[i, h]) - math.log(total)) <= m / 2 * 2.0 ** -24 + 2.0 ** -18, (i, h)
+    assert kv.take_status(ctx) == 0
+
+
+@pytest.mark.parametrize("n,ctx_len,H,K,D,typ", [(4500, 0, 4, 2, 128, BF16), (3001, 0, 2, 1, 256, F16), (2050, 7000, 2, 1, 64, F16), (300, 20000, 4, 1, 128, BF16),
+                                                 (4200, 0, 24, 4, 256, F16), (1100, 0, 800, 2, 128, BF16)])
+def test_prompt_long_rows_key_by_key(env, n, ctx_len, H, K, D, typ):
+    gpu, ctx = env
+    m, g = n + ctx_len, gen(n)
+    level, dims = R.signature(m, D)
+    k, v = (torch.zeros(m, K, D, dtype=typ, device="cuda") for _ in range(2))
+    k[:, :, 0] = -level.cuda().to(typ)[:, None]
+    for h in range(K):
+        v[torch.arange(m, device="cuda"), h, (dims.cuda() + h) % D] = 1
+    q = randn(g, n, H, D, dtype=typ)
+    q[..., 0] = 1
+    o = torch.empty_like(q)
+    gpu.attn_prompt(ctx, q, k, v, o, ints([0, n]), ints([0, m]), scale=math.log(2))
+    for i in {0, 31, 32, 127, 128, n // 2, n - 129, n - 2, n - 1}:
+        w = R.signature_output(level[:ctx_len + i + 1], dims[:ctx_len + i + 1], D)
+        for h in {0, H // K - 1, H // 2, H - 1}:
+            x = w.roll(h // (H // K))
+            close(o[i, h], x, R.signature_bound(x, ctx_len + i + 1, typ), ("o", i, h))
