@@ -1248,3 +1248,33 @@ def test_prompt_long_rows_key_by_key(env, n, ctx_len, H, K, D, typ):
         for h in {0, H // K - 1, H // 2, H - 1}:
             x = w.roll(h // (H // K))
             close(o[i, h], x, R.signature_bound(x, ctx_len + i + 1, typ), ("o", i, h))
+
+
+# ---------------------------------------------------------------- workgroups of 8 waves
+@pytest.mark.parametrize("typ,H,K,D", [(BF16, 20, 2, 128), (F16, 20, 4, 128), (F16, 24, 4, 256), (BF16, 20, 1, 256)])
+def test_prompt_wide_form(env, typ, H, K, D):
+    """Long sequences and heads enough that the card is full take 256 queries to a workgroup (fewer heads have
+    their tiles' keys halved instead): odd ends, keys and queries that differ, a short sequence beside."""
+    gpu, ctx = env
+    for i, (lq, lk) in enumerate([([4101], None), ([4096], [4133]), ([4353], [4200]), ([8100, 97], None)]):
+        check_prompt(prompt_case(gpu, ctx, gen(70 + i), typ, H, K, D, lq, lk, gap=i & 1), typ, heads=[H - 1])
+
+
+@pytest.mark.parametrize("typ,H,K,D", [(BF16, 20, 2, 128), (F16, 24, 4, 256)])
+def test_prompt_wide_form_hidden_values(env, typ, H, K, D):
+    """NaN and infinities that some rows of a workgroup see and others do not, at its first and last keys."""
+    gpu, ctx = env
+
+    def spoil(k, v):
+        for at, val in ((0, 1e4), (3840, float("nan")), (3999, float("inf")), (4095, -float("inf")), (4300, float("nan"))):
+            v[at, 0, at % 7] = val
+        k[4200, 0, :] = float("nan")
+        k[-3:], v[-3:] = float("nan"), float("inf")             # the gap behind the sequence
+    q, k, v, o, z, lq, lk = prompt_case(gpu, ctx, gen(80), typ, H, K, D, [4400], gap=3, nan=spoil)
+    for a, b in ((0, 40), (3800, 4400)):                         # the rows around
+        sees = torch.arange(4400, device="cuda")[None] <= torch.arange(a, b, device="cuda")[:, None]
+        w = R.attention(q[a:b, 0], k[:4400, 0], v[:4400, 0], sees, D ** -0.5)
+        eo, el = R.attention_bounds(*w, 4400, D, typ)
+        close(o[a:b, 0], w[0], eo, ("o", a))
+        close(z[a:b, 0], w[1], el, ("lse", a))
+    assert bool(torch.isfinite(o[:4200, H - 1].float()).all()) and bool((o[4400:] == 7).all())
