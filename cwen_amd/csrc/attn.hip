@@ -1029,8 +1029,7 @@ int attn_prompt_launch(const cwen_ctx *ctx, int type, int D, const PromptArgs &a
   // 247 us against 252, 16384 2.91 ms and 3.10).  Heads of 64 gain nothing (32768: 4.9 ms and 4.7).
   const bool wide = !split && D != 64 && a.total_q >= 4096ll * a.n_seq;
   const int BM = wide ? 256 : 128;
-  const long long items = (a.total_q + BM - 1) / BM + a.n_seq;
-  if (items * a.nh > INT32_MAX) return CWEN_EINVAL;
+  const long long items = (a.total_q + BM - 1) / BM + a.n_seq;    // items * nh fits a launch (the entry point has checked)
   return by_type(type, D, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int dim = decltype(d)::value;

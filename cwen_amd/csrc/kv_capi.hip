@@ -232,6 +232,7 @@ int cwen_kv_status(cwen_ctx *ctx, const cwen_kv *kv, int *bits, void *stream) {
 }
 
 // ------------------------------------------------------------ attention
+constexpr long long launch_max = 1 << 24;       // workgroups of 256: a launch has less than 2^32 threads
 static int check_heads(int nh, int nkv, int D, float scale) {
   if (nh < 1 || nkv < 1 || nh > 65535 || nh % nkv || (D != 64 && D != 128 && D != 256)) return CWEN_EINVAL;
   return scale > 0 && isfinite(scale * 1.44269504f) ? CWEN_OK : CWEN_EINVAL;     // exponents are powers of two
@@ -247,6 +248,7 @@ int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, con
   if (n_seq < 0 || n_seq > 65536 || total_q < 0 || total_k < 0 || total_q >= 1 << 30 || total_k >= 1 << 30) return CWEN_EINVAL;
   if (!cu_k && total_q != total_k) return CWEN_EINVAL;
   if (n_seq == 0 || total_q == 0) return CWEN_OK;
+  if (((total_q + 127ll) / 128 + n_seq) * n_head >= launch_max) return CWEN_EINVAL;
   const long long qr = (long long)n_head * head_dim, kr = (long long)n_kv_head * head_dim;
   if (!ok_rows(q, q_ts, qr) || !ok_rows(o, o_ts, qr) || !cu_q || !aligned4(cu_q) || !aligned4(cu_k) || !aligned4(lse))
     return CWEN_EINVAL;
@@ -273,6 +275,7 @@ int cwen_attn_tree(cwen_ctx *ctx, const cwen_kv *kv, int layer, const void *q, l
   if (max_nodes < 0 || max_nodes > CWEN_TREE_MAX || max_len < 0) return CWEN_EINVAL;
   if (mask && ((uintptr_t)mask % 8 || mw < 1 || mw > CWEN_TREE_MAX / 64 || max_nodes > 64 * mw)) return CWEN_EINVAL;
   if (n_seq == 0 || total == 0 || max_nodes == 0) return CWEN_OK;
+  if ((n_head + 31ll) / 32 * total >= launch_max) return CWEN_EINVAL;
   const long long qr = (long long)n_head * kv->head_dim;
   if (!ok_rows(q, q_ts, qr) || !ok_rows(o, o_ts, qr) || !seqs || !cu || !aligned4(seqs) || !aligned4(cu) || !aligned4(lse))
     return CWEN_EINVAL;

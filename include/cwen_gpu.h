@@ -354,7 +354,8 @@ int cwen_rope_kv(cwen_ctx *ctx, const cwen_rope *r, int xtype, const void *q, lo
  * cu_q[s] .. cu_q[s+1]-1 and keys cu_k[s] .. cu_k[s+1]-1 (device, n_seq + 1
  * non-decreasing ints within 0..total_q and 0..total_k; cu_k NULL: cu_q);
  * its query i sees keys j <= i + (keys - queries).  Rows of o that no
- * sequence covers are left as they were; lengths may be 0. */
+ * sequence covers are left as they were; lengths may be 0.  CWEN_EINVAL also
+ * when (total_q / 128, rounded up, + n_seq) * n_head reaches 2^24. */
 int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, const void *k, long long k_ts,
                      const void *v, long long v_ts, void *o, long long o_ts, float *lse, const int *cu_q,
                      const int *cu_k, int n_seq, int total_q, int total_k, int n_head, int n_kv_head, int head_dim,
@@ -372,7 +373,8 @@ int cwen_attn_prompt(cwen_ctx *ctx, int type, const void *q, long long q_ts, con
  * overlap, nor replays of graphs that captured them.  max_len: the expected
  * longest context; it guides the launch and may be wrong.  CWEN_EINVAL also
  * when (n_seq + 64) * (row tiles of max_nodes * heads per KV head) * (tiles of
- * max_pages * page positions) passes 2^31. */
+ * max_pages * page positions) passes 2^31, or total * (n_head / 32, rounded up)
+ * reaches 2^24. */
 #define CWEN_TREE_MAX 256
 int cwen_attn_tree(cwen_ctx *ctx, const cwen_kv *kv, int layer, const void *q, long long q_ts, void *o, long long o_ts,
                    float *lse, const int *seqs, const int *cu, const unsigned long long *mask, int mw, int n_seq,

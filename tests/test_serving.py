@@ -277,7 +277,7 @@ def test_scales_past_the_powers_of_two(scale, rc):
     go on to the device, which is not here; no launch is made without one.)"""
     L = gpu.lib()
     if rc is None and __import__("torch").cuda.is_available():
-        pytest.skip("made-up addresses")
+        pytest.skip("made-up addresses: never where a device would take them")
     got = (L.cwen_attn_prompt(CTX, gpu.T_F16, P, 512, P + 8192, 256, P + 16384, 256, P + 24576, 512, None, P, P, 1, 2, 2, 4, 2, 128, scale, None),
            L.cwen_attn_tree(CTX, kv(), 0, P, 512, P + 8192, 512, None, P, P, None, 0, 1, 2, 2, 5, 4, scale, None))
     assert got == (rc, rc) if rc else EINVAL not in got
@@ -304,3 +304,17 @@ def test_signatures_show_a_lost_or_wrong_block(n, D):
                 moved = dims.clone()
                 moved[one] = dims[b + away:b + away + 16]
                 assert seen(R.signature_output(level, moved, D)), ("wrong", b, away)
+
+
+def test_calls_past_a_launch_are_refused():
+    """A launch has less than 2^32 threads: more sequences x heads than that in one call are refused before the device is asked."""
+    L = gpu.lib()
+    prompt = lambda n, t, nh: L.cwen_attn_prompt(CTX, gpu.T_F16, P, nh * 64, P + (1 << 44), 64, P + (1 << 45), 64, P + (1 << 46), nh * 64, None, P, P, n, t, t,
+                                                 nh, 1, 64, 1.0, None)
+    big = kv(max_seqs=65536, max_pages=16, n_kv_head=1, head_dim=64)
+    tree = lambda t, nh: L.cwen_attn_tree(CTX, big, 0, P, nh * 64, P + (1 << 46), nh * 64, None, P, P, None, 0, 65536, t, 1, 5, nh, 1.0, None)
+    for f, n in ((prompt, (65536, 65536, 256)), (prompt, (1, (1 << 30) - 1, 2)), (tree, (1 << 23, 64)), (tree, (1 << 23, 33))):
+        assert f(*n) == EINVAL, n
+    if not __import__("torch").cuda.is_available():            # taken, and then there is no device
+        for f, n in ((prompt, (65536, 128, 255)), (tree, ((1 << 24) - 1, 32))):
+            assert f(*n) not in (EINVAL, OK), n
