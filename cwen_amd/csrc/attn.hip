@@ -143,9 +143,9 @@ template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a,
 }
 
 // Bound by the matrix cores, and there by power: 32768 tokens of 32/8 heads of 128 in bf16 take
-// 7.6 ms, 1.16 PFLOP/s with the matrix pipes 57 % busy at 1.94 GHz (a product of 8192^3 reaches
-// 1.21); 9 prompts of 16301 tokens in all 339 us (0.91), 4096 tokens of 24/4 heads of 256 in f16
-// 228 us (0.90: the longest row sets the time).
+// 7.6 to 7.9 ms, 1.11 to 1.16 PFLOP/s with the matrix pipes 57 % busy at 1.94 GHz (a product of
+// 8192^3 reaches 1.2 to 1.38); 9 prompts of 16301 tokens in all 339 to 355 us (0.87 to 0.91), 4096 tokens
+// of 24/4 heads of 256 in f16 228 to 231 us (0.90: the longest row sets the time).
 // RW KW waves share double-buffered tiles of KW BN keys: RW of them have 32 queries
 // of one head each, and with KW = 2 the first RW take one half of every tile's keys, the
 // others, for the same queries, the other; their sums meet at the end.
@@ -517,7 +517,8 @@ __device__ __forceinline__ float max64(float v) {
 }
 
 // Bound by a chain of six trips to memory, then by the pages' bytes: one node of 24/4 heads of 256
-// behind 4096 positions 10.8 us (16.8 MB), 64 of them behind up to 8000 102 us.
+// behind 4096 positions 9.7 to 10.8 us (16.8 MB), 64 of them behind up to 8000 102 us, 48 of 32/8 heads
+// of 128 behind up to 12000 218 us (1.2 GB, 5.5 TB/s).
 // Few rows: one tile of 32, the chunk's keys dealt to 4 waves 32 at a time.  A wave
 // has its own K and V rows in LDS and no barrier in its loop: the next K rows
 // are requested when the scores are done, the next V rows after the outputs, so
@@ -723,8 +724,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) __attribute__(
 }
 
 // Bound by the pages' bytes while rows are few (48 trees of up to 24 nodes behind up to 12000
-// positions, 32/8 heads of 128: 130 us, 617 MB, 4.75 TB/s), by matrix work and the partials with
-// more (48 nodes of 24/4 heads of 256 behind 32000: 65 us).
+// positions, 32/8 heads of 128: 128 to 130 us, 617 MB, 4.8 TB/s), by matrix work and the partials with
+// more (48 nodes of 24/4 heads of 256 behind 32000: 64 us).
 // Many rows: 4 waves of 32 rows share double-buffered tiles of BN keys.
 template <typename T, int D, int BN>
 __global__ __launch_bounds__(256, 2) void tree_many_kernel(TreeArgs a, TreeLaunch p) {
@@ -1019,14 +1020,16 @@ template <typename F> int by_type(int type, int D, F f) {
 int attn_prompt_launch(const cwen_ctx *ctx, int type, int D, const PromptArgs &a, hipStream_t st) {
   const long long tiles = (a.total_q + 127) / 128 + a.n_seq;      // of 128 rows, at most
   // Up to 2.5 workgroups per CU (heads of 64: 4.5) the longest row sets the time, so its keys
-  // go to two halves of a workgroup: heads of 128, 32/8: 2048 tokens 47 us against 62 (4096, 4 per
-  // CU: 158 against 143); of 256, 24/4: 2048 79 against 112 (4096 260 against 252); of 64, 16/4: 2048
-  // 26 against 38, 8192 174 against 184 (40 prompts of 125 20 against 16).
+  // go to two halves of a workgroup: heads of 128, 32/8: 2048 tokens 48 us against 56 (2560: 76 against
+  // 74, 4096: 159 against 144); of 256, 24/4: 2048 73 against 101 (4096 241 against 238); of 64, 16/4: 2048
+  // 26 against 36, 8192 178 against 184 (40 prompts of 125 14.4 against 11.3).
   const bool split = 2 * tiles * a.nh <= (D == 64 ? 9ll : 5ll) * ctx->ncu;
   // Sequences of 4096 tokens and more on average: workgroups of 8 waves read K and V half as often as
   // those of 4, which leave fewer waves idle in short sequences and more workgroups to a CU (heads of 128,
-  // 32/8: one prompt of 32768 7.57 ms against 7.90, 4 of 4096 757 us against 720; of 256, 24/4: 4096
-  // 247 us against 252, 16384 2.91 ms and 3.10).  Heads of 64 gain nothing (32768: 4.9 ms and 4.7).
+  // 32/8: one prompt of 4096 140 us against 144, of 32768 7.77 ms against 7.98, 9 of 1811 345 us against 297; at
+  // the line the sides differ by 2 %, 4 prompts of 4096 the other way, 556 against 545; of 256, 24/4: 4096
+  // 229 us against 238, 16384 2.99 ms against 3.19).  Heads of 64, 32/8, are not built so: 4096 106 us against 101,
+  // 32768 4.80 ms against 5.11.
   const bool wide = !split && D != 64 && a.total_q >= 4096ll * a.n_seq;
   const int BM = wide ? 256 : 128;
   const long long items = (a.total_q + BM - 1) / BM + a.n_seq;    // items * nh fits a launch (the entry point has checked)

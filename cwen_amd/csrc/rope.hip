@@ -2,8 +2,10 @@
 // with the write into the paged cache.
 //
 // The turn of pair i at position p is p * turns[i] whole circles.  The product
-// is taken and reduced to (-1/2, 1/2] in f64 (at p = 2^31 the reduced angle
-// still holds 2^-22 of a circle), the sine and cosine in f32.  A workgroup
+// is taken and reduced to (-1/2, 1/2] in f64, the sine and cosine in f32.  turns[i] <=
+// 1 / 2 pi carries about a dozen roundings of 2^-53 (its power, scaling, division) and the
+// product one: p 2^-52 of a circle at most, 2^-21 at the last position, and less than the
+// rounding to f32 (2^-26 of a circle) up to position 2^26.  A workgroup
 // computes them once per token into LDS and turns every head with them; an f64
 // product per head instead would cost as much as the head's memory traffic.
 // Memory bound past a few hundred tokens: every element is read and written
@@ -65,7 +67,7 @@ __host__ __device__ constexpr int rope_items(int D, int n_rot, bool halves) { re
 // tokens of 5/1 heads of 128 take 9.3 us instead of 13.6, 100000 of one head of 64 12 instead
 // of 56 (two tokens to a workgroup lose to one in f32: 16 heads of 64 15 against 12.5).  A
 // decode step of 32 heads takes 3.2 us, a launch's own length; 8192 tokens of 32/8
-// heads of 128 in bf16 32 us (201 MB, 6.3 TB/s: a large copy reaches 4.8).
+// heads of 128 in bf16 32 us (201 MB, 6.3 TB/s: a copy of 256 MiB reaches 5.4, a plain kernel 6.2).
 template <typename TX, typename TY, bool HALVES, bool GROUP>
 __global__ __launch_bounds__(THREADS) void rope_kernel(RopeParams p, RopeTab tab) {
   __shared__ float2 s_cs[GROUP ? 2048 : 128];   // tok n_rot / 2 <= 256 / items * 8 items
