@@ -143,9 +143,9 @@ template <int BM> __device__ __forceinline__ Item find_item(const PromptArgs &a,
 }
 
 // Bound by the matrix cores, and there by power: 32768 tokens of 32/8 heads of 128 in bf16 take
-// 7.6 to 7.9 ms, 1.11 to 1.16 PFLOP/s with the matrix pipes 57 % busy at 1.94 GHz (a product of
-// 8192^3 reaches 1.2 to 1.38); 9 prompts of 16301 tokens in all 339 to 355 us (0.87 to 0.91), 4096 tokens
-// of 24/4 heads of 256 in f16 228 to 231 us (0.90: the longest row sets the time).
+// 7.55 to 7.9 ms, 1.11 to 1.17 PFLOP/s with the matrix pipes 57 % busy at 1.94 GHz (a product of
+// 8192^3 reaches 1.2 to 1.38); 9 prompts of 16301 tokens in all 334 to 355 us (0.87 to 0.92), 4096 tokens
+// of 24/4 heads of 256 in f16 225 to 231 us (0.89 to 0.92: the longest row sets the time).
 // RW KW waves share double-buffered tiles of KW BN keys: RW of them have 32 queries
 // of one head each, and with KW = 2 the first RW take one half of every tile's keys, the
 // others, for the same queries, the other; their sums meet at the end.
