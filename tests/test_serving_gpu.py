@@ -1278,3 +1278,24 @@ def test_prompt_wide_form_hidden_values(env, typ, H, K, D):
         close(o[a:b, 0], w[0], eo, ("o", a))
         close(z[a:b, 0], w[1], el, ("lse", a))
     assert bool(torch.isfinite(o[:4200, H - 1].float()).all()) and bool((o[4400:] == 7).all())
+
+
+@pytest.mark.parametrize("typ,H,K,D,n", [(F16, 2, 1, 64, 300), (BF16, 2, 1, 256, 300), (F16, 800, 2, 128, 200), (BF16, 20, 2, 128, 4200)])
+def test_prompt_scores_of_minus_infinity(env, typ, H, K, D, n):
+    """Keys with scores of -inf weigh nothing, whole tiles of them too; the first rows, which see no
+    others, are NaN with lse -inf.  In every form, with keys before the queries."""
+    gpu, ctx = env
+    off, g = 40, gen(n)
+    q, k, v = randn(g, n, H, D, dtype=typ), randn(g, n + off, K, D, dtype=typ), randn(g, n + off, K, D, dtype=typ)
+    gone = torch.zeros(n + off, dtype=torch.bool, device="cuda")
+    gone[:off + 5], gone[64:192], gone[n - 3:n] = True, True, True
+    q[..., 0], k[gone, :, 0] = 1, -math.inf
+    o, z = torch.empty_like(q), torch.empty(n, H, device="cuda")
+    gpu.attn_prompt(ctx, q, k, v, o, ints([0, n]), ints([0, n + off]), lse=z)
+    counts = (torch.arange(n + off, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None] + off) & ~gone[None]
+    for h in (0, H - 1):
+        w = R.attention(q[:, h], k[:, h // (H // K)].nan_to_num(neginf=0), v[:, h // (H // K)], counts, D ** -0.5)
+        eo, el = R.attention_bounds(*w, n + off, D, typ)
+        want = torch.where(counts.any(1)[:, None], w[0], torch.full_like(w[0], float("nan")))
+        close(o[:, h], want, eo, ("o", h))
+        close(z[:, h], w[1], el, ("lse", h))
