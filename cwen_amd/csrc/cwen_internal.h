@@ -390,6 +390,35 @@ struct TypeBF16 {
   typedef __bf16 vec8 __attribute__((ext_vector_type(8)));
 };
 
+// 8 elements at a 16-byte aligned address (f32: two such).
+template <typename T> struct Io;
+template <> struct Io<float> {
+  static __device__ __forceinline__ void load(const float *p, float (&x)[8]) {
+    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(float *p, const float (&x)[8]) {
+    *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
+    *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <typename T, typename V> struct Io16 {
+  static __device__ __forceinline__ void load(const T *p, float (&x)[8]) {
+    const V a = *(const V *)p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)a[j];
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&x)[8]) {
+    V a;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = (T)x[j];
+    *(V *)p = a;
+  }
+};
+template <> struct Io<TypeF16::elem> : Io16<TypeF16::elem, TypeF16::vec8> {};
+template <> struct Io<TypeBF16::elem> : Io16<TypeBF16::elem, TypeBF16::vec8> {};
+
 // ------------------------------------------------------------ rope.hip
 struct cwen_rope {
   int head_dim, n_rot, layout;
@@ -440,6 +469,49 @@ struct TreeArgs {
   float scale;
 };
 int attn_tree_launch(const cwen_ctx *ctx, const TreeArgs &a, hipStream_t st);
+
+// ------------------------------------------------------------ gdn_seq.hip, gdn_prompt.hip
+// Packed sequences over a pool's slots, as cwen_gpu.h describes them.
+struct GdnSeqs {
+  const int *cu, *count, *src, *dst;   // all but cu nullable
+  int n_seq, total, n_slots;
+  int *status;
+};
+struct GdnConvArgs {
+  GdnSeqs s;
+  const void *x;
+  void *y;                  // nullable
+  long long xs, ys;
+  const float *kw;
+  float *hist;              // the layer's slots
+  int C;
+};
+int gdn_conv_launch(int xtype, int ytype, const GdnConvArgs &a, hipStream_t st);
+struct GdnRuleArgs {
+  GdnSeqs s;
+  const void *q, *k, *v;
+  void *o;                  // nullable
+  long long qs, ks, vs, os, gs;
+  const float *a, *b, *A, *dt;   // A, dt: both or neither
+  float *state;             // the layer's slots
+  int nkh, nvh, group;      // group: value heads per key head, or 0 for h % nkh
+};
+int gdn_step_launch(int xtype, int otype, int D, const GdnRuleArgs &a, hipStream_t st);
+int gdn_prompt_launch(int xtype, int otype, int D, const GdnRuleArgs &a, void *work, hipStream_t st);
+size_t gdn_prompt_bytes(int xtype, int otype, int D, int nkh, int nvh, int n_seq, int total);
+
+// ------------------------------------------------------------ logprobs.hip
+struct LogprobArgs {
+  const void *x;
+  long long ls;
+  int V, rows, top;
+  const int *tokens;
+  float *logprob, *entropy, *lse, *top_lp;
+  int *rank, *top_ids;
+  float *work;
+};
+int logprobs_launch(int type, const LogprobArgs &a, hipStream_t st);
+size_t logprobs_bytes(int rows, int V, int top);
 
 // ------------------------------------------------------------ cache pages (device)
 __device__ __forceinline__ void kv_raise(const cwen_kv &kv, int bits) {

@@ -24,34 +24,6 @@ struct RopeTab {
   int tok;                       // tokens of a workgroup
 };
 
-template <typename T> struct Io;
-template <> struct Io<float> {
-  static __device__ __forceinline__ void load(const float *p, float (&x)[8]) {
-    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-  static __device__ __forceinline__ void store(float *p, const float (&x)[8]) {
-    *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
-    *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-  }
-};
-template <typename T, typename V> struct Io16 {
-  static __device__ __forceinline__ void load(const T *p, float (&x)[8]) {
-    const V a = *(const V *)p;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)a[j];
-  }
-  static __device__ __forceinline__ void store(T *p, const float (&x)[8]) {
-    V a;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = (T)x[j];
-    *(V *)p = a;
-  }
-};
-template <> struct Io<TypeF16::elem> : Io16<TypeF16::elem, TypeF16::vec8> {};
-template <> struct Io<TypeBF16::elem> : Io16<TypeBF16::elem, TypeBF16::vec8> {};
-
 __device__ __forceinline__ void turn(float &x, float &y, float2 cs) {
   const float a = x * cs.x - y * cs.y;
   y = x * cs.y + y * cs.x;

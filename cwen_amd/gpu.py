@@ -61,6 +61,15 @@ SIGNATURES = [
     ("cwen_attn_prompt", _I, [_VP, _I, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I,
                               C.c_float, _VP]),
     ("cwen_attn_tree", _I, [_VP, _VP, _I, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, C.c_float, _VP]),
+    ("cwen_gdn_status", _I, [_VP, _VP, C.POINTER(_I), _VP]),
+    ("cwen_gdn_conv", _I, [_VP, _VP, _I, _I, _VP, _LL, _VP, _I, _VP, _LL, _VP, _VP, _VP, _VP, _I, _I, _VP]),
+    ("cwen_gdn_step", _I, [_VP, _VP, _I, _I, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _LL, _VP, _VP, _I, _VP, _LL, _VP, _VP, _VP,
+                           _VP, _I, _I, _VP]),
+    ("cwen_gdn_prompt", _I, [_VP, _VP, _I, _I, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _LL, _VP, _VP, _I, _VP, _LL, _VP, _VP, _VP,
+                             _VP, _I, _I, _VP, C.c_size_t, _VP]),
+    ("cwen_gdn_prompt_work", _I, [_VP, _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    ("cwen_logprobs", _I, [_VP, _I, _VP, _LL, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, C.c_size_t, _VP]),
+    ("cwen_logprobs_work", _I, [_I, _I, _I, C.POINTER(C.c_size_t)]),
     ("cwen_model_create", _I, [_VP, _VP, C.POINTER(_VP)]),
     ("cwen_model_free", _I, [_VP]),
     ("cwen_model_set", _I, [_VP, _I, _I, _I, _VP, _VP, _I, _I]),
@@ -595,6 +604,169 @@ def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: 
     check("cwen_attn_tree", lib().cwen_attn_tree(
         ctx.h, kv.ref_c, layer, _ptr(q), qs, _ptr(o), os_, _ptr(lse), _vec("seqs", seqs, None), _vec("cu", cu, n + 1),
         _ptr(mask), mw, n, T, max_nodes, max_len, H, D ** -0.5 if scale is None else scale, _stream_of(ctx, stream)))
+
+
+GDN_MOD, GDN_GROUP, GDN_ARG, GDN_SEQ_MAX = 0, 1, 1, 4096
+LOGPROBS_TOP = 64
+
+
+class GdnPoolC(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_layers", "n_slots", "nkh", "nvh", "dk", "key_head")] + \
+               [(n, C.c_void_p) for n in ("state", "hist", "status")]
+
+
+class GdnPool:
+    """The GatedDeltaNet states of many sequences over torch tensors (cwen_gdn_pool): state
+    [layers, slots, value heads, dk, dk] and hist [layers, slots, channels, 3], float32, either
+    may be None.  GdnPool.empty allocates one.  key_head: "mod" or "group"."""
+
+    def __init__(self, nkh: int, nvh: int, dk: int, state=None, hist=None, key_head: str = "mod"):
+        import torch
+        if state is None and hist is None:
+            raise ValueError("state or hist expected")
+        some = state if state is not None else hist
+        L, N = some.shape[:2]
+        self.channels = (2 * nkh + nvh) * dk
+        for name, t, shape in (("state", state, (L, N, nvh, dk, dk)), ("hist", hist, (L, N, self.channels, 3))):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != some.device):
+                raise ValueError(f"{name}: contiguous float32 {shape} on {some.device} expected, got {tuple(t.shape)} {t.dtype}")
+        self.state, self.hist, self.status = state, hist, torch.zeros(1, dtype=torch.int32, device=some.device)
+        self.nkh, self.nvh, self.dk, self.slots = nkh, nvh, dk, N
+        self.c = GdnPoolC(L, N, nkh, nvh, dk, {"mod": GDN_MOD, "group": GDN_GROUP}[key_head], _ptr(state), _ptr(hist), _ptr(self.status))
+        self.ref_c = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, n_layers: int, n_slots: int, nkh: int, nvh: int, dk: int = 128, key_head: str = "mod", device="cuda") -> "GdnPool":
+        import torch
+        f = lambda *n: torch.zeros(n, dtype=torch.float32, device=device)
+        return cls(nkh, nvh, dk, f(n_layers, n_slots, nvh, dk, dk), f(n_layers, n_slots, (2 * nkh + nvh) * dk, 3), key_head)
+
+    def prompt_work(self, total: int, n_seq: int, dtype, out_dtype):
+        """Scratch for gdn_prompt calls of up to `total` rows in n_seq sequences of these types."""
+        import torch
+        if not _FLOATS:
+            _torch_tables()
+        n = C.c_size_t()
+        check("cwen_gdn_prompt_work", lib().cwen_gdn_prompt_work(self.ref_c, _FLOATS[dtype], _FLOATS[out_dtype], n_seq, total, C.byref(n)))
+        return torch.empty(n.value, dtype=torch.uint8, device=self.status.device)
+
+    def take_status(self, ctx: Context, stream=None) -> int:
+        """The GDN_* bits raised since the last call, cleared.  Synchronous."""
+        _on(ctx, self.status)
+        bits = C.c_int()
+        check("cwen_gdn_status", lib().cwen_gdn_status(ctx.h, self.ref_c, C.byref(bits), _stream_of(ctx, stream)))
+        return bits.value
+
+
+def _seqs(cu, count, src, dst) -> tuple:
+    """The packed sequences' vectors as arguments: (cu, count, src, dst), n_seq."""
+    n = cu.numel() - 1
+    if n < 0:
+        raise ValueError("cu: at least one border expected")
+    at = lambda name, t: None if t is None else _vec(name, t, n)
+    return (_vec("cu", cu, None), at("count", count), at("src", src), at("dst", dst)), n
+
+
+def _row_stride(t, T: int, row: int) -> int:
+    return t.stride(0) if T > 1 else row
+
+
+def gdn_conv(ctx: Context, pool: GdnPool, layer: int, x, kw, y, cu, src=None, dst=None, count=None, stream=None) -> None:
+    """y = silu of the causal convolution of packed rows x [rows, channels] (cwen_gdn_conv); kw [channels, 4]
+    float32; y may be None (the history alone moves)."""
+    T, Cn = x.shape
+    if Cn != pool.channels or (y is not None and tuple(y.shape) != (T, Cn)):
+        raise ValueError(f"x {tuple(x.shape)}, y {None if y is None else tuple(y.shape)}: the pool has {pool.channels} channels")
+    if x.numel() and any(t is not None and t.stride(1) != 1 for t in (x, y)):
+        raise ValueError("a row's elements must lie in a row")
+    _on(ctx, pool.status, x, kw, y, cu, src, dst, count)
+    seqs, n = _seqs(cu, count, src, dst)
+    check("cwen_gdn_conv", lib().cwen_gdn_conv(
+        ctx.h, pool.ref_c, layer, _type(x), _ptr(x), _row_stride(x, T, Cn), _vec("kw", kw, 4 * Cn, "float32"),
+        _type(x if y is None else y), _ptr(y), 0 if y is None else _row_stride(y, T, Cn), *seqs, n, T, _stream_of(ctx, stream)))
+
+
+def _gdn_rule(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, src, dst, A, dt, count) -> tuple:
+    """The arguments that gdn_step and gdn_prompt have in common, and the number of sequences."""
+    T = q.shape[0]
+    _on(ctx, pool.status, q, k, v, a, b, o, cu, src, dst, A, dt, count)
+    qs, ks = _heads("q", q, (T, pool.nkh, pool.dk)), _heads("k", k, (T, pool.nkh, pool.dk), q.dtype)
+    vs = _heads("v", v, (T, pool.nvh, pool.dk), q.dtype)
+    os_ = 0 if o is None else _heads("o", o, (T, pool.nvh, pool.dk))
+    for name, t in (("a", a), ("b", b)):
+        if tuple(t.shape) != (T, pool.nvh) or str(t.dtype) != "torch.float32" or (t.numel() and t.stride(1) != 1):
+            raise ValueError(f"{name}: float32 [{T}, {pool.nvh}] with a row's elements in a row expected")
+    gs = _row_stride(a, T, pool.nvh)
+    if gs != _row_stride(b, T, pool.nvh):
+        raise ValueError("a and b must have one row stride")
+    if (A is None) != (dt is None):
+        raise ValueError("A and dt come together")
+    per_head = lambda name, t: None if t is None else _vec(name, t, pool.nvh, "float32")
+    seqs, n = _seqs(cu, count, src, dst)
+    return (ctx.h, pool.ref_c, layer, _type(q), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(a), _ptr(b), gs, per_head("A", A),
+            per_head("dt", dt), _type(q if o is None else o), _ptr(o), os_, *seqs, n, T), n
+
+
+def gdn_step(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, src=None, dst=None, A=None, dt=None, count=None,
+             stream=None) -> None:
+    """The gated delta rule for one or a few rows of each sequence (cwen_gdn_step): q, k [rows, key heads, dk], v, o
+    [rows, value heads, dk], a, b float32 [rows, value heads]; o may be None (the states alone move)."""
+    args, _ = _gdn_rule(ctx, pool, layer, q, k, v, a, b, o, cu, src, dst, A, dt, count)
+    check("cwen_gdn_step", lib().cwen_gdn_step(*args, _stream_of(ctx, stream)))
+
+
+def gdn_prompt(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, src=None, dst=None, A=None, dt=None, count=None,
+               work=None, stream=None) -> None:
+    """The gated delta rule over packed prompts (cwen_gdn_prompt), arguments as gdn_step; work: a prompt_work of the
+    pool for at least this size (None: allocated for the call)."""
+    args, n = _gdn_rule(ctx, pool, layer, q, k, v, a, b, o, cu, src, dst, A, dt, count)
+    s = _stream_of(ctx, stream)
+    if work is None:
+        work = pool.prompt_work(q.shape[0], n, q.dtype, q.dtype if o is None else o.dtype)
+        _in_use(work, stream)
+    _on(ctx, work)
+    check("cwen_gdn_prompt", lib().cwen_gdn_prompt(*args, _ptr(work), work.numel() * work.element_size(), s))
+
+
+def _in_use(t, stream) -> None:
+    """Keep a tensor allocated for one call from being handed out again before a stream other than the current one is done with it."""
+    if stream is not None and t.numel():
+        import torch
+        t.record_stream(torch.cuda.ExternalStream(stream, device=t.device) if isinstance(stream, int) else stream)
+
+
+def logprobs_work(rows: int, V: int, top: int = 0, device="cuda"):
+    """Scratch for logprobs calls of this size."""
+    import torch
+    n = C.c_size_t()
+    check("cwen_logprobs_work", lib().cwen_logprobs_work(rows, V, top, C.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def logprobs(ctx: Context, logits, tokens=None, logprob=None, rank=None, entropy=None, lse=None, top_ids=None, top_logprobs=None,
+             work=None, stream=None) -> None:
+    """Log probabilities over logits [rows, vocab] (cwen_logprobs): logprob, entropy, lse float32 [rows], rank and tokens
+    int32 [rows], top_ids int32 and top_logprobs float32 [rows, top], each may be None; work: a logprobs_work of this
+    size (None: allocated for the call)."""
+    rows, V = logits.shape
+    if logits.numel() and logits.stride(1) != 1:
+        raise ValueError("a row's logits must lie in a row")
+    _on(ctx, logits, tokens, logprob, rank, entropy, lse, top_ids, top_logprobs)
+    top = next((t.shape[1] for t in (top_ids, top_logprobs) if t is not None and t.dim() == 2), 0)
+    vec = lambda name, t, n, d: None if t is None else _vec(name, t, n, d)
+    for name, t in (("top_ids", top_ids), ("top_logprobs", top_logprobs)):
+        if t is not None and tuple(t.shape) != (rows, top):
+            raise ValueError(f"{name}: [{rows}, {top}] expected, got {tuple(t.shape)}")
+    s = _stream_of(ctx, stream)
+    if work is None:
+        work = logprobs_work(rows, V, top, logits.device)
+        _in_use(work, stream)
+    _on(ctx, work)
+    check("cwen_logprobs", lib().cwen_logprobs(
+        ctx.h, _type(logits), _ptr(logits), _row_stride(logits, rows, V), V, rows, vec("tokens", tokens, rows, "int32"),
+        vec("logprob", logprob, rows, "float32"), vec("rank", rank, rows, "int32"), vec("entropy", entropy, rows, "float32"),
+        vec("lse", lse, rows, "float32"), top, vec("top_ids", top_ids, rows * top, "int32"),
+        vec("top_logprobs", top_logprobs, rows * top, "float32"), _ptr(work), work.numel() * work.element_size(), s))
 
 
 # ---------------------------------------------------------------- model

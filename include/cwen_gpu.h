@@ -215,6 +215,116 @@ int cwen_gdn_block(cwen_ctx *ctx, cwen_gdn *g, const float *qkv, int qs, const f
  * layer. */
 int cwen_gdn_commit(cwen_gdn *g, int n);
 
+/* ---- GatedDeltaNet layers of many sequences ----
+ * A pool holds the states of many sequences, one slot each.  The caller owns the
+ * memory (DEVICE memory); calls work on it in stream order, without a copy to the
+ * host, an allocation or a wait (cwen_gdn_status waits), so calls can be captured.
+ * In `layer` of a slot lie the recurrent state [nvh][dk][dk] (row = key
+ * dimension) and the convolution's history [C][3], C = (2 * nkh + nvh) * dk
+ * channels, oldest input first: what cwen_gdn_set_state takes for one sequence.
+ *
+ * cwen_gdn_conv, cwen_gdn_step and cwen_gdn_prompt take packed sequences.
+ * Sequence i < n_seq holds the rows cu[i] .. cu[i+1]-1 (device, n_seq + 1
+ * non-decreasing ints within 0..total); the call takes its first count[i] of
+ * them (device, 0 .. its rows; count NULL: all).  It starts from slot src[i] of
+ * the pool, or from zeros where src[i] is -1 (src NULL: all from zeros), and
+ * leaves its end state in slot dst[i], or nowhere where dst[i] is -1 (dst NULL:
+ * none).  So src = dst moves a sequence on; src != dst forks it (with no rows:
+ * a plain copy, or a cleared slot); dst = -1 scores drafted rows without moving
+ * the state, and a second call with the accepted counts (and no outputs) moves
+ * it.  No slot that a sequence ends in may be another's src or dst in the call.
+ * A sequence with an invalid slot or count, or whose dst another one names, is
+ * left out whole: its rows of the output and its slot stay as they were, and
+ * CWEN_GDN_ARG is raised in *status.  Rows that no sequence takes stay as they
+ * were.  Calls that share slots must not overlap. */
+typedef struct {
+  int n_layers;            /* 1..32767                                             */
+  int n_slots;             /* 1..65536                                             */
+  int nkh, nvh;            /* key and value heads; nvh a multiple of nkh, <= 4096  */
+  int dk;                  /* 64 or 128: dims of a key and of a value head         */
+  int key_head;            /* CWEN_GDN_*: which key head value head h reads        */
+  float *state;            /* [n_layers][n_slots][nvh][dk][dk], 16-byte aligned; may be NULL for cwen_gdn_conv */
+  float *hist;             /* [n_layers][n_slots][C][3], 16-byte aligned; NULL unless for cwen_gdn_conv */
+  int *status;             /* 1 int                                                */
+} cwen_gdn_pool;
+enum { CWEN_GDN_MOD = 0,   /* h % nkh (run.c:2027)                                 */
+       CWEN_GDN_GROUP = 1  /* h / (nvh / nkh)                                      */ };
+#define CWEN_GDN_ARG 1     /* a sequence's slot or count is invalid, or its dst is named twice */
+/* Sequences of one call at most. */
+#define CWEN_GDN_SEQ_MAX 4096
+/* Read the status bits to the HOST and clear them.  Synchronous. */
+int cwen_gdn_status(cwen_ctx *ctx, const cwen_gdn_pool *pool, int *bits, void *stream);
+
+/* The causal convolution of a layer's mixed rows: y[t][c] = silu(sum_j kw[c][j]
+ * x[t - 3 + j][c]), j < 4, the inputs before a sequence's first row from its
+ * history (conv1d_update + silu, run.c:2183-2200).  x [total] rows of C
+ * elements, x_ts apart, kw [C][4] f32 (device, 16-byte aligned), y (nullable:
+ * the history alone moves) likewise; element types xtype and ytype (F32, F16,
+ * BF16), computed in f32 and rounded once.  Pointers 16-byte aligned, strides
+ * multiples of 8; y must not overlap x. */
+int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *x, long long x_ts,
+                  const float *kw, int ytype, void *y, long long y_ts, const int *cu, const int *count, const int *src,
+                  const int *dst, int n_seq, int total, void *stream);
+
+/* The gated delta rule, row after row; per row and value head h, with k and q
+ * the rows of its key head over their lengths (x / sqrt(sum x^2 + 1e-6)):
+ *   S *= g;  d = beta (v - S^T k);  S += k d^T;  o = S^T q / sqrt(dk)
+ * (gdn_step without its gated norm, run.c:2014-2180).  q, k [total][nkh][dk], v
+ * and o [total][nvh][dk], rows q_ts .. o_ts apart, element types xtype (q, k,
+ * v) and otype (F32, F16, BF16); a, b f32 [total], rows g_ts floats apart: with
+ * A and dt (f32 [nvh]) g = exp(A[h] softplus(a + dt[h])) and beta = sigmoid(b)
+ * (run.c:2697-2698), with both NULL g = exp(a) and beta = b.  a log decay above
+ * 0 or a beta outside 0..2 gives unspecified values.  o is nullable (the states
+ * alone move).  Pointers of q, k, v and o 16-byte aligned, their strides
+ * multiples of 8; o must not overlap q, k or v (it may lie beside them in rows
+ * of the same bytes).  States are held and moved in f32.
+ *
+ * cwen_gdn_step does it as written, the state in registers: for one or a few
+ * rows of each sequence.  A row's result does not depend on the other rows or
+ * sequences of the call: a block's rows are the bits of single ones.
+ * cwen_gdn_prompt takes chunks of 32 rows on the matrix cores: with d_i of a
+ * chunk from (1 + L) d = r, L_ij = beta_i g_j+1..g_i k_i.k_j (j < i), r_i =
+ * beta_i (v_i - g_1..g_i S^T k_i).  Operands are rounded to f16 in pieces whose
+ * sum holds 21 bits or more, the outputs' products where xtype and otype are 16
+ * bits to single f16 values; sums are f32.  `work`: device scratch of
+ * cwen_gdn_prompt_work's bytes, 256-byte aligned, free again when the call's
+ * launches are done. */
+int cwen_gdn_step(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *q, long long q_ts,
+                  const void *k, long long k_ts, const void *v, long long v_ts, const float *a, const float *b,
+                  long long g_ts, const float *A, const float *dt, int otype, void *o, long long o_ts, const int *cu,
+                  const int *count, const int *src, const int *dst, int n_seq, int total, void *stream);
+int cwen_gdn_prompt(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *q, long long q_ts,
+                    const void *k, long long k_ts, const void *v, long long v_ts, const float *a, const float *b,
+                    long long g_ts, const float *A, const float *dt, int otype, void *o, long long o_ts, const int *cu,
+                    const int *count, const int *src, const int *dst, int n_seq, int total, void *work,
+                    size_t work_bytes, void *stream);
+int cwen_gdn_prompt_work(const cwen_gdn_pool *pool, int xtype, int otype, int n_seq, int total, size_t *bytes);
+
+/* ---- log probabilities ----
+ * For each of `rows` rows of V logits (device, element type F32, F16 or BF16,
+ * rows `ls` elements apart), x a row:
+ *   lse      ln sum_i exp(x_i)
+ *   entropy  -sum_i p_i ln p_i, p_i = exp(x_i - lse)
+ *   logprob  x_t - lse of the row's token t = tokens[row]
+ *   rank     how many logits come before it: greater, or equal at a lower index
+ *   top_ids, top_logprobs [rows][top]: the `top` largest logits' indices in that
+ *            order (ties: lower index first, as argmax_of, run.c:2647-2668) and
+ *            their log probabilities
+ * Every output is nullable; logprob and rank need `tokens` (device).  top <=
+ * CWEN_LOGPROBS_TOP; with fewer than `top` logits the rest is -1 and -inf.
+ * Logits of -inf have probability 0 (logprob -inf) and take no part in the
+ * entropy; a row of nothing else has lse -inf and NaN in the others.  A NaN or
+ * +inf makes the row's lse, entropy and log probabilities NaN; NaN takes no part
+ * in ranks and the top.  A token outside 0..V-1, or whose logit is NaN, has
+ * logprob NaN and rank -1.  Sums are f32 in a fixed order that depends on rows,
+ * V and the address's alignment only.  `work`: device scratch of
+ * cwen_logprobs_work's bytes, 16-byte aligned. */
+#define CWEN_LOGPROBS_TOP 64
+int cwen_logprobs(cwen_ctx *ctx, int type, const void *logits, long long ls, int V, int rows, const int *tokens,
+                  float *logprob, int *rank, float *entropy, float *lse, int top, int *top_ids, float *top_logprobs,
+                  void *work, size_t work_bytes, void *stream);
+int cwen_logprobs_work(int rows, int V, int top, size_t *bytes);
+
 /* ---- rotary positions ----
  * Turns the first n_rot dims of each head by angles a_i = pos * f_i, i <
  * n_rot / 2: the pair (x, y) becomes m (x cos a - y sin a, x sin a + y cos a);
