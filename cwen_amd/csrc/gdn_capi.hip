@@ -91,6 +91,7 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
     if (!clear_of(x, x_ts * xe, (long long)C * xe, y, y_ts * ye, (long long)C * ye, total, true)) return CWEN_EINVAL;
   }
   if (n_seq == 0) return CWEN_OK;
+  if (gdn_pieces(total, n_seq, 32) >= 2 * launch_max) return CWEN_EINVAL;      // workgroups of 128
   OnDevice dev(ctx->device);
   if (dev.rc) return dev.rc;
   const GdnConvArgs a = {{cu, count, src, dst, n_seq, total, pool->n_slots, pool->status}, x, y, x_ts, y_ts, kw,
@@ -107,6 +108,7 @@ int cwen_gdn_step(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
   const int rc = check_rule(ctx, pool, layer, xtype, q, q_ts, k, k_ts, v, v_ts, a, b, g_ts, A, dt, otype, o, o_ts, cu, count, src, dst,
                             n_seq, total, &args, &none);
   if (rc || none) return rc;
+  if ((long long)n_seq * pool->nvh >= launch_max) return CWEN_EINVAL;
   OnDevice dev(ctx->device);
   return dev.rc ? dev.rc : gdn_step_launch(xtype, otype, pool->dk, args, (hipStream_t)stream);
 }
@@ -131,7 +133,7 @@ int cwen_gdn_prompt(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xty
   const int rc = check_rule(ctx, pool, layer, xtype, q, q_ts, k, k_ts, v, v_ts, a, b, g_ts, A, dt, otype, o, o_ts, cu, count, src, dst,
                             n_seq, total, &args, &none);
   if (rc || none) return rc;
-  if (gdn_pieces(total, n_seq, 32) * pool->nvh >= launch_max) return CWEN_EINVAL;
+  if (gdn_pieces(total, n_seq, 32) * pool->nvh * 2 >= launch_max) return CWEN_EINVAL;
   const size_t need = gdn_prompt_bytes(xtype, otype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
   if (need && (!work || ((uintptr_t)work & 255u))) return CWEN_EINVAL;
   if (work_bytes < need) return CWEN_ESCRATCH;

@@ -228,8 +228,3 @@ int gdn_step_launch(int xtype, int otype, int D, const GdnRuleArgs &a, hipStream
   CWEN_HIP_TRY(hipGetLastError());
   return CWEN_OK;
 }
-
-size_t gdn_prompt_bytes(int, int, int, int, int, int, int) { return 0; }
-int gdn_prompt_launch(int xtype, int otype, int D, const GdnRuleArgs &a, void *, hipStream_t st) {
-  return gdn_step_launch(xtype, otype, D, a, st);
-}

@@ -694,7 +694,7 @@ def _gdn_rule(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, src
     vs = _heads("v", v, (T, pool.nvh, pool.dk), q.dtype)
     os_ = 0 if o is None else _heads("o", o, (T, pool.nvh, pool.dk))
     for name, t in (("a", a), ("b", b)):
-        if tuple(t.shape) != (T, pool.nvh) or str(t.dtype) != "torch.float32" or (t.numel() and t.stride(1) != 1):
+        if tuple(t.shape) != (T, pool.nvh) or str(t.dtype) != "torch.float32" or (t.numel() and pool.nvh > 1 and t.stride(1) != 1):
             raise ValueError(f"{name}: float32 [{T}, {pool.nvh}] with a row's elements in a row expected")
     gs = _row_stride(a, T, pool.nvh)
     if gs != _row_stride(b, T, pool.nvh):

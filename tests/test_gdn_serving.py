@@ -87,8 +87,8 @@ def test_rule_refusals():
     n = C.c_size_t()
     assert gpu.lib().cwen_gdn_prompt_work(pool(), BF16, BF16, 1, 40, C.byref(n)) == OK
     if n.value:
-        assert rule("prompt", total=40, wb=n.value - 1) == ESCRATCH
-        assert rule("prompt", total=40, work=None) == EINVAL and rule("prompt", total=40, work=P + 64) == EINVAL
+        assert rule("prompt", o=None, total=40, wb=n.value - 1) == ESCRATCH
+        assert rule("prompt", o=None, total=40, work=None) == EINVAL and rule("prompt", o=None, total=40, work=P + 64) == EINVAL
     assert rule("prompt", c=pool(nvh=4096, nkh=1), vs=4096 * 64, os=4096 * 64, gs=4096, qs=4096 * 64, ks=4096 * 64, total=1 << 20,
                 q=P, k=P, v=P, o=None) == EINVAL          # chunks times heads past a launch
     L = gpu.lib()
