@@ -50,6 +50,7 @@ int check_rule(const cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xt
   }
   *none = n_seq == 0;
   const long long layer_floats = (long long)pool->n_slots * pool->nvh * D * D;
+  if (total == 1) q_ts = k_ts = kr, v_ts = o_ts = vr, g_ts = pool->nvh;       // strides of nothing
   *out = {{cu, count, src, dst, n_seq, total, pool->n_slots, pool->status}, q, k, v, o, q_ts, k_ts, v_ts, o_ts, g_ts, a, b, A, dt,
           pool->state + layer * layer_floats, pool->nkh, pool->nvh, pool->key_head == CWEN_GDN_GROUP ? pool->nvh / pool->nkh : 0};
   return CWEN_OK;
@@ -134,6 +135,7 @@ int cwen_gdn_prompt(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xty
                             n_seq, total, &args, &none);
   if (rc || none) return rc;
   if (gdn_pieces(total, n_seq, 32) * pool->nvh * 2 >= launch_max) return CWEN_EINVAL;
+  if (total > 1 && (v_ts >= 1 << 24 || (o && o_ts >= 1 << 24))) return CWEN_EINVAL;      // a chunk's rows by 32-bit offsets
   const size_t need = gdn_prompt_bytes(xtype, otype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
   if (need && (!work || ((uintptr_t)work & 255u))) return CWEN_EINVAL;
   if (work_bytes < need) return CWEN_ESCRATCH;

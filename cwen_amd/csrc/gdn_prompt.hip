@@ -2,10 +2,10 @@
 //
 // With G_i the log decays of a chunk's rows summed up to row i, D_ij = exp(G_i -
 // G_j) and S the state before the chunk, the rows' updates d_i solve
-//   (1 + L) d = r,  L_ij = beta_i D_ij k_i.k_j (j < i),  r_i = beta_i (v_i - e^G_i S^T k_i)
+//   (1 + L) d = beta r,  L_ij = beta_i D_ij k_i.k_j (j < i),  r_i = v_i - e^G_i S^T k_i
 // and   o_i = (e^G_i S^T q_i + sum_(j <= i) D_ij q_i.k_j d_j) / sqrt(D)
 //       S  <- e^G_31 S + sum_i e^(G_31 - G_i) k_i d_i^T.
-// T = (1 + L)^-1 and the scores A_ij = D_ij q_i.k_j / sqrt(D) do not depend on
+// T = (1 + L)^-1 beta and the scores A_ij = D_ij q_i.k_j do not depend on
 // the state: a first launch forms them for all chunks side by side, a second
 // one runs over the chunks of each sequence and head, S in registers.
 //
@@ -19,12 +19,12 @@
 // waves.  K and Q are laid out in that order by the first launch.
 //
 // Precision: f32 values enter a product as two f16 values, x s = hi + lo with a
-// power of two s, 21 bits and more below the column's largest.  One s serves a
-// chunk's S, r and d: with the largest |S| and |v| of a column at 2^8 .. 2^9,
-// |S^T k| <= sqrt(128) 2^9, and r and d (which the rule does not enlarge) stay
-// below 2^15.  Keys and queries of 16 bits are exact f16 values after a power of
-// two; what is left of their length (rho, 1 .. 2) goes into the rows' factors.  f32
-// ones are normalised and split.
+// power of two s per column: 22 bits, and down to 2^-25 of a unit.  The unit is
+// taken anew, the larger of |S| and |v| at 1 .. 2, every 8 chunks and whenever a
+// chunk's largest |v| is outside 1/8 .. 16 units; so |S^T k|, r and d (|S| grows by
+// the rows' |v| at most) stay below 2^14.  Keys and queries of 16 bits are exact
+// f16 values after a power of two; what is left of their length (rho, 1 .. 2) goes into
+// the rows' factors.  f32 ones are normalised and split.
 #include <math.h>
 #include "gdn_seq.h"
 #include "attn_core.h"
@@ -43,11 +43,11 @@ template <int D, bool KL, bool OF> struct Rec {
   static constexpr int K = 0, KLO = OP, Q = KL ? 2 * OP : OP, QLO = 3 * OP, KEY = KL ? 4 * OP : 2 * OP;
   static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = OF ? 8192 : 6144, HEAD = F + 1024;
 };
-// The factors: per row beta, beta e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31.  The scores
+// The factors: per row e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31 (beta is in T's columns).  The scores
 // and the last of the rows' factors are in units of O_UNIT, so that the low halves of small scores are no
 // subnormals, and without 1 / sqrt(D).
 constexpr float O_UNIT = 1.f / 64;
-enum { F_BETA = 0, F_X = 32, F_D = 64, F_O = 96, F_END = 128 };
+enum { F_X = 0, F_D = 32, F_O = 64, F_END = 96 };
 
 // Whether the outputs are formed with both halves of S, A and d.  Single ones are
 // off by 2^-12 of S, A and d: beside the rounding to bf16 (2^-9) that does not show,
@@ -61,9 +61,10 @@ struct PromptWork {
 __device__ __forceinline__ int operand_at(int row, int d, int U) {       // half index
   return (((row >> 4) * U + (d >> 5)) * 64 + ((d & 15) >> 2) * 16 + (row & 15)) * 8 + (d & 3) + ((d >> 4) & 1) * 4;
 }
-// x as an f16 value, subnormals kept.  The opaque copy keeps the compiler from
-// folding a product or sum into the conversion: v_fma_mixlo_f16 gives 0 for
-// subnormal results, which the low halves of values around 1 are.
+// x as an f16 value.  The opaque copy gives it one rounding to f32 first: left to
+// itself, the compiler folds the product or sum before the conversion into one of
+// the value's uses and not into another (v_fma_mixlo_f16), and now and then the
+// two are different values; their difference is lost then.
 __device__ __forceinline__ _Float16 f16_of(float x) { return (_Float16)f32_of(x); }
 __device__ __forceinline__ floatx4_t mma(half8_t a, half8_t b, floatx4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -71,16 +72,18 @@ __device__ __forceinline__ floatx4_t mma(half8_t a, half8_t b, floatx4_t c) {
 __device__ __forceinline__ int value_head(const GdnRuleArgs &a, int hk, int r) { return a.group ? hk * a.group + r : hk + a.nkh * r; }
 
 // ---- first launch: a workgroup has one chunk of one key head ----
-constexpr int PREP_WAVES = 2;
+// Bound by the trips to memory and the steps of the solve, not by its bytes or operations: all loads stand at the
+// start, and LDS is used twice, so that four workgroups share a CU.
+constexpr int PREP_WAVES = 4;
 
 template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {
   constexpr bool KL = sizeof(TX) == 4;
   typedef Rec<D, KL, OF> R;
-  constexpr int U = R::U, GS = 33, HEADS = 2 * PREP_WAVES;               // HEADS value heads at a time
-  __shared__ __align__(16) char s_key[R::KEY];
+  constexpr int U = R::U, GS = 33, HEADS = 4, HB = R::F + 64;     // HEADS value heads at a time, two a wave
+  constexpr int BYTES = R::KEY > HEADS * HB ? R::KEY : HEADS * HB;
+  // First K and Q; then, for a head, the rows of L (read 4 floats at a time), then its T hi, T lo, A operands.
+  __shared__ __align__(16) char s_mem[BYTES];
   __shared__ float s_G[N * GS], s_P[N * GS], s_rho[N], s_sig[N];
-  // L of a head, then its T hi, T lo, A operands (rows of L are read 4 floats at a time)
-  __shared__ __align__(16) char s_head[HEADS][R::F + 64];
   __shared__ float2 s_gb[HEADS][N];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int z = blockIdx.x / a.nkh, hk = blockIdx.x - z * a.nkh;
@@ -90,99 +93,105 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
   const int t0 = (z - gdn_piece0(q.first, s, N)) * N, rows = min(q.n - t0, N);
   if (t0 < 0 || rows <= 0) return;
   const long long first = (long long)q.first + t0;
+  const int n = lane & 31, sub = 2 * wave + (lane >> 5), grp = a.nvh / a.nkh;
+  // The gates of value head r0 + sub, row n.
+  auto gate = [&](int r0, float &g, float &beta, int &hv) {
+    const int r = r0 + sub;
+    const bool have = sub < HEADS && r < grp;
+    hv = have ? value_head(a, hk, r) : -1;
+    g = beta = 0.f;
+    if (have && n < rows) {
+      g = a.a[(first + n) * a.gs + hv];
+      beta = a.b[(first + n) * a.gs + hv];
+    }
+  };
 
   // K and Q into LDS as operands: 8 threads a row
   constexpr int PER = D / 8;
+  const int row = tid >> 3;
+  float x[2][PER], g, beta;
+  int hv;
 #pragma unroll
-  for (int op = 0; op < 2; ++op)
-    for (int row = tid >> 3; row < N; row += 8 * PREP_WAVES) {
-      const TX *p = (const TX *)(op ? a.q : a.k) + (first + min(row, rows - 1)) * (op ? a.qs : a.ks) + hk * D + (tid & 7) * PER;
-      float x[PER], ss = 0.f;
+  for (int op = 0; op < 2; ++op) {
+    const TX *p = (const TX *)(op ? a.q : a.k) + (first + min(row, rows - 1)) * (op ? a.qs : a.ks) + hk * D + (tid & 7) * PER;
 #pragma unroll
-      for (int i = 0; i < PER; i += 8) Io<TX>::load(p + i, *(float(*)[8])&x[i]);
+    for (int i = 0; i < PER; i += 8) Io<TX>::load(p + i, *(float(*)[8])&x[op][i]);
+  }
+  gate(0, g, beta, hv);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (row >= rows) x[i] = 0.f;
-        ss = fmaf(x[i], x[i], ss);
-      }
-      ss += dpp<0xB1>(ss);
-      ss += dpp<0x4E>(ss);
-      ss += dpp<0x141>(ss);
-      const float inv = 1.f / sqrtf(ss + 1e-6f);
-      // 16 bits: the power of two below 1 / length, exact; the rest is a factor of the row
-      const float f = KL ? inv : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) & 0x7f800000u);
-      if ((tid & 7) == 0) (op ? s_sig : s_rho)[row] = KL || f == 0.f ? 1.f : inv / f;
-      _Float16 *hi = (_Float16 *)(s_key + (op ? R::Q : R::K)), *lo = (_Float16 *)(s_key + (op ? R::QLO : R::KLO));
+  for (int op = 0; op < 2; ++op) {
+    float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < PER; i += 4) {
-        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-        half4 h, l;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float y = x[i + j] * f;
-          h[j] = f16_of(y);
-          l[j] = f16_of(y - (float)h[j]);
-        }
-        const int at = operand_at(row, (tid & 7) * PER + i, U);
-        *(half4 *)(hi + at) = h;
-        if (KL) *(half4 *)(lo + at) = l;
-      }
+    for (int i = 0; i < PER; ++i) {
+      if (row >= rows) x[op][i] = 0.f;
+      ss = fmaf(x[op][i], x[op][i], ss);
     }
+    ss += dpp<0xB1>(ss);
+    ss += dpp<0x4E>(ss);
+    ss += dpp<0x141>(ss);
+    const float inv = 1.f / sqrtf(ss + 1e-6f);
+    // 16 bits: the power of two below 1 / length, exact; the rest is a factor of the row
+    const float f = KL ? inv : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) & 0x7f800000u);
+    if ((tid & 7) == 0) (op ? s_sig : s_rho)[row] = KL || f == 0.f ? 1.f : inv / f;
+    _Float16 *hi = (_Float16 *)(s_mem + (op ? R::Q : R::K)), *lo = (_Float16 *)(s_mem + (op ? R::QLO : R::KLO));
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+      half4 h, l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = x[op][i + j] * f;
+        h[j] = f16_of(y);
+        l[j] = f16_of(y - (float)h[j]);
+      }
+      const int at = operand_at(row, (tid & 7) * PER + i, U);
+      *(half4 *)(hi + at) = h;
+      if (KL) *(half4 *)(lo + at) = l;
+    }
+  }
   __syncthreads();
   {
     char *out = w.key + ((long long)z * a.nkh + hk) * R::KEY;
-    for (int i = tid * 16; i < R::KEY; i += 64 * PREP_WAVES * 16) *(uint4 *)(out + i) = *(const uint4 *)(s_key + i);
+#pragma unroll
+    for (int i = 0; i < R::KEY; i += 64 * PREP_WAVES * 16) *(uint4 *)(out + i + tid * 16) = *(const uint4 *)(s_mem + i + tid * 16);
   }
-  // k_i.k_j and q_i.k_j: the waves take the rows' halves
-  for (int mt = wave; mt < 2; mt += PREP_WAVES) {
-    floatx4_t g[2] = {}, p[2] = {};
+  // k_i.k_j (waves 0, 1) and q_i.k_j (2, 3), 16 rows i each
+  {
+    const int mt = wave & 1;
+    const bool isq = wave >> 1;
+    floatx4_t c[2] = {};
+    auto op = [&](int base, int m, int u) { return *(const half8_t *)(s_mem + base + ((m * U + u) * 64 + lane) * 16); };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      auto op = [&](int base, int m) { return *(const half8_t *)(s_key + base + ((m * U + u) * 64 + lane) * 16); };
-      const half8_t km = op(R::K, mt), qm = op(R::Q, mt);
+      const half8_t m = op(isq ? R::Q : R::K, mt, u);
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        const half8_t kn = op(R::K, nt);
-        g[nt] = mma(km, kn, g[nt]);
-        p[nt] = mma(qm, kn, p[nt]);
-        if (KL) {
-          const half8_t kl = op(R::KLO, nt);
-          g[nt] = mma(km, kl, mma(op(R::KLO, mt), kn, g[nt]));
-          p[nt] = mma(qm, kl, mma(op(R::QLO, mt), kn, p[nt]));
-        }
+        const half8_t kn = op(R::K, nt, u);
+        c[nt] = mma(m, kn, c[nt]);
+        if (KL) c[nt] = mma(m, op(R::KLO, nt, u), mma(op(isq ? R::QLO : R::KLO, mt, u), kn, c[nt]));
       }
     }
+    float *to = isq ? s_P : s_G;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * mt + 4 * (lane >> 4) + i, col = 16 * nt + (lane & 15);
-        s_G[row * GS + col] = g[nt][i];
-        s_P[row * GS + col] = p[nt][i];
-      }
+      for (int i = 0; i < 4; ++i) to[(16 * mt + 4 * (lane >> 4) + i) * GS + 16 * nt + (lane & 15)] = c[nt][i];
   }
   __syncthreads();
 
   // The value heads: 32 lanes each, lane n the column n of L, T and A.
-  const int n = lane & 31, sub = 2 * wave + (lane >> 5), grp = a.nvh / a.nkh;
+  if (wave >= HEADS / 2) return;
   const float rho = s_rho[n], sig = s_sig[n];
   for (int r0 = 0; r0 < grp; r0 += HEADS) {
-    const int r = r0 + sub;
-    const bool have = r < grp;
-    const int hv = value_head(a, hk, have ? r : 0);
-    float g = 0.f, beta = 0.f;
-    if (have && n < rows) {
-      g = a.a[(first + n) * a.gs + hv];
-      beta = a.b[(first + n) * a.gs + hv];
-      if (a.A) {
-        const float y = g + a.dt[hv];
-        g = a.A[hv] * (y > 20.f ? y : log1pf(expf(y)));
-        beta = 1.f / (1.f + expf(-beta));
-      }
+    if (r0) gate(r0, g, beta, hv);
+    if (a.A && hv >= 0 && n < rows) {
+      const float y = g + a.dt[hv];
+      g = a.A[hv] * (y > 20.f ? y : log1pf(expf(y)));
+      beta = 1.f / (1.f + expf(-beta));
     }
     s_gb[sub][n] = make_float2(g, beta);
-    float *L = (float *)s_head[sub];
-    _Float16 *op = (_Float16 *)s_head[sub];
+    float *L = (float *)(s_mem + sub * HB);
+    _Float16 *op = (_Float16 *)L;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     // Decays from n to i, added up from n on: no difference of sums that are far larger.
     float acc = 0.f, pre = 0.f, dec = 1.f;
@@ -196,11 +205,11 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
       L[i * N + n] = i > n ? gb.y * s_rho[i] * rho * dec * s_G[i * GS + n] : 0.f;
       A[i] = i >= n ? s_sig[i] * rho * dec * s_P[i * GS + n] / O_UNIT : 0.f;
     }
-    if (have) {
-      float *F = (float *)(w.head + ((long long)z * a.nvh + hv) * R::HEAD + R::F);
+    char *out = w.head + ((long long)z * a.nvh + max(hv, 0)) * R::HEAD;
+    if (hv >= 0) {
+      float *F = (float *)(out + R::F);
       const float e = expf(pre);
-      F[F_BETA + n] = beta;
-      F[F_X + n] = beta * e * rho;
+      F[F_X + n] = e * rho;
       F[F_D + n] = rho * dec;
       F[F_O + n] = e * sig / O_UNIT;
       if (n == N - 1) F[F_END] = e;
@@ -225,49 +234,307 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = operand_at(i, n, 1);
-      const _Float16 h = f16_of(T[i]), x = f16_of(A[i]);
+      const float t = T[i] * beta;
+      const _Float16 h = f16_of(t), x = f16_of(A[i]);
       op[R::T / 2 + at] = h;
-      op[R::TLO / 2 + at] = f16_of(T[i] - (float)h);
+      op[R::TLO / 2 + at] = f16_of(t - (float)h);
       op[R::A / 2 + at] = x;
       if (OF) op[R::ALO / 2 + at] = f16_of(A[i] - (float)x);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (have) {
-      char *out = w.head + ((long long)z * a.nvh + hv) * R::HEAD;
+    if (hv >= 0) {
 #pragma unroll
-      for (int i = 0; i < R::F; i += 512) *(uint4 *)(out + i + n * 16) = *(const uint4 *)(s_head[sub] + i + n * 16);
+      for (int i = 0; i < R::F; i += 512) *(uint4 *)(out + i + n * 16) = *(const uint4 *)(s_mem + sub * HB + i + n * 16);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
 // ---- second launch: NW waves of 16 columns of one head's state, over a sequence's chunks ----
+// One more wave of the workgroup brings the records into LDS, two chunks ahead: the loads take the time of
+// their bytes to issue, which a wave of the chain would wait out.
 // The column's largest over the 4 lanes that share it.
 __device__ __forceinline__ float max_groups(float x) {
   const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
   return max_halves(fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1])));
 }
-// x f, f a power of two, as two f16 values (below 2^-14 as 0, 2^-22 of the column's largest).
-__device__ __forceinline__ void split(float x, float f, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)(x * f);
-  lo = (_Float16)fmaf(x, f, -(float)hi);
+// Two operands whose sum is x, one multiply-add that rounds to f16 for each low half (the compiler takes two
+// instructions and a half).  The block reads x behind the conversions that gave h0 .. h3, so a matrix result in x is
+// complete; its last instruction is the wait that a vector result needs before a matrix instruction reads it.
+__device__ __forceinline__ void split8(const float (&x)[8], half8_t &hi, half8_t &lo) {
+  half2_t h0 = {(_Float16)x[0], (_Float16)x[1]}, h1 = {(_Float16)x[2], (_Float16)x[3]};
+  half2_t h2 = {(_Float16)x[4], (_Float16)x[5]}, h3 = {(_Float16)x[6], (_Float16)x[7]}, l0, l1, l2, l3;
+  asm("v_fma_mixlo_f16 %0, %8, 1.0, -%4 op_sel_hi:[0,0,1]\n"
+      "v_fma_mixlo_f16 %1, %10, 1.0, -%5 op_sel_hi:[0,0,1]\n"
+      "v_fma_mixlo_f16 %2, %12, 1.0, -%6 op_sel_hi:[0,0,1]\n"
+      "v_fma_mixlo_f16 %3, %14, 1.0, -%7 op_sel_hi:[0,0,1]\n"
+      "v_fma_mixhi_f16 %0, %9, 1.0, -%4 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n"
+      "v_fma_mixhi_f16 %1, %11, 1.0, -%5 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n"
+      "v_fma_mixhi_f16 %2, %13, 1.0, -%6 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n"
+      "v_fma_mixhi_f16 %3, %15, 1.0, -%7 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n"
+      "s_nop 1"
+      : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "+v"(h0), "+v"(h1), "+v"(h2), "+v"(h3)
+      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+  hi = (half8_t){h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+  lo = (half8_t){l0[0], l0[1], l1[0], l1[1], l2[0], l2[1], l3[0], l3[1]};
 }
-// Any value.  The opaque copy makes its high half one value: left to itself, the
-// compiler folds the product or sum before it into one of the half's two uses,
-// where it is rounded once instead of twice and now and then is another.
-__device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
-  x = f32_of(x);
-  hi = (_Float16)x;
-  lo = (_Float16)(x - (float)hi);
+// The high one alone.
+__device__ __forceinline__ half8_t high8(const float (&x)[8]) {
+  return (half8_t){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3], (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
 }
 
-template <typename TX, typename TO, int D, int NW> __global__ __launch_bounds__(64 * NW) void chain_kernel(GdnRuleArgs a, PromptWork w) {
-  constexpr bool KL = sizeof(TX) == 4, OF = full_out<TX, TO>();
+template <typename TX, typename TO, int D, int NW> struct Chain {
+  static constexpr bool KL = sizeof(TX) == 4, OF = full_out<TX, TO>();
   typedef Rec<D, KL, OF> R;
-  constexpr int U = R::U, DT = D / 16, SL = D / (16 * NW), KB = (R::KEY + R::HEAD) / 1024;
-  __shared__ __align__(1024) char s_buf[2][R::KEY + R::HEAD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  const int per = a.nvh * SL, s = blockIdx.x / per, i0 = blockIdx.x - s * per, grp = a.nvh / a.nkh;
+  static constexpr int U = R::U, DT = D / 16, KB = (R::KEY + R::HEAD) / 1024, XS = sizeof(TX), OS = sizeof(TO);
+  static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
+  typedef char Buf[R::KEY + R::HEAD];
+
+  int lane, n, g;
+  // the sequence
+  long long v_chunk, o_chunk;        // bytes of a chunk's rows
+  const char *v0;
+  char *o0;
+  int rows;
+  uint32_t v_row, o_row;             // bytes of a row
+  uint32_t v_at[VP], o_at[OP];
+  char *s_v, *s_o;                   // the wave's columns of a chunk, row by row
+  float out_unit;
+  // the state, divided by the column's unit, and the present chunk's values
+  floatx4_t S[DT];
+  float unit, per_unit, v[8], vmax;
+  uint4 vr[3][VP];                   // values on their way: chunk c's in vr[c % 3]
+  float far[XS == 4 ? 8 : 4];    // the chunk's after that, by columns (16 bits: two a float)
+
+  // A chunk's rows of v and o as buffers that end with the sequence: loads past it give 0, stores past it (and to no o)
+  // do nothing, so no row needs a comparison.  A lane takes 16 bytes at a time; LDS turns rows into columns.
+  __device__ __forceinline__ uint32_t bytes_of(int c, uint32_t row, int es) const {
+    const int left = min(rows - c * N, N);
+    return c >= 0 && left > 0 ? (uint32_t)(left - 1) * row + D * es : 0u;
+  }
+  __device__ __forceinline__ void load_v(int c, uint4 (&to)[VP]) const {
+    const auto r = make_rsrc(v0 + c * v_chunk, bytes_of(c, v_row, XS));
+#pragma unroll
+    for (int i = 0; i < VP; ++i) to[i] = bload16(r, v_at[i]);
+  }
+  __device__ __forceinline__ void turn_v(const uint4 (&from)[VP]) {
+    typedef typename std::conditional<std::is_same<TX, TypeBF16::elem>::value, TypeBF16, TypeF16>::type Type;
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < VP; ++i) *(uint4 *)(s_v + (i * 64 + lane) * 16) = from[i];
+    asm volatile("" ::: "memory");
+    if constexpr (XS == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) far[e] = ((const float *)s_v)[((e >> 2) * 16 + 4 * g + (e & 3)) * 16 + n];
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 x = __builtin_bit_cast(f2, AttnOps<Type>::tr(s_v + (mt * 16 + 4 * g + (n >> 2)) * 32 + (n & 3) * 8));
+        far[2 * mt] = x[0];
+        far[2 * mt + 1] = x[1];
+      }
+    }
+  }
+  // The turned values become the present ones; vmax: their column's largest.
+  __device__ __forceinline__ void take_v() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (XS == 4) {
+        v[e] = far[e];
+      } else {
+        const uint32_t x = __builtin_bit_cast(uint32_t, far[e >> 1]);
+        if constexpr (std::is_same<TX, TypeBF16::elem>::value) v[e] = __builtin_bit_cast(float, e & 1 ? x & 0xffff0000u : x << 16);
+        else v[e] = (float)__builtin_bit_cast(half2_t, x)[e & 1];
+      }
+    }
+    vmax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]));
+    vmax = max_groups(vmax);
+  }
+  // The unit for the larger of |S| and `most` (a |v|) to lie in 1 .. 2; returns what S has to be multiplied by.
+  __device__ __forceinline__ float renew(float most) {
+    float mx = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fabsf(S[t][i]));
+    mx = fmaxf(max_groups(mx) * unit, most);
+    const int ex = min(max((int)(__builtin_bit_cast(uint32_t, mx) >> 23), 1), 253);
+    const float old = unit;
+    unit = __builtin_bit_cast(float, ex << 23);
+    per_unit = __builtin_bit_cast(float, (254 - ex) << 23);
+    // (a column that fell further than 2^100 since holds nothing beside what it held)
+    return fminf(old * per_unit, 0x1p100f);
+  }
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  __device__ __forceinline__ void read_o(u32x4 (&x)[OP]) const {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < OP; ++i) x[i] = *(const u32x4 *)(s_o + (i * 64 + lane) * 16);
+    asm volatile("" ::: "memory");
+  }
+  __device__ __forceinline__ void store_o(int c, const u32x4 (&x)[OP]) const {
+    const auto r = make_rsrc(o0 + c * o_chunk, o0 ? bytes_of(c, o_row, OS) : 0u);
+#pragma unroll
+    for (int i = 0; i < OP; ++i) __builtin_amdgcn_raw_buffer_store_b128(x[i], r, o_at[i], 0, 0);
+  }
+
+  // Chunk c, whose record is in `b` behind the barrier.  v holds its values, `far` those of c + 1, vr_2 those of c + 2;
+  // vr_4 takes c + 4's.
+  __device__ __forceinline__ void chunk(int c, Buf &b, const uint4 (&vr_2)[VP], uint4 (&vr_4)[VP]) {
+    const float *F = (const float *)(b + R::KEY + R::F);
+    u32x4 o_last[OP];
+    read_o(o_last);
+    lds_barrier();
+    asm volatile("" ::: "memory");
+    auto op = [&](int base, int i) __attribute__((always_inline)) { return *(const half8_t *)(b + base + (i * 64 + lane) * 16); };
+    auto rows4 = [&](int f, int mt) __attribute__((always_inline)) { return *(const floatx4_t *)(F + f + 16 * mt + 4 * g); };
+    // lane i of 16: rows 4 g + i / 4, dims 4 (i % 4) ..; it gets dim i of the four rows
+    auto kt = [&](int base, int t) __attribute__((always_inline)) {
+      const char *p = b + base + ((t >> 1) * 64 + (n & 3) * 16 + 4 * g + (n >> 2)) * 16 + (t & 1) * 8;
+      const auto x = AttnOps<TypeF16>::tr(p), y = AttnOps<TypeF16>::tr(p + U * 1024);
+      return (half8_t){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+    // Operands are asked for a stage before the product that takes them (stages do not mix): left to itself the
+    // compiler reads each one just ahead of its product, and the wave, alone on its SIMD, waits for LDS 30 times a chunk.
+    half8_t K[2 * U], KL_[2 * U];
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+      K[i] = op(R::K, i);
+      if (KL) KL_[i] = op(R::KLO, i);
+    }
+    floatx4_t fx[2], fd[2], fo[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) fx[mt] = rows4(F_X, mt);
+    // The present values in units, and whether the next ones call for new units in the chunks to come: at least every
+    // 8, and where their |v| leaves what the present one is good for.  In between |S| grows by the rows' |v| < 16 units
+    // at most.
+    float w[8], ratio = 1.f;
+    const float vmax_here = vmax, unit_here = unit;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v[e] * per_unit;
+    take_v();
+    const float vu = vmax * per_unit;
+    if (!__all((c & 7) != 7 && vu < 16.f && vu >= 0.125f)) ratio = renew(fmaxf(vmax_here, vmax));
+    store_o(c - 1, o_last);
+    load_v(c + 4, vr_4);
+    half8_t T[2], TL[2], Q[2 * U], QL[2 * U];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) T[mt] = op(R::KEY + R::T, mt), TL[mt] = op(R::KEY + R::TLO, mt);
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+      Q[i] = op(R::Q, i);
+      if (KL) QL[i] = op(R::QLO, i);
+    }
+    half8_t hi[U], lo[U];
+    floatx4_t X[2] = {}, Y[2] = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = S[2 * u + (j >> 2)][j & 3];
+      split8(x, hi[u], lo[u]);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        X[mt] = mma(K[mt * U + u], lo[u], X[mt]);
+        X[mt] = mma(K[mt * U + u], hi[u], X[mt]);
+        if (KL) X[mt] = mma(KL_[mt * U + u], hi[u], X[mt]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    half8_t KT[DT], KTL[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      KT[t] = kt(R::K, t);
+      if (KL) KTL[t] = kt(R::KLO, t);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) fd[mt] = rows4(F_D, mt), fo[mt] = rows4(F_O, mt);
+    const float end = F[F_END];
+    half8_t A[2], AL[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      A[mt] = op(R::KEY + R::A, mt);
+      if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+    }
+    half8_t rh, rl;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
+        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+        if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
+      }
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = fmaf(-fx[e >> 2][e & 3], X[e >> 2][e & 3], w[e]);
+    split8(r, rh, rl);
+    floatx4_t d[2] = {};
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, d[mt])));
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[t][i] *= end * ratio;
+    __builtin_amdgcn_sched_barrier(0);
+    turn_v(vr_2);
+    half8_t dh, dl, oh, ol;
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = d[e >> 2][e & 3];
+      y[e] = x[e] * (fd[e >> 2][e & 3] * ratio);
+    }
+    split8(y, dh, dl);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) S[t] = mma(KT[t], dl, S[t]);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) S[t] = mma(KT[t], dh, S[t]);
+    if (KL)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) S[t] = mma(KTL[t], dh, S[t]);
+    if (OF) split8(x, oh, ol);
+    else oh = high8(x);
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      floatx4_t y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = fo[mt][i] * Y[mt][i];
+      y = mma(A[mt], oh, y);
+      if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ((TO *)s_o)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
+    }
+  }
+};
+
+// The nth longest sequence (of up to 64; more stay in their order), so that no long one starts when the others are done.
+__device__ __forceinline__ int nth_longest(const GdnSeqs &a, int nth) {
+  if (a.n_seq == 1 || a.n_seq > 64) return nth;
+  const int lane = threadIdx.x & 63, n = lane < a.n_seq ? gdn_seq(a, lane).n : -1;
+  int rank = 0;
+  for (int j = 0; j < a.n_seq; ++j) {
+    const int m = __builtin_amdgcn_readlane(n, j);
+    rank += m > n || (m == n && j < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < a.n_seq && rank == nth));
+}
+
+// Three records in LDS, an array each: in one, the compiler would wait for the loads into one record
+// before it reads another.
+template <typename TX, typename TO, int D, int NW>
+__global__ __launch_bounds__(64 * (NW + 1)) __attribute__((amdgpu_waves_per_eu(1, 2))) void chain_kernel(GdnRuleArgs a, PromptWork w) {
+  typedef Chain<TX, TO, D, NW> C;
+  typedef typename C::R R;
+  constexpr int SL = D / (16 * NW);
+  __shared__ __align__(1024) typename C::Buf b0, b1, b2;
+  __shared__ __align__(16) char s_v[NW][N * 16 * C::XS], s_o[NW][N * 16 * C::OS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = a.nvh * SL, nth = blockIdx.x / per, i0 = blockIdx.x - nth * per, grp = a.nvh / a.nkh;
+  const int s = nth_longest(a.s, nth);
   // Workgroups of one key head share its operands: on one XCD (block b runs on XCD b % 8).
   int hk, rest;
   if (a.nkh % 8 == 0) {
@@ -285,189 +552,103 @@ template <typename TX, typename TO, int D, int NW> __global__ __launch_bounds__(
     return;
   }
   if (q.n == 0 && (q.dst < 0 || q.dst == q.src)) return;
-  const int col = slice * 16 * NW + wave * 16 + n, chunks = (q.n + N - 1) / N;
-  const long long z0 = gdn_piece0(q.first, s, N);
-  const char *key = w.key + (z0 * a.nkh + hk) * R::KEY, *head = w.head + (z0 * a.nvh + hv) * R::HEAD;
-  const long long key_step = (long long)a.nkh * R::KEY, head_step = (long long)a.nvh * R::HEAD;
-  auto land = [&](int c) __attribute__((always_inline)) {
+  const int chunks = (q.n + N - 1) / N;
+  if (wave == NW) {
+    if (!chunks) return;
+    const long long z0 = gdn_piece0(q.first, s, N), key_step = (long long)a.nkh * R::KEY, head_step = (long long)a.nvh * R::HEAD;
+    const char *key = w.key + (z0 * a.nkh + hk) * R::KEY + lane * 16, *head = w.head + (z0 * a.nvh + hv) * R::HEAD + lane * 16;
+    // The next record, in order; past the last one that one again, so that there is always one to count.
+    int c = 0;
+    auto land = [&](typename C::Buf &to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < (KB + NW - 1) / NW; ++p) {
-      const int kb = p * NW + wave;
-      if (kb < KB) {
-        const char *from = kb < R::KEY / 1024 ? key + c * key_step + kb * 1024 : head + c * head_step + (kb * 1024 - R::KEY);
-        __builtin_amdgcn_global_load_lds((attn_glb_t *)(from + lane * 16), (attn_lds_t *)(s_buf[c & 1] + kb * 1024), 16, 0, 0);
-      }
+      for (int i = 0; i < R::KEY / 1024; ++i)
+        __builtin_amdgcn_global_load_lds((attn_glb_t *)(key + i * 1024), (attn_lds_t *)(to + i * 1024), 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < R::HEAD / 1024; ++i)
+        __builtin_amdgcn_global_load_lds((attn_glb_t *)(head + i * 1024), (attn_lds_t *)(to + R::KEY + i * 1024), 16, 0, 0);
+      if (++c < chunks) key += key_step, head += head_step;
+    };
+    // Buffer c % 3 is read until the barrier of chunk c + 1, behind which chunk c + 3 goes there.
+    auto next = [&](typename C::Buf &to) __attribute__((always_inline)) {
+      wait_loads<C::KB>();
+      lds_barrier();
+      asm volatile("" ::: "memory");
+      land(to);
+    };
+    land(b0);
+    land(b1);
+    for (int i = 0;;) {
+      next(b2);
+      if (++i == chunks) break;
+      next(b0);
+      if (++i == chunks) break;
+      next(b1);
+      if (++i == chunks) break;
     }
-  };
-  const TX *vp = (const TX *)a.v + (long long)q.first * a.vs + hv * D + col;
-  TX vr[8];
-  auto load_v = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) vr[e] = vp[(long long)min(c * N + (e >> 2) * 16 + 4 * g + (e & 3), q.n - 1) * a.vs];
-  };
-  floatx4_t S[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t) S[t] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
-  const long long slot = (long long)a.nvh * D * D, at = (long long)hv * D * D + 4 * g * D + col;
-  if (chunks) {
-    land(0);
-    load_v(0);
+    wait_loads<0>();            // what was asked for past the end lands before the LDS is given up
+    return;
   }
+  C p;
+  p.lane = lane;
+  p.n = lane & 15;
+  p.g = lane >> 4;
+  const int c0 = (slice * NW + wave) * 16;             // the wave's first column
+  const long long slot = (long long)a.nvh * D * D, at = (long long)hv * D * D + 4 * p.g * D + c0 + p.n;
+#pragma unroll
+  for (int t = 0; t < C::DT; ++t) p.S[t] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
   if (q.src >= 0) {
-    const float *p = a.state + q.src * slot + at;
+    const float *from = a.state + q.src * slot + at;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < C::DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) S[t][i] = p[(16 * t + i) * D];
+      for (int i = 0; i < 4; ++i) p.S[t][i] = from[(16 * t + i) * D];
   }
-  float unit = 1.f;             // S holds the state divided by it
-  float o[8];                   // the last chunk's outputs
-  auto store_o = [&](int c) __attribute__((always_inline)) {
-    TO *p = (TO *)a.o + (long long)q.first * a.os + hv * D + col;
+  p.unit = p.per_unit = 1.f;
+  if (chunks) {
+    p.rows = q.n;
+    p.v0 = (const char *)a.v + (q.first * a.vs + hv * D) * C::XS;
+    p.o0 = a.o ? (char *)a.o + (q.first * a.os + hv * D) * C::OS : nullptr;
+    p.v_row = (uint32_t)a.vs * C::XS;
+    p.o_row = (uint32_t)a.os * C::OS;
+    p.v_chunk = a.vs * C::XS * N;
+    p.o_chunk = a.os * C::OS * N;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int row = c * N + (e >> 2) * 16 + 4 * g + (e & 3);
-      if (row < q.n) p[(long long)row * a.os] = (TO)o[e];
+    for (int i = 0; i < C::VP; ++i) p.v_at[i] = (i * 64 + p.lane) / C::XS * p.v_row + c0 * C::XS + p.lane % C::XS * 16;
+#pragma unroll
+    for (int i = 0; i < C::OP; ++i) p.o_at[i] = (i * 64 + p.lane) / C::OS * p.o_row + c0 * C::OS + p.lane % C::OS * 16;
+    p.s_v = s_v[wave];
+    p.s_o = s_o[wave];
+    p.out_unit = O_UNIT / sqrtf((float)D);
+    p.load_v(0, p.vr[0]);
+    p.load_v(1, p.vr[1]);
+    p.load_v(2, p.vr[2]);
+    p.turn_v(p.vr[0]);
+    p.take_v();
+    p.turn_v(p.vr[1]);
+    p.load_v(3, p.vr[0]);
+    const float ratio = p.renew(p.vmax);
+#pragma unroll
+    for (int t = 0; t < C::DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p.S[t][i] *= ratio;
+    for (int c = 0;;) {
+      p.chunk(c, b0, p.vr[2], p.vr[1]);
+      if (++c == chunks) break;
+      p.chunk(c, b1, p.vr[0], p.vr[2]);
+      if (++c == chunks) break;
+      p.chunk(c, b2, p.vr[1], p.vr[0]);
+      if (++c == chunks) break;
     }
-  };
-  for (int c = 0; c < chunks; ++c) {
-    const char *b = s_buf[c & 1], *h = b + R::KEY;
-    wait_loads<0>();
-    lds_barrier();
-    asm volatile("" ::: "memory");
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c * N + (e >> 2) * 16 + 4 * g + (e & 3) < q.n ? (float)vr[e] : 0.f;
-    // The last outputs leave here, so that the wait above never meets a store that has just begun.
-    if (a.o && c) store_o(c - 1);
-    if (c + 1 < chunks) {
-      land(c + 1);
-      load_v(c + 1);
-    }
-    auto op = [&](int base, int i) __attribute__((always_inline)) { return *(const half8_t *)(b + base + (i * 64 + lane) * 16); };
-    // the new unit: the largest at 2^8 .. 2^9
-    float mx = 0.f;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) mx = fmaxf(fmaxf(fmaxf(mx, fabsf(S[t][0])), fmaxf(fabsf(S[t][1]), fabsf(S[t][2]))), fabsf(S[t][3]));
-    mx *= unit;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e]));
-    mx = max_groups(mx);
-    const int ex = min(max((int)(__builtin_bit_cast(uint32_t, mx) >> 23) - 8, 1), 253);
-    const float new_unit = __builtin_bit_cast(float, ex << 23), per_unit = __builtin_bit_cast(float, (254 - ex) << 23);
-    // (a column that fell further than 2^100 within a chunk holds nothing beside what it held)
-    const float ratio = fminf(unit * per_unit, 0x1p100f);
-    unit = new_unit;
-    half8_t hi[U], lo[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        _Float16 x, y;
-        split(S[2 * u + (j >> 2)][j & 3], ratio, x, y);
-        hi[u][j] = x;
-        lo[u][j] = y;
-      }
-    floatx4_t X[2] = {}, Y[2] = {};
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const half8_t k = op(R::K, mt * U + u);
-        X[mt] = mma(k, lo[u], X[mt]);
-        X[mt] = mma(k, hi[u], X[mt]);
-        if (KL) X[mt] = mma(op(R::KLO, mt * U + u), hi[u], X[mt]);
-      }
-    if (a.o) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const half8_t x = op(R::Q, mt * U + u);
-          Y[mt] = mma(x, hi[u], Y[mt]);
-          if (OF) Y[mt] = mma(x, lo[u], Y[mt]);
-          if (KL) Y[mt] = mma(op(R::QLO, mt * U + u), hi[u], Y[mt]);
-        }
-    }
-    const float *F = (const float *)(h + R::F);
-    auto rows4 = [&](int f, int mt) __attribute__((always_inline)) { return *(const floatx4_t *)(F + f + 16 * mt + 4 * g); };
-    half8_t rh, rl;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const floatx4_t fb = rows4(F_BETA, mt), fx = rows4(F_X, mt);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        _Float16 x, y;
-        split(fmaf(fb[i], v[4 * mt + i] * per_unit, -fx[i] * X[mt][i]), x, y);
-        rh[4 * mt + i] = x;
-        rl[4 * mt + i] = y;
-      }
-    }
-    floatx4_t d[2] = {};
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const half8_t th = op(R::KEY + R::T, mt);
-      d[mt] = mma(th, rh, mma(th, rl, mma(op(R::KEY + R::TLO, mt), rh, d[mt])));
-    }
-    half8_t dh, dl;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const floatx4_t fd = rows4(F_D, mt);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        _Float16 x, y;
-        split(d[mt][i] * fd[i], x, y);
-        dh[4 * mt + i] = x;
-        dl[4 * mt + i] = y;
-      }
-    }
-    const float end = F[F_END] * ratio;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      // lane i of 16: rows 4 g + i / 4, dims 4 (i % 4) ..; it gets dim i of the four rows
-      auto kt = [&](int base) __attribute__((always_inline)) {
-        const char *p = b + base + ((t >> 1) * 64 + (n & 3) * 16 + 4 * g + (n >> 2)) * 16 + (t & 1) * 8;
-        const auto x = AttnOps<TypeF16>::tr(p), y = AttnOps<TypeF16>::tr(p + U * 1024);
-        return (half8_t){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) S[t][i] *= end;
-      const half8_t k = kt(R::K);
-      S[t] = mma(k, dh, mma(k, dl, S[t]));
-      if (KL) S[t] = mma(kt(R::KLO), dh, S[t]);
-    }
-    if (a.o) {
-      half8_t oh, ol;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          _Float16 x, y;
-          split(d[mt][i], x, y);
-          oh[4 * mt + i] = x;
-          ol[4 * mt + i] = y;
-        }
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const floatx4_t fo = rows4(F_O, mt);
-        floatx4_t y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = fo[i] * Y[mt][i];
-        const half8_t A = op(R::KEY + R::A, mt);
-        y = mma(A, oh, y);
-        if (OF) y = mma(A, ol, mma(op(R::KEY + R::ALO, mt), oh, y));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[4 * mt + i] = y[i] * (unit * O_UNIT / sqrtf((float)D));
-      }
-    }
+    typename C::u32x4 o_last[C::OP];
+    p.read_o(o_last);
+    p.store_o(chunks - 1, o_last);
   }
-  if (a.o && chunks) store_o(chunks - 1);
   if (q.dst >= 0) {
-    float *p = a.state + q.dst * slot + at;
+    float *to = a.state + q.dst * slot + at;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < C::DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[(16 * t + i) * D] = S[t][i] * unit;
+      for (int i = 0; i < 4; ++i) to[(16 * t + i) * D] = p.S[t][i] * p.unit;
   }
 }
 
@@ -481,12 +662,18 @@ void sizes_of(int xtype, int otype, int D, size_t *key, size_t *head) {
   else sizes<false, true>(D, key, head);
 }
 
+template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
+  constexpr int SL = D / (16 * NW);
+  hipLaunchKernelGGL((chain_kernel<TX, TO, D, NW>), dim3((unsigned)((long long)a.s.n_seq * a.nvh * SL)), dim3(64 * (NW + 1)), 0, st, a, w);
+}
 template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
-  constexpr bool OF = full_out<TX, TO>();
-  constexpr int NW = 4;
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
-  hipLaunchKernelGGL((prep_kernel<TX, D, OF>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
-  hipLaunchKernelGGL((chain_kernel<TX, TO, D, NW>), dim3((unsigned)((long long)a.s.n_seq * a.nvh * (D / (16 * NW)))), dim3(64 * NW), 0, st, a, w);
+  hipLaunchKernelGGL((prep_kernel<TX, D, full_out<TX, TO>()>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
+  // Waves of a workgroup: two where there are few of them (8192 rows of 48 heads of 128: 192 workgroups; with four,
+  // 96, a chunk takes a sixth longer, the waves' reads of LDS and the loads into it being in each other's way), else
+  // four, which bring a record for twice the columns (16301 rows in 9 sequences: an eighth less).
+  if ((long long)a.s.n_seq * a.nvh * (D / 32) <= 512) launch_chain<TX, TO, D, 2>(a, w, st);
+  else launch_chain<TX, TO, D, 4>(a, w, st);
 }
 template <typename TX, typename TO> void launch_d(int D, const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   if (D == 128) launch<TX, TO, 128>(a, w, st);

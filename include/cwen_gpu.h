@@ -276,8 +276,8 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
  * (run.c:2697-2698), with both NULL g = exp(a) and beta = b.  a log decay above
  * 0 or a beta outside 0..2 gives unspecified values.  o is nullable (the states
  * alone move).  Pointers of q, k, v and o 16-byte aligned, their strides
- * multiples of 8; o must not overlap q, k or v (it may lie beside them in rows
- * of the same bytes).  States are held and moved in f32.
+ * multiples of 8 (the prompt's v_ts and o_ts below 2^24); o must not overlap q,
+ * k or v (it may lie beside them in rows of the same bytes).  States are held and moved in f32.
  *
  * cwen_gdn_step does it as written, the state in registers: for one or a few
  * rows of each sequence.  A row's result does not depend on the other rows or
