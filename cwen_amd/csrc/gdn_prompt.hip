@@ -41,7 +41,7 @@ template <int D, bool KL, bool OF> struct Rec {
   static constexpr int U = D / 32;
   static constexpr int OP = N * D * 2;                       // bytes of an operand
   static constexpr int K = 0, KLO = OP, Q = KL ? 2 * OP : OP, QLO = 3 * OP, KEY = KL ? 4 * OP : 2 * OP;
-  static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = OF ? 8192 : 6144, HEAD = F + 1024;
+  static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = OF ? 8192 : 6144, HEAD = F + 512;
 };
 // The factors: per row e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31 (beta is in T's columns).  The scores
 // and the last of the rows' factors are in units of O_UNIT, so that the low halves of small scores are no
@@ -79,7 +79,7 @@ constexpr int PREP_WAVES = 4;
 template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {
   constexpr bool KL = sizeof(TX) == 4;
   typedef Rec<D, KL, OF> R;
-  constexpr int U = R::U, GS = 33, HEADS = 4, HB = R::F + 64;     // HEADS value heads at a time, two a wave
+  constexpr int U = R::U, GS = 33, LS = N, HEADS = 4, HB = R::F + 64;     // HEADS value heads at a time, two a wave
   constexpr int BYTES = R::KEY > HEADS * HB ? R::KEY : HEADS * HB;
   // First K and Q; then, for a head, the rows of L (read 4 floats at a time), then its T hi, T lo, A operands.
   __shared__ __align__(16) char s_mem[BYTES];
@@ -172,10 +172,14 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
       }
     }
     float *to = isq ? s_P : s_G;
+    const float *len = isq ? s_sig : s_rho;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[(16 * mt + 4 * (lane >> 4) + i) * GS + 16 * nt + (lane & 15)] = c[nt][i];
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * mt + 4 * (lane >> 4) + i, k = 16 * nt + (lane & 15);
+        to[r * GS + k] = c[nt][i] * (len[r] * s_rho[k] * (isq ? 1.f / O_UNIT : 1.f));
+      }
   }
   __syncthreads();
 
@@ -189,55 +193,92 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
       g = a.A[hv] * (y > 20.f ? y : log1pf(expf(y)));
       beta = 1.f / (1.f + expf(-beta));
     }
-    s_gb[sub][n] = make_float2(g, beta);
+    const float eg = expf(g);
+    s_gb[sub][n] = make_float2(eg, beta);
     float *L = (float *)(s_mem + sub * HB);
     _Float16 *op = (_Float16 *)L;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    // Decays from n to i, added up from n on: no difference of sums that are far larger.
-    float acc = 0.f, pre = 0.f, dec = 1.f;
+    // Decays from n to i and up to n, multiplied up: no difference of sums that are far larger.
+    float dec = 0.f, pre = 1.f;
     float A[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float2 gb = s_gb[sub][i];
-      acc = i > n ? acc + gb.x : 0.f;
-      pre += i <= n ? gb.x : 0.f;
-      dec = i > n ? expf(acc) : 1.f;
-      L[i * N + n] = i > n ? gb.y * s_rho[i] * rho * dec * s_G[i * GS + n] : 0.f;
-      A[i] = i >= n ? s_sig[i] * rho * dec * s_P[i * GS + n] / O_UNIT : 0.f;
+      dec = i == n ? 1.f : dec * gb.x;
+      pre *= i <= n ? gb.x : 1.f;
+      L[i * LS + n] = gb.y * dec * s_G[i * GS + n];             // (only i > n is read)
+      A[i] = i >= n ? dec * s_P[i * GS + n] : 0.f;
     }
     char *out = w.head + ((long long)z * a.nvh + max(hv, 0)) * R::HEAD;
     if (hv >= 0) {
       float *F = (float *)(out + R::F);
-      const float e = expf(pre);
-      F[F_X + n] = e * rho;
+      F[F_X + n] = pre * rho;
       F[F_D + n] = rho * dec;
-      F[F_O + n] = e * sig / O_UNIT;
-      if (n == N - 1) F[F_END] = e;
+      F[F_O + n] = pre * sig / O_UNIT;
+      if (n == N - 1) F[F_END] = pre;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    // T column by column: T_in = [i = n] - sum_(j < i) L_ij T_jn
-    float T[N];
+    // (1 + L)^-1 in blocks of 16 rows: the two on the diagonal column by column, T_in = [i = n] - sum_(j < i) L_ij T_jn,
+    // both at once; the third is -T22 (L21 T11), on the matrix cores in f32.
+    float T[16];
+    {
+      const int h = n >> 4, m = n & 15;
+      const float *Lh = L + 16 * h * LS + 16 * h;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float t = i == n ? 1.f : 0.f;
+      for (int i = 0; i < 16; ++i) {
+        float t = i == m ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < i; j += 4) {
-        const float4 l = *(const float4 *)(L + i * N + j);
-        t = fmaf(-l.x, T[j], t);
-        if (j + 1 < i) t = fmaf(-l.y, T[j + 1], t);
-        if (j + 2 < i) t = fmaf(-l.z, T[j + 2], t);
-        if (j + 3 < i) t = fmaf(-l.w, T[j + 3], t);
+        for (int j = 0; j < i; j += 4) {
+          const float4 l = *(const float4 *)(Lh + i * LS + j);
+          t = fmaf(-l.x, T[j], t);
+          if (j + 1 < i) t = fmaf(-l.y, T[j + 1], t);
+          if (j + 2 < i) t = fmaf(-l.z, T[j + 2], t);
+          if (j + 3 < i) t = fmaf(-l.w, T[j + 3], t);
+        }
+        T[i] = t;
       }
-      T[i] = t;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 16; ++i) L[(16 * h + i) * LS + 16 * h + m] = T[i];      // over L11 and L22
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    floatx4_t T21[2];                  // of the wave's two heads: rows 16 + 4 g + i, column m
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float *Lw = (const float *)(s_mem + (2 * wave + e) * HB);
+      const int m = lane & 15, g4 = lane >> 4;
+      floatx4_t M = {}, t = {};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        M = __builtin_amdgcn_mfma_f32_16x16x4f32(Lw[(16 + m) * LS + 4 * g4 + k], Lw[(4 * g4 + k) * LS + m], M, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x4f32(Lw[(16 + m) * LS + 16 + 4 * g4 + k], -M[k], t, 0, 0, 0);
+      T21[e] = t;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    auto put = [&](_Float16 *to, int i, int col, float t) {
+      const int at = operand_at(i, col, 1);
+      const _Float16 h = f16_of(t);
+      to[R::T / 2 + at] = h;
+      to[R::TLO / 2 + at] = f16_of(t - (float)h);
+    };
+#pragma unroll
+    for (int i = 0; i < 16; ++i) put(op, 16 * (n >> 4) + i, n, T[i] * beta);
+    // rows 0 .. 15 of the later columns: nothing (zeros of the earlier lanes' blocks)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (n >= 16) put(op, i, n, 0.f);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int m = lane & 15;
+      const float b = s_gb[2 * wave + e][m].y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put((_Float16 *)(s_mem + (2 * wave + e) * HB), 16 + 4 * (lane >> 4) + i, m, T21[e][i] * b);
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = operand_at(i, n, 1);
-      const float t = T[i] * beta;
-      const _Float16 h = f16_of(t), x = f16_of(A[i]);
-      op[R::T / 2 + at] = h;
-      op[R::TLO / 2 + at] = f16_of(t - (float)h);
+      const _Float16 x = f16_of(A[i]);
       op[R::A / 2 + at] = x;
       if (OF) op[R::ALO / 2 + at] = f16_of(A[i] - (float)x);
     }
@@ -286,7 +327,7 @@ __device__ __forceinline__ half8_t high8(const float (&x)[8]) {
 template <typename TX, typename TO, int D, int NW> struct Chain {
   static constexpr bool KL = sizeof(TX) == 4, OF = full_out<TX, TO>();
   typedef Rec<D, KL, OF> R;
-  static constexpr int U = R::U, DT = D / 16, KB = (R::KEY + R::HEAD) / 1024, XS = sizeof(TX), OS = sizeof(TO);
+  static constexpr int U = R::U, DT = D / 16, KB = R::KEY / 1024 + R::HEAD / 1024 + 1, XS = sizeof(TX), OS = sizeof(TO);
   static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
   typedef char Buf[R::KEY + R::HEAD];
 
@@ -298,7 +339,8 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   int rows;
   uint32_t v_row, o_row;             // bytes of a row
   uint32_t v_at[VP], o_at[OP];
-  char *s_v, *s_o;                   // the wave's columns of a chunk, row by row
+  char *s_io;                        // the wave's columns of a chunk, row by row: values, then outputs, of which the
+                                     // values are read before outputs are written, and outputs before the next values
   float out_unit;
   // the state, divided by the column's unit, and the present chunk's values
   floatx4_t S[DT];
@@ -321,20 +363,21 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     typedef typename std::conditional<std::is_same<TX, TypeBF16::elem>::value, TypeBF16, TypeF16>::type Type;
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < VP; ++i) *(uint4 *)(s_v + (i * 64 + lane) * 16) = from[i];
+    for (int i = 0; i < VP; ++i) *(uint4 *)(s_io + (i * 64 + lane) * 16) = from[i];
     asm volatile("" ::: "memory");
     if constexpr (XS == 4) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) far[e] = ((const float *)s_v)[((e >> 2) * 16 + 4 * g + (e & 3)) * 16 + n];
+      for (int e = 0; e < 8; ++e) far[e] = ((const float *)s_io)[((e >> 2) * 16 + 4 * g + (e & 3)) * 16 + n];
     } else {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         typedef float f2 __attribute__((ext_vector_type(2)));
-        const f2 x = __builtin_bit_cast(f2, AttnOps<Type>::tr(s_v + (mt * 16 + 4 * g + (n >> 2)) * 32 + (n & 3) * 8));
+        const f2 x = __builtin_bit_cast(f2, AttnOps<Type>::tr(s_io + (mt * 16 + 4 * g + (n >> 2)) * 32 + (n & 3) * 8));
         far[2 * mt] = x[0];
         far[2 * mt + 1] = x[1];
       }
     }
+    asm volatile("" ::: "memory");
   }
   // The turned values become the present ones; vmax: their column's largest.
   __device__ __forceinline__ void take_v() {
@@ -372,7 +415,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   __device__ __forceinline__ void read_o(u32x4 (&x)[OP]) const {
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < OP; ++i) x[i] = *(const u32x4 *)(s_o + (i * 64 + lane) * 16);
+    for (int i = 0; i < OP; ++i) x[i] = *(const u32x4 *)(s_io + (i * 64 + lane) * 16);
     asm volatile("" ::: "memory");
   }
   __device__ __forceinline__ void store_o(int c, const u32x4 (&x)[OP]) const {
@@ -420,14 +463,6 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     if (!__all((c & 7) != 7 && vu < 16.f && vu >= 0.125f)) ratio = renew(fmaxf(vmax_here, vmax));
     store_o(c - 1, o_last);
     load_v(c + 4, vr_4);
-    half8_t T[2], TL[2], Q[2 * U], QL[2 * U];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) T[mt] = op(R::KEY + R::T, mt), TL[mt] = op(R::KEY + R::TLO, mt);
-#pragma unroll
-    for (int i = 0; i < 2 * U; ++i) {
-      Q[i] = op(R::Q, i);
-      if (KL) QL[i] = op(R::QLO, i);
-    }
     half8_t hi[U], lo[U];
     floatx4_t X[2] = {}, Y[2] = {};
 #pragma unroll
@@ -444,6 +479,28 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    half8_t T[2], TL[2], Q[2 * U], QL[2 * U];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) T[mt] = op(R::KEY + R::T, mt), TL[mt] = op(R::KEY + R::TLO, mt);
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+      Q[i] = op(R::Q, i);
+      if (KL) QL[i] = op(R::QLO, i);
+    }
+    half8_t rh, rl;
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = fmaf(-fx[e >> 2][e & 3], X[e >> 2][e & 3], w[e]);
+    split8(r, rh, rl);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
+        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+        if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
     half8_t KT[DT], KTL[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
@@ -459,19 +516,6 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       A[mt] = op(R::KEY + R::A, mt);
       if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
     }
-    half8_t rh, rl;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
-        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
-        if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
-      }
-    float r[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = fmaf(-fx[e >> 2][e & 3], X[e >> 2][e & 3], w[e]);
-    split8(r, rh, rl);
     floatx4_t d[2] = {};
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, d[mt])));
@@ -506,7 +550,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       y = mma(A[mt], oh, y);
       if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ((TO *)s_o)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
+      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
     }
   }
 };
@@ -526,12 +570,12 @@ __device__ __forceinline__ int nth_longest(const GdnSeqs &a, int nth) {
 // Three records in LDS, an array each: in one, the compiler would wait for the loads into one record
 // before it reads another.
 template <typename TX, typename TO, int D, int NW>
-__global__ __launch_bounds__(64 * (NW + 1)) __attribute__((amdgpu_waves_per_eu(1, 2))) void chain_kernel(GdnRuleArgs a, PromptWork w) {
+__global__ __launch_bounds__(64 * (NW + 1), NW == 4 && sizeof(TX) == 2 ? 3 : 1) void chain_kernel(GdnRuleArgs a, PromptWork w) {
   typedef Chain<TX, TO, D, NW> C;
   typedef typename C::R R;
   constexpr int SL = D / (16 * NW);
   __shared__ __align__(1024) typename C::Buf b0, b1, b2;
-  __shared__ __align__(16) char s_v[NW][N * 16 * C::XS], s_o[NW][N * 16 * C::OS];
+  __shared__ __align__(16) char s_io[NW][N * 16 * (C::XS > C::OS ? C::XS : C::OS)];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = a.nvh * SL, nth = blockIdx.x / per, i0 = blockIdx.x - nth * per, grp = a.nvh / a.nkh;
   const int s = nth_longest(a.s, nth);
@@ -566,6 +610,10 @@ __global__ __launch_bounds__(64 * (NW + 1)) __attribute__((amdgpu_waves_per_eu(1
 #pragma unroll
       for (int i = 0; i < R::HEAD / 1024; ++i)
         __builtin_amdgcn_global_load_lds((attn_glb_t *)(head + i * 1024), (attn_lds_t *)(to + R::KEY + i * 1024), 16, 0, 0);
+      constexpr int most = R::HEAD / 1024 * 1024;
+      static_assert(R::KEY % 1024 == 0 && R::HEAD - most == 512, "a record ends in half a load");
+      if (lane < 32)
+        __builtin_amdgcn_global_load_lds((attn_glb_t *)(head + most), (attn_lds_t *)(to + R::KEY + most), 16, 0, 0);
       if (++c < chunks) key += key_step, head += head_step;
     };
     // Buffer c % 3 is read until the barrier of chunk c + 1, behind which chunk c + 3 goes there.
@@ -616,8 +664,7 @@ __global__ __launch_bounds__(64 * (NW + 1)) __attribute__((amdgpu_waves_per_eu(1
     for (int i = 0; i < C::VP; ++i) p.v_at[i] = (i * 64 + p.lane) / C::XS * p.v_row + c0 * C::XS + p.lane % C::XS * 16;
 #pragma unroll
     for (int i = 0; i < C::OP; ++i) p.o_at[i] = (i * 64 + p.lane) / C::OS * p.o_row + c0 * C::OS + p.lane % C::OS * 16;
-    p.s_v = s_v[wave];
-    p.s_o = s_o[wave];
+    p.s_io = s_io[wave];
     p.out_unit = O_UNIT / sqrtf((float)D);
     p.load_v(0, p.vr[0]);
     p.load_v(1, p.vr[1]);
