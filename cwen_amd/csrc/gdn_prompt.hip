@@ -570,7 +570,7 @@ __device__ __forceinline__ int nth_longest(const GdnSeqs &a, int nth) {
 // Three records in LDS, an array each: in one, the compiler would wait for the loads into one record
 // before it reads another.
 template <typename TX, typename TO, int D, int NW>
-__global__ __launch_bounds__(64 * (NW + 1), NW == 4 && sizeof(TX) == 2 ? 3 : 1) void chain_kernel(GdnRuleArgs a, PromptWork w) {
+__global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) void chain_kernel(GdnRuleArgs a, PromptWork w) {
   typedef Chain<TX, TO, D, NW> C;
   typedef typename C::R R;
   constexpr int SL = D / (16 * NW);
@@ -716,11 +716,13 @@ template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRu
 template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
   hipLaunchKernelGGL((prep_kernel<TX, D, full_out<TX, TO>()>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
-  // Waves of a workgroup: two where there are few of them (8192 rows of 48 heads of 128: 192 workgroups; with four,
-  // 96, a chunk takes a sixth longer, the waves' reads of LDS and the loads into it being in each other's way), else
-  // four, which bring a record for twice the columns (16301 rows in 9 sequences: an eighth less).
+  // Waves of a workgroup: two where there are few sequences and heads, which spreads them over the CUs (8192 rows of 48
+  // heads of 128 in bf16: 298 us, with four 345).  Else all of a head's columns: a record then comes once, and two of
+  // the chain's waves share a SIMD (16301 rows in 9 sequences: 254 us, with four 300).  Eight waves of f32 operands do
+  // not fit the registers.
+  constexpr int MANY = D == 128 && sizeof(TX) == 2 ? 8 : 4;
   if ((long long)a.s.n_seq * a.nvh * (D / 32) <= 512) launch_chain<TX, TO, D, 2>(a, w, st);
-  else launch_chain<TX, TO, D, 4>(a, w, st);
+  else launch_chain<TX, TO, D, MANY>(a, w, st);
 }
 template <typename TX, typename TO> void launch_d(int D, const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   if (D == 128) launch<TX, TO, 128>(a, w, st);

@@ -47,26 +47,73 @@ struct Entry {
   int i;
 };
 __device__ __forceinline__ bool before(Entry a, Entry b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
-__device__ __forceinline__ Entry of_lane(Entry a, int l) { return {__shfl(a.v, l), __shfl(a.i, l)}; }
-// The bitonic step between lanes x apart; down: the lower lane keeps the entry that comes first.
-__device__ __forceinline__ Entry step(Entry a, int x, bool down) {
-  const int lane = threadIdx.x & 63;
-  const Entry b = {__shfl_xor(a.v, x), __shfl_xor(a.i, x)};
-  const bool first = ((lane & x) == 0) == down;
-  return before(b, a) == first ? b : a;
+__device__ __forceinline__ Entry of_lane(Entry a, int l) {
+  return {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, a.v), l)), __builtin_amdgcn_readlane(a.i, l)};
+}
+// The value of the lane X apart (lane ^ X), by row permutes and swaps: a shuffle through LDS takes 100 cycles.
+template <int X> __device__ __forceinline__ int apart(int v) {
+  auto perm = [](int x, auto ctrl) { return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, false); };
+  if constexpr (X == 1) return perm(v, std::integral_constant<int, 0xB1>{});
+  else if constexpr (X == 2) return perm(v, std::integral_constant<int, 0x4E>{});
+  else if constexpr (X == 4) return perm(perm(v, std::integral_constant<int, 0x141>{}), std::integral_constant<int, 0x1B>{});
+  else if constexpr (X == 8) return perm(v, std::integral_constant<int, 0x128>{});
+  else if constexpr (X == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return __builtin_amdgcn_inverse_ballot_w64(0xFFFF0000FFFF0000ull) ? (int)p[0] : (int)p[1];
+  } else {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_inverse_ballot_w64(0xFFFFFFFF00000000ull) ? (int)p[0] : (int)p[1];
+  }
+}
+template <int X> __device__ __forceinline__ float apart(float v) { return __builtin_bit_cast(float, apart<X>(__builtin_bit_cast(int, v))); }
+template <int X> __device__ __forceinline__ Entry apart(Entry a) { return {apart<X>(a.v), apart<X>(a.i)}; }
+// The lanes whose bit X is clear, and of those and the others (in blocks of K) the ones that keep the entry that comes first.
+constexpr unsigned long long lanes_clear(int x) {
+  unsigned long long m = 0;
+  for (int l = 0; l < 64; ++l)
+    if (!(l & x)) m |= 1ull << l;
+  return m;
+}
+constexpr unsigned long long keep_first(int x, int k) {
+  unsigned long long m = 0;
+  for (int l = 0; l < 64; ++l)
+    if (!(l & x) == !(l & k)) m |= 1ull << l;
+  return m;
+}
+// Bitonic steps X, X / 2, .. 1; in every other block of K lanes the other way round.
+template <int X, int K> __device__ __forceinline__ Entry steps(Entry a) {
+  const Entry b = apart<X>(a);
+  const bool first = __builtin_amdgcn_inverse_ballot_w64(K < 64 ? keep_first(X, K) : lanes_clear(X));
+  a = before(b, a) == first ? b : a;
+  if constexpr (X > 1) return steps<X / 2, K>(a);
+  else return a;
 }
 __device__ __forceinline__ Entry sorted(Entry a) {
-  const int lane = threadIdx.x & 63;
-  for (int k = 2; k <= 64; k *= 2)
-    for (int x = k / 2; x > 0; x /= 2) a = step(a, x, (lane & k) == 0);
-  return a;
+  return steps<32, 64>(steps<16, 32>(steps<8, 16>(steps<4, 8>(steps<2, 4>(steps<1, 2>(a))))));
 }
+// The other way round: lane 63 - l.
+__device__ __forceinline__ Entry turned(Entry a) { return apart<32>(apart<16>(apart<8>(apart<4>(apart<2>(apart<1>(a)))))); }
 // The 64 first of two sorted lists.
 __device__ __forceinline__ Entry merged(Entry a, Entry b) {
-  b = of_lane(b, 63 - (threadIdx.x & 63));
-  a = before(b, a) ? b : a;
-  for (int x = 32; x > 0; x /= 2) a = step(a, x, true);
-  return a;
+  b = turned(b);
+  return steps<32, 64>(before(b, a) ? b : a);
+}
+// Over the wave.
+__device__ __forceinline__ Sums joined(Sums r) {
+  r = joined(r, {apart<1>(r.m), apart<1>(r.s), apart<1>(r.t)});
+  r = joined(r, {apart<2>(r.m), apart<2>(r.s), apart<2>(r.t)});
+  r = joined(r, {apart<4>(r.m), apart<4>(r.s), apart<4>(r.t)});
+  r = joined(r, {apart<8>(r.m), apart<8>(r.s), apart<8>(r.t)});
+  r = joined(r, {apart<16>(r.m), apart<16>(r.s), apart<16>(r.t)});
+  return joined(r, {apart<32>(r.m), apart<32>(r.s), apart<32>(r.t)});
+}
+__device__ __forceinline__ int added(int c) {
+  c += apart<1>(c);
+  c += apart<2>(c);
+  c += apart<4>(c);
+  c += apart<8>(c);
+  c += apart<16>(c);
+  return c + apart<32>(c);
 }
 
 struct Best {
@@ -110,6 +157,25 @@ struct Best {
   }
 };
 
+// One wanted entry: each lane's own, its indexes coming in their order.
+struct Most {
+  Entry mine, last;
+  __device__ __forceinline__ void start(float *, int *, int) { mine = last = {-INFINITY, NONE}; }
+  __device__ __forceinline__ void offer(float v, int i) {
+    if (before({v, i}, mine)) mine = {v, i};
+  }
+  __device__ __forceinline__ void flush() {
+    auto step = [&](Entry b) { mine = before(b, mine) ? b : mine; };
+    step(apart<1>(mine));
+    step(apart<2>(mine));
+    step(apart<4>(mine));
+    step(apart<8>(mine));
+    step(apart<16>(mine));
+    step(apart<32>(mine));
+    if (threadIdx.x & 63) mine = {-INFINITY, NONE};
+  }
+};
+
 // Words of one part's result: m, s, t, count, then the list.
 __host__ __device__ constexpr int part_words(int top) { return 4 + 2 * ((top + 1) & ~1); }
 
@@ -140,8 +206,9 @@ template <typename T> __device__ __forceinline__ float token_logit(const Logprob
   return tok >= 0 && tok < a.V ? (float)((const T *)a.x)[row * a.ls + tok] : NAN;
 }
 
-template <typename T> __global__ __launch_bounds__(THREADS) void part_kernel(LogprobArgs a, Split sp) {
-  constexpr int E = 16 / sizeof(T);
+// TOP: 0 no largest logits are wanted, 1 one, 2 more.  RANK: whether ranks are.
+template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) void part_kernel(LogprobArgs a, Split sp) {
+  constexpr int E = 16 / sizeof(T), VECS = 64 / (16 * E / 4);      // 16 logits at a time
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
   __shared__ float s_qv[WAVES][128], s_sums[WAVES][3];
   __shared__ int s_qi[WAVES][128], s_cnt[WAVES];
@@ -150,25 +217,73 @@ template <typename T> __global__ __launch_bounds__(THREADS) void part_kernel(Log
   const T *x = (const T *)a.x + row * a.ls;
   // Whole 16-byte pieces lie behind `head` logits; the first part takes those too, the last one the row's end.
   const int head = min((int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T), a.V), nvec = (a.V - head) / E;
-  const int tok = a.rank && a.tokens ? a.tokens[row] : -1;
-  const float xt = a.rank ? token_logit<T>(a, row) : NAN;
+  const int tok = RANK ? a.tokens[row] : -1;
+  // What comes before the token: from its logit on at lower indexes, from the next float on at higher ones.
+  const float xt = RANK ? token_logit<T>(a, row) : NAN;
+  const float above = __builtin_bit_cast(float, xt == 0.f ? 1 : __builtin_bit_cast(int, xt) + (xt < 0.f ? -1 : 1));
   Sums r = {-INFINITY, 0.f, 0.f};
+  float ref = 0.f;                    // r.m, or 0 before there is one
   int cnt = 0;
-  Best best;
-  best.start(s_qv[wave], s_qi[wave], max(a.top, 1));
+  typename std::conditional<TOP == 2, Best, Most>::type best;
+  best.start(s_qv[wave], s_qi[wave], a.top);
+  auto grow = [&](float v) {          // all lanes
+    if (__any(v > r.m + LAG)) {
+      renew(r, fmaxf(r.m, v));
+      ref = r.m == -INFINITY ? 0.f : r.m;
+    }
+  };
+  auto add = [&](float v) {
+    const float d = v - ref, e = exp_of(d);
+    r.s += e;
+    r.t = fmaf(e, fmaxf(d, -200.f), r.t);       // e is 0 there, and 0 times -infinity is not
+  };
   auto one = [&](float v, int i, bool in) {       // all lanes; in: there is one
     v = in ? v : -INFINITY;
-    if (__any(v > r.m + LAG)) renew(r, fmaxf(r.m, v));
-    const float d = fmaxf(v - (r.m == -INFINITY ? 0.f : r.m), -1e30f), e = exp_of(d);
-    r.s += v != v ? v : e;
-    r.t = fmaf(e, d, r.t);
-    cnt += in && (v > xt || (v == xt && i < tok)) ? 1 : 0;
-    if (a.top) best.offer(in ? v : -INFINITY, in ? i : NONE);
+    grow(v);
+    add(v);
+    if (RANK) cnt += in && v >= (i < tok ? xt : above) ? 1 : 0;
+    if (TOP) best.offer(v, in ? i : NONE);
   };
   const int v0 = part * sp.vecs, v1 = min(nvec, v0 + sp.vecs);
-  if (part == 0)
-    for (int i = 0; i < head; i += THREADS) one(i + (int)threadIdx.x < head ? (float)x[i + threadIdx.x] : 0.f, i + threadIdx.x, i + (int)threadIdx.x < head);
-  for (int u = v0; u < v1; u += THREADS) {
+  if (part == 0) one((int)threadIdx.x < head ? (float)x[threadIdx.x] : 0.f, threadIdx.x, (int)threadIdx.x < head);
+  const int tokvec = RANK ? (tok - head) / E : 0;               // (a token in front of the pieces: one of piece 0 or none)
+  int u = v0;
+  for (; u + THREADS * VECS <= v1; u += THREADS * VECS) {
+    vec w[VECS];
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) w[k] = *(const vec *)(x + head + (long long)(u + THREADS * k + threadIdx.x) * E);
+    float f[VECS][E], most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        f[k][e] = (float)w[k][e];
+        most = fmaxf(most, f[k][e]);
+      }
+    grow(most);
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) add(f[k][e]);
+    if (RANK) {
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) {
+        const int p = u + THREADS * k + threadIdx.x;
+        const float from = p < tokvec && tok >= head ? xt : above;
+#pragma unroll
+        for (int e = 0; e < E; ++e) cnt += f[k][e] >= from ? 1 : 0;
+        if (p == tokvec)
+          for (int e = 0; e < E; ++e) cnt += (float)w[k][e] == xt && head + p * E + e < tok ? 1 : 0;
+      }
+    }
+    if (TOP && __any(most >= (TOP == 1 ? best.mine.v : best.last.v))) {
+#pragma unroll
+      for (int k = 0; k < VECS; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) best.offer(f[k][e], head + (u + THREADS * k + (int)threadIdx.x) * E + e);
+    }
+  }
+  for (; u < v1; u += THREADS) {
     const int p = u + threadIdx.x;
     const bool in = p < v1;
     vec w = {};
@@ -179,9 +294,9 @@ template <typename T> __global__ __launch_bounds__(THREADS) void part_kernel(Log
     const int t0 = head + nvec * E;
     one(t0 + (int)threadIdx.x < a.V ? (float)x[t0 + threadIdx.x] : 0.f, t0 + threadIdx.x, t0 + (int)threadIdx.x < a.V);
   }
-  if (a.top) best.flush();
-  for (int d = 32; d > 0; d /= 2) r = joined(r, {__shfl_xor(r.m, d), __shfl_xor(r.s, d), __shfl_xor(r.t, d)});
-  for (int d = 32; d > 0; d /= 2) cnt += __shfl_xor(cnt, d);
+  if (TOP) best.flush();
+  r = joined(r);
+  cnt = added(cnt);
   Best::settle();
   s_qv[wave][lane] = best.mine.v;
   s_qi[wave][lane] = best.mine.i;
@@ -195,7 +310,7 @@ template <typename T> __global__ __launch_bounds__(THREADS) void part_kernel(Log
   for (int w = 1; w < WAVES; ++w) {
     r = joined(r, {s_sums[w][0], s_sums[w][1], s_sums[w][2]});
     cnt += s_cnt[w];
-    if (a.top) l = merged(l, {s_qv[w][lane], s_qi[w][lane]});
+    if (TOP) l = merged(l, {s_qv[w][lane], s_qi[w][lane]});
   }
   if (sp.n == 1) {
     finish(a, row, r, cnt, token_logit<T>(a, row), l);
@@ -206,8 +321,12 @@ template <typename T> __global__ __launch_bounds__(THREADS) void part_kernel(Log
   if (lane < a.top) *(float2 *)(o + 4 + 2 * lane) = make_float2(l.v, __builtin_bit_cast(float, l.i));
 }
 
-template <typename T> __global__ __launch_bounds__(64) void join_kernel(LogprobArgs a, int parts) {
-  const int lane = threadIdx.x & 63, row = blockIdx.x, words = part_words(a.top);
+// The parts of a row together: every wave asks for all of its lists at once, and merges those that can
+// still matter.
+template <typename T> __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int parts) {
+  __shared__ float s_v[WAVES][64];
+  __shared__ int s_i[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x, words = part_words(a.top);
   const float *w = a.work + (long long)row * parts * words;
   Sums r = {-INFINITY, 0.f, 0.f};
   int cnt = 0;
@@ -216,30 +335,54 @@ template <typename T> __global__ __launch_bounds__(64) void join_kernel(LogprobA
     r = {f.x, f.y, f.z};
     cnt = __builtin_bit_cast(int, f.w);
   }
-  for (int d = 32; d > 0; d /= 2) r = joined(r, {__shfl_xor(r.m, d), __shfl_xor(r.s, d), __shfl_xor(r.t, d)});
-  for (int d = 32; d > 0; d /= 2) cnt += __shfl_xor(cnt, d);
+  const float xt = token_logit<T>(a, row);
   Entry l = {-INFINITY, NONE};
-  if (a.top)
-    for (int p = 0; p < parts; ++p) {
-      Entry e = {-INFINITY, NONE};
-      if (lane < a.top) {
-        const float2 f = *(const float2 *)(w + p * words + 4 + 2 * lane);
-        e = {f.x, __builtin_bit_cast(int, f.y)};
-      }
-      l = merged(l, e);
+  if (a.top) {
+    constexpr int LISTS = SPLITS / WAVES;
+    float2 e[LISTS];
+#pragma unroll
+    for (int k = 0; k < LISTS; ++k) {
+      const int p = k * WAVES + wave;
+      e[k] = make_float2(-INFINITY, __builtin_bit_cast(float, NONE));
+      if (p < parts && lane < a.top) e[k] = *(const float2 *)(w + p * words + 4 + 2 * lane);
     }
-  finish(a, row, r, cnt, token_logit<T>(a, row), l);
+#pragma unroll
+    for (int k = 0; k < LISTS; ++k) {
+      const Entry b = {e[k].x, __builtin_bit_cast(int, e[k].y)};
+      if (k == 0) l = b;
+      else if (__any(before(b, of_lane(l, a.top - 1)))) l = merged(l, b);
+    }
+    s_v[wave][lane] = l.v;
+    s_i[wave][lane] = l.i;
+    __syncthreads();
+  }
+  if (wave) return;
+  if (a.top)
+    for (int k = 1; k < WAVES; ++k) {
+      const Entry b = {s_v[k][lane], s_i[k][lane]};
+      if (__any(before(b, of_lane(l, a.top - 1)))) l = merged(l, b);
+    }
+  r = joined(r);
+  cnt = added(cnt);
+  finish(a, row, r, cnt, xt, l);
 }
 
 // Parts of a row: enough workgroups for the card, 4096 logits or more each.
 int parts_of(int rows, int V) { return std::max(1, std::min({SPLITS, (1024 + rows - 1) / std::max(rows, 1), V / 4096})); }
 
+template <typename T, int TOP> void launch_parts(const LogprobArgs &a, const Split &sp, hipStream_t st) {
+  const dim3 grid((unsigned)(a.rows * sp.n));
+  if (a.rank) hipLaunchKernelGGL((part_kernel<T, TOP, true>), grid, dim3(THREADS), 0, st, a, sp);
+  else hipLaunchKernelGGL((part_kernel<T, TOP, false>), grid, dim3(THREADS), 0, st, a, sp);
+}
 template <typename T> void launch(const LogprobArgs &a, hipStream_t st) {
   constexpr int E = 16 / sizeof(T);
   const int n = parts_of(a.rows, a.V);
   const Split sp = {n, (a.V / E + n - 1) / n};
-  hipLaunchKernelGGL((part_kernel<T>), dim3((unsigned)(a.rows * n)), dim3(THREADS), 0, st, a, sp);
-  if (n > 1) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)a.rows), dim3(64), 0, st, a, n);
+  if (a.top == 0) launch_parts<T, 0>(a, sp, st);
+  else if (a.top == 1) launch_parts<T, 1>(a, sp, st);
+  else launch_parts<T, 2>(a, sp, st);
+  if (n > 1) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)a.rows), dim3(THREADS), 0, st, a, n);
 }
 
 }  // namespace
