@@ -4,6 +4,12 @@
 
 namespace {
 
+// x / (1 + exp(-x)) with the hardware's exp2 and reciprocal, each off by an ulp.  With the exact division the
+// convolution is bound by its instructions (8192 rows of 10240 channels in bf16: 108 us instead of 72).
+__device__ __forceinline__ float silu_near(float x) {
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * x));
+}
+
 // ---- convolution ----
 // A thread has 8 channels of the TB rows of one piece, the last three inputs
 // and the taps in registers, so that a row is read once by its own piece and the
@@ -57,7 +63,7 @@ template <typename TX, typename TY> __global__ __launch_bounds__(CONV_THREADS) v
       Io<TX>::load(x + (long long)t * a.xs, cur);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        out[e] = silu_f(conv4(in[0][e], in[1][e], in[2][e], cur[e], w[e]));
+        out[e] = silu_near(conv4(in[0][e], in[1][e], in[2][e], cur[e], w[e]));
         in[0][e] = in[1][e];
         in[1][e] = in[2][e];
         in[2][e] = cur[e];
@@ -131,23 +137,40 @@ template <typename TX, typename TO, int D> __global__ __launch_bounds__(256) voi
   const TX *kp = (const TX *)a.k + (long long)q.first * a.ks + hk * D + i0;
   const TX *vp = (const TX *)a.v + (long long)q.first * a.vs + hv * D + j0;
   const float *ap = a.a + (long long)q.first * a.gs + hv, *bp = a.b + (long long)q.first * a.gs + hv;
-  const float A = a.A ? a.A[hv] : 0.f, dt = a.A ? a.dt[hv] : 0.f, scale = 1.f / sqrtf((float)D);
-  for (int t = 0; t < q.n; ++t) {
-    typedef TX vec4 __attribute__((ext_vector_type(4)));
-    float k[R], x[R];
+  const float scale = 1.f / sqrtf((float)D);
+  typedef TX vec4 __attribute__((ext_vector_type(4)));
+  // A row's operands are asked for while the row before is computed, its gates with those of 64 rows, one a lane.
+  float k1[R], x1[R];
+  vec4 v1 = {};
+  float g64 = 0.f, beta64 = 0.f;
+  auto ask = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < R; r += 8) {
-      Io<TX>::load(kp + t * a.ks + r, *(float(*)[8])&k[r]);
-      Io<TX>::load(qp + t * a.qs + r, *(float(*)[8])&x[r]);
+      Io<TX>::load(kp + t * a.ks + r, *(float(*)[8])&k1[r]);
+      Io<TX>::load(qp + t * a.qs + r, *(float(*)[8])&x1[r]);
     }
-    const vec4 v = *(const vec4 *)(vp + t * a.vs);
-    float g = ap[t * a.gs], beta = bp[t * a.gs];
-    if (a.A) {
-      const float y = g + dt;
-      g = A * (y > 20.f ? y : log1pf(expf(y)));
-      beta = 1.f / (1.f + expf(-beta));
+    v1 = *(const vec4 *)(vp + t * a.vs);
+  };
+  if (q.n) ask(0);
+  for (int t = 0; t < q.n; ++t) {
+    if ((t & 63) == 0) {
+      const int u = min(t + lane, q.n - 1);
+      g64 = ap[u * a.gs];
+      beta64 = bp[u * a.gs];
+      if (a.A) {
+        const float y = g64 + a.dt[hv];
+        g64 = a.A[hv] * (y > 20.f ? y : log1pf(expf(y)));
+        beta64 = 1.f / (1.f + expf(-beta64));
+      }
+      g64 = expf(g64);
     }
-    g = expf(g);
+    const float g = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g64), t & 63));
+    const float beta = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, beta64), t & 63));
+    float k[R], x[R];
+    const vec4 v = v1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) k[r] = k1[r], x[r] = x1[r];
+    if (t + 1 < q.n) ask(t + 1);
     float kk = 0.f, qq = 0.f, kq = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -155,27 +178,32 @@ template <typename TX, typename TO, int D> __global__ __launch_bounds__(256) voi
       qq = fmaf(x[r], x[r], qq);
       kq = fmaf(k[r], x[r], kq);
     }
-    const float kn = 1.f / sqrtf(sum_rows(kk) + 1e-6f), qn = 1.f / sqrtf(sum_rows(qq) + 1e-6f);
-    float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+    const float kn = 1.f / sqrtf(sum_rows(kk) + 1e-6f);
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       u.x = fmaf(S[r].x, k[r], u.x); u.y = fmaf(S[r].y, k[r], u.y); u.z = fmaf(S[r].z, k[r], u.z); u.w = fmaf(S[r].w, k[r], u.w);
-      w.x = fmaf(S[r].x, x[r], w.x); w.y = fmaf(S[r].y, x[r], w.y); w.z = fmaf(S[r].z, x[r], w.z); w.w = fmaf(S[r].w, x[r], w.w);
     }
     const float gk = g * kn;
     float4 d;
     d.x = beta * ((float)v[0] - gk * sum_rows(u.x)); d.y = beta * ((float)v[1] - gk * sum_rows(u.y));
     d.z = beta * ((float)v[2] - gk * sum_rows(u.z)); d.w = beta * ((float)v[3] - gk * sum_rows(u.w));
     if (a.o) {
-      const float gq = g * qn, c = sum_rows(kq) * kn * qn;
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        w.x = fmaf(S[r].x, x[r], w.x); w.y = fmaf(S[r].y, x[r], w.y); w.z = fmaf(S[r].z, x[r], w.z); w.w = fmaf(S[r].w, x[r], w.w);
+      }
+      const float qn = 1.f / sqrtf(sum_rows(qq) + 1e-6f), gq = g * qn, c = sum_rows(kq) * kn * qn;
       w = make_float4(sum_rows(w.x), sum_rows(w.y), sum_rows(w.z), sum_rows(w.w));
       if (rg == 0) {
-        typedef TO vec4 __attribute__((ext_vector_type(4)));
-        *(vec4 *)((TO *)a.o + (long long)(q.first + t) * a.os + hv * D + j0) =
-            (vec4){(TO)(scale * fmaf(gq, w.x, c * d.x)), (TO)(scale * fmaf(gq, w.y, c * d.y)),
+        typedef TO out4 __attribute__((ext_vector_type(4)));
+        *(out4 *)((TO *)a.o + (long long)(q.first + t) * a.os + hv * D + j0) =
+            (out4){(TO)(scale * fmaf(gq, w.x, c * d.x)), (TO)(scale * fmaf(gq, w.y, c * d.y)),
                    (TO)(scale * fmaf(gq, w.z, c * d.z)), (TO)(scale * fmaf(gq, w.w, c * d.w))};
       }
     }
+    if (t + 1 == q.n && q.dst < 0) return;          // the last row's state is nobody's
     d.x *= kn; d.y *= kn; d.z *= kn; d.w *= kn;
 #pragma unroll
     for (int r = 0; r < R; ++r) {

@@ -143,7 +143,10 @@ struct Best {
     qi[lane] = rest.i;
     n = max(n - 64, 0);
   }
+  // The lanes' largest of several logits each: as many logits as are wanted are not below the last of so many lanes.
+  __device__ __forceinline__ void hint(float most) { last.v = of_lane(sorted({most, NONE}), top - 1).v; }
   __device__ __forceinline__ void offer(float v, int i) {
+    if (!__any(v >= last.v)) return;
     const bool in = before({v, i}, last);
     const unsigned long long who = __ballot(in);
     if (!who) return;
@@ -161,6 +164,7 @@ struct Best {
 struct Most {
   Entry mine, last;
   __device__ __forceinline__ void start(float *, int *, int) { mine = last = {-INFINITY, NONE}; }
+  __device__ __forceinline__ void hint(float) {}
   __device__ __forceinline__ void offer(float v, int i) {
     if (before({v, i}, mine)) mine = {v, i};
   }
@@ -208,7 +212,7 @@ template <typename T> __device__ __forceinline__ float token_logit(const Logprob
 
 // TOP: 0 no largest logits are wanted, 1 one, 2 more.  RANK: whether ranks are.
 template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) void part_kernel(LogprobArgs a, Split sp) {
-  constexpr int E = 16 / sizeof(T), VECS = 64 / (16 * E / 4);      // 16 logits at a time
+  constexpr int E = 16 / sizeof(T), VECS = 16 / E;      // 16 logits at a time
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
   __shared__ float s_qv[WAVES][128], s_sums[WAVES][3];
   __shared__ int s_qi[WAVES][128], s_cnt[WAVES];
@@ -276,6 +280,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
           for (int e = 0; e < E; ++e) cnt += (float)w[k][e] == xt && head + p * E + e < tok ? 1 : 0;
       }
     }
+    if (TOP == 2 && u == v0) best.hint(most);
     if (TOP && __any(most >= (TOP == 1 ? best.mine.v : best.last.v))) {
 #pragma unroll
       for (int k = 0; k < VECS; ++k)
@@ -367,8 +372,15 @@ template <typename T> __global__ __launch_bounds__(THREADS) void join_kernel(Log
   finish(a, row, r, cnt, xt, l);
 }
 
-// Parts of a row: enough workgroups for the card, 4096 logits or more each.
-int parts_of(int rows, int V) { return std::max(1, std::min({SPLITS, (1024 + rows - 1) / std::max(rows, 1), V / 4096})); }
+// Parts of a row: three workgroups a CU together (96 rows of bf16, top 20: 38 us; two or four a CU 40 to 44: a wave's first
+// list costs it 1 us), but two turns of the loop each (one f32 row: 31 parts 19 us, 61 parts 21, the join taking longer), in
+// whole turns (what is left over goes piece by piece).
+Split split_of(int rows, int V, int E) {
+  const int turn = THREADS * 16 / E, most = std::max(1, std::min({SPLITS, 768 / std::max(rows, 1), V / 8192}));
+  int vecs = std::max(1, (V / E + most * turn / 2) / (most * turn)) * turn;
+  while ((V / E + vecs - 1) / vecs > SPLITS) vecs += turn;
+  return {std::max(1, (V / E + vecs - 1) / vecs), vecs};
+}
 
 template <typename T, int TOP> void launch_parts(const LogprobArgs &a, const Split &sp, hipStream_t st) {
   const dim3 grid((unsigned)(a.rows * sp.n));
@@ -377,8 +389,8 @@ template <typename T, int TOP> void launch_parts(const LogprobArgs &a, const Spl
 }
 template <typename T> void launch(const LogprobArgs &a, hipStream_t st) {
   constexpr int E = 16 / sizeof(T);
-  const int n = parts_of(a.rows, a.V);
-  const Split sp = {n, (a.V / E + n - 1) / n};
+  const Split sp = split_of(a.rows, a.V, E);
+  const int n = sp.n;
   if (a.top == 0) launch_parts<T, 0>(a, sp, st);
   else if (a.top == 1) launch_parts<T, 1>(a, sp, st);
   else launch_parts<T, 2>(a, sp, st);
@@ -388,7 +400,7 @@ template <typename T> void launch(const LogprobArgs &a, hipStream_t st) {
 }  // namespace
 
 size_t logprobs_bytes(int rows, int V, int top) {
-  const int n = parts_of(rows, V);
+  const int n = std::max(split_of(rows, V, 4).n, split_of(rows, V, 8).n);
   return n > 1 ? (size_t)rows * n * part_words(top) * sizeof(float) : 0;
 }
 

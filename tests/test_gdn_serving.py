@@ -119,6 +119,10 @@ def test_logprobs_refusals():
     for a in ((-1, 10, 0), (1, 0, 0), (1, 10, 65), (1, 10, -1)):
         assert L.cwen_logprobs_work(*a, C.byref(n)) == EINVAL
     assert L.cwen_logprobs_work(1, 10, 0, None) == EINVAL
+    for V in list(range(1, 70)) + [4095, 4096, 4097, 8191, 8192, 248320, 1 << 30]:      # every size has a division
+        for rows in (1, 2, 96, 1500, (1 << 18) - 1):
+            assert L.cwen_logprobs_work(rows, V, 64, C.byref(n)) == OK
+            assert n.value <= rows * 64 * (4 + 128) * 4 and (n.value > 0) == (rows <= 96 and V > 12000), (rows, V, n.value)
 
 
 PROG = r"""
