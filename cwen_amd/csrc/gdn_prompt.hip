@@ -251,9 +251,22 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         M = __builtin_amdgcn_mfma_f32_16x16x4f32(Lw[(16 + m) * LS + 4 * g4 + k], Lw[(4 * g4 + k) * LS + m], M, 0, 0, 0);
+      // (a row of M that is not finite makes the rows from it on so, and must not reach those before it)
+      int clear = 16;
+      if (__any(!(fabsf(M[0]) + fabsf(M[1]) + fabsf(M[2]) + fabsf(M[3]) < INFINITY))) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t = __builtin_amdgcn_mfma_f32_16x16x4f32(Lw[(16 + m) * LS + 16 + 4 * g4 + k], -M[k], t, 0, 0, 0);
-      T21[e] = t;
+        for (int k = 15; k >= 0; --k)
+          if (__any(4 * g4 == (k & 12) && !(fabsf(M[k & 3]) < INFINITY))) clear = k;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) M[k] = 4 * g4 + k < clear ? M[k] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float T22 = m >= 4 * g4 + k ? Lw[(16 + m) * LS + 16 + 4 * g4 + k] : 0.f;
+        t = __builtin_amdgcn_mfma_f32_16x16x4f32(T22, -M[k], t, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) T21[e][k] = 4 * g4 + k < clear ? t[k] : NAN;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     auto put = [&](_Float16 *to, int i, int col, float t) {
@@ -263,7 +276,7 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
       to[R::TLO / 2 + at] = f16_of(t - (float)h);
     };
 #pragma unroll
-    for (int i = 0; i < 16; ++i) put(op, 16 * (n >> 4) + i, n, T[i] * beta);
+    for (int i = 0; i < 16; ++i) put(op, 16 * (n >> 4) + i, n, i >= (n & 15) ? T[i] * beta : 0.f);   // (beta may be NaN)
     // rows 0 .. 15 of the later columns: nothing (zeros of the earlier lanes' blocks)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -301,11 +314,14 @@ __device__ __forceinline__ float max_groups(float x) {
 }
 // Two operands whose sum is x, one multiply-add that rounds to f16 for each low half (the compiler takes two
 // instructions and a half).  The block reads x behind the conversions that gave h0 .. h3, so a matrix result in x is
-// complete; its last instruction is the wait that a vector result needs before a matrix instruction reads it.
+// complete.  Its first instruction is the wait that a matrix instruction's addend needs before it may be overwritten (7
+// cycles here), its last the one that a vector result needs before a matrix instruction reads it: the compiler puts
+// neither in front of or behind assembly.
 __device__ __forceinline__ void split8(const float (&x)[8], half8_t &hi, half8_t &lo) {
   half2_t h0 = {(_Float16)x[0], (_Float16)x[1]}, h1 = {(_Float16)x[2], (_Float16)x[3]};
   half2_t h2 = {(_Float16)x[4], (_Float16)x[5]}, h3 = {(_Float16)x[6], (_Float16)x[7]}, l0, l1, l2, l3;
-  asm("v_fma_mixlo_f16 %0, %8, 1.0, -%4 op_sel_hi:[0,0,1]\n"
+  asm("s_nop 7\n"
+      "v_fma_mixlo_f16 %0, %8, 1.0, -%4 op_sel_hi:[0,0,1]\n"
       "v_fma_mixlo_f16 %1, %10, 1.0, -%5 op_sel_hi:[0,0,1]\n"
       "v_fma_mixlo_f16 %2, %12, 1.0, -%6 op_sel_hi:[0,0,1]\n"
       "v_fma_mixlo_f16 %3, %14, 1.0, -%7 op_sel_hi:[0,0,1]\n"
@@ -395,9 +411,16 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]));
     vmax = max_groups(vmax);
+    if (__any(vmax == INFINITY)) {       // an infinite value is no measure for the rows before it
+      vmax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+      vmax = max_groups(vmax);
+    }
   }
-  // The unit for the larger of |S| and `most` (a |v|) to lie in 1 .. 2; returns what S has to be multiplied by.
-  __device__ __forceinline__ float renew(float most) {
+  // The unit for the larger of |S| and `most` (a |v|) to lie in 1 .. 2, in the columns that call for it: what a column
+  // gets does not depend on its neighbours.  Returns what S has to be multiplied by.
+  __device__ __forceinline__ float renew(float most, bool call) {
     float mx = 0.f;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -406,10 +429,18 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     mx = fmaxf(max_groups(mx) * unit, most);
     const int ex = min(max((int)(__builtin_bit_cast(uint32_t, mx) >> 23), 1), 253);
     const float old = unit;
-    unit = __builtin_bit_cast(float, ex << 23);
-    per_unit = __builtin_bit_cast(float, (254 - ex) << 23);
+    unit = call ? __builtin_bit_cast(float, ex << 23) : unit;
+    per_unit = call ? __builtin_bit_cast(float, (254 - ex) << 23) : per_unit;
     // (a column that fell further than 2^100 since holds nothing beside what it held)
     return fminf(old * per_unit, 0x1p100f);
+  }
+  __device__ __forceinline__ int row_of(int e) const { return (e >> 2) * 16 + 4 * g + (e & 3); }
+  // The first of a column's rows that is not finite, or N.
+  __device__ __forceinline__ int first_odd(const float (&x)[8]) const {
+    float back = 0.f;             // N - row
+#pragma unroll
+    for (int e = 7; e >= 0; --e) back = fabsf(x[e]) < INFINITY ? back : fmaxf(back, (float)(N - row_of(e)));
+    return N - (int)max_groups(back);
   }
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   __device__ __forceinline__ void read_o(u32x4 (&x)[OP]) const {
@@ -460,7 +491,8 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     for (int e = 0; e < 8; ++e) w[e] = v[e] * per_unit;
     take_v();
     const float vu = vmax * per_unit;
-    if (!__all((c & 7) != 7 && vu < 16.f && vu >= 0.125f)) ratio = renew(fmaxf(vmax_here, vmax));
+    const bool stay = (c & 7) != 7 && vu < 16.f && vu >= 0.125f;
+    if (!__all(stay)) ratio = renew(fmaxf(vmax_here, vmax), !stay);
     store_o(c - 1, o_last);
     load_v(c + 4, vr_4);
     half8_t hi[U], lo[U];
@@ -472,11 +504,12 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       for (int j = 0; j < 8; ++j) x[j] = S[2 * u + (j >> 2)][j & 3];
       split8(x, hi[u], lo[u]);
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        X[mt] = mma(K[mt * U + u], lo[u], X[mt]);
-        X[mt] = mma(K[mt * U + u], hi[u], X[mt]);
-        if (KL) X[mt] = mma(KL_[mt * U + u], hi[u], X[mt]);
-      }
+      for (int mt = 0; mt < 2; ++mt) X[mt] = mma(K[mt * U + u], lo[u], X[mt]);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) X[mt] = mma(K[mt * U + u], hi[u], X[mt]);
+      if (KL)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) X[mt] = mma(KL_[mt * U + u], hi[u], X[mt]);
     }
     __builtin_amdgcn_sched_barrier(0);
     half8_t T[2], TL[2], Q[2 * U], QL[2 * U];
@@ -500,6 +533,37 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
         if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
         if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
       }
+    floatx4_t d[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3];
+    // A row that is not finite must not reach the rows before it, whose products with it are 0 times that.
+    int clear = N;                // rows from here on are not finite in this column
+    half8_t oh = high8(x), ol;
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) odd = __builtin_amdgcn_fdot2((half2_t){oh[e], oh[e + 1]}, (half2_t){0, 0}, odd, false);
+    if (__any(odd != 0.f)) {      // (0 or NaN)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)rh[e];
+      clear = first_odd(x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (row_of(e) >= clear) rh[e] = rl[e] = (_Float16)0.f;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const half8_t t = op(R::KEY + R::T, mt), u = op(R::KEY + R::TLO, mt);
+        d[mt] = mma(t, rh, mma(u, rh, mma(t, rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3];
+      clear = min(clear, first_odd(x));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = row_of(e) < clear ? x[e] : 0.f;
+      oh = high8(x);
+    }
     __builtin_amdgcn_sched_barrier(0);
     half8_t KT[DT], KTL[DT];
 #pragma unroll
@@ -508,30 +572,16 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       if (KL) KTL[t] = kt(R::KLO, t);
     }
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) fd[mt] = rows4(F_D, mt), fo[mt] = rows4(F_O, mt);
+    for (int mt = 0; mt < 2; ++mt) fd[mt] = rows4(F_D, mt);
     const float end = F[F_END];
-    half8_t A[2], AL[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      A[mt] = op(R::KEY + R::A, mt);
-      if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
-    }
-    floatx4_t d[2] = {};
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, d[mt])));
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[t][i] *= end * ratio;
-    __builtin_amdgcn_sched_barrier(0);
     turn_v(vr_2);
-    half8_t dh, dl, oh, ol;
-    float x[8], y[8];
+    half8_t dh, dl;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = d[e >> 2][e & 3];
-      y[e] = x[e] * (fd[e >> 2][e & 3] * ratio);
-    }
+    for (int e = 0; e < 8; ++e) y[e] = row_of(e) < clear ? x[e] * (fd[e >> 2][e & 3] * ratio) : NAN;
     split8(y, dh, dl);
 #pragma unroll
     for (int t = 0; t < DT; ++t) S[t] = mma(KT[t], dl, S[t]);
@@ -540,8 +590,14 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     if (KL)
 #pragma unroll
       for (int t = 0; t < DT; ++t) S[t] = mma(KTL[t], dh, S[t]);
+    half8_t A[2], AL[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      fo[mt] = rows4(F_O, mt);
+      A[mt] = op(R::KEY + R::A, mt);
+      if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+    }
     if (OF) split8(x, oh, ol);
-    else oh = high8(x);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       floatx4_t y;
@@ -550,7 +606,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       y = mma(A[mt], oh, y);
       if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
+      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(16 * mt + 4 * g + i < clear ? y[i] * (unit_here * out_unit) : NAN);
     }
   }
 };
@@ -673,7 +729,7 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
     p.take_v();
     p.turn_v(p.vr[1]);
     p.load_v(3, p.vr[0]);
-    const float ratio = p.renew(p.vmax);
+    const float ratio = p.renew(p.vmax, true);
 #pragma unroll
     for (int t = 0; t < C::DT; ++t)
 #pragma unroll

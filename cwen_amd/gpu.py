@@ -720,19 +720,19 @@ def gdn_prompt(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, sr
     """The gated delta rule over packed prompts (cwen_gdn_prompt), arguments as gdn_step; work: a prompt_work of the
     pool for at least this size (None: allocated for the call)."""
     args, n = _gdn_rule(ctx, pool, layer, q, k, v, a, b, o, cu, src, dst, A, dt, count)
-    s = _stream_of(ctx, stream)
     if work is None:
-        work = pool.prompt_work(q.shape[0], n, q.dtype, q.dtype if o is None else o.dtype)
-        _in_use(work, stream)
+        work = _scratch(lambda: pool.prompt_work(q.shape[0], n, q.dtype, q.dtype if o is None else o.dtype), stream)
     _on(ctx, work)
-    check("cwen_gdn_prompt", lib().cwen_gdn_prompt(*args, _ptr(work), work.numel() * work.element_size(), s))
+    check("cwen_gdn_prompt", lib().cwen_gdn_prompt(*args, _ptr(work), work.numel() * work.element_size(), _stream_of(ctx, stream)))
 
 
-def _in_use(t, stream) -> None:
-    """Keep a tensor allocated for one call from being handed out again before a stream other than the current one is done with it."""
-    if stream is not None and t.numel():
-        import torch
-        t.record_stream(torch.cuda.ExternalStream(stream, device=t.device) if isinstance(stream, int) else stream)
+def _scratch(make, stream):
+    """A tensor for one call on `stream`, from that stream's memory: free for what follows there, and only there."""
+    if stream is None:
+        return make()
+    import torch
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+        return make()
 
 
 def logprobs_work(rows: int, V: int, top: int = 0, device="cuda"):
@@ -757,16 +757,15 @@ def logprobs(ctx: Context, logits, tokens=None, logprob=None, rank=None, entropy
     for name, t in (("top_ids", top_ids), ("top_logprobs", top_logprobs)):
         if t is not None and tuple(t.shape) != (rows, top):
             raise ValueError(f"{name}: [{rows}, {top}] expected, got {tuple(t.shape)}")
-    s = _stream_of(ctx, stream)
     if work is None:
-        work = logprobs_work(rows, V, top, logits.device)
-        _in_use(work, stream)
+        work = _scratch(lambda: logprobs_work(rows, V, top, logits.device), stream)
     _on(ctx, work)
     check("cwen_logprobs", lib().cwen_logprobs(
         ctx.h, _type(logits), _ptr(logits), _row_stride(logits, rows, V), V, rows, vec("tokens", tokens, rows, "int32"),
         vec("logprob", logprob, rows, "float32"), vec("rank", rank, rows, "int32"), vec("entropy", entropy, rows, "float32"),
         vec("lse", lse, rows, "float32"), top, vec("top_ids", top_ids, rows * top, "int32"),
-        vec("top_logprobs", top_logprobs, rows * top, "float32"), _ptr(work), work.numel() * work.element_size(), s))
+        vec("top_logprobs", top_logprobs, rows * top, "float32"), _ptr(work), work.numel() * work.element_size(),
+        _stream_of(ctx, stream)))
 
 
 # ---------------------------------------------------------------- model

@@ -275,7 +275,9 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
  * A and dt (f32 [nvh]) g = exp(A[h] softplus(a + dt[h])) and beta = sigmoid(b)
  * (run.c:2697-2698), with both NULL g = exp(a) and beta = b.  a log decay above
  * 0 or a beta outside 0..2 gives unspecified values.  o is nullable (the states
- * alone move).  Pointers of q, k, v and o 16-byte aligned, their strides
+ * alone move).  A value of v that is not finite makes its column of the head not
+ * finite from its row on, a key or gate the whole head; a query its row alone.
+ * Pointers of q, k, v and o 16-byte aligned, their strides
  * multiples of 8 (the prompt's v_ts and o_ts below 2^24); o must not overlap q,
  * k or v (it may lie beside them in rows of the same bytes).  States are held and moved in f32.
  *
@@ -285,8 +287,8 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
  * cwen_gdn_prompt takes chunks of 32 rows on the matrix cores: with d_i of a
  * chunk from (1 + L) d = r, L_ij = beta_i g_j+1..g_i k_i.k_j (j < i), r_i =
  * beta_i (v_i - g_1..g_i S^T k_i).  Operands are rounded to f16 in pieces whose
- * sum holds 21 bits or more, for outputs of BF16 from operands of 16 bits to single
- * f16 values; sums are f32.  `work`: device scratch of
+ * sum holds 21 bits or more, below the column's largest |S| and |v| of the chunk;
+ * for outputs of BF16 from operands of 16 bits to single f16 values; sums are f32.  `work`: device scratch of
  * cwen_gdn_prompt_work's bytes, 256-byte aligned, free again when the call's
  * launches are done. */
 int cwen_gdn_step(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *q, long long q_ts,

@@ -256,6 +256,60 @@ def test_rule_wide_range(env):
         check_rule(env, name, [70, 3], 2, 4, 128, BF16, BF16, 6, raw=False, change=change)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("name", ["step", "prompt"])
+def test_rule_values_that_are_not_finite(env, name, bad):
+    """They reach their own column, head or row, never an earlier row, another sequence or the rows of no sequence."""
+    gpu, ctx = env
+    for i, (tx, to, nkh, nvh, D) in enumerate(((F32, F32, 2, 4, 64), (BF16, BF16, 2, 4, 128), (F16, F16, 1, 3, 128))):
+        lens, first = [75, 40], 1
+        T = first + sum(lens) + 3
+        call = gpu.gdn_step if name == "step" else gpu.gdn_prompt
+        q, k, v, a, b, _, _ = rule_inputs(gen(500 + i), T, nkh, nvh, D, tx, raw=False)
+        cu, dst = ints(borders(lens, first)), ints([0, 1])
+
+        def run():
+            pool = gpu.GdnPool.empty(1, 2, nkh, nvh, D)
+            o = torch.full((T, nvh, D), 7.0, device="cuda", dtype=to)
+            call(ctx, pool, 0, q, k, v, a, b, o, cu, None, dst)
+            return o, pool.state[0].clone()
+
+        for t in (q, k, v, a, b):                                # rows of no sequence hold anything
+            t[0], t[-3:] = bad, math.nan
+        clean, state = run()
+        assert bool(torch.isfinite(clean).all()) and bool(torch.isfinite(state).all())
+        for what, row in (("v", 0), ("v", 45), ("v", 31), ("k", 13), ("k", 64), ("q", 20), ("a", 33), ("b", 50), ("b", 7)):
+            if what == "a" and bad == -math.inf:
+                continue                                          # a decay to nothing: a number like others
+            t = {"q": q, "k": k, "v": v, "a": a, "b": b}[what]
+            at = first + row
+            keep = t[at].clone()
+            if what == "v":
+                t[at, 1, 5] = bad
+            elif what in "kq":
+                t[at, 0, 3] = bad
+            else:
+                t[at, 1] = bad
+            o, s = run()
+            t[at] = keep
+            heads = [h for h in range(nvh) if h % nkh == 0] if what in "kq" else [1]
+            others = [h for h in range(nvh) if h not in heads]
+            tell = (name, what, row, tx)
+            assert torch.equal(o[:, others], clean[:, others]) and torch.equal(s[:, others], state[:, others]), tell
+            assert torch.equal(o[:at, heads], clean[:at, heads]), tell                       # earlier rows
+            assert torch.equal(o[first + 75:], clean[first + 75:]) and torch.equal(s[1], state[1]), tell
+            end = first + 75
+            if what == "v":
+                cols = [c for c in range(D) if c != 5]
+                assert torch.equal(o[:, 1, cols], clean[:, 1, cols]) and torch.equal(s[0, 1][:, cols], state[0, 1][:, cols]), tell
+                assert not bool(torch.isfinite(o[at:end, 1, 5]).any()) and not bool(torch.isfinite(s[0, 1, :, 5]).any()), tell
+            elif what == "q":                                     # (an infinite one: over its length, NaN)
+                assert torch.equal(o[at + 1:end], clean[at + 1:end]) and torch.equal(s, state), tell
+                assert not bool(torch.isfinite(o[at, heads]).any()), tell
+            else:
+                assert not bool(torch.isfinite(o[at:end, heads]).any()) and not bool(torch.isfinite(s[0, heads]).any()), tell
+
+
 def test_step_rows_do_not_depend_on_the_call(env):
     """A block's rows are the bits of single ones, alone or among other sequences; scored rows leave the slots alone, the
     accepted counts move them."""
