@@ -434,13 +434,13 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     // (a column that fell further than 2^100 since holds nothing beside what it held)
     return fminf(old * per_unit, 0x1p100f);
   }
-  __device__ __forceinline__ int row_of(int e) const { return (e >> 2) * 16 + 4 * g + (e & 3); }
-  // The first of a column's rows that is not finite, or N.
+  // The first of a column's rows that is not finite, or N, less 4 g (value e of a lane is row at(e) + 4 g).
+  static __device__ constexpr int at(int e) { return (e >> 2) * 16 + (e & 3); }
   __device__ __forceinline__ int first_odd(const float (&x)[8]) const {
-    float back = 0.f;             // N - row
+    int first = N;
 #pragma unroll
-    for (int e = 7; e >= 0; --e) back = fabsf(x[e]) < INFINITY ? back : fmaxf(back, (float)(N - row_of(e)));
-    return N - (int)max_groups(back);
+    for (int e = 7; e >= 0; --e) first = fabsf(x[e]) < INFINITY ? first : at(e);
+    return -(int)max_groups(-(float)min(first + 4 * g, N)) - 4 * g;
   }
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   __device__ __forceinline__ void read_o(u32x4 (&x)[OP]) const {
@@ -533,37 +533,6 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
         if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
         if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
       }
-    floatx4_t d[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
-    float x[8], y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3];
-    // A row that is not finite must not reach the rows before it, whose products with it are 0 times that.
-    int clear = N;                // rows from here on are not finite in this column
-    half8_t oh = high8(x), ol;
-    float odd = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) odd = __builtin_amdgcn_fdot2((half2_t){oh[e], oh[e + 1]}, (half2_t){0, 0}, odd, false);
-    if (__any(odd != 0.f)) {      // (0 or NaN)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)rh[e];
-      clear = first_odd(x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (row_of(e) >= clear) rh[e] = rl[e] = (_Float16)0.f;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const half8_t t = op(R::KEY + R::T, mt), u = op(R::KEY + R::TLO, mt);
-        d[mt] = mma(t, rh, mma(u, rh, mma(t, rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3];
-      clear = min(clear, first_odd(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = row_of(e) < clear ? x[e] : 0.f;
-      oh = high8(x);
-    }
     __builtin_amdgcn_sched_barrier(0);
     half8_t KT[DT], KTL[DT];
 #pragma unroll
@@ -574,14 +543,21 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) fd[mt] = rows4(F_D, mt);
     const float end = F[F_END];
+    floatx4_t d[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[t][i] *= end * ratio;
     turn_v(vr_2);
-    half8_t dh, dl;
+    float x[8], y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = row_of(e) < clear ? x[e] * (fd[e >> 2][e & 3] * ratio) : NAN;
+    for (int e = 0; e < 8; ++e) {
+      x[e] = d[e >> 2][e & 3];
+      y[e] = x[e] * (fd[e >> 2][e & 3] * ratio);
+    }
+    half8_t dh, dl;
     split8(y, dh, dl);
 #pragma unroll
     for (int t = 0; t < DT; ++t) S[t] = mma(KT[t], dl, S[t]);
@@ -590,12 +566,41 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     if (KL)
 #pragma unroll
       for (int t = 0; t < DT; ++t) S[t] = mma(KTL[t], dh, S[t]);
+    __builtin_amdgcn_sched_barrier(0);
     half8_t A[2], AL[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       fo[mt] = rows4(F_O, mt);
       A[mt] = op(R::KEY + R::A, mt);
       if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+    }
+    // A row of d that is not finite leaves nothing finite in its column of S.  But it must not reach the outputs of the rows
+    // before it, whose products with it are 0 times that, neither here nor in d: there those rows are solved anew.
+    half8_t oh = high8(x), ol;
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) odd = __builtin_amdgcn_fdot2((half2_t){oh[e], oh[e + 1]}, (half2_t){0, 0}, odd, false);
+    if (__any(odd != 0.f)) {      // (0 or NaN)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)rh[e];
+      int clear = first_odd(x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (at(e) >= clear) rh[e] = rl[e] = (_Float16)0.f;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const half8_t t = op(R::KEY + R::T, mt), u = op(R::KEY + R::TLO, mt);
+        d[mt] = mma(t, rh, mma(u, rh, mma(t, rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3];
+      clear = min(clear, first_odd(x));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = at(e) < clear ? x[e] : 0.f;
+        if (at(e) >= clear) Y[e >> 2][e & 3] = NAN;
+      }
+      oh = high8(x);
     }
     if (OF) split8(x, oh, ol);
 #pragma unroll
@@ -606,7 +611,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       y = mma(A[mt], oh, y);
       if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(16 * mt + 4 * g + i < clear ? y[i] * (unit_here * out_unit) : NAN);
+      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
     }
   }
 };
