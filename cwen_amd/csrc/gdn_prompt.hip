@@ -411,12 +411,13 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]));
     vmax = max_groups(vmax);
-    if (__any(vmax == INFINITY)) {       // an infinite value is no measure for the rows before it
-      vmax = 0.f;
+  }
+  // Of the finite ones: an infinite value is no measure for the rows before it.
+  __device__ __forceinline__ void finite_vmax() {
+    vmax = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
-      vmax = max_groups(vmax);
-    }
+    for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+    vmax = max_groups(vmax);
   }
   // The unit for the larger of |S| and `most` (a |v|) to lie in 1 .. 2, in the columns that call for it: what a column
   // gets does not depend on its neighbours.  Returns what S has to be multiplied by.
@@ -490,9 +491,14 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = v[e] * per_unit;
     take_v();
-    const float vu = vmax * per_unit;
-    const bool stay = (c & 7) != 7 && vu < 16.f && vu >= 0.125f;
-    if (!__all(stay)) ratio = renew(fmaxf(vmax_here, vmax), !stay);
+    auto stay = [&]() __attribute__((always_inline)) {
+      const float vu = vmax * per_unit;
+      return (c & 7) != 7 && vu < 16.f && vu >= 0.125f;
+    };
+    if (!__all(stay())) {
+      if (__any(vmax == INFINITY)) finite_vmax();
+      ratio = renew(fmaxf(vmax_here, vmax), !stay());
+    }
     store_o(c - 1, o_last);
     load_v(c + 4, vr_4);
     half8_t hi[U], lo[U];
@@ -543,6 +549,17 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) fd[mt] = rows4(F_D, mt);
     const float end = F[F_END];
+    // (two waves have registers for these as well by now; of more, three share a SIMD's)
+    half8_t A[2], AL[2];
+    auto ask_a = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        fo[mt] = rows4(F_O, mt);
+        A[mt] = op(R::KEY + R::A, mt);
+        if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+      }
+    };
+    if (NW <= 2) ask_a();
     floatx4_t d[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
@@ -550,6 +567,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[t][i] *= end * ratio;
+    __builtin_amdgcn_sched_barrier(0);
     turn_v(vr_2);
     float x[8], y[8];
 #pragma unroll
@@ -557,6 +575,13 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       x[e] = d[e >> 2][e & 3];
       y[e] = x[e] * (fd[e >> 2][e & 3] * ratio);
     }
+    // A row of d that is not finite leaves nothing finite in its column of S.  But it must not reach the outputs of the rows
+    // before it, whose products with it are 0 times that, neither here nor in d: there those rows are solved anew.
+    float odd = 0.f;
+    half8_t oh = high8(x), ol;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) odd = __builtin_amdgcn_fdot2((half2_t){oh[e], oh[e + 1]}, (half2_t){0, 0}, odd, false);
+    const bool is_odd = __any(odd != 0.f);        // (0 or NaN)
     half8_t dh, dl;
     split8(y, dh, dl);
 #pragma unroll
@@ -566,21 +591,11 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     if (KL)
 #pragma unroll
       for (int t = 0; t < DT; ++t) S[t] = mma(KTL[t], dh, S[t]);
-    __builtin_amdgcn_sched_barrier(0);
-    half8_t A[2], AL[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      fo[mt] = rows4(F_O, mt);
-      A[mt] = op(R::KEY + R::A, mt);
-      if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+    if (NW > 2) {
+      __builtin_amdgcn_sched_barrier(0);
+      ask_a();
     }
-    // A row of d that is not finite leaves nothing finite in its column of S.  But it must not reach the outputs of the rows
-    // before it, whose products with it are 0 times that, neither here nor in d: there those rows are solved anew.
-    half8_t oh = high8(x), ol;
-    float odd = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) odd = __builtin_amdgcn_fdot2((half2_t){oh[e], oh[e + 1]}, (half2_t){0, 0}, odd, false);
-    if (__any(odd != 0.f)) {      // (0 or NaN)
+    if (is_odd) {                 // (behind the state's products: ahead of them its values would not fit the registers)
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = (float)rh[e];
       int clear = first_odd(x);
@@ -732,6 +747,7 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
     p.load_v(2, p.vr[2]);
     p.turn_v(p.vr[0]);
     p.take_v();
+    p.finite_vmax();
     p.turn_v(p.vr[1]);
     p.load_v(3, p.vr[0]);
     const float ratio = p.renew(p.vmax, true);
