@@ -134,7 +134,8 @@ int cwen_gdn_prompt(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xty
   const int rc = check_rule(ctx, pool, layer, xtype, q, q_ts, k, k_ts, v, v_ts, a, b, g_ts, A, dt, otype, o, o_ts, cu, count, src, dst,
                             n_seq, total, &args, &none);
   if (rc || none) return rc;
-  if (gdn_pieces(total, n_seq, 32) * pool->nvh * 2 >= launch_max) return CWEN_EINVAL;
+  // (the second launch has up to 640 threads a sequence and head)
+  if (gdn_pieces(total, n_seq, 32) * pool->nvh * 2 >= launch_max || (long long)n_seq * pool->nvh * 4 >= launch_max) return CWEN_EINVAL;
   if (total > 1 && (v_ts >= 1 << 24 || (o && o_ts >= 1 << 24))) return CWEN_EINVAL;      // a chunk's rows by 32-bit offsets
   const size_t need = gdn_prompt_bytes(xtype, otype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
   if (need && (!work || ((uintptr_t)work & 255u))) return CWEN_EINVAL;

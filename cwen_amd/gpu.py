@@ -721,17 +721,17 @@ def gdn_prompt(ctx: Context, pool: GdnPool, layer: int, q, k, v, a, b, o, cu, sr
     pool for at least this size (None: allocated for the call)."""
     args, n = _gdn_rule(ctx, pool, layer, q, k, v, a, b, o, cu, src, dst, A, dt, count)
     if work is None:
-        work = _scratch(lambda: pool.prompt_work(q.shape[0], n, q.dtype, q.dtype if o is None else o.dtype), stream)
+        work = _scratch(lambda: pool.prompt_work(q.shape[0], n, q.dtype, q.dtype if o is None else o.dtype), stream, q.device)
     _on(ctx, work)
     check("cwen_gdn_prompt", lib().cwen_gdn_prompt(*args, _ptr(work), work.numel() * work.element_size(), _stream_of(ctx, stream)))
 
 
-def _scratch(make, stream):
+def _scratch(make, stream, device):
     """A tensor for one call on `stream`, from that stream's memory: free for what follows there, and only there."""
     if stream is None:
         return make()
     import torch
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream):
         return make()
 
 
@@ -758,7 +758,7 @@ def logprobs(ctx: Context, logits, tokens=None, logprob=None, rank=None, entropy
         if t is not None and tuple(t.shape) != (rows, top):
             raise ValueError(f"{name}: [{rows}, {top}] expected, got {tuple(t.shape)}")
     if work is None:
-        work = _scratch(lambda: logprobs_work(rows, V, top, logits.device), stream)
+        work = _scratch(lambda: logprobs_work(rows, V, top, logits.device), stream, logits.device)
     _on(ctx, work)
     check("cwen_logprobs", lib().cwen_logprobs(
         ctx.h, _type(logits), _ptr(logits), _row_stride(logits, rows, V), V, rows, vec("tokens", tokens, rows, "int32"),

@@ -274,7 +274,8 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
  * v) and otype (F32, F16, BF16); a, b f32 [total], rows g_ts floats apart: with
  * A and dt (f32 [nvh]) g = exp(A[h] softplus(a + dt[h])) and beta = sigmoid(b)
  * (run.c:2697-2698), with both NULL g = exp(a) and beta = b.  a log decay above
- * 0 or a beta outside 0..2 gives unspecified values.  o is nullable (the states
+ * 0, a beta outside 0..2, or a row of q or k longer than 2^63 (its squares' sum
+ * is f32) gives unspecified values.  o is nullable (the states
  * alone move).  A value of v that is not finite makes its column of the head not
  * finite from its row on, a key or gate the whole head; a query its row alone.
  * Pointers of q, k, v and o 16-byte aligned, their strides

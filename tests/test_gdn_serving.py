@@ -92,6 +92,7 @@ def test_rule_refusals():
     assert rule("prompt", c=pool(nvh=4096, nkh=1), vs=4096 * 64, os=4096 * 64, gs=4096, qs=4096 * 64, ks=4096 * 64, total=1 << 20,
                 q=P, k=P, v=P, o=None) == EINVAL          # chunks times heads past a launch
     L = gpu.lib()
+    assert rule("prompt", c=pool(nvh=1024, nkh=1), vs=1024 * 64, os=1024 * 64, gs=1024, o=None, n=4096) == EINVAL       # sequences times heads past one
     assert L.cwen_gdn_prompt_work(pool(), BF16, BF16, 1, 40, None) == EINVAL
     assert L.cwen_gdn_prompt_work(pool(), 3, BF16, 1, 40, C.byref(n)) == ETYPE
     assert L.cwen_gdn_prompt_work(pool(), BF16, BF16, -1, 40, C.byref(n)) == EINVAL
