@@ -793,12 +793,15 @@ template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRu
 template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
   hipLaunchKernelGGL((prep_kernel<TX, D, full_out<TX, TO>()>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
-  // Waves of a workgroup: two where there are few sequences and heads, which spreads them over the CUs (8192 rows of 48
-  // heads of 128 in bf16: 298 us, with four 345).  Else all of a head's columns: a record then comes once, and two of
-  // the chain's waves share a SIMD (16301 rows in 9 sequences: 254 us, with four 300).  Eight waves of f32 operands do
-  // not fit the registers.
-  constexpr int MANY = D == 128 && sizeof(TX) == 2 ? 8 : 4;
-  if ((long long)a.s.n_seq * a.nvh * (D / 32) <= 512) launch_chain<TX, TO, D, 2>(a, w, st);
+  // Waves of a workgroup: the fewest with which the workgroups have a CU each.  Few waves beside each other are faster
+  // (1024 rows of 48 heads of 128 in bf16, both launches: 62 us with two, 66 with four, 85 with eight), two workgroups on
+  // a CU are not (two such sequences: 86, 77, 96).  Past that all of a head's columns: a record then comes once, and two of
+  // the chain's waves share a SIMD (four: 142, 134, 108; 48: 1353, 1234, 1019).  Eight waves of f32 operands do not fit the
+  // registers.
+  constexpr int MANY = D == 128 && sizeof(TX) == 2 ? 8 : 4, CUS = 256;
+  const long long heads = (long long)a.s.n_seq * a.nvh;
+  if (heads * (D / 32) <= CUS) launch_chain<TX, TO, D, 2>(a, w, st);
+  else if (heads * (D / 64) <= CUS) launch_chain<TX, TO, D, 4>(a, w, st);
   else launch_chain<TX, TO, D, MANY>(a, w, st);
 }
 template <typename TX, typename TO> void launch_d(int D, const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {

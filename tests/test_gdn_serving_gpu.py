@@ -246,6 +246,51 @@ def test_rule_hard_inputs(env, name, kind):
         check_rule(env, name, [70, 33], 2, 4, (64, 128)[i % 2], tx, to, 300 + i, raw=False, change=HARD[kind])
 
 
+# Sequences and heads for launches of two, four and eight (f32: four) waves a workgroup.
+WIDE = [([33, 64, 5, 97, 1], 4, 12, 128), ([33, 64, 5, 97, 1], 8, 16, 128), ([40, 31, 32, 1, 0, 65, 96, 7, 64, 33], 8, 16, 128),
+        ([40, 31, 32, 1, 0, 65, 96, 7, 64, 33], 8, 16, 64), ([40, 31, 32, 1, 0, 65, 96, 7, 64, 33], 28, 28, 64)]
+
+
+@pytest.mark.parametrize("tx,to", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32)])
+def test_prompt_of_many_heads(env, tx, to):
+    for i, (lens, nkh, nvh, D) in enumerate(WIDE):
+        check_rule(env, "prompt", lens, nkh, nvh, D, tx, to, 700 + i, key_head="mod" if i % 2 else "group")
+        check_rule(env, "prompt", lens, nkh, nvh, D, tx, to, 710 + i, raw=False, count=[n - n // 4 for n in lens],
+                   change=list(HARD.values())[i % len(HARD)])
+
+
+@pytest.mark.parametrize("tx,to", [(F32, F32), (BF16, BF16), (F16, F16)])
+def test_prompt_of_many_heads_with_values_that_are_not_finite(env, tx, to):
+    """In one column of every head of a sequence: rows before, other columns and other sequences stay as they are."""
+    gpu, ctx = env
+    for i, (lens, nkh, nvh, D) in enumerate(WIDE):
+        T, at, n = sum(lens), sum(lens[:3]), lens[3] if lens[3] > 70 else 0
+        if not n:
+            at, n = sum(lens[:6]), lens[6]
+        q, k, v, a, b, _, _ = rule_inputs(gen(720 + i), T, nkh, nvh, D, tx, raw=False)
+        cu, dst = ints(borders(lens, 0)), ints(list(range(len(lens))))
+
+        def run():
+            pool = gpu.GdnPool.empty(1, len(lens), nkh, nvh, D)
+            o = torch.full((T, nvh, D), 7.0, device="cuda", dtype=to)
+            gpu.gdn_prompt(ctx, pool, 0, q, k, v, a, b, o, cu, None, dst)
+            return o, pool.state[0].clone()
+
+        clean, state = run()
+        seq = lens.index(n)
+        for row, bad in ((0, math.nan), (33, math.inf), (63, -math.inf), (70, math.nan)):
+            keep = v[at + row].clone()
+            v[at + row, :, 9] = bad
+            o, s = run()
+            v[at + row] = keep
+            cols, rest = [c for c in range(D) if c != 9], [r for r in range(len(lens)) if r != seq]
+            tell = (lens, nvh, D, row, bad, tx)
+            assert torch.equal(o[:, :, cols], clean[:, :, cols]) and torch.equal(s[:, :, :, cols], state[:, :, :, cols]), tell
+            assert torch.equal(o[:at + row], clean[:at + row]) and torch.equal(o[at + n:], clean[at + n:]), tell
+            assert torch.equal(s[rest], state[rest]), tell
+            assert not bool(torch.isfinite(o[at + row:at + n, :, 9]).any()) and not bool(torch.isfinite(s[seq, :, :, 9]).any()), tell
+
+
 def test_rule_wide_range(env):
     """Values of f32's and bf16's range, beside columns of small ones: each column by its own size."""
     def change(q, k, v, a, b):
