@@ -345,6 +345,10 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   typedef Rec<D, KL, OF> R;
   static constexpr int U = R::U, DT = D / 16, KB = R::KEY / 1024 + R::HEAD / 1024 + 1, XS = sizeof(TX), OS = sizeof(TO);
   static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
+  // Of two waves each has another one that forms its outputs, a chunk later, from S's and d's halves in LDS (f32 heads of
+  // 128 have no room for them and a fourth record).
+  static constexpr bool SPLIT = NW == 2 && (XS == 2 || D == 64);
+  static constexpr int HALVES = OF ? 2 : 1, EX = HALVES * (U + 1) * 1024 + 512, NV = SPLIT ? 4 : 3;
   typedef char Buf[R::KEY + R::HEAD];
 
   int lane, n, g;
@@ -361,7 +365,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   // the state, divided by the column's unit, and the present chunk's values
   floatx4_t S[DT];
   float unit, per_unit, v[8], vmax;
-  uint4 vr[3][VP];                   // values on their way: chunk c's in vr[c % 3]
+  uint4 vr[NV][VP];                  // values on their way: chunk c's in vr[c % NV]
   float far[XS == 4 ? 8 : 4];    // the chunk's after that, by columns (16 bits: two a float)
 
   // A chunk's rows of v and o as buffers that end with the sequence: loads past it give 0, stores past it (and to no o)
@@ -458,10 +462,11 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 
   // Chunk c, whose record is in `b` behind the barrier.  v holds its values, `far` those of c + 1, vr_2 those of c + 2;
   // vr_4 takes c + 4's.
-  __device__ __forceinline__ void chunk(int c, Buf &b, const uint4 (&vr_2)[VP], uint4 (&vr_4)[VP]) {
+  __device__ __forceinline__ void chunk(int c, Buf &b, const uint4 (&vr_2)[VP], uint4 (&vr_4)[VP], char *ex) {
     const float *F = (const float *)(b + R::KEY + R::F);
     u32x4 o_last[OP];
-    read_o(o_last);
+    if (!SPLIT) read_o(o_last);
+    asm volatile("" ::: "memory");
     lds_barrier();
     asm volatile("" ::: "memory");
     auto op = [&](int base, int i) __attribute__((always_inline)) { return *(const half8_t *)(b + base + (i * 64 + lane) * 16); };
@@ -499,7 +504,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       if (__any(vmax == INFINITY)) finite_vmax();
       ratio = renew(fmaxf(vmax_here, vmax), !stay());
     }
-    store_o(c - 1, o_last);
+    if (!SPLIT) store_o(c - 1, o_last);
     load_v(c + 4, vr_4);
     half8_t hi[U], lo[U];
     floatx4_t X[2] = {}, Y[2] = {};
@@ -509,6 +514,10 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = S[2 * u + (j >> 2)][j & 3];
       split8(x, hi[u], lo[u]);
+      if (SPLIT) {
+        *(half8_t *)(ex + (u * 64 + lane) * 16) = hi[u];
+        if (OF) *(half8_t *)(ex + ((U + 1 + u) * 64 + lane) * 16) = lo[u];
+      }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) X[mt] = mma(K[mt * U + u], lo[u], X[mt]);
 #pragma unroll
@@ -521,24 +530,26 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     half8_t T[2], TL[2], Q[2 * U], QL[2 * U];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) T[mt] = op(R::KEY + R::T, mt), TL[mt] = op(R::KEY + R::TLO, mt);
+    if (!SPLIT)
 #pragma unroll
-    for (int i = 0; i < 2 * U; ++i) {
-      Q[i] = op(R::Q, i);
-      if (KL) QL[i] = op(R::QLO, i);
-    }
+      for (int i = 0; i < 2 * U; ++i) {
+        Q[i] = op(R::Q, i);
+        if (KL) QL[i] = op(R::QLO, i);
+      }
     half8_t rh, rl;
     float r[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) r[e] = fmaf(-fx[e >> 2][e & 3], X[e >> 2][e & 3], w[e]);
     split8(r, rh, rl);
+    if (!SPLIT)
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
-        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
-        if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
-      }
+        for (int mt = 0; mt < 2; ++mt) {
+          Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
+          if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+          if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
+        }
     __builtin_amdgcn_sched_barrier(0);
     half8_t KT[DT], KTL[DT];
 #pragma unroll
@@ -559,7 +570,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
         if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
       }
     };
-    if (NW <= 2) ask_a();
+    if (NW <= 2 && !SPLIT) ask_a();
     floatx4_t d[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) d[mt] = mma(T[mt], rh, mma(TL[mt], rh, mma(T[mt], rl, (floatx4_t){0.f, 0.f, 0.f, 0.f})));
@@ -595,10 +606,11 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       __builtin_amdgcn_sched_barrier(0);
       ask_a();
     }
+    int clear = N;                // (less 4 g)
     if (is_odd) {                 // (behind the state's products: ahead of them its values would not fit the registers)
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = (float)rh[e];
-      int clear = first_odd(x);
+      clear = first_odd(x);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (at(e) >= clear) rh[e] = rl[e] = (_Float16)0.f;
@@ -618,6 +630,12 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       oh = high8(x);
     }
     if (OF) split8(x, oh, ol);
+    if constexpr (SPLIT) {
+      *(half8_t *)(ex + (U * 64 + lane) * 16) = oh;
+      if (OF) *(half8_t *)(ex + ((2 * U + 1) * 64 + lane) * 16) = ol;
+      *(float2 *)(ex + HALVES * (U + 1) * 1024 + lane * 8) = make_float2(unit_here, __builtin_bit_cast(float, clear));
+      return;
+    }
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       floatx4_t y;
@@ -628,6 +646,59 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
       for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
     }
+  }
+
+  // The other wave's part of chunk c, behind the barrier of chunk c + 1.
+  __device__ __forceinline__ void outputs(int c, Buf &b, const char *ex) {
+    asm volatile("" ::: "memory");
+    lds_barrier();
+    asm volatile("" ::: "memory");
+    if (!o0) return;
+    const float *F = (const float *)(b + R::KEY + R::F);
+    auto op = [&](const char *from, int i) __attribute__((always_inline)) { return *(const half8_t *)(from + (i * 64 + lane) * 16); };
+    half8_t Q[2 * U], QL[2 * U], hi[U], lo[U], A[2], AL[2], oh, ol;
+    floatx4_t Y[2] = {}, fo[2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      hi[u] = op(ex, u);
+      if (OF) lo[u] = op(ex, U + 1 + u);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+      Q[i] = op(b + R::Q, i);
+      if (KL) QL[i] = op(b + R::QLO, i);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      fo[mt] = *(const floatx4_t *)(F + F_O + 16 * mt + 4 * g);
+      A[mt] = op(b + R::KEY + R::A, mt);
+      if (OF) AL[mt] = op(b + R::KEY + R::ALO, mt);
+    }
+    oh = op(ex, U);
+    if (OF) ol = op(ex, 2 * U + 1);
+    const float2 column = *(const float2 *)(ex + HALVES * (U + 1) * 1024 + lane * 8);       // its unit; its first row that is not finite
+    const int clear = __builtin_bit_cast(int, column.y);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
+        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+        if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
+      }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      floatx4_t y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = 16 * mt + i < clear ? fo[mt][i] * Y[mt][i] : NAN;
+      y = mma(A[mt], oh, y);
+      if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (column.x * out_unit));
+    }
+    u32x4 o[OP];
+    read_o(o);
+    store_o(c, o);
   }
 };
 
@@ -646,12 +717,17 @@ __device__ __forceinline__ int nth_longest(const GdnSeqs &a, int nth) {
 // Three records in LDS, an array each: in one, the compiler would wait for the loads into one record
 // before it reads another.
 template <typename TX, typename TO, int D, int NW>
-__global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) void chain_kernel(GdnRuleArgs a, PromptWork w) {
+__global__ __launch_bounds__(64 * (Chain<TX, TO, D, NW>::SPLIT ? 2 * NW + 1 : NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1)
+void chain_kernel(GdnRuleArgs a, PromptWork w) {
   typedef Chain<TX, TO, D, NW> C;
   typedef typename C::R R;
-  constexpr int SL = D / (16 * NW);
+  constexpr bool SPLIT = C::SPLIT;
+  constexpr int SL = D / (16 * NW), OUT = SPLIT ? NW : 0;        // waves of outputs, before those of the chain
   __shared__ __align__(1024) typename C::Buf b0, b1, b2;
-  __shared__ __align__(16) char s_io[NW][N * 16 * (C::XS > C::OS ? C::XS : C::OS)];
+  __shared__ __align__(1024) char b3_[SPLIT ? sizeof(typename C::Buf) : 16];
+  __shared__ __align__(16) char s_io[OUT + NW][N * 16 * (C::XS > C::OS ? C::XS : C::OS)];
+  __shared__ __align__(16) char s_ex[SPLIT ? 2 : 1][SPLIT ? NW : 1][SPLIT ? C::EX : 16];
+  typename C::Buf &b3 = (typename C::Buf &)b3_;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = a.nvh * SL, nth = blockIdx.x / per, i0 = blockIdx.x - nth * per, grp = a.nvh / a.nkh;
   const int s = nth_longest(a.s, nth);
@@ -673,7 +749,7 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
   }
   if (q.n == 0 && (q.dst < 0 || q.dst == q.src)) return;
   const int chunks = (q.n + N - 1) / N;
-  if (wave == NW) {
+  if (wave == OUT + NW) {
     if (!chunks) return;
     const long long z0 = gdn_piece0(q.first, s, N), key_step = (long long)a.nkh * R::KEY, head_step = (long long)a.nvh * R::HEAD;
     const char *key = w.key + (z0 * a.nkh + hk) * R::KEY + lane * 16, *head = w.head + (z0 * a.nvh + hv) * R::HEAD + lane * 16;
@@ -692,7 +768,7 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
         __builtin_amdgcn_global_load_lds((attn_glb_t *)(head + most), (attn_lds_t *)(to + R::KEY + most), 16, 0, 0);
       if (++c < chunks) key += key_step, head += head_step;
     };
-    // Buffer c % 3 is read until the barrier of chunk c + 1, behind which chunk c + 3 goes there.
+    // Buffer c % 3 is read until the barrier of chunk c + 1, behind which chunk c + 3 goes there (SPLIT: c % 4, c + 2, c + 4).
     auto next = [&](typename C::Buf &to) __attribute__((always_inline)) {
       wait_loads<C::KB>();
       lds_barrier();
@@ -704,11 +780,16 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
     for (int i = 0;;) {
       next(b2);
       if (++i == chunks) break;
+      if (SPLIT) {
+        next(b3);
+        if (++i == chunks) break;
+      }
       next(b0);
       if (++i == chunks) break;
       next(b1);
       if (++i == chunks) break;
     }
+    if (SPLIT) lds_barrier();
     wait_loads<0>();            // what was asked for past the end lands before the LDS is given up
     return;
   }
@@ -716,7 +797,32 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
   p.lane = lane;
   p.n = lane & 15;
   p.g = lane >> 4;
-  const int c0 = (slice * NW + wave) * 16;             // the wave's first column
+  const int part = SPLIT && wave >= NW ? wave - NW : wave, c0 = (slice * NW + part) * 16;             // the wave's first column
+  p.rows = q.n;
+  p.o0 = a.o ? (char *)a.o + (q.first * a.os + hv * D) * C::OS : nullptr;
+  p.o_row = (uint32_t)a.os * C::OS;
+  p.o_chunk = a.os * C::OS * N;
+#pragma unroll
+  for (int i = 0; i < C::OP; ++i) p.o_at[i] = (i * 64 + lane) / C::OS * p.o_row + c0 * C::OS + lane % C::OS * 16;
+  p.s_io = s_io[wave];
+  p.out_unit = O_UNIT / sqrtf((float)D);
+  if constexpr (SPLIT) {
+    if (wave < NW) {
+      if (!chunks) return;
+      lds_barrier();                                   // of chunk 0
+      for (int c = 0;;) {
+        p.outputs(c, b0, s_ex[0][part]);
+        if (++c == chunks) break;
+        p.outputs(c, b1, s_ex[1][part]);
+        if (++c == chunks) break;
+        p.outputs(c, b2, s_ex[0][part]);
+        if (++c == chunks) break;
+        p.outputs(c, b3, s_ex[1][part]);
+        if (++c == chunks) break;
+      }
+      return;
+    }
+  }
   const long long slot = (long long)a.nvh * D * D, at = (long long)hv * D * D + 4 * p.g * D + c0 + p.n;
 #pragma unroll
   for (int t = 0; t < C::DT; ++t) p.S[t] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
@@ -729,19 +835,11 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
   }
   p.unit = p.per_unit = 1.f;
   if (chunks) {
-    p.rows = q.n;
     p.v0 = (const char *)a.v + (q.first * a.vs + hv * D) * C::XS;
-    p.o0 = a.o ? (char *)a.o + (q.first * a.os + hv * D) * C::OS : nullptr;
     p.v_row = (uint32_t)a.vs * C::XS;
-    p.o_row = (uint32_t)a.os * C::OS;
     p.v_chunk = a.vs * C::XS * N;
-    p.o_chunk = a.os * C::OS * N;
 #pragma unroll
     for (int i = 0; i < C::VP; ++i) p.v_at[i] = (i * 64 + p.lane) / C::XS * p.v_row + c0 * C::XS + p.lane % C::XS * 16;
-#pragma unroll
-    for (int i = 0; i < C::OP; ++i) p.o_at[i] = (i * 64 + p.lane) / C::OS * p.o_row + c0 * C::OS + p.lane % C::OS * 16;
-    p.s_io = s_io[wave];
-    p.out_unit = O_UNIT / sqrtf((float)D);
     p.load_v(0, p.vr[0]);
     p.load_v(1, p.vr[1]);
     p.load_v(2, p.vr[2]);
@@ -749,23 +847,38 @@ __global__ __launch_bounds__(64 * (NW + 1), NW >= 4 && sizeof(TX) == 2 ? 3 : 1) 
     p.take_v();
     p.finite_vmax();
     p.turn_v(p.vr[1]);
-    p.load_v(3, p.vr[0]);
+    p.load_v(3, p.vr[3 % C::NV]);
     const float ratio = p.renew(p.vmax, true);
 #pragma unroll
     for (int t = 0; t < C::DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) p.S[t][i] *= ratio;
-    for (int c = 0;;) {
-      p.chunk(c, b0, p.vr[2], p.vr[1]);
-      if (++c == chunks) break;
-      p.chunk(c, b1, p.vr[0], p.vr[2]);
-      if (++c == chunks) break;
-      p.chunk(c, b2, p.vr[1], p.vr[0]);
-      if (++c == chunks) break;
+    if constexpr (SPLIT) {
+      for (int c = 0;;) {
+        p.chunk(c, b0, p.vr[2], p.vr[0], s_ex[0][part]);
+        if (++c == chunks) break;
+        p.chunk(c, b1, p.vr[3], p.vr[1], s_ex[1][part]);
+        if (++c == chunks) break;
+        p.chunk(c, b2, p.vr[0], p.vr[2], s_ex[0][part]);
+        if (++c == chunks) break;
+        p.chunk(c, b3, p.vr[1], p.vr[3], s_ex[1][part]);
+        if (++c == chunks) break;
+      }
+      asm volatile("" ::: "memory");
+      lds_barrier();
+    } else {
+      for (int c = 0;;) {
+        p.chunk(c, b0, p.vr[2], p.vr[1], nullptr);
+        if (++c == chunks) break;
+        p.chunk(c, b1, p.vr[0], p.vr[2], nullptr);
+        if (++c == chunks) break;
+        p.chunk(c, b2, p.vr[1], p.vr[0], nullptr);
+        if (++c == chunks) break;
+      }
+      typename C::u32x4 o_last[C::OP];
+      p.read_o(o_last);
+      p.store_o(chunks - 1, o_last);
     }
-    typename C::u32x4 o_last[C::OP];
-    p.read_o(o_last);
-    p.store_o(chunks - 1, o_last);
   }
   if (q.dst >= 0) {
     float *to = a.state + q.dst * slot + at;
@@ -788,7 +901,7 @@ void sizes_of(int xtype, int otype, int D, size_t *key, size_t *head) {
 
 template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   constexpr int SL = D / (16 * NW);
-  hipLaunchKernelGGL((chain_kernel<TX, TO, D, NW>), dim3((unsigned)((long long)a.s.n_seq * a.nvh * SL)), dim3(64 * (NW + 1)), 0, st, a, w);
+  hipLaunchKernelGGL((chain_kernel<TX, TO, D, NW>), dim3((unsigned)((long long)a.s.n_seq * a.nvh * SL)), dim3(64 * (Chain<TX, TO, D, NW>::SPLIT ? 2 * NW + 1 : NW + 1)), 0, st, a, w);
 }
 template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
