@@ -345,8 +345,9 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   typedef Rec<D, KL, OF> R;
   static constexpr int U = R::U, DT = D / 16, KB = R::KEY / 1024 + R::HEAD / 1024 + 1, XS = sizeof(TX), OS = sizeof(TO);
   static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
-  // Of two waves each has another one that forms its outputs, a chunk later, from S's and d's halves in LDS (f32 heads of
-  // 128 have no room for them and a fourth record).
+  // Of two waves each has another one that forms its outputs, a chunk later, from S's and d's halves in LDS: what a chunk
+  // takes is one wave's products and instructions, one after the other (8192 rows of 48 heads of 128 in bf16: 312 us, with
+  // the outputs among them 341).  f32 heads of 128 have no room for that and a fourth record.
   static constexpr bool SPLIT = NW == 2 && (XS == 2 || D == 64);
   static constexpr int HALVES = OF ? 2 : 1, EX = HALVES * (U + 1) * 1024 + 512, NV = SPLIT ? 4 : 3;
   typedef char Buf[R::KEY + R::HEAD];
@@ -907,8 +908,8 @@ template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, con
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
   hipLaunchKernelGGL((prep_kernel<TX, D, full_out<TX, TO>()>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
   // Waves of a workgroup: the fewest with which the workgroups have a CU each.  Few waves beside each other are faster
-  // (1024 rows of 48 heads of 128 in bf16, both launches: 62 us with two, 66 with four, 85 with eight), two workgroups on
-  // a CU are not (two such sequences: 86, 77, 96).  Past that all of a head's columns: a record then comes once, and two of
+  // (1024 rows of 48 heads of 128 in bf16, both launches, before the outputs had waves of their own: 62 us with two, 66 with
+  // four, 85 with eight), two workgroups on a CU are not (two such sequences: 86, 77, 96).  Past that all of a head's columns: a record then comes once, and two of
   // the chain's waves share a SIMD (four: 142, 134, 108; 48: 1353, 1234, 1019).  Eight waves of f32 operands do not fit the
   // registers.
   constexpr int MANY = D == 128 && sizeof(TX) == 2 ? 8 : 4, CUS = 256;
