@@ -601,6 +601,73 @@ def model_step(gpu, ctx, pool, ws, h, cu, src, dst, rule, count=None, emit=True,
     return h
 
 
+def test_many_sequences(env):
+    """As many as one call takes, of no, one or a few rows; more than a wave has lanes."""
+    gpu, ctx = env
+    for S in (65, 200, 4096):
+        r = random.Random(S)
+        lens = [r.choice([0, 1, 1, 2, 3]) if S == 4096 else r.choice([0, 1, 2, 31, 33, 70]) for _ in range(S)]
+        for name in ("step", "prompt"):
+            check_rule(env, name, lens, 1, 1, 64, BF16, F32, 800 + S, first=2)
+        g, T = gen(S), sum(lens)
+        pool = gpu.GdnPool.empty(1, S, 1, 1, 64)
+        pool.hist.normal_(generator=g)
+        before, slots = pool.hist[0].double().cpu(), r.sample(range(S), S)
+        x, kw, y = randn(g, T, pool.channels), randn(g, pool.channels, 4), torch.empty(T, pool.channels, device="cuda")
+        gpu.gdn_conv(ctx, pool, 0, x, kw, y, ints(borders(lens)), ints(slots), ints(slots))
+        assert pool.take_status(ctx) == 0
+        want, bound, hist, at = torch.empty(T, pool.channels, dtype=torch.float64), torch.empty(T, pool.channels, dtype=torch.float64), before.clone(), 0
+        xc, kc = x.cpu(), kw.cpu()
+        for j, n in enumerate(lens):
+            want[at:at + n], hist[slots[j]], b = R.conv(xc[at:at + n], before[slots[j]], kc)
+            bound[at:at + n] = R.rounded(want[at:at + n], b, F32)
+            at += n
+        close(y, want, bound, ("conv", S))
+        assert torch.equal(pool.hist[0].double().cpu(), hist)
+
+
+def test_far_rows_and_slots(env):
+    """Rows and slots behind 2^31 elements: the bits of the same call on near ones."""
+    gpu, ctx = env
+    nkh, nvh, D, T, far = 16, 48, 128, 140, 2 ** 24 - 8
+    g = gen(90)
+    q, k, v, a, b, A, dt = rule_inputs(g, T, nkh, nvh, D, BF16)
+    a, b = a.contiguous(), b.contiguous()
+    big, out, gates = (torch.empty(T, far, device="cuda", dtype=t) for t in (BF16, BF16, F32))
+    place = lambda to, at, x: to[:, at:at + x[0].numel()].copy_(x.flatten(1)).unflatten(1, x.shape[1:])
+    Q, K, V = place(big, 0, q), place(big, 2048, k), place(big, 4096, v)
+    far_a, far_b = place(gates, 0, a), place(gates, 64, b)
+    O = out[:, :nvh * D].unflatten(1, (nvh, D))
+    cu = ints([0, T - 3, T])
+    near, wide = gpu.GdnPool.empty(1, 2, nkh, nvh, D), gpu.GdnPool.empty(2, 1400, nkh, nvh, D)
+    assert (T - 1) * far > 2 ** 31 and 2799 * nvh * D * D > 2 ** 31
+    for call in (gpu.gdn_prompt, gpu.gdn_step):
+        near.state.normal_(generator=g)
+        wide.state[1, [3, 1399]] = near.state[0]
+        o = torch.empty(T, nvh, D, device="cuda", dtype=BF16)
+        call(ctx, near, 0, q.contiguous(), k.contiguous(), v.contiguous(), a, b, o, cu, ints([0, 1]), ints([0, 1]), A, dt)
+        call(ctx, wide, 1, Q, K, V, far_a, far_b, O, cu, ints([3, 1399]), ints([3, 1399]), A, dt)
+        assert torch.equal(o, O) and torch.equal(near.state[0], wide.state[1, [3, 1399]])
+    del gates
+    x, kw = big[:, :near.channels], randn(g, near.channels, 4)
+    y = torch.empty(T, near.channels, device="cuda", dtype=BF16)
+    gpu.gdn_conv(ctx, near, 0, x.contiguous(), kw, y, cu, None, ints([0, 1]))
+    gpu.gdn_conv(ctx, wide, 1, x, kw, out[:, :near.channels], cu, None, ints([3, 1399]))
+    assert torch.equal(y, out[:, :near.channels]) and torch.equal(near.hist[0], wide.hist[1, [3, 1399]])
+    V, tok = 100003, ints([7, 1, 100002] * 47)[:T]
+    x = out[:, 64:64 + V]
+    x.normal_(generator=g)
+    res = []
+    for z in (x, x.contiguous()):
+        lp, H, ids = torch.empty(T, device="cuda"), torch.empty(T, device="cuda"), torch.empty(T, 5, device="cuda", dtype=torch.int32)
+        gpu.logprobs(ctx, z, tok, lp, entropy=H, top_ids=ids)
+        res.append((lp, H, ids))
+    assert torch.equal(res[0][2], res[1][2])
+    z = torch.log_softmax(x.double(), 1)
+    for lp, H, _ in res:                                   # (sums split by the rows' alignment)
+        close(lp, z[torch.arange(T, device="cuda"), tok.long()], R.logprobs_bound(V, V // 256 + 32, z[torch.arange(T, device="cuda"), tok.long()]).cpu(), "far")
+
+
 def test_requests_from_prompt_to_answer(env):
     """Two layers and a head over packed requests: prompts, a fork, drafted chains scored and kept, log probabilities; the
     same tokens as one prompt give the same answers."""
