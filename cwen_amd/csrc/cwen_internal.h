@@ -498,7 +498,7 @@ struct GdnRuleArgs {
 };
 int gdn_step_launch(int xtype, int otype, int D, const GdnRuleArgs &a, hipStream_t st);
 int gdn_prompt_launch(int xtype, int otype, int D, const GdnRuleArgs &a, void *work, hipStream_t st);
-size_t gdn_prompt_bytes(int xtype, int otype, int D, int nkh, int nvh, int n_seq, int total);
+size_t gdn_prompt_bytes(int xtype, int D, int nkh, int nvh, int n_seq, int total);
 
 // ------------------------------------------------------------ logprobs.hip
 struct LogprobArgs {

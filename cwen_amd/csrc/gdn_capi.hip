@@ -121,7 +121,7 @@ int cwen_gdn_prompt_work(const cwen_gdn_pool *pool, int xtype, int otype, int n_
   if (rc) return rc;
   if (!elem_size(xtype) || !elem_size(otype)) return CWEN_ETYPE;
   if (n_seq < 0 || n_seq > CWEN_GDN_SEQ_MAX || total < 0 || total >= 1 << 30) return CWEN_EINVAL;
-  if (n_seq) *bytes = gdn_prompt_bytes(xtype, otype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
+  if (n_seq) *bytes = gdn_prompt_bytes(xtype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
   return CWEN_OK;
 }
 
@@ -137,7 +137,7 @@ int cwen_gdn_prompt(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xty
   // (the second launch has up to 640 threads a sequence and head)
   if (gdn_pieces(total, n_seq, 32) * pool->nvh * 2 >= launch_max || (long long)n_seq * pool->nvh * 4 >= launch_max) return CWEN_EINVAL;
   if (total > 1 && (v_ts >= 1 << 24 || (o && o_ts >= 1 << 24))) return CWEN_EINVAL;      // a chunk's rows by 32-bit offsets
-  const size_t need = gdn_prompt_bytes(xtype, otype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
+  const size_t need = gdn_prompt_bytes(xtype, pool->dk, pool->nkh, pool->nvh, n_seq, total);
   if (need && (!work || ((uintptr_t)work & 255u))) return CWEN_EINVAL;
   if (work_bytes < need) return CWEN_ESCRATCH;
   OnDevice dev(ctx->device);

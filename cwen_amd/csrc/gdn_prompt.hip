@@ -35,24 +35,19 @@ constexpr int N = 32;                       // rows of a chunk
 
 // A chunk's record of a key head: K hi [, K lo], Q hi [, Q lo] as operands:
 // row 16 mt + m, dims 32 u + 4 g + j and 32 u + 16 + 4 g + j (j < 4) at half
-// ((mt U + u) 64 + 16 g + m) 8, U = D / 32.  Of a value head: T hi, T lo, A hi
-// [, A lo] as operands (rows mt, the chunk's rows as dims), then the factors.
-template <int D, bool KL, bool OF> struct Rec {
+// ((mt U + u) 64 + 16 g + m) 8, U = D / 32.  Of a value head: T hi, T lo, A hi,
+// A lo as operands (rows mt, the chunk's rows as dims), then the factors.
+template <int D, bool KL> struct Rec {
   static constexpr int U = D / 32;
   static constexpr int OP = N * D * 2;                       // bytes of an operand
   static constexpr int K = 0, KLO = OP, Q = KL ? 2 * OP : OP, QLO = 3 * OP, KEY = KL ? 4 * OP : 2 * OP;
-  static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = OF ? 8192 : 6144, HEAD = F + 512;
+  static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = 8192, HEAD = F + 512;
 };
 // The factors: per row e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31 (beta is in T's columns).  The scores
 // and the last of the rows' factors are in units of O_UNIT, so that the low halves of small scores are no
 // subnormals, and without 1 / sqrt(D).
 constexpr float O_UNIT = 1.f / 64;
 enum { F_X = 0, F_D = 32, F_O = 64, F_END = 96 };
-
-// Whether the outputs are formed with both halves of S, A and d.  Single ones are
-// off by 2^-12 of S, A and d: beside the rounding to bf16 (2^-9) that does not show,
-// beside the one to f16 it would.
-template <typename TX, typename TO> constexpr bool full_out() { return sizeof(TX) == 4 || !std::is_same<TO, TypeBF16::elem>::value; }
 
 struct PromptWork {
   char *key, *head;          // [piece][key head], [piece][value head]
@@ -77,9 +72,9 @@ __device__ __forceinline__ int value_head(const GdnRuleArgs &a, int hk, int r) {
 // TB/s).
 constexpr int PREP_WAVES = 4;
 
-template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {
+template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {
   constexpr bool KL = sizeof(TX) == 4;
-  typedef Rec<D, KL, OF> R;
+  typedef Rec<D, KL> R;
   constexpr int U = R::U, GS = 33, LS = N, HEADS = 4, HB = R::F + 64;     // HEADS value heads at a time, two a wave
   constexpr int BYTES = R::KEY > HEADS * HB ? R::KEY : HEADS * HB;
   // First K and Q; then, for a head, the rows of L (read 4 floats at a time), then its T hi, T lo, A operands.
@@ -294,7 +289,7 @@ template <typename TX, int D, bool OF> __global__ __launch_bounds__(64 * PREP_WA
       const int at = operand_at(i, n, 1);
       const _Float16 x = f16_of(A[i]);
       op[R::A / 2 + at] = x;
-      if (OF) op[R::ALO / 2 + at] = f16_of(A[i] - (float)x);
+      op[R::ALO / 2 + at] = f16_of(A[i] - (float)x);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (hv >= 0) {
@@ -342,15 +337,15 @@ __device__ __forceinline__ half8_t high8(const float (&x)[8]) {
 }
 
 template <typename TX, typename TO, int D, int NW> struct Chain {
-  static constexpr bool KL = sizeof(TX) == 4, OF = full_out<TX, TO>();
-  typedef Rec<D, KL, OF> R;
+  static constexpr bool KL = sizeof(TX) == 4;
+  typedef Rec<D, KL> R;
   static constexpr int U = R::U, DT = D / 16, KB = R::KEY / 1024 + R::HEAD / 1024 + 1, XS = sizeof(TX), OS = sizeof(TO);
   static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
   // Of two waves each has another one that forms its outputs, a chunk later, from S's and d's halves in LDS: what a chunk
   // takes is one wave's products and instructions, one after the other (8192 rows of 48 heads of 128 in bf16: 312 us, with
   // the outputs among them 341).  f32 heads of 128 have no room for that and a fourth record.
   static constexpr bool SPLIT = NW == 2 && (XS == 2 || D == 64);
-  static constexpr int HALVES = OF ? 2 : 1, EX = HALVES * (U + 1) * 1024 + 512, NV = SPLIT ? 4 : 3;
+  static constexpr int EX = 2 * (U + 1) * 1024 + 512, NV = SPLIT ? 4 : 3;
   typedef char Buf[R::KEY + R::HEAD];
 
   int lane, n, g;
@@ -518,7 +513,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       split8(x, hi[u], lo[u]);
       if (SPLIT) {
         *(half8_t *)(ex + (u * 64 + lane) * 16) = hi[u];
-        if (OF) *(half8_t *)(ex + ((U + 1 + u) * 64 + lane) * 16) = lo[u];
+        *(half8_t *)(ex + ((U + 1 + u) * 64 + lane) * 16) = lo[u];
       }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) X[mt] = mma(K[mt * U + u], lo[u], X[mt]);
@@ -549,7 +544,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
-          if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+          Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
           if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
         }
     __builtin_amdgcn_sched_barrier(0);
@@ -569,7 +564,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       for (int mt = 0; mt < 2; ++mt) {
         fo[mt] = rows4(F_O, mt);
         A[mt] = op(R::KEY + R::A, mt);
-        if (OF) AL[mt] = op(R::KEY + R::ALO, mt);
+        AL[mt] = op(R::KEY + R::ALO, mt);
       }
     };
     if (NW <= 2 && !SPLIT) ask_a();
@@ -629,13 +624,12 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
         x[e] = at(e) < clear ? x[e] : 0.f;
         if (at(e) >= clear) Y[e >> 2][e & 3] = NAN;
       }
-      oh = high8(x);
     }
-    if (OF) split8(x, oh, ol);
+    split8(x, oh, ol);
     if constexpr (SPLIT) {
       *(half8_t *)(ex + (U * 64 + lane) * 16) = oh;
-      if (OF) *(half8_t *)(ex + ((2 * U + 1) * 64 + lane) * 16) = ol;
-      *(float2 *)(ex + HALVES * (U + 1) * 1024 + lane * 8) = make_float2(unit_here, __builtin_bit_cast(float, clear));
+      *(half8_t *)(ex + ((2 * U + 1) * 64 + lane) * 16) = ol;
+      *(float2 *)(ex + 2 * (U + 1) * 1024 + lane * 8) = make_float2(unit_here, __builtin_bit_cast(float, clear));
       return;
     }
 #pragma unroll
@@ -643,8 +637,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       floatx4_t y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = fo[mt][i] * Y[mt][i];
-      y = mma(A[mt], oh, y);
-      if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
+      y = mma(A[mt], ol, mma(AL[mt], oh, mma(A[mt], oh, y)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (unit_here * out_unit));
     }
@@ -663,7 +656,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       hi[u] = op(ex, u);
-      if (OF) lo[u] = op(ex, U + 1 + u);
+      lo[u] = op(ex, U + 1 + u);
     }
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
@@ -674,18 +667,18 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     for (int mt = 0; mt < 2; ++mt) {
       fo[mt] = *(const floatx4_t *)(F + F_O + 16 * mt + 4 * g);
       A[mt] = op(b + R::KEY + R::A, mt);
-      if (OF) AL[mt] = op(b + R::KEY + R::ALO, mt);
+      AL[mt] = op(b + R::KEY + R::ALO, mt);
     }
     oh = op(ex, U);
-    if (OF) ol = op(ex, 2 * U + 1);
-    const float2 column = *(const float2 *)(ex + HALVES * (U + 1) * 1024 + lane * 8);       // its unit; its first row that is not finite
+    ol = op(ex, 2 * U + 1);
+    const float2 column = *(const float2 *)(ex + 2 * (U + 1) * 1024 + lane * 8);       // its unit; its first row that is not finite
     const int clear = __builtin_bit_cast(int, column.y);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         Y[mt] = mma(Q[mt * U + u], hi[u], Y[mt]);
-        if (OF) Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
+        Y[mt] = mma(Q[mt * U + u], lo[u], Y[mt]);
         if (KL) Y[mt] = mma(QL[mt * U + u], hi[u], Y[mt]);
       }
 #pragma unroll
@@ -693,8 +686,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
       floatx4_t y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = 16 * mt + i < clear ? fo[mt][i] * Y[mt][i] : NAN;
-      y = mma(A[mt], oh, y);
-      if (OF) y = mma(A[mt], ol, mma(AL[mt], oh, y));
+      y = mma(A[mt], ol, mma(AL[mt], oh, mma(A[mt], oh, y)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) ((TO *)s_io)[(16 * mt + 4 * g + i) * 16 + n] = (TO)(y[i] * (column.x * out_unit));
     }
@@ -891,14 +883,10 @@ void chain_kernel(GdnRuleArgs a, PromptWork w) {
   }
 }
 
-template <bool KL, bool OF> void sizes(int D, size_t *key, size_t *head) {
-  *key = D == 128 ? Rec<128, KL, OF>::KEY : Rec<64, KL, OF>::KEY;
-  *head = Rec<128, KL, OF>::HEAD;
-}
-void sizes_of(int xtype, int otype, int D, size_t *key, size_t *head) {
-  if (xtype == CWEN_T_F32) sizes<true, true>(D, key, head);
-  else if (otype == CWEN_T_BF16) sizes<false, false>(D, key, head);
-  else sizes<false, true>(D, key, head);
+void sizes_of(int xtype, int D, size_t *key, size_t *head) {
+  if (xtype == CWEN_T_F32) *key = D == 128 ? Rec<128, true>::KEY : Rec<64, true>::KEY;
+  else *key = D == 128 ? Rec<128, false>::KEY : Rec<64, false>::KEY;
+  *head = Rec<128, true>::HEAD;             // of every form
 }
 
 template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
@@ -907,7 +895,7 @@ template <typename TX, typename TO, int D, int NW> void launch_chain(const GdnRu
 }
 template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, const PromptWork &w, hipStream_t st) {
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
-  hipLaunchKernelGGL((prep_kernel<TX, D, full_out<TX, TO>()>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
+  hipLaunchKernelGGL((prep_kernel<TX, D>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
   // Waves of a workgroup: the fewest with which the workgroups have a CU each.  Few waves beside each other are faster
   // (1024 rows of 48 heads of 128 in bf16, both launches, before the outputs had waves of their own: 62 us with two, 66 with
   // four, 85 with eight), two workgroups on a CU are not (two such sequences: 86, 77, 96).  Past that all of a head's columns: a record then comes once, and two of
@@ -931,15 +919,15 @@ template <typename TX> void launch_o(int otype, int D, const GdnRuleArgs &a, con
 
 }  // namespace
 
-size_t gdn_prompt_bytes(int xtype, int otype, int D, int nkh, int nvh, int n_seq, int total) {
+size_t gdn_prompt_bytes(int xtype, int D, int nkh, int nvh, int n_seq, int total) {
   size_t key, head;
-  sizes_of(xtype, otype, D, &key, &head);
+  sizes_of(xtype, D, &key, &head);
   return (size_t)gdn_pieces(total, n_seq, N) * (nkh * key + nvh * head);
 }
 
 int gdn_prompt_launch(int xtype, int otype, int D, const GdnRuleArgs &a, void *work, hipStream_t st) {
   size_t key, head;
-  sizes_of(xtype, otype, D, &key, &head);
+  sizes_of(xtype, D, &key, &head);
   const PromptWork w = {(char *)work, (char *)work + (size_t)gdn_pieces(a.s.total, a.s.n_seq, N) * a.nkh * key};
   if (xtype == CWEN_T_F32) launch_o<float>(otype, D, a, w, st);
   else if (xtype == CWEN_T_F16) launch_o<TypeF16::elem>(otype, D, a, w, st);
