@@ -1,0 +1,29 @@
+"""The bounds of the chunked delta rule reject an operand that has lost its low half: a model of the chunks' products on the CPU."""
+import pytest
+
+import gdn_chunks as G
+
+SIZES = [(1, 1, 2, 64), (33, 1, 2, 128), (100, 2, 4, 64), (257, 1, 3, 128), (600, 1, 2, 64)]
+
+
+@pytest.fixture(scope="module", params=SIZES, ids=lambda s: "x".join(map(str, s)))
+def prompt(request):
+    x = G.inputs(*request.param, seed=request.param[0])
+    return (request.param[0], x, *G.reference(*x))
+
+
+def test_two_halves_are_well_within_the_bounds(prompt):
+    n, x, want, limits = prompt
+    o, s = G.share(G.chunks(*x), want, limits)
+    assert o < 0.2 and s < 0.2, (o, s)
+
+
+@pytest.mark.parametrize("name", G.OPERANDS)
+def test_a_single_half_is_far_outside(prompt, name):
+    """In the outputs (the rows before the state enter those of later chunks only), and in the state where it enters that."""
+    n, x, want, limits = prompt
+    o, s = G.share(G.chunks(*x, single=(name,)), want, limits)
+    if name != "y" or n > G.N:
+        assert o > 3, o
+    if name in ("r", "T", "y", "K"):
+        assert s > 3, s
