@@ -21,8 +21,10 @@
 // Precision: f32 values enter a product as two f16 values, x s = hi + lo with a
 // power of two s per column: 22 bits, and down to 2^-25 of a unit.  The unit is
 // taken anew, the larger of |S| and |v| at 1 .. 2, every 8 chunks and whenever a
-// chunk's largest |v| is outside 1/8 .. 16 units; so |S^T k|, r and d (|S| grows by
-// the rows' |v| at most) stay below 2^14.  Keys and queries of 16 bits are exact
+// chunk's largest |v| is outside 1/8 .. 16 units.  A row lengthens a column of S by
+// beta |v| < 32 units at most, from 2 sqrt(D) before the 9 chunks that a unit can have
+// to go through: |S|, |S^T k| and r stay below 9300 units, d = beta (v - S^T k) below
+// 18600, and with rho below 37200, where f16 ends at 65504.  Keys and queries of 16 bits are exact
 // f16 values after a power of two; what is left of their length (rho, 1 .. 2) goes into
 // the rows' factors.  f32 ones are normalised and split.
 #include <math.h>
@@ -486,8 +488,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) fx[mt] = rows4(F_X, mt);
     // The present values in units, and whether the next ones call for new units in the chunks to come: at least every
-    // 8, and where their |v| leaves what the present one is good for.  In between |S| grows by the rows' |v| < 16 units
-    // at most.
+    // 8, and where their |v| leaves what the present one is good for.
     float w[8], ratio = 1.f;
     const float vmax_here = vmax, unit_here = unit;
 #pragma unroll

@@ -64,7 +64,7 @@ def _unit(x):
     return torch.exp2(torch.floor(torch.log2(x.clamp(min=2.0 ** -120))))
 
 
-def bounds(g, m):
+def bounds(g, m, wider=1, linear=0):
     """Of each output [n, H, D] and of the state's columns' lengths [H, D], for keys, queries, values and gates that are
     independent of each other; g the log decays, m the largest of a column's |state| + |v| in a row's chunk and the one before.
 
@@ -75,15 +75,19 @@ def bounds(g, m):
     they let it decay, and errors of independent signs add as their squares.  The largest of the columns may be twice that.
     An output has the state's error along q, and its own: S and q, and the 32 terms of the scores times x, from two operands
     each.  Queries have no direction in common with keys or errors: a product with one of length 1 is 1 / sqrt(D), 4 / sqrt(D)
-    among all the outputs."""
+    among all the outputs.
+
+    `wider`: those errors that many times over; `linear`: besides, an error of that many 2^-22 m a row that is the same in
+    every row, so that rows' errors add up."""
     n, D = m.shape[0], m.shape[2]
     e = 2.0 ** -22 * m
     fall = torch.exp(2 * g.double())[..., None]
-    square, before = torch.zeros_like(e[0]), torch.empty_like(e)
+    square, line, before = torch.zeros_like(e[0]), torch.zeros_like(e[0]), torch.empty_like(e)
     for t in range(n):
-        square = square * fall[t] + 8 * e[t] ** 2
-        before[t] = square
-    return 4 / math.sqrt(D) * (before.sqrt() + math.sqrt(2 * N + 4) * e) / math.sqrt(D), 2 * square.sqrt()
+        square = square * fall[t] + 8 * (wider * e[t]) ** 2
+        line = line * fall[t].sqrt() + linear * e[t]
+        before[t] = square.sqrt() + line
+    return 4 / math.sqrt(D) * (before + wider * math.sqrt(2 * N + 4) * e) / math.sqrt(D), 2 * square.sqrt() + line
 
 
 def share(got, want, limits):
@@ -99,7 +103,7 @@ def inputs(n, nkh, nvh, D, seed, dtype=torch.float32):
     return q, k, v, -torch.exp(1.5 * r(n, nvh) - 3), torch.sigmoid(r(n, nvh)), 0.2 * r(nvh, D, D)
 
 
-def reference(q, k, v, g, beta, S, key_head="mod"):
+def reference(q, k, v, g, beta, S, key_head="mod", wider=1, linear=0):
     """(outputs, end state) in 64 bits, and the bounds of both."""
     n, H, D = v.shape
     S = torch.zeros(H, D, D, dtype=torch.float64) if S is None else S.double()
@@ -111,4 +115,30 @@ def reference(q, k, v, g, beta, S, key_head="mod"):
         size[t] = torch.maximum(before, S.norm(dim=1)) + v[t].double().abs()
     m = torch.stack([size[c:c + N].amax(0) for c in range(0, n, N)])
     m[1:] = torch.maximum(m[1:], m[:-1])
-    return (o, S), bounds(g, m.repeat_interleave(N, 0)[:n])
+    return (o, S), bounds(g, m.repeat_interleave(N, 0)[:n], wider, linear)
+
+
+def long_betas(kind, n, H, D, seed, dtype=torch.float32):
+    """Inputs with betas above 1, and how far the bounds of `bounds` widen (wider, linear).  With keys that are independent
+    d's errors, and T's besides, grow by a beta each: 4 times.
+
+    With one key for all rows T's entries are 4 in every row: a row's d has errors of 32 of them and of as many right hand sides,
+    sqrt(2 * 32) * 4 2^-22 M, where the bounds count sqrt(8) 2^-22 M: 12 times.  And errors of sums that are alike in every row
+    add up: the key's length is off by up to 4 * 2^-24 (a sum, a root, a quotient, a product), which enters d and y, times beta
+    each: 4 2^-22 M; the sum T r has partial sums of 8 M (its terms of 4 M alternate), and a matrix instruction's adds of its 32
+    terms, 8 of 4 at a time, may each cut 2^-23 of that off: 8 * 8 / 2 = 32 2^-22 M.  The value's sign alternates there, so that the
+    state grows by two values a row, and the values grow to 16 units of their column right after the unit was chosen."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g)
+    q, k, v = r(n, H, D).to(dtype), r(n, H, D).to(dtype), r(n, H, D)
+    gate, beta = torch.zeros(n, H), torch.full((n, H), 1.5 if kind == "1.5" else 2.0)
+    if kind in ("2", "1.5"):
+        gate = -torch.exp(1.5 * r(n, H) - 3)
+        return (q, k, v.to(dtype), gate, beta, 0.2 * r(H, D, D)), dict(wider=4)
+    k.zero_()
+    k[:, :, 5] = 1.0078125                   # of length 1.98 in powers of two
+    if kind == "spread":
+        k.copy_(r(1, H, D).to(dtype).expand_as(k))
+    t = torch.arange(n)[:, None, None]
+    v = (1 + 0.2 * torch.rand(1, H, D, generator=g)) * torch.where(t < 9 * N, 1.0, 13 * (1 - 2.0 * (t % 2)))
+    return (q, k, v.to(dtype), gate, beta, torch.zeros(H, D, D)), dict(wider=12, linear=36)

@@ -27,3 +27,13 @@ def test_a_single_half_is_far_outside(prompt, name):
         assert o > 3, o
     if name in ("r", "T", "y", "K"):
         assert s > 3, s
+
+
+@pytest.mark.parametrize("kind", ["2", "1.5", "one", "spread"])
+def test_betas_above_one(kind):
+    """The model's operands stay below f16's largest value, and the errors within the wider bounds."""
+    for n, H, D in ((16 * G.N + 20, 2, 64), (75, 1, 128)):
+        x, wider = G.long_betas(kind, n, H, D, n)
+        want, limits = G.reference(*x, **wider)
+        o, s = G.share(G.chunks(*x), want, limits)
+        assert o < 0.5 and s < 0.5, (o, s)

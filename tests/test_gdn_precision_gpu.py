@@ -2,6 +2,7 @@
 import pytest
 
 import gdn_chunks as G
+import gdn_ref as R
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,35 @@ def test_the_outputs_type_only_rounds_them(env, tx, to):
         assert torch.equal(s, t), (lens, nvh, D)
         far = (p.double() - o.double()).abs() - o.double().abs() * (torch.finfo(to).eps / 2 + 2.0 ** -24)
         assert far.max() <= (2.0 ** -25 if to == F16 else 0), (lens, nvh, D, far.max(), int((far > 0).sum()), "of", far.numel())
+
+
+@pytest.mark.parametrize("tx", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["2", "1.5", "one", "spread"])
+def test_betas_above_one(env, kind, tx):
+    """Betas to 2, where the state grows by two values a row: prompts in every launch width, and steps."""
+    gpu, ctx = env
+    for n, S, H, D in ((16 * G.N + 20, 1, 2, 128), (16 * G.N + 20, 3, 20, 64), (16 * G.N + 20, 40, 2, 128), (16 * G.N + 20, 70, 2, 128),
+                       (10 * G.N, 70, 2, 64)):
+        x, wider = G.long_betas(kind, n, H, D, n + D, tx)
+        want, limits = G.reference(*x, **wider)
+        _, _, M = R.rule(*x[:3], x[3].double(), x[4].double(), x[5])
+        q, k, v, a, b = (t.cuda().repeat(S, *[1] * (t.dim() - 1)) for t in x[:5])
+        cu, slots = ints(borders([n] * S)), ints(list(range(S)))
+        for call in (gpu.gdn_prompt, gpu.gdn_step):
+            pool = gpu.GdnPool.empty(1, S, H, H, D)
+            pool.state[0] = x[5].cuda()
+            o = torch.empty(S * n, H, D, device="cuda")
+            call(ctx, pool, 0, q, k, v, a, b, o, cu, slots, slots)
+            assert pool.take_status(ctx) == 0
+            for i in range(S):
+                got = o[i * n:(i + 1) * n], pool.state[0, i]
+                assert i == 0 or all(torch.equal(x, y) for x, y in zip(got, first)), (call.__name__, i)
+                first = got
+            got = [t.cpu() for t in first]
+            worst = G.share(got, want, limits)
+            print(call.__name__, kind, tx, n, H, D, worst, flush=True)
+            if call is gpu.gdn_prompt:
+                assert max(worst) < 1, (n, D, worst)
+            else:
+                eo, es = R.step_bounds(n, D, M, F32)
+                assert bool(((got[0] - want[0]).abs() <= eo).all()) and bool(((got[1] - want[1]).abs() <= es[:, None]).all()), (n, D)
