@@ -17,10 +17,11 @@
 #include <math.h>
 #include <algorithm>
 #include "cwen_internal.h"
+#include "logprobs_table.h"
 
 namespace {
 
-constexpr int THREADS = 256, WAVES = 4, LIST = CWEN_LOGPROBS_TOP, SPLITS = 64;
+constexpr int THREADS = LP_THREADS, WAVES = 4, SPLITS = LP_SPLITS;
 constexpr float LAG = 8.f, LOG2E = 1.44269504088896340736f;
 constexpr int NONE = 0x7fffffff;            // index of a list entry that is none
 
@@ -187,11 +188,6 @@ struct Most {
 // Words of one part's result: m, s, t, count, then the list.
 __host__ __device__ constexpr int part_words(int top) { return 4 + 2 * ((top + 1) & ~1); }
 
-struct Split {
-  int n;              // parts of a row
-  int vecs;           // 16-byte pieces of a part
-};
-
 __device__ __forceinline__ void finish(const LogprobArgs &a, int row, Sums r, int before_it, float xt, Entry e) {
   const int lane = threadIdx.x & 63;
   const float ls = (float)log((double)r.s);
@@ -215,8 +211,8 @@ template <typename T> __device__ __forceinline__ float token_logit(const Logprob
 }
 
 // TOP: 0 no largest logits are wanted, 1 one, 2 more.  RANK: whether ranks are.
-template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) void part_kernel(LogprobArgs a, Split sp) {
-  constexpr int E = 16 / sizeof(T), VECS = 16 / E;      // 16 logits at a time
+template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) void part_kernel(LogprobArgs a, lp_split sp) {
+  constexpr int E = 16 / sizeof(T), VECS = LP_LOGITS / E;
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
   __shared__ float s_qv[WAVES][128], s_sums[WAVES][3];
   __shared__ int s_qi[WAVES][128], s_cnt[WAVES];
@@ -252,7 +248,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
     if (RANK) cnt += in && v >= (i < tok ? xt : above) ? 1 : 0;
     if (TOP) best.offer(v, in ? i : NONE);
   };
-  const int v0 = part * sp.vecs, v1 = min(nvec, v0 + sp.vecs);
+  const int v0 = part * sp.vecs, v1 = part == sp.n - 1 ? nvec : min(nvec, v0 + sp.vecs);
   if (part == 0) one((int)threadIdx.x < head ? (float)x[threadIdx.x] : 0.f, threadIdx.x, (int)threadIdx.x < head);
   const int tokvec = RANK ? (tok - head) / E : 0;               // (a token in front of the pieces: one of piece 0 or none)
   int u = v0;
@@ -376,24 +372,14 @@ template <typename T> __global__ __launch_bounds__(THREADS) void join_kernel(Log
   finish(a, row, r, cnt, xt, l);
 }
 
-// Parts of a row: three workgroups a CU together (96 rows of bf16, top 20: 38 us; two or four a CU 40 to 44: a wave's first
-// list costs it 1 us), but two turns of the loop each (one f32 row: 31 parts 19 us, 61 parts 21, the join taking longer), in
-// whole turns (what is left over goes piece by piece).
-Split split_of(int rows, int V, int E) {
-  const int turn = THREADS * 16 / E, most = std::max(1, std::min({SPLITS, 768 / std::max(rows, 1), V / 8192}));
-  int vecs = std::max(1, (V / E + most * turn / 2) / (most * turn)) * turn;
-  while ((V / E + vecs - 1) / vecs > SPLITS) vecs += turn;
-  return {std::max(1, (V / E + vecs - 1) / vecs), vecs};
-}
-
-template <typename T, int TOP> void launch_parts(const LogprobArgs &a, const Split &sp, hipStream_t st) {
+template <typename T, int TOP> void launch_parts(const LogprobArgs &a, const lp_split &sp, hipStream_t st) {
   const dim3 grid((unsigned)(a.rows * sp.n));
   if (a.rank) hipLaunchKernelGGL((part_kernel<T, TOP, true>), grid, dim3(THREADS), 0, st, a, sp);
   else hipLaunchKernelGGL((part_kernel<T, TOP, false>), grid, dim3(THREADS), 0, st, a, sp);
 }
 template <typename T> void launch(const LogprobArgs &a, hipStream_t st) {
   constexpr int E = 16 / sizeof(T);
-  const Split sp = split_of(a.rows, a.V, E);
+  const lp_split sp = lp_divide(a.rows, a.V, E);
   const int n = sp.n;
   if (a.top == 0) launch_parts<T, 0>(a, sp, st);
   else if (a.top == 1) launch_parts<T, 1>(a, sp, st);
@@ -404,7 +390,7 @@ template <typename T> void launch(const LogprobArgs &a, hipStream_t st) {
 }  // namespace
 
 size_t logprobs_bytes(int rows, int V, int top) {
-  const int n = std::max(split_of(rows, V, 4).n, split_of(rows, V, 8).n);
+  const int n = std::max(lp_divide(rows, V, 4).n, lp_divide(rows, V, 8).n);
   return n > 1 ? (size_t)rows * n * part_words(top) * sizeof(float) : 0;
 }
 

@@ -1,0 +1,57 @@
+"""Log probabilities on the GPU where rows are cut into parts."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def env():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from cwen_amd import gpu
+    ctx = gpu.Context(0)
+    yield gpu, ctx
+    torch.cuda.synchronize()
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def run(env, x, tok, top):
+    gpu, ctx = env
+    rows = x.shape[0]
+    f, i = (lambda *s: torch.empty(s, device="cuda")), (lambda *s: torch.empty(s, device="cuda", dtype=torch.int32))
+    out = {"logprob": f(rows), "rank": i(rows), "entropy": f(rows), "lse": f(rows), "top_ids": i(rows, top), "top_logprobs": f(rows, top)}
+    gpu.logprobs(ctx, x, tok, **out)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_in_parts(env, dtype):
+    """Vocabularies that are no whole number of turns, in one part and in several, aligned or not: every logit counts once (in
+    the ranks).  Tokens stand at the ends of parts; logits are multiples of 1/8, so that there are ties."""
+    for j, (rows, V) in enumerate(((1, 20000), (1, 50257), (3, 151936), (7, 16385), (300, 50257), (200, 32003), (385, 20001), (500, 50257))):
+        for gap in (0, 3):
+            g = gen(10 * j + gap)
+            x = torch.randint(-40, 41, (rows, V + gap), device="cuda", generator=g).float().div(8).to(dtype)[:, gap:]
+            tok = torch.randint(0, V, (rows,), device="cuda", generator=g)
+            ends = torch.tensor([0, V - 1, V // 2, 4095, 4096, 8191, 8192, 12288], device="cuda")
+            tok[::2] = ends[torch.arange(tok[::2].numel(), device="cuda") % 8]
+            x[1::3, V - 1] = 6
+            out = run(env, x, tok.int(), 20)
+            z, r = torch.log_softmax(x.double(), 1), torch.arange(rows, device="cuda")
+            xt, at = x[r, tok][:, None], torch.arange(V, device="cuda")[None]
+            assert torch.equal(out["rank"].long(), ((x > xt) | ((x == xt) & (at < tok[:, None]))).sum(1)), (rows, V, gap)
+            order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :20]
+            assert torch.equal(out["top_ids"].long(), order), (rows, V, gap)
+            # a thread adds up to V / 256 terms, each sum off by 2^-24; fewer than 100 roundings more; |x - m| <= 11 in the entropy's sum
+            bound = 2.0 ** -24 * (V / 256 + 100)
+            for name, want in (("logprob", z[r, tok]), ("lse", torch.logsumexp(x.double(), 1)), ("top_logprobs", torch.gather(z, 1, order))):
+                assert (out[name].double() - want).abs().max() <= bound + 2.0 ** -23 * want.abs().max(), (rows, V, gap, name)
+            H = -(torch.exp(z) * z).sum(1)
+            assert (out["entropy"].double() - H).abs().max() <= 12 * bound, (rows, V, gap)

@@ -1,0 +1,64 @@
+"""How the log probabilities' rows are cut into parts, without a GPU."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+from cwen_amd import gpu
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def run_c(tmp_path, text):
+    src = tmp_path / "t.c"
+    src.write_text('#include <limits.h>\n#include <stdio.h>\n#include "logprobs_table.h"\n'
+                   '#define CHECK(x) do { if (!(x)) { printf("line %d: %s\\n", __LINE__, #x); return 1; } } while (0)\n' + text)
+    for cc in (["gcc", "-std=c11", "-fsanitize=undefined", "-fno-sanitize-recover"], ["g++", "-std=c++17", "-x", "c++"]):
+        subprocess.run([*cc, "-O1", "-Wall", "-Wextra", "-Wno-unused-function", f"-I{ROOT / 'cwen_amd' / 'csrc'}", "-o", str(tmp_path / "t"), str(src)],
+                       check=True)
+        r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True)
+        assert r.returncode == 0, r.stdout + r.stderr
+
+
+DIVISION = r"""
+static int one(int rows, int V, int E) {
+  const lp_split s = lp_divide(rows, V, E);
+  const int turn = LP_THREADS * LP_LOGITS / E, pieces = V / E, rest = pieces - (s.n - 1) * s.vecs;
+  CHECK(s.n >= 1 && s.n <= LP_SPLITS && s.vecs >= 1);
+  CHECK(s.n == 1 || (long long)s.n * rows <= LP_WORKGROUPS);      // no second round of workgroups, no join for many rows
+  CHECK(s.n == 1 || V >= 2 * 8192);
+  if (s.n > 1) {
+    CHECK(s.vecs % turn == 0);
+    CHECK(rest >= turn / 2);                                     // no part that holds next to nothing,
+    CHECK(rest < s.vecs + turn / 2);                             // nor one that holds far more than the others
+  }
+  return 0;
+}
+int main(void) {
+  static const int some[] = {1, 2, 3, 4, 7, 8, 12, 24, 48, 95, 96, 97, 128, 200, 256, 300, 383, 384, 385, 767, 768, 769, 1500, 4096, (1 << 18) - 1};
+  for (int i = 0; i < (int)(sizeof some / sizeof *some); ++i)
+    for (int E = 4; E <= 8; E += 4) {
+      for (int V = 1; V < 300000; V += 1 + V / 97)
+        if (one(some[i], V, E)) { printf("rows %d V %d E %d\n", some[i], V, E); return 1; }
+      static const int names[] = {32000, 50257, 128256, 151936, 201088, 248320, 262144, 1 << 20, (1 << 30) - 1, 1 << 30};
+      for (int j = 0; j < (int)(sizeof names / sizeof *names); ++j)
+        if (one(some[i], names[j], E)) { printf("rows %d V %d E %d\n", some[i], names[j], E); return 1; }
+    }
+  for (int rows = 1; rows < 1600; ++rows)
+    for (int E = 4; E <= 8; E += 4)
+      if (one(rows, 151936, E) || one(rows, 248320, E)) { printf("rows %d E %d\n", rows, E); return 1; }
+  return 0;
+}
+"""
+
+
+def test_division_of_rows(tmp_path):
+    run_c(tmp_path, DIVISION)
+
+
+def test_many_rows_need_no_scratch():
+    """Whatever the vocabulary: rows that fill the card have one part each."""
+    n = C.c_size_t()
+    for V in (6000, 13000, 50257, 128256, 151936, 201088, 248320, 262144):
+        for rows in (385, 768, 1500, (1 << 18) - 1):
+            assert gpu.lib().cwen_logprobs_work(rows, V, 20, C.byref(n)) == 0 and n.value == 0, (rows, V, n.value)
+        assert gpu.lib().cwen_logprobs_work(1, V, 20, C.byref(n)) == 0 and (n.value > 0) == (V > 16384), (V, n.value)
