@@ -187,6 +187,7 @@ struct Most {
 
 // Words of one part's result: m, s, t, count, then the list.
 __host__ __device__ constexpr int part_words(int top) { return 4 + 2 * ((top + 1) & ~1); }
+static_assert(LP_WORKGROUPS * part_words(CWEN_LOGPROBS_TOP) * 4 == CWEN_LOGPROBS_WORK_MAX, "scratch that serves every call");
 
 __device__ __forceinline__ void finish(const LogprobArgs &a, int row, Sums r, int before_it, float xt, Entry e) {
   const int lane = threadIdx.x & 63;

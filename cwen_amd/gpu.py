@@ -608,6 +608,7 @@ def attn_tree(ctx: Context, kv: PagedKV, layer: int, q, o, seqs, cu, max_nodes: 
 
 GDN_MOD, GDN_GROUP, GDN_ARG, GDN_SEQ_MAX = 0, 1, 1, 4096
 LOGPROBS_TOP = 64
+LOGPROBS_WORK_MAX = 768 * (16 + 8 * LOGPROBS_TOP)      # bytes of `work` that serve every logprobs call
 
 
 class GdnPoolC(C.Structure):
@@ -736,7 +737,7 @@ def _scratch(make, stream, device):
 
 
 def logprobs_work(rows: int, V: int, top: int = 0, device="cuda"):
-    """Scratch for logprobs calls of this size."""
+    """Scratch for logprobs calls of these rows, V and top (fewer rows can need more: LOGPROBS_WORK_MAX bytes serve every call)."""
     import torch
     n = C.c_size_t()
     check("cwen_logprobs_work", lib().cwen_logprobs_work(rows, V, top, C.byref(n)))
@@ -747,7 +748,7 @@ def logprobs(ctx: Context, logits, tokens=None, logprob=None, rank=None, entropy
              work=None, stream=None) -> None:
     """Log probabilities over logits [rows, vocab] (cwen_logprobs): logprob, entropy, lse float32 [rows], rank and tokens
     int32 [rows], top_ids int32 and top_logprobs float32 [rows, top], each may be None; work: a logprobs_work of this
-    size (None: allocated for the call)."""
+    size, or LOGPROBS_WORK_MAX bytes (None: allocated for the call)."""
     rows, V = logits.shape
     if logits.numel() and logits.stride(1) != 1:
         raise ValueError("a row's logits must lie in a row")

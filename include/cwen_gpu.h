@@ -322,8 +322,11 @@ int cwen_gdn_prompt_work(const cwen_gdn_pool *pool, int xtype, int otype, int n_
  * in ranks and the top.  A token outside 0..V-1, or whose logit is NaN, has
  * logprob NaN and rank -1.  Sums are f32 in a fixed order that depends on rows,
  * V and the address's alignment only.  `work`: device scratch of
- * cwen_logprobs_work's bytes, 16-byte aligned. */
+ * cwen_logprobs_work's bytes for these rows, V and top, 16-byte aligned.  More
+ * rows can need less (few rows are cut into more parts); CWEN_LOGPROBS_WORK_MAX
+ * bytes serve every call. */
 #define CWEN_LOGPROBS_TOP 64
+#define CWEN_LOGPROBS_WORK_MAX (768 * (16 + 8 * CWEN_LOGPROBS_TOP))
 int cwen_logprobs(cwen_ctx *ctx, int type, const void *logits, long long ls, int V, int rows, const int *tokens,
                   float *logprob, int *rank, float *entropy, float *lse, int top, int *top_ids, float *top_logprobs,
                   void *work, size_t work_bytes, void *stream);

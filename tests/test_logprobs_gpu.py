@@ -55,3 +55,16 @@ def test_rows_in_parts(env, dtype):
                 assert (out[name].double() - want).abs().max() <= bound + 2.0 ** -23 * want.abs().max(), (rows, V, gap, name)
             H = -(torch.exp(z) * z).sum(1)
             assert (out["entropy"].double() - H).abs().max() <= 12 * bound, (rows, V, gap)
+
+
+def test_one_scratch_for_every_call(env):
+    """Batches of all sizes with one scratch give the bits of calls with their own."""
+    gpu, ctx = env
+    x = torch.randn(500, 40000, device="cuda", generator=gen(5))
+    work = torch.empty(gpu.LOGPROBS_WORK_MAX, dtype=torch.uint8, device="cuda")
+    for rows in (500, 1, 37, 384, 385, 2, 200):
+        got = [[torch.empty(rows, device="cuda"), torch.empty(rows, 64, dtype=torch.int32, device="cuda")] for _ in range(2)]
+        for (lse, ids), w in zip(got, (work, None)):
+            gpu.logprobs(ctx, x[:rows], lse=lse, top_ids=ids, work=w)
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]), rows
+        assert torch.equal(got[0][1].long(), torch.sort(x[:rows], dim=1, descending=True, stable=True).indices[:, :64]), rows

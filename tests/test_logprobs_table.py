@@ -62,3 +62,17 @@ def test_many_rows_need_no_scratch():
         for rows in (385, 768, 1500, (1 << 18) - 1):
             assert gpu.lib().cwen_logprobs_work(rows, V, 20, C.byref(n)) == 0 and n.value == 0, (rows, V, n.value)
         assert gpu.lib().cwen_logprobs_work(1, V, 20, C.byref(n)) == 0 and (n.value > 0) == (V > 16384), (V, n.value)
+
+
+def test_scratch_that_serves_every_call():
+    """The scratch of a call is not less for fewer rows; the stated maximum covers all of them."""
+    n, most = C.c_size_t(), 0
+    for rows in [*range(1, 400), 500, 768, 769, 1500]:
+        for V in (1, 8192, 16384, 20000, 50257, 128256, 151936, 201088, 248320, 262144, 1 << 24, 1 << 30):
+            for top in (0, 1, 2, 5, 20, 63, 64):
+                assert gpu.lib().cwen_logprobs_work(rows, V, top, C.byref(n)) == 0
+                assert n.value <= 768 * (16 + 8 * (top + 1)) and n.value <= gpu.LOGPROBS_WORK_MAX, (rows, V, top, n.value)
+                most = max(most, n.value)
+    assert most == gpu.LOGPROBS_WORK_MAX
+    header = (ROOT / "include" / "cwen_gpu.h").read_text()
+    assert "#define CWEN_LOGPROBS_WORK_MAX (768 * (16 + 8 * CWEN_LOGPROBS_TOP))" in header
