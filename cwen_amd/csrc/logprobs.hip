@@ -225,7 +225,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
   const int tok = RANK ? a.tokens[row] : -1;
   // What comes before the token: from its logit on at lower indexes, from the next float on at higher ones.
   const float xt = RANK ? token_logit<T>(a, row) : NAN;
-  const float above = __builtin_bit_cast(float, xt == 0.f ? 1 : __builtin_bit_cast(int, xt) + (xt < 0.f ? -1 : 1));
+  const float above = __builtin_bit_cast(float, lp_above(__builtin_bit_cast(unsigned, xt)));
   Sums r = {-INFINITY, 0.f, 0.f};
   float ref = 0.f;                    // r.m, or 0 before there is one
   int cnt = 0;
@@ -251,7 +251,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
   };
   const int v0 = part * sp.vecs, v1 = part == sp.n - 1 ? nvec : min(nvec, v0 + sp.vecs);
   if (part == 0) one((int)threadIdx.x < head ? (float)x[threadIdx.x] : 0.f, threadIdx.x, (int)threadIdx.x < head);
-  const int tokvec = RANK ? (tok - head) / E : 0;               // (a token in front of the pieces: one of piece 0 or none)
+  const int tokvec = RANK ? lp_piece(tok, head, E) : -1;
   int u = v0;
   for (; u + THREADS * VECS <= v1; u += THREADS * VECS) {
     vec w[VECS];
@@ -274,7 +274,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
 #pragma unroll
       for (int k = 0; k < VECS; ++k) {
         const int p = u + THREADS * k + threadIdx.x;
-        const float from = p < tokvec && tok >= head ? xt : above;
+        const float from = p < tokvec ? xt : above;
 #pragma unroll
         for (int e = 0; e < E; ++e) cnt += f[k][e] >= from ? 1 : 0;
         if (p == tokvec)

@@ -1,5 +1,5 @@
-// How rows of logits are cut into parts, shared by the host and plain C++ (the
-// CPU tests compile this file alone).
+// How rows of logits are cut into parts, and what comes before a token, shared
+// by host, kernels and plain C++ (the CPU tests compile this file alone).
 #pragma once
 #if defined(__HIP__) || defined(__HIPCC__)
 #define LP_FN __host__ __device__ __forceinline__
@@ -45,3 +45,8 @@ LP_FN lp_split lp_divide(int rows, int V, int E) {
   if (s.n > 1 && pieces - (s.n - 1) * s.vecs < turn / 2) --s.n;
   return s;
 }
+
+// The piece that token `tok` lies in, where pieces of E logits begin behind `head` logits; -1 for one in front of them (or none).
+LP_FN int lp_piece(int tok, int head, int E) { return tok < head ? -1 : (tok - head) / E; }
+// The bits of the next f32 above one that is a number below +inf.
+LP_FN unsigned lp_above(unsigned bits) { return (bits & 0x7fffffffu) == 0 ? 1 : bits & 0x80000000u ? bits - 1 : bits + 1; }

@@ -13,7 +13,7 @@ def run_c(tmp_path, text):
     src.write_text('#include <limits.h>\n#include <stdio.h>\n#include "logprobs_table.h"\n'
                    '#define CHECK(x) do { if (!(x)) { printf("line %d: %s\\n", __LINE__, #x); return 1; } } while (0)\n' + text)
     for cc in (["gcc", "-std=c11", "-fsanitize=undefined", "-fno-sanitize-recover"], ["g++", "-std=c++17", "-x", "c++"]):
-        subprocess.run([*cc, "-O1", "-Wall", "-Wextra", "-Wno-unused-function", f"-I{ROOT / 'cwen_amd' / 'csrc'}", "-o", str(tmp_path / "t"), str(src)],
+        subprocess.run([*cc, "-O1", "-Wall", "-Wextra", "-Wno-unused-function", f"-I{ROOT / 'cwen_amd' / 'csrc'}", "-o", str(tmp_path / "t"), str(src), "-lm"],
                        check=True)
         r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True)
         assert r.returncode == 0, r.stdout + r.stderr
@@ -76,3 +76,30 @@ def test_scratch_that_serves_every_call():
     assert most == gpu.LOGPROBS_WORK_MAX
     header = (ROOT / "include" / "cwen_gpu.h").read_text()
     assert "#define CWEN_LOGPROBS_WORK_MAX (768 * (16 + 8 * CWEN_LOGPROBS_TOP))" in header
+
+
+PLACES = r"""
+#include <math.h>
+#include <string.h>
+static float f(unsigned b) { float x; memcpy(&x, &b, 4); return x; }
+int main(void) {
+  static const int toks[] = {INT_MIN, INT_MIN + 1, -9, -1, 0, 1, 2, 3, 4, 7, 8, 9, 4095, 4096, (1 << 30) - 1, 1 << 30, INT_MAX - 1, INT_MAX};
+  for (int i = 0; i < (int)(sizeof toks / sizeof *toks); ++i)
+    for (int E = 4; E <= 8; E += 4)
+      for (int head = 0; head < E; ++head) {
+        const int p = lp_piece(toks[i], head, E);
+        CHECK((p >= 0) == (toks[i] >= head));
+        CHECK(p < 0 || ((long long)p * E + head <= toks[i] && toks[i] < ((long long)p + 1) * E + head));
+      }
+  static const unsigned bits[] = {0, 0x80000000u, 1, 0x80000001u, 0x80000002u, 0x007fffff, 0x00800000, 0x3f800000, 0xbf800000u, 0x7f7fffff, 0xff7fffffu, 0xff800000u};
+  for (int i = 0; i < (int)(sizeof bits / sizeof *bits); ++i) CHECK(f(lp_above(bits[i])) == nextafterf(f(bits[i]), INFINITY));
+  static const unsigned none[] = {0x7f800000, 0x7fc00000, 0x7fffffff, 0xffc00000u, 0xffffffffu};      /* +inf and NaN: any bits, no overflow */
+  for (int i = 0; i < (int)(sizeof none / sizeof *none); ++i) CHECK(lp_above(none[i]) != none[i]);
+  return 0;
+}
+"""
+
+
+def test_places_of_tokens(tmp_path):
+    """Any int as a token, any bits as its logit, without an overflow."""
+    run_c(tmp_path, PLACES)
