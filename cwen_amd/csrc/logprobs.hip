@@ -1,10 +1,11 @@
 // Log probabilities of given tokens, their ranks, entropies and the largest
 // logits, in one pass over the logits.
 //
-// A thread keeps m, s = sum e^(x - m) and t = sum e^(x - m) (x - m) of its
-// logits; then lse = m + ln s and the entropy is ln s - t / s.  The reference m
-// is renewed only when a logit outgrows it by more than LAG: s stays below
-// e^LAG times the number of logits.
+// A thread keeps m, its largest logit, s = sum e^(x - m) and t = sum e^(x - m)
+// (x - m); then lse = m + ln s and the entropy is ln s - t / s.  The largest one's
+// own term is exactly 1, so that a token near certainty keeps its digits, and the 16
+// terms of a turn are summed by themselves first, so that many small ones are not
+// lost one by one beside a large sum.
 //
 // A wave keeps the 64 largest logits seen, one a lane, sorted by value and then
 // by index.  A logit that comes before the last of the wanted ones goes into a
@@ -22,7 +23,7 @@
 namespace {
 
 constexpr int THREADS = LP_THREADS, WAVES = 4, SPLITS = LP_SPLITS;
-constexpr float LAG = 8.f, LOG2E = 1.44269504088896340736f;
+constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int NONE = 0x7fffffff;            // index of a list entry that is none
 
 // ---- sums
@@ -191,18 +192,18 @@ static_assert(LP_WORKGROUPS * part_words(CWEN_LOGPROBS_TOP) * 4 == CWEN_LOGPROBS
 
 __device__ __forceinline__ void finish(const LogprobArgs &a, int row, Sums r, int before_it, float xt, Entry e) {
   const int lane = threadIdx.x & 63;
-  const float ls = (float)log((double)r.s);
+  const double ls = log((double)r.s);
   if (lane == 0) {
     const int tok = a.tokens ? a.tokens[row] : -1;
     const bool there = tok >= 0 && tok < a.V && xt == xt;
-    if (a.lse) a.lse[row] = r.m == -INFINITY && r.s == 0.f ? -INFINITY : (float)((double)r.m + log((double)r.s));
-    if (a.entropy) a.entropy[row] = r.m == -INFINITY ? NAN : (float)(log((double)r.s) - (double)r.t / (double)r.s);
-    if (a.logprob) a.logprob[row] = there ? (xt - r.m) - ls : NAN;
+    if (a.lse) a.lse[row] = r.m == -INFINITY && r.s == 0.f ? -INFINITY : (float)((double)r.m + ls);
+    if (a.entropy) a.entropy[row] = r.m == -INFINITY ? NAN : (float)(ls - (double)r.t / (double)r.s);
+    if (a.logprob) a.logprob[row] = there ? (float)((double)xt - r.m - ls) : NAN;
     if (a.rank) a.rank[row] = there ? before_it : -1;
   }
   if (lane < a.top) {
     if (a.top_ids) a.top_ids[(long long)row * a.top + lane] = e.i == NONE ? -1 : e.i;
-    if (a.top_lp) a.top_lp[(long long)row * a.top + lane] = e.i == NONE ? -INFINITY : (e.v - r.m) - ls;
+    if (a.top_lp) a.top_lp[(long long)row * a.top + lane] = e.i == NONE ? -INFINITY : (float)((double)e.v - r.m - ls);
   }
 }
 
@@ -232,7 +233,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
   typename std::conditional<TOP == 2, Best, Most>::type best;
   best.start(s_qv[wave], s_qi[wave], a.top);
   auto grow = [&](float v) {          // all lanes
-    if (__any(v > r.m + LAG)) {
+    if (__any(v > r.m)) {
       renew(r, fmaxf(r.m, v));
       ref = r.m == -INFINITY ? 0.f : r.m;
     }
@@ -240,7 +241,7 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
   auto add = [&](float v) {
     const float d = v - ref, e = exp_of(d);
     r.s += e;
-    r.t = fmaf(e, fmaxf(d, -200.f), r.t);       // e is 0 there, and 0 times -infinity is not
+    r.t = fmaf(e, fmaxf(d, -200.f), r.t);
   };
   auto one = [&](float v, int i, bool in) {       // all lanes; in: there is one
     v = in ? v : -INFINITY;
@@ -266,10 +267,17 @@ template <typename T, int TOP, bool RANK> __global__ __launch_bounds__(THREADS) 
         most = fmaxf(most, f[k][e]);
       }
     grow(most);
+    float s4[4] = {}, t4[4] = {};
 #pragma unroll
     for (int k = 0; k < VECS; ++k)
 #pragma unroll
-      for (int e = 0; e < E; ++e) add(f[k][e]);
+      for (int e = 0; e < E; ++e) {
+        const float d = f[k][e] - ref, x = exp_of(d);
+        s4[e & 3] += x;
+        t4[e & 3] = fmaf(x, fmaxf(d, -200.f), t4[e & 3]);       // x is 0 there, and 0 times -infinity is not
+      }
+    r.s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    r.t += (t4[0] + t4[1]) + (t4[2] + t4[3]);
     if (RANK) {
 #pragma unroll
       for (int k = 0; k < VECS; ++k) {

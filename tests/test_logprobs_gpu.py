@@ -68,3 +68,37 @@ def test_one_scratch_for_every_call(env):
             gpu.logprobs(ctx, x[:rows], lse=lse, top_ids=ids, work=w)
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]), rows
         assert torch.equal(got[0][1].long(), torch.sort(x[:rows], dim=1, descending=True, stable=True).indices[:, :64]), rows
+
+
+def test_many_small_terms_beside_a_large_one(env):
+    """A thread's small terms, each below half a step of its sum, are not lost: 944 of e^-17 behind one of 1."""
+    rows, V = 400, 248320                                       # one part a row, 61 turns
+    x = torch.full((rows, V), -9.1, device="cuda")
+    x[:, :4096] = 0
+    x[:, 4096:8192:16] = 7.99
+    tok = torch.full((rows,), 4096, device="cuda", dtype=torch.int32)
+    out = run(env, x, tok, 1)
+    z = torch.log_softmax(x[0].double(), 0)
+    # 61 turns' sums, 6 roundings in a turn, 15 joins and 3 of exp, 2^-24 of the sum each; the entropy's second sum is 0.05 of
+    # the first, with 16 more roundings of its factors
+    bound = 85 * 2.0 ** -24
+    for name, want, b in (("logprob", z[4096], bound), ("lse", torch.logsumexp(x[0].double(), 0), bound), ("entropy", -(torch.exp(z) * z).sum(), 1.1 * bound)):
+        off = (out[name].double() - want).abs().max()
+        assert off <= b + 2.0 ** -24 * want.abs(), (name, off / 2.0 ** -24)
+
+
+def test_tokens_near_certainty(env):
+    """Log probabilities around -3e-4 keep an f32 sum's roundings, not those of a logit's exponential."""
+    rows, V = 2000, 8192
+    g = gen(3)
+    x, r = torch.randn(rows, V, device="cuda", generator=g), torch.arange(rows, device="cuda")
+    tok = torch.randint(V, (rows,), device="cuda", generator=g)
+    x[r, tok] = 17 + torch.rand(rows, device="cuda", generator=g)
+    out = run(env, x, tok.int(), 1)
+    want = torch.log_softmax(x.double(), 1)[r, tok]
+    assert -1e-3 < want.min() and want.max() < -1e-4
+    # the sum is 1 and a little: 2 turns, 6 roundings in one and 9 joins, half a step of 2^-23 each at most, 1 / sqrt(3) of that
+    # in the mean: sqrt(17 / 3) 2^-24
+    for got in (out["logprob"], out["top_logprobs"][:, 0]):
+        off = (got.double() - want) * 2.0 ** 24
+        assert off.abs().max() <= 17 and off.square().mean().sqrt() <= 3, (off.abs().max(), off.square().mean().sqrt())
