@@ -19,12 +19,15 @@
 // waves.  K and Q are laid out in that order by the first launch.
 //
 // Precision: f32 values enter a product as two f16 values, x s = hi + lo with a
-// power of two s per column: 22 bits, and down to 2^-25 of a unit.  The unit is
-// taken anew, the larger of |S| and |v| at 1 .. 2, every 8 chunks and whenever a
-// chunk's largest |v| is outside 1/8 .. 16 units.  A row lengthens a column of S by
-// beta |v| < 32 units at most, from 2 sqrt(D) before the 9 chunks that a unit can have
-// to go through: |S|, |S^T k| and r stay below 9300 units, d = beta (v - S^T k) below
-// 18600, and with rho below 37200, where f16 ends at 65504.  Keys and queries of 16 bits are exact
+// power of two s per column: 22 bits, and down to 2^-25 of a unit.  What counts beside
+// |S| is beta |v|: T, whose columns have beta as a factor, is divided by a power of two
+// of the chunk and head, its scale, that is not below the betas (1 for betas above 1/4),
+// and r is multiplied by it, v and S^T k each.  The unit is taken anew, the larger of
+// |S| and scale |v| at 1 .. 2, every 8 chunks and whenever a chunk's largest scale |v|
+// is outside 1/8 .. 16 units.  A row lengthens a column of S by beta |v| < 32 units
+// at most, from 2 sqrt(D) before the 9 chunks that a unit can have to go through: |S|,
+// |S^T k| and r stay below 9300 units, d = beta (v - S^T k) below 18600, and with rho
+// below 37200, where f16 ends at 65504.  Keys and queries of 16 bits are exact
 // f16 values after a power of two; what is left of their length (rho, 1 .. 2) goes into
 // the rows' factors.  f32 ones are normalised and split.
 #include <math.h>
@@ -45,11 +48,12 @@ template <int D, bool KL> struct Rec {
   static constexpr int K = 0, KLO = OP, Q = KL ? 2 * OP : OP, QLO = 3 * OP, KEY = KL ? 4 * OP : 2 * OP;
   static constexpr int T = 0, TLO = 2048, A = 4096, ALO = 6144, F = 8192, HEAD = F + 512;
 };
-// The factors: per row e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31 (beta is in T's columns).  The scores
+// The factors: per row scale e^G rho, rho e^(G_31 - G), e^G sigma; then e^G_31, the scale and the next chunk's (beta is in
+// T's columns).  The scores
 // and the last of the rows' factors are in units of O_UNIT, so that the low halves of small scores are no
 // subnormals, and without 1 / sqrt(D).
 constexpr float O_UNIT = 1.f / 64;
-enum { F_X = 0, F_D = 32, F_O = 64, F_END = 96 };
+enum { F_X = 0, F_D = 32, F_O = 64, F_END = 96, F_SCALE = 97, F_NEXT = 98 };
 
 struct PromptWork {
   char *key, *head;          // [piece][key head], [piece][value head]
@@ -67,6 +71,23 @@ __device__ __forceinline__ floatx4_t mma(half8_t a, half8_t b, floatx4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ int value_head(const GdnRuleArgs &a, int hk, int r) { return a.group ? hk * a.group + r : hk + a.nkh * r; }
+
+// The scale of a chunk and head, from its rows' betas in 32 lanes; one that is no number does not count.
+__device__ __forceinline__ float scale_of(float beta) {
+  float x = fmaxf(beta, 0.f);
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  x = fmaxf(x, dpp<0x140>(x));
+  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  x = fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
+  const float up = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, fminf(x, 1.f)) + 0x7fffffu) & 0x7f800000u);
+  return x > 0.25f ? 1.f : fmaxf(up, 0x1p-60f);
+}
+// The value that the wave's lower (e = 0) or upper 32 lanes have in common.
+__device__ __forceinline__ float of_half(float x, int e) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 32 * e));
+}
 
 // ---- first launch: a workgroup has one chunk of one key head ----
 // Bound by the trips to memory and the steps of the solve, not by its bytes or operations: all loads stand at the
@@ -92,22 +113,24 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
   if (t0 < 0 || rows <= 0) return;
   const long long first = (long long)q.first + t0;
   const int n = lane & 31, sub = 2 * wave + (lane >> 5), grp = a.nvh / a.nkh;
-  // The gates of value head r0 + sub, row n.
-  auto gate = [&](int r0, float &g, float &beta, int &hv) {
+  // The gates of value head r0 + sub, row n, and the next chunk's beta there.
+  const int rows_next = q.n - t0 - N;
+  auto gate = [&](int r0, float &g, float &beta, float &beta_next, int &hv) {
     const int r = r0 + sub;
     const bool have = sub < HEADS && r < grp;
     hv = have ? value_head(a, hk, r) : -1;
-    g = beta = 0.f;
+    g = beta = beta_next = 0.f;
     if (have && n < rows) {
       g = a.a[(first + n) * a.gs + hv];
       beta = a.b[(first + n) * a.gs + hv];
     }
+    if (have && n < rows_next) beta_next = a.b[(first + N + n) * a.gs + hv];
   };
 
   // K and Q into LDS as operands: 8 threads a row
   constexpr int PER = D / 8;
   const int row = tid >> 3;
-  float x[2][PER], g, beta;
+  float x[2][PER], g, beta, beta_next;
   int hv;
 #pragma unroll
   for (int op = 0; op < 2; ++op) {
@@ -115,7 +138,7 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
 #pragma unroll
     for (int i = 0; i < PER; i += 8) Io<TX>::load(p + i, *(float(*)[8])&x[op][i]);
   }
-  gate(0, g, beta, hv);
+  gate(0, g, beta, beta_next, hv);
 #pragma unroll
   for (int op = 0; op < 2; ++op) {
     float ss = 0.f;
@@ -185,12 +208,14 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
   if (wave >= HEADS / 2) return;
   const float rho = s_rho[n], sig = s_sig[n];
   for (int r0 = 0; r0 < grp; r0 += HEADS) {
-    if (r0) gate(r0, g, beta, hv);
+    if (r0) gate(r0, g, beta, beta_next, hv);
     if (a.A && hv >= 0 && n < rows) {
       const float y = g + a.dt[hv];
       g = a.A[hv] * (y > 20.f ? y : log1pf(expf(y)));
       beta = 1.f / (1.f + expf(-beta));
     }
+    if (a.A && hv >= 0 && n < rows_next) beta_next = 1.f / (1.f + expf(-beta_next));
+    const float scale = scale_of(beta), per_scale = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, scale));
     const float eg = expf(g);
     s_gb[sub][n] = make_float2(eg, beta);
     float *L = (float *)(s_mem + sub * HB);
@@ -207,13 +232,18 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
       L[i * LS + n] = gb.y * dec * s_G[i * GS + n];             // (only i > n is read)
       A[i] = i >= n ? dec * s_P[i * GS + n] : 0.f;
     }
+    const float next = scale_of(beta_next);
     char *out = w.head + ((long long)z * a.nvh + max(hv, 0)) * R::HEAD;
     if (hv >= 0) {
       float *F = (float *)(out + R::F);
-      F[F_X + n] = pre * rho;
+      F[F_X + n] = pre * rho * scale;
       F[F_D + n] = rho * dec;
       F[F_O + n] = pre * sig / O_UNIT;
-      if (n == N - 1) F[F_END] = pre;
+      if (n == N - 1) {
+        F[F_END] = pre;
+        F[F_SCALE] = scale;
+        F[F_NEXT] = next;
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     // (1 + L)^-1 in blocks of 16 rows: the two on the diagonal column by column, T_in = [i = n] - sum_(j < i) L_ij T_jn,
@@ -274,7 +304,7 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
       to[R::TLO / 2 + at] = f16_of(t - (float)h);
     };
 #pragma unroll
-    for (int i = 0; i < 16; ++i) put(op, 16 * (n >> 4) + i, n, i >= (n & 15) ? T[i] * beta : 0.f);   // (beta may be NaN)
+    for (int i = 0; i < 16; ++i) put(op, 16 * (n >> 4) + i, n, i >= (n & 15) ? T[i] * (beta * per_scale) : 0.f);   // (beta may be NaN)
     // rows 0 .. 15 of the later columns: nothing (zeros of the earlier lanes' blocks)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -282,7 +312,7 @@ template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int m = lane & 15;
-      const float b = s_gb[2 * wave + e][m].y;
+      const float b = s_gb[2 * wave + e][m].y * of_half(per_scale, e);
 #pragma unroll
       for (int i = 0; i < 4; ++i) put((_Float16 *)(s_mem + (2 * wave + e) * HB), 16 + 4 * (lane >> 4) + i, m, T21[e][i] * b);
     }
@@ -361,9 +391,9 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   char *s_io;                        // the wave's columns of a chunk, row by row: values, then outputs, of which the
                                      // values are read before outputs are written, and outputs before the next values
   float out_unit;
-  // the state, divided by the column's unit, and the present chunk's values
+  // the state, divided by the column's unit, and the present chunk's values, with its scale
   floatx4_t S[DT];
-  float unit, per_unit, v[8], vmax;
+  float unit, per_unit, v[8], vmax, scale;
   uint4 vr[NV][VP];                  // values on their way: chunk c's in vr[c % NV]
   float far[XS == 4 ? 8 : 4];    // the chunk's after that, by columns (16 bits: two a float)
 
@@ -398,7 +428,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     }
     asm volatile("" ::: "memory");
   }
-  // The turned values become the present ones; vmax: their column's largest.
+  // The turned values become the present ones; vmax: their column's largest, times their scale.
   __device__ __forceinline__ void take_v() {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -413,16 +443,16 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     vmax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]));
-    vmax = max_groups(vmax);
+    vmax = max_groups(vmax) * scale;
   }
   // Of the finite ones: an infinite value is no measure for the rows before it.
   __device__ __forceinline__ void finite_vmax() {
     vmax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
-    vmax = max_groups(vmax);
+    vmax = max_groups(vmax) * scale;
   }
-  // The unit for the larger of |S| and `most` (a |v|) to lie in 1 .. 2, in the columns that call for it: what a column
+  // The unit for the larger of |S| and `most` (a scaled |v|) to lie in 1 .. 2, in the columns that call for it: what a column
   // gets does not depend on its neighbours.  Returns what S has to be multiplied by.
   __device__ __forceinline__ float renew(float most, bool call) {
     float mx = 0.f;
@@ -478,6 +508,7 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     };
     // Operands are asked for a stage before the product that takes them (stages do not mix): left to itself the
     // compiler reads each one just ahead of its product, and the wave, alone on its SIMD, waits for LDS 30 times a chunk.
+    const float scale_next = F[F_NEXT];
     half8_t K[2 * U], KL_[2 * U];
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
@@ -487,12 +518,13 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
     floatx4_t fx[2], fd[2], fo[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) fx[mt] = rows4(F_X, mt);
-    // The present values in units, and whether the next ones call for new units in the chunks to come: at least every
-    // 8, and where their |v| leaves what the present one is good for.
+    // The present values, scaled, in units, and whether the next ones call for new units in the chunks to come: at least
+    // every 8, and where their scaled |v| leaves what the present one is good for.
     float w[8], ratio = 1.f;
-    const float vmax_here = vmax, unit_here = unit;
+    const float vmax_here = vmax, unit_here = unit, to_units = per_unit * scale;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = v[e] * per_unit;
+    for (int e = 0; e < 8; ++e) w[e] = v[e] * to_units;
+    scale = scale_next;
     take_v();
     auto stay = [&]() __attribute__((always_inline)) {
       const float vu = vmax * per_unit;
@@ -828,8 +860,9 @@ void chain_kernel(GdnRuleArgs a, PromptWork w) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) p.S[t][i] = from[(16 * t + i) * D];
   }
-  p.unit = p.per_unit = 1.f;
+  p.unit = p.per_unit = p.scale = 1.f;
   if (chunks) {
+    p.scale = *(const float *)(w.head + ((long long)gdn_piece0(q.first, s, N) * a.nvh + hv) * R::HEAD + R::F + 4 * F_SCALE);
     p.v0 = (const char *)a.v + (q.first * a.vs + hv * D) * C::XS;
     p.v_row = (uint32_t)a.vs * C::XS;
     p.v_chunk = a.vs * C::XS * N;

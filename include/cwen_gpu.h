@@ -288,11 +288,10 @@ int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype
  * cwen_gdn_prompt takes chunks of 32 rows on the matrix cores: with d_i of a
  * chunk from (1 + L) d = r, L_ij = beta_i g_j+1..g_i k_i.k_j (j < i), r_i =
  * beta_i (v_i - g_1..g_i S^T k_i).  Operands are rounded to f16 in pieces whose
- * sum holds 21 bits or more, below the column's largest |S| and |v| of the chunk
- * (so a state far below its |v|, of betas near 2^-n alone, keeps 24 - n bits of
- * its own); sums are f32, outputs of 16 bits those of F32 rounded once.  `work`:
- * device scratch of cwen_gdn_prompt_work's bytes, 256-byte aligned, free again
- * when the call's launches are done. */
+ * sum holds 21 bits or more, below the column's largest |S| and |v|, times the
+ * largest beta, of the chunk and its neighbours; sums are f32, outputs of 16 bits
+ * those of F32 rounded once.  `work`: device scratch of cwen_gdn_prompt_work's
+ * bytes, 256-byte aligned, free again when the call's launches are done. */
 int cwen_gdn_step(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *q, long long q_ts,
                   const void *k, long long k_ts, const void *v, long long v_ts, const float *a, const float *b,
                   long long g_ts, const float *A, const float *dt, int otype, void *o, long long o_ts, const int *cu,

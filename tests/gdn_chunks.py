@@ -2,7 +2,8 @@
 
 An f32 value x enters a product as two f16 values, hi + lo: off by 2^-22 |x|, and by 2^-25 of its column's unit at least.
 `chunks` forms the products of chunks of 32 rows from such operands (sums in 64 bits, results in 32); `single` names
-operands that are left as their hi alone, 2^-11 off instead."""
+operands that are left as their hi alone, 2^-11 off instead.  A chunk's values and T are scaled by a power of two that its
+betas call for, so that what counts beside |S| is beta |v|."""
 import math
 
 import torch
@@ -14,7 +15,13 @@ N = 32
 OPERANDS = ("S", "r", "T", "y", "x", "A", "K", "Q")
 
 
-def chunks(q, k, v, g, beta, S, single=(), key_head="mod"):
+def scales(beta):
+    """Per chunk and head: the power of two not below the chunk's largest beta, or 1 for betas above 1/4."""
+    most = torch.stack([beta[c:c + N].float().amax(0) for c in range(0, beta.shape[0], N)])
+    return torch.where(most > 0.25, 1.0, torch.exp2(torch.ceil(torch.log2(most.clamp(min=2.0 ** -60)))))
+
+
+def chunks(q, k, v, g, beta, S, single=(), key_head="mod", scaled=True):
     """As gdn_ref.rule on f32 tensors, without M."""
     n, H, D = v.shape
     m = [h % k.shape[1] if key_head == "mod" else h // (H // k.shape[1]) for h in range(H)]
@@ -28,6 +35,7 @@ def chunks(q, k, v, g, beta, S, single=(), key_head="mod"):
     def product(a, b):                                                     # without the product of the two low halves
         return (a[0] @ b[0] + a[1] @ b[0] + a[0] @ b[1]).float()
 
+    scale = scales(beta) if scaled else torch.ones(-(-n // N), H)
     k, q, v = per_head(length(k)), per_head(length(q)), v.float().transpose(0, 1)
     g, beta = g.float().t(), beta.float().t()
     pad = -n % N
@@ -38,7 +46,8 @@ def chunks(q, k, v, g, beta, S, single=(), key_head="mod"):
     low = torch.ones(N, N).tril().bool()
     for c in range((n + pad) // N):
         at, after = slice(c * N, c * N + N), slice(c * N + N, c * N + 2 * N)
-        here, nxt = v[:, at].abs().amax(1), v[:, after].abs().amax(1) if (c + 1) * N < n + pad else torch.zeros(H, D)
+        sc, here = scale[c][:, None], v[:, at].abs().amax(1) * scale[c][:, None]
+        nxt = v[:, after].abs().amax(1) * scale[c + 1][:, None] if (c + 1) * N < n + pad else torch.zeros(H, D)
         if unit is None:
             unit = _unit(torch.maximum(S.abs().amax(1), here))
         s = S / unit[:, None]
@@ -47,10 +56,10 @@ def chunks(q, k, v, g, beta, S, single=(), key_head="mod"):
         K, Q, SS = halves("K", k[:, at]), halves("Q", q[:, at]), halves("S", s)
         turned = tuple(x.transpose(1, 2) for x in K)
         L = beta[:, at, None] * decay * product(K, turned) * low.tril(-1)
-        T = (torch.linalg.inv((torch.eye(N) + L).double()).float() * beta[:, None, at])
+        T = torch.linalg.inv((torch.eye(N) + L).double()).float() * (beta[:, None, at] / sc[..., None])
         A = halves("A", 64 * decay * product(Q, turned))
         eG = torch.exp(G).float()[..., None]
-        r = v[:, at] / unit[:, None] - eG * product(K, SS)
+        r = v[:, at] * sc[..., None] / unit[:, None] - eG * sc[..., None] * product(K, SS)
         d = product(halves("T", T), halves("r", r))
         o[:, at] = (eG * product(Q, SS) + product(A, halves("x", d)) / 64) * unit[:, None]
         y = d * torch.exp(G[:, -1:] - G).float()[..., None]
@@ -66,11 +75,12 @@ def _unit(x):
 
 def bounds(g, m, wider=1, linear=0):
     """Of each output [n, H, D] and of the state's columns' lengths [H, D], for keys, queries, values and gates that are
-    independent of each other; g the log decays, m the largest of a column's |state| + |v| in a row's chunk and the one before.
+    independent of each other; g the log decays, m the largest of a column's |state| + s |v| in a row's chunk and the one before,
+    s the chunk's scale.
 
     An operand's element is off by 2^-22 of itself at most, and by 2^-25 of its column's unit, which is no more than 8 m; below
-    2^-22 m, with a sign of its own.  A row's d has the errors of S, k, v, r and T in it, each times a vector of length 1 or
-    less; beta <= 1 of it enters the state along k, with the errors of y and k there and 2^-22 m more for lengths, decays
+    2^-22 m, with a sign of its own.  A row's d has the errors of S, k, s v, s r and T / s in it, each times a vector of length 1
+    or less; it enters the state along k, with the errors of y and k there and 2^-22 m more for lengths, decays
     and sums in f32 (2^-24 times the root of their terms): sqrt(8) 2^-22 m a row.  Later rows do not enlarge what is there,
     they let it decay, and errors of independent signs add as their squares.  The largest of the columns may be twice that.
     An output has the state's error along q, and its own: S and q, and the 32 terms of the scores times x, from two operands
@@ -106,16 +116,26 @@ def inputs(n, nkh, nvh, D, seed, dtype=torch.float32):
 def reference(q, k, v, g, beta, S, key_head="mod", wider=1, linear=0):
     """(outputs, end state) in 64 bits, and the bounds of both."""
     n, H, D = v.shape
+    scale = scales(beta)
     S = torch.zeros(H, D, D, dtype=torch.float64) if S is None else S.double()
     o, size = torch.empty(n, H, D, dtype=torch.float64), torch.empty(n, H, D, dtype=torch.float64)
     for t in range(n):
         r = slice(t, t + 1)
         before = S.norm(dim=1)
         o[t], S, _ = R.rule(q[r], k[r], v[r], g[r].double(), beta[r].double(), S, key_head)
-        size[t] = torch.maximum(before, S.norm(dim=1)) + v[t].double().abs()
+        size[t] = torch.maximum(before, S.norm(dim=1)) + v[t].double().abs() * scale[t // N].double()[:, None]
     m = torch.stack([size[c:c + N].amax(0) for c in range(0, n, N)])
     m[1:] = torch.maximum(m[1:], m[:-1])
     return (o, S), bounds(g, m.repeat_interleave(N, 0)[:n], wider, linear)
+
+
+def small_betas(n, H, D, seed, dtype=torch.float32):
+    """A head each of betas around 2^-3, 2^-8, .. : the state is far below the values.  The last head's betas are small in its
+    first chunks, then near 1 for a chunk, then small again."""
+    q, k, v, g, beta, _ = inputs(n, H, H, D, seed, dtype)
+    beta = beta * torch.exp2(-3.0 - 5 * torch.arange(H))
+    beta[96:128, -1] = 0.9
+    return q, k, v, g, beta, None
 
 
 def long_betas(kind, n, H, D, seed, dtype=torch.float32):

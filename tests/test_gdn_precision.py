@@ -37,3 +37,13 @@ def test_betas_above_one(kind):
         want, limits = G.reference(*x, **wider)
         o, s = G.share(G.chunks(*x), want, limits)
         assert o < 0.5 and s < 0.5, (o, s)
+
+
+def test_small_betas():
+    """A state of small betas alone keeps the bits that others do; without a scale it would not."""
+    x = G.small_betas(200, 6, 64, 1)
+    want, limits = G.reference(*x)
+    o, s = G.share(G.chunks(*x), want, limits)
+    assert o < 0.2 and s < 0.2, (o, s)
+    o, s = G.share(G.chunks(*x, scaled=False), want, limits)
+    assert o > 3 and s > 3, (o, s)

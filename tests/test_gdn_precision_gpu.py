@@ -119,3 +119,20 @@ def test_betas_above_one(env, kind, tx):
             else:
                 eo, es = R.step_bounds(n, D, M, F32)
                 assert bool(((got[0] - want[0]).abs() <= eo).all()) and bool(((got[1] - want[1]).abs() <= es[:, None]).all()), (n, D)
+
+
+@pytest.mark.parametrize("tx", [F32, F16, BF16])
+def test_small_betas(env, tx):
+    """A prompt whose state is far below its values keeps as many bits of the state, in every launch width."""
+    gpu, ctx = env
+    for n, S, H, D in ((200, 1, 6, 128), (333, 2, 6, 64), (200, 16, 6, 128), (200, 24, 6, 128), (161, 24, 6, 64)):
+        x = G.small_betas(n, H, D, n + D, tx)
+        want, limits = G.reference(*x)
+        q, k, v, a, b = (t.cuda().repeat(S, *[1] * (t.dim() - 1)) for t in x[:5])
+        pool = gpu.GdnPool.empty(1, S, H, H, D)
+        o, slots = torch.empty(S * n, H, D, device="cuda"), ints(list(range(S)))
+        gpu.gdn_prompt(ctx, pool, 0, q, k, v, a, b, o, ints(borders([n] * S)), None, slots)
+        for i in range(0, S, max(1, S - 1)):
+            worst = G.share((o[i * n:(i + 1) * n].cpu(), pool.state[0, i].cpu()), want, limits)
+            print(tx, n, S, D, worst, flush=True)
+            assert max(worst) < 1, (n, S, D, worst)
