@@ -91,8 +91,8 @@ __device__ __forceinline__ float of_half(float x, int e) {
 
 // ---- first launch: a workgroup has one chunk of one key head ----
 // Bound by the trips to memory and the steps of the solve, not by its bytes or operations: all loads stand at the
-// start, and LDS is used twice, so that four workgroups share a CU (16301 rows of 16/48 heads of 128 in bf16: 121 us, 3.9
-// TB/s).
+// start, and LDS is used twice.  Three workgroups share a CU, by their registers and by LDS (16301 rows of 16/48 heads of
+// 128 in bf16: 143 us, 3.7 TB/s).
 constexpr int PREP_WAVES = 4;
 
 template <typename TX, int D> __global__ __launch_bounds__(64 * PREP_WAVES) void prep_kernel(GdnRuleArgs a, PromptWork w) {
@@ -374,8 +374,8 @@ template <typename TX, typename TO, int D, int NW> struct Chain {
   static constexpr int U = R::U, DT = D / 16, KB = R::KEY / 1024 + R::HEAD / 1024 + 1, XS = sizeof(TX), OS = sizeof(TO);
   static constexpr int VP = XS / 2, OP = OS / 2;     // a wave's loads and stores of a chunk
   // Of two waves each has another one that forms its outputs, a chunk later, from S's and d's halves in LDS: what a chunk
-  // takes is one wave's products and instructions, one after the other (8192 rows of 48 heads of 128 in bf16: 312 us, with
-  // the outputs among them 341).  f32 heads of 128 have no room for that and a fourth record.
+  // takes is one wave's products and instructions, one after the other (8192 rows of 48 heads of 128 in bf16, both launches:
+  // 406 us, with the outputs among them 449).  f32 heads of 128 have no room for that and a fourth record.
   static constexpr bool SPLIT = NW == 2 && (XS == 2 || D == 64);
   static constexpr int EX = 2 * (U + 1) * 1024 + 512, NV = SPLIT ? 4 : 3;
   typedef char Buf[R::KEY + R::HEAD];
@@ -931,9 +931,11 @@ template <typename TX, typename TO, int D> void launch(const GdnRuleArgs &a, con
   const long long pieces = gdn_pieces(a.s.total, a.s.n_seq, N);
   hipLaunchKernelGGL((prep_kernel<TX, D>), dim3((unsigned)(pieces * a.nkh)), dim3(64 * PREP_WAVES), 0, st, a, w);
   // Waves of a workgroup: the fewest with which the workgroups have a CU each.  Few waves beside each other are faster
-  // (1024 rows of 48 heads of 128 in bf16, both launches, before the outputs had waves of their own: 62 us with two, 66 with
-  // four, 85 with eight), two workgroups on a CU are not (two such sequences: 86, 77, 96).  Past that all of a head's columns: a record then comes once, and two of
-  // the chain's waves share a SIMD (four: 142, 134, 108; 48: 1353, 1234, 1019).  Eight waves of f32 operands do not fit the
+  // (1024 rows of 48 heads of 128 in bf16, both launches: 63 us with two, 71 with four, 91 with eight), two workgroups on a
+  // CU are not (two such sequences: 116, 82, 104).  Past that all of a head's columns: a record then comes once, and two of
+  // the chain's waves share a SIMD (four: 177, 147, 119; 48: 2058, 1365, 1179).  Short sequences are the same: 8 of 64 rows
+  // 54, 38, 37; 40 of 16 rows 194, 103, 92; 40 of 256 rows 564, 359, 315.  (Workgroups of eight have a CU each, so one head
+  // more than there are CUs is a second round: five sequences 133, six 212.)  Eight waves of f32 operands do not fit the
   // registers.
   constexpr int MANY = D == 128 && sizeof(TX) == 2 ? 8 : 4, CUS = 256;
   const long long heads = (long long)a.s.n_seq * a.nvh;

@@ -260,8 +260,10 @@ int cwen_gdn_status(cwen_ctx *ctx, const cwen_gdn_pool *pool, int *bits, void *s
  * history (conv1d_update + silu, run.c:2183-2200).  x [total] rows of C
  * elements, x_ts apart, kw [C][4] f32 (device, 16-byte aligned), y (nullable:
  * the history alone moves) likewise; element types xtype and ytype (F32, F16,
- * BF16), computed in f32 and rounded once.  Pointers 16-byte aligned, strides
- * multiples of 8; y must not overlap x. */
+ * BF16), computed in f32 and rounded once; silu(z) with the hardware's exp2 and
+ * reciprocal: off by (6 + 2 |z|) 2^-24 of itself, 0 below z = -87 (so not the
+ * bits of cwen_gdn_block's).  Pointers 16-byte aligned, strides multiples of 8; y must
+ * not overlap x. */
 int cwen_gdn_conv(cwen_ctx *ctx, const cwen_gdn_pool *pool, int layer, int xtype, const void *x, long long x_ts,
                   const float *kw, int ytype, void *y, long long y_ts, const int *cu, const int *count, const int *src,
                   const int *dst, int n_seq, int total, void *stream);

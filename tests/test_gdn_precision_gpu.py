@@ -136,3 +136,21 @@ def test_small_betas(env, tx):
             worst = G.share((o[i * n:(i + 1) * n].cpu(), pool.state[0, i].cpu()), want, limits)
             print(tx, n, S, D, worst, flush=True)
             assert max(worst) < 1, (n, S, D, worst)
+
+
+def test_silu_of_the_convolution(env):
+    """Taps that pass the input on: silu alone, to the stated share of itself."""
+    gpu, ctx = env
+    pool = gpu.GdnPool(1, 2, 64, hist=torch.zeros(1, 1, 256, 3, device="cuda"))
+    kw = torch.zeros(256, 4, device="cuda")
+    kw[:, 3] = 1
+    span = torch.linspace(-86.5, 90, 39000, device="cuda"), torch.logspace(-30, 4, 1000, device="cuda"), -torch.logspace(-30, 1, 960, device="cuda")
+    x = torch.cat(span).view(160, 256)
+    low = torch.linspace(-3e38, -87.5, 256, device="cuda")[None]
+    y = torch.empty(161, 256, device="cuda")
+    gpu.gdn_conv(ctx, pool, 0, torch.cat([x, low]), kw, y, ints([0, 161]))
+    z = x.double()
+    want = z * torch.sigmoid(z)
+    # the exponent's product 1.22 |z|, exp2 2, the sum 1, the reciprocal 2, the product 1, each 2^-24
+    assert ((y[:160].double() - want).abs() <= (6 + 2 * z.abs()) * 2.0 ** -24 * want.abs() + 2.0 ** -126).all()
+    assert y[160].abs().max() < 2e-36
